@@ -1,0 +1,371 @@
+"""The kernels of the 4-bit cache on the GPU: writing, reading back, and attention, against 64 bits.
+
+Tolerances of attention, before any run: the cached numbers are exact, so with scores up to ``s`` and values up to ``v`` in magnitude
+a weight is off by about the score's rounding, ``s`` times a few float32 roundings (2^-24) over the sum of 16 to 256 products, and
+the exponential's (2^-22); all of it is below ``v (s + 4) 2^-18`` in the result.  In bfloat16 the result is rounded to 2^-9 of itself,
+and the probabilities may be float16 (2^-12 of each, at most ``v 2^-12`` together).
+"""
+
+import pytest
+import torch
+
+import fp4_plain
+from torchllms_b200.cache import fp4
+
+pytestmark = pytest.mark.gpu
+DT = {"f32": torch.float32, "bf16": torch.bfloat16}
+
+
+def ops():
+    from torchllms_b200.kernels import get_ops
+    return get_ops()
+
+
+# ------------------------------------------------------------------------------------------------- writing
+
+def turned(x, cs, interleaved):
+    """The rotation in float32, every product and sum rounded by itself."""
+    n = 2 * cs.shape[1]
+    c, s = cs[:, None, :, 0], cs[:, None, :, 1]
+    a, b = (x[..., 0:n:2], x[..., 1:n:2]) if interleaved else (x[..., :n // 2], x[..., n // 2:n])
+    y0, y1 = a * c - b * s, b * c + a * s
+    y = torch.stack([y0, y1], -1).flatten(-2) if interleaved else torch.cat([y0, y1], -1)
+    return torch.cat([y, x[..., n:]], -1)
+
+
+@pytest.mark.parametrize("T,H,KV,D,rot,page,interleaved,dtype,splits", [
+    (1, 4, 2, 64, 64, 16, True, "bf16", 1),
+    (1, 8, 1, 128, 128, 16, False, "f32", 1),
+    (7, 3, 1, 32, 32, 48, True, "f32", 1),
+    (33, 6, 2, 48, 48, 16, False, "bf16", 1),        # half of the rotated part is no multiple of eight
+    (300, 4, 4, 16, 10, 32, False, "f32", 1),
+    (300, 4, 4, 16, 10, 32, True, "bf16", 1),        # the rotated part ends inside a run of eight
+    (515, 14, 2, 128, 64, 64, True, "bf16", 1),
+    (70, 8, 2, 256, 128, 16, False, "bf16", 1),
+    (5, 32, 8, 128, 128, 16, True, "bf16", 3),       # float32 partial sums
+    (9, 4, 2, 64, 64, 16, False, "f32", 2),
+])
+def test_rows_are_rotated_and_held_in_4_bits(T, H, KV, D, rot, page, interleaved, dtype, splits):
+    g = torch.Generator().manual_seed(T + D)
+    n_pages = -(-T // page) + 3
+    x = torch.randn((splits, T, (H + 2 * KV) * D), generator=g) * torch.exp2(torch.randint(-6, 7, (1, T, 1), generator=g).float())
+    x = x.to(DT[dtype]) if splits == 1 else x
+    positions = torch.randint(0, 900, (T,), generator=g).int()
+    table = torch.randn((900, rot // 2, 2), generator=g)
+    slots = torch.randperm(n_pages * page, generator=g)[:T].int()
+    dev = [t.cuda() for t in (x, positions, table, slots)]
+    pages = [torch.randint(0, 200, fp4.page_shape(n_pages, KV, page, D), generator=g).to(torch.uint8).cuda() for _ in range(2)]
+    before = [p.clone() for p in pages]
+    q = ops().rope_kv_write_fp4(dev[0][0] if splits == 1 else dev[0], dev[1], dev[2], n_heads=H, n_kv_heads=KV, head_dim=D,
+                                interleaved=interleaved, k_pages=pages[0], v_pages=pages[1], slot_mapping=dev[3], page_size=page,
+                                out_dtype=DT[dtype])
+    # bit for bit what the definition makes of the rows in float32
+    rows = dev[0][0].float()
+    for sp in range(1, splits):
+        rows = rows + dev[0][sp]
+    rows = rows.view(T, H + 2 * KV, D)
+    y = turned(rows[:, :H + KV], dev[2][dev[1].long()], interleaved)
+    assert torch.equal(q, y[:, :H].to(DT[dtype]))
+    expect = [b.clone() for b in before]
+    fp4.store(expect[0], y[:, H:], dev[3], page)
+    fp4.store(expect[1], rows[:, H + KV:], dev[3], page)
+    for got, want, held in zip(pages, expect, (y[:, H:], rows[:, H + KV:])):
+        mine = [fp4.load(t, dev[3], page, D) for t in (got, want)]
+        assert torch.equal(mine[0], mine[1]) and torch.equal(mine[0].double().cpu(), fp4_plain.quantized(held.cpu()))
+    # other slots are as they were, byte for byte
+    rest = torch.tensor(sorted(set(range(n_pages * page)) - set(slots.tolist()))).cuda()
+    for got, was in zip(pages, before):
+        for a, b in zip(fp4.rows_of(got, D), fp4.rows_of(was, D)):
+            pick = lambda t: t[rest // page, :, rest % page // 16, rest % 16]  # noqa: E731
+            assert torch.equal(pick(a), pick(b))
+    # reading back, in either dtype: exactly what is there
+    for out_dtype in DT.values():
+        k, v = ops().kv_read_fp4(pages[0], pages[1], dev[3], head_dim=D, page_size=page, out_dtype=out_dtype)
+        assert torch.equal(k.float(), fp4.load(pages[0], dev[3], page, D)) and torch.equal(v.float(), fp4.load(pages[1], dev[3], page, D))
+
+
+def test_hard_numbers_and_rows_without_a_cache():
+    H, KV, D, page = 2, 2, 32, 16
+    x = torch.zeros((6, (H + 2 * KV) * D))
+    v = x[:, (H + KV) * D:].view(6, KV, D)
+    v[0, 0, 3], v[1, 0, 17], v[2], v[3], v[4, :, ::3] = float("inf"), float("nan"), -1e30, 2e-5, 1e-45
+    g = torch.Generator().manual_seed(1)
+    v[5] = torch.randint(-64, 65, (KV, D), generator=g) / 8.0            # quotients halfway between two codes
+    pages = [torch.zeros(fp4.page_shape(1, KV, page, D), dtype=torch.uint8).cuda() for _ in range(2)]
+    table, positions, slots = torch.tensor([[[1.0, 0.0]]]).expand(1, D // 2, 2).contiguous().cuda(), torch.zeros(6, dtype=torch.int32).cuda(), \
+        torch.arange(6, dtype=torch.int32).cuda()
+    kw = dict(n_heads=H, n_kv_heads=KV, head_dim=D, interleaved=True, page_size=page)
+    q = ops().rope_kv_write_fp4(x.cuda(), positions, table, k_pages=pages[0], v_pages=pages[1], slot_mapping=slots, **kw)
+    _k, got = ops().kv_read_fp4(pages[0], pages[1], slots, head_dim=D, page_size=page)
+    want = fp4_plain.quantized(v).float()
+    assert torch.equal(got.cpu().isnan(), want.isnan()) and torch.equal(got.cpu().nan_to_num(), want.nan_to_num())
+    assert got[0, 0, :16].isnan().all() and not got[0, 0, 16:].isnan().any() and (got[2] == -61440).all()
+    alone = ops().rope_kv_write_fp4(x.cuda(), positions, table, k_pages=None, v_pages=None, slot_mapping=None, **kw)
+    assert torch.equal(alone, q)
+    empty = ops().kv_read_fp4(pages[0], pages[1], slots[:0], head_dim=D, page_size=page)
+    assert empty[0].shape == (0, KV, D)
+
+
+def test_rows_whose_norm_was_deferred():
+    from torchllms_b200.kernels.lazy import RowScaled
+    T, H, KV, D, page = 5, 4, 2, 64, 16
+    g = torch.Generator().manual_seed(2)
+    x, ssq = torch.randn((2, T, (H + 2 * KV) * D), generator=g).cuda(), torch.rand((T, 3), generator=g).cuda() + 0.5
+    rs = RowScaled(x, ssq, 256, 1e-5)
+    table, positions = torch.randn((9, D // 2, 2), generator=g).cuda(), torch.arange(T, dtype=torch.int32).cuda()
+    kw = dict(n_heads=H, n_kv_heads=KV, head_dim=D, interleaved=False, slot_mapping=positions, page_size=page, out_dtype=torch.bfloat16)
+    a, b = ([torch.zeros(fp4.page_shape(1, KV, page, D), dtype=torch.uint8).cuda() for _ in range(2)] for _ in range(2))
+    q = ops().rope_kv_write_fp4(rs, positions, table, k_pages=a[0], v_pages=a[1], **kw)
+    want = ops().rope_kv_write_fp4((x[0] + x[1]) * rs.scale()[:, None], positions, table, k_pages=b[0], v_pages=b[1], **kw)
+    assert (q.float() - want.float()).abs().max() <= 2.0 ** -7 * want.float().abs().max()       # (a factor rounded another way)
+    for s, t in zip(a, b):
+        off = fp4.load(s, positions, page, D) - fp4.load(t, positions, page, D)
+        assert (off != 0).float().mean() < 0.01
+
+
+# ------------------------------------------------------------------------------------------------- attention
+
+def batch(H, KV, D, page, q_lens, kv_lens, window=None, dtype="bf16", seed=0, poison=True, sharp=1.0):
+    """A step over a cache in which everything that no query may see is byte 255 (scales that are not numbers) and blocks
+    before the window have no page."""
+    g = torch.Generator().manual_seed(seed)
+    blocks = [-(-n // page) for n in kv_lens]
+    n_pages = sum(blocks) + 2
+    order = torch.randperm(n_pages, generator=g).tolist()
+    table = torch.full((len(kv_lens), max(blocks) + 3), -1, dtype=torch.int32)
+    seen = torch.zeros((n_pages, page), dtype=torch.bool)
+    for b, (n, L) in enumerate(zip(q_lens, kv_lens)):
+        first = max(0, L - n - window + 1) if window else 0
+        for j in range(blocks[b]):
+            p = order.pop()
+            if n and (j + 1) * page > first:
+                table[b, j] = p
+                at = torch.arange(page) + j * page
+                seen[p] = (at >= first) & (at < L)
+    gain = torch.exp(0.5 * torch.randn((KV, 1, D), generator=g))
+    pages = []
+    for k in (gain, torch.ones_like(gain)):
+        x = torch.randn((n_pages, KV, page, D), generator=g) * k
+        codes, scales = fp4.encode(x)
+        if poison:
+            codes[~seen[:, None].expand(-1, KV, -1)] = 255
+            scales[~seen[:, None].expand(-1, KV, -1)] = 255
+        parts = [t.reshape(n_pages, KV, page // 16, -1) for t in (codes, scales)]
+        pages.append(torch.cat(parts, -1).contiguous().cuda())
+    q_start = torch.zeros(len(q_lens) + 1, dtype=torch.int32)
+    q_start[1:] = torch.cumsum(torch.tensor(q_lens), 0)
+    q = (torch.randn((int(q_start[-1]), H, D), generator=g) * sharp).to(DT[dtype])
+    return dict(q=q.cuda(), k_pages=pages[0], v_pages=pages[1], block_table=table.cuda(), q_start=q_start.cuda(),
+                kv_len=torch.tensor(kv_lens, dtype=torch.int32).cuda()), \
+        dict(n_seqs=len(q_lens), max_q_len=max(q_lens), max_kv_len=max(kv_lens), scale=D ** -0.5, window=window, page_size=page)
+
+
+def judge(got, a, kw):
+    want, s, v = fp4_plain.attention(a["q"], a["k_pages"], a["v_pages"], a["block_table"], a["q_start"], a["kv_len"], kw["page_size"],
+                                     kw["scale"], kw["window"])
+    bound = v * (s + 4.0) * 2.0 ** -18
+    if got.dtype == torch.bfloat16:
+        bound = bound + v * 2.0 ** -12 + want.abs() * 2.0 ** -8
+    off = (got.double().cpu() - want).abs()
+    assert (off <= bound).all(), (float((off / bound).max()), float(off.max()))
+
+
+SHAPES = [
+    # H, KV, D, page, q_lens, kv_lens, window
+    pytest.param(4, 2, 64, 16, [1], [1], None, id="first_token"),
+    pytest.param(32, 8, 64, 16, [1], [333], None, id="one_64"),
+    pytest.param(8, 2, 128, 16, [1, 1, 1], [17, 640, 1], None, id="three_128"),
+    pytest.param(8, 1, 128, 48, [1, 1], [500, 49], None, id="pages_of_48"),
+    pytest.param(7, 1, 128, 32, [1, 3, 2], [65, 200, 2], None, id="group_of_7"),
+    pytest.param(16, 16, 64, 128, [1, 4], [129, 1000], None, id="no_groups"),
+    pytest.param(24, 1, 64, 16, [1, 1], [70, 300], None, id="group_of_24"),
+    pytest.param(4, 2, 64, 16, [1, 1, 2], [600, 90, 300], 64, id="window_64"),
+    pytest.param(4, 2, 128, 64, [1, 5], [700, 390], 129, id="window_129"),
+    pytest.param(4, 4, 64, 16, [1, 1], [50, 500], 1, id="window_1"),
+    pytest.param(4, 2, 64, 16, [5, 3, 1], [2, 3, 0], None, id="rows_that_see_nothing"),
+    pytest.param(4, 2, 128, 16, [0, 1, 0, 2], [30, 31, 0, 64], None, id="requests_without_tokens"),
+    pytest.param(6, 2, 48, 16, [1, 9], [40, 100], None, id="heads_of_48"),
+    pytest.param(2, 1, 16, 16, [1, 20], [300, 20], 33, id="heads_of_16"),
+    pytest.param(4, 1, 256, 32, [1, 2], [90, 400], None, id="heads_of_256"),
+    pytest.param(8, 2, 128, 16, [64], [64], None, id="prompt_64"),
+    pytest.param(4, 2, 64, 16, [131], [131], None, id="prompt_131"),
+    pytest.param(4, 1, 128, 16, [200, 17], [329, 17], None, id="portions"),
+    pytest.param(6, 2, 64, 16, [150, 97], [150, 460], 100, id="portions_window"),
+]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("H,KV,D,page,q_lens,kv_lens,window", SHAPES)
+def test_attention_is_the_formula(H, KV, D, page, q_lens, kv_lens, window, dtype):
+    a, kw = batch(H, KV, D, page, q_lens, kv_lens, window, dtype)
+    judge(ops().paged_attention_fp4(**a, **kw), a, kw)
+    ops().check_status()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_large_and_tiny_queries(dtype):
+    """Queries of 1e4 and of 1e-6 (scores that are one-hot, or all alike), and rows of zeros."""
+    for sharp in (1e4, 1e-6, 0.0):
+        a, kw = batch(8, 2, 64, 16, [1, 3], [100, 230], None, dtype, sharp=sharp)
+        judge(ops().paged_attention_fp4(**a, **kw), a, kw)
+
+
+def test_a_number_that_is_none_shows_in_the_rows_that_see_it():
+    a, kw = batch(4, 2, 64, 16, [1, 1, 4], [40, 40, 40])
+    v = fp4.rows_of(a["v_pages"], 64)[1]
+    v[int(a["block_table"][0, 1]), 0, 0, 3, 1] = 255               # key 19 of the first request, head 0, coordinates 16 to 31
+    k = fp4.rows_of(a["k_pages"], 64)[1]
+    k[int(a["block_table"][2, 2]), 1, 0, 6, 0] = 255               # key 38 of the third, head 1: tokens at 38 and 39 see it
+    got = ops().paged_attention_fp4(**a, **kw).isnan().cpu()
+    want = torch.zeros_like(got)
+    want[0, :2, 16:32] = True
+    want[4:, 2:] = True
+    assert torch.equal(got, want)
+
+
+def test_slices_streams_and_outputs():
+    """Some requests of a step, tables that are slices, an output shared by two calls, another stream, a recorded graph."""
+    a, kw = batch(8, 2, 64, 16, [1, 1, 9, 5], [200, 33, 90, 5])
+    whole = ops().paged_attention_fp4(**a, **kw)
+    judge(whole, a, kw)
+    wide = torch.full((4, a["block_table"].shape[1] + 7), -1, dtype=torch.int32).cuda()
+    wide[:, 2:-5] = a["block_table"]
+    out = torch.full_like(whole, 9.0)
+    cut = lambda lo, hi: dict(q=a["q"], k_pages=a["k_pages"], v_pages=a["v_pages"], block_table=wide[lo:hi, 2:-5],  # noqa: E731
+                              q_start=a["q_start"][lo:hi + 1], kv_len=a["kv_len"][lo:hi])
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        ops().paged_attention_fp4(**cut(0, 2), **dict(kw, n_seqs=2, max_q_len=1), n_tokens=2, out=out)
+        ops().paged_attention_fp4(**cut(2, 4), **dict(kw, n_seqs=2, max_kv_len=90), out=out, allow_split=False)
+    torch.cuda.current_stream().wait_stream(s)
+    judge(out, a, kw)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        again = ops().paged_attention_fp4(**a, **kw)
+    again.zero_()
+    graph.replay()
+    assert torch.equal(again, whole)
+
+
+def test_the_same_call_gives_the_same_bits():
+    a, kw = batch(8, 2, 128, 16, [1] * 5, [3000, 900, 64, 1, 2222])
+    first = ops().paged_attention_fp4(**a, **kw)
+    for _ in range(5):
+        assert torch.equal(ops().paged_attention_fp4(**a, **kw), first)
+
+
+def test_pages_behind_two_to_the_31_bytes():
+    """A cache of 2.6 GB a side whose used pages lie at its end."""
+    KV, D, page = 8, 128, 64
+    n = 72000
+    k, v = (torch.empty(fp4.page_shape(n, KV, page, D), dtype=torch.uint8, device="cuda") for _ in range(2))
+    assert k.numel() > 2 ** 31
+    a, kw = batch(8, KV, D, page, [1, 2], [100, 150])
+    used = a["k_pages"].shape[0]
+    k[-used:], v[-used:] = a["k_pages"], a["v_pages"]
+    far = dict(a, k_pages=k, v_pages=v, block_table=torch.where(a["block_table"] >= 0, a["block_table"] + n - used, a["block_table"]))
+    assert torch.equal(ops().paged_attention_fp4(**far, **kw), ops().paged_attention_fp4(**a, **kw))
+    slots = torch.tensor([(n - 1) * page + 5, (n - 2) * page], dtype=torch.int32).cuda()
+    got = ops().kv_read_fp4(k, v, slots, head_dim=D, page_size=page)
+    near = ops().kv_read_fp4(a["k_pages"], a["v_pages"], slots - (n - used) * page, head_dim=D, page_size=page)
+    assert torch.equal(torch.stack(got).nan_to_num(7.0), torch.stack(near).nan_to_num(7.0))
+    x = torch.randn((2, 3 * KV * D), device="cuda")
+    table = torch.ones((1, D // 2, 2), device="cuda")
+    ops().rope_kv_write_fp4(x, torch.zeros(2, dtype=torch.int32, device="cuda"), table, n_heads=KV, n_kv_heads=KV, head_dim=D, interleaved=True,
+                            k_pages=k, v_pages=v, slot_mapping=slots, page_size=page)
+    _, back = ops().kv_read_fp4(k, v, slots, head_dim=D, page_size=page)
+    assert torch.equal(back.double().cpu(), fp4_plain.quantized(x[:, 2 * KV * D:].view(2, KV, D).cpu()))
+
+
+def test_refusals():
+    from torchllms_b200.kernels.native import KernelError
+    a, kw = batch(4, 2, 64, 16, [1, 2], [30, 40])
+
+    def refused(match, **changes):
+        args = dict(a, **kw)
+        args.update(changes)
+        with pytest.raises(KernelError, match=match):
+            ops().paged_attention_fp4(**args)
+    refused("GPU", q=a["q"].cpu())
+    refused("float32 or bfloat16", q=a["q"].half())
+    refused("contiguous", q=a["q"].transpose(0, 1))
+    refused("4-bit pages", k_pages=a["k_pages"][..., :-16].contiguous())
+    refused("uint8", v_pages=a["v_pages"].to(torch.int8))
+    refused("alike", v_pages=a["v_pages"][:-1])
+    refused("multiple of 16 tokens", page_size=8)
+    refused("positive multiple", q=a["q"][:, :3].contiguous())
+    refused("too narrow", max_kv_len=100000)
+    refused("cover every request", n_seqs=3)
+    refused("at least one key", window=0)
+    refused("int32", kv_len=a["kv_len"].long())
+    refused("unit column stride", block_table=a["block_table"].t())
+    refused("q's shape", out=a["q"][:1])
+    refused("unknown attention implementation", impl="fastest")
+    x = torch.zeros((2, 8 * 64), dtype=torch.bfloat16).cuda()
+    write = dict(n_heads=4, n_kv_heads=2, head_dim=64, interleaved=True, k_pages=a["k_pages"], v_pages=a["v_pages"],
+                 slot_mapping=torch.zeros(2, dtype=torch.int32).cuda(), page_size=16)
+    positions, table = torch.zeros(2, dtype=torch.int32).cuda(), torch.zeros((4, 32, 2)).cuda()
+    for match, changes in (("qkv must be", dict(n_heads=5)), ("cannot widen", dict(out_dtype=torch.float32)), ("multiple of 16", dict(page_size=24)),
+                           ("go together", dict(v_pages=None)), ("one cache slot", dict(slot_mapping=positions[:1])),
+                           ("multiple of 16 coordinates", dict(head_dim=60))):
+        with pytest.raises(KernelError, match=match):
+            ops().rope_kv_write_fp4(x, positions, table, **dict(write, **changes))
+    with pytest.raises(KernelError, match="at most head_dim / 2"):
+        ops().rope_kv_write_fp4(x, positions, torch.zeros((4, 33, 2)).cuda(), **write)
+    with pytest.raises(KernelError, match="vector of slots"):
+        ops().kv_read_fp4(a["k_pages"], a["v_pages"], positions, head_dim=64, page_size=16, out_dtype=torch.float16)
+    with pytest.raises(KernelError, match="GPU"):
+        ops().kv_read_fp4(a["k_pages"], a["v_pages"], positions.cpu(), head_dim=64, page_size=16)
+
+
+# ------------------------------------------------------------------------------------------------- the engine
+
+@pytest.mark.parametrize("name,dtype", [("A", "float32"), ("B", "float32"), ("C", "float32"), ("C", "bfloat16")])
+def test_engine_with_a_4_bit_cache_is_the_plain_model_with_one(tmp_path, monkeypatch, name, dtype):
+    import random
+
+    import numpy as np
+
+    import plain_llama
+    import traces
+    from helpers import TINY, tiny_folder
+    from test_fp4_cache import with_4_bit_cache
+    from torchllms_b200.engine.replay import Replayer
+    cfg, seed, _page = TINY[name]
+    folder = tiny_folder(tmp_path, name, dtype=DT["f32" if dtype == "float32" else "bf16"])
+    rng = random.Random(seed)
+    lengths = [1, 7, 33, 64, 50, 120] + ([310] if name == "C" else [])
+    reqs = {f"r{i}": [rng.randrange(cfg["vocab_size"]) for _ in range(n)] for i, n in enumerate(lengths)}
+    model = plain_llama.PlainModel(folder)
+    stored = {} if dtype == "float32" else dict(stored=plain_llama.to_bfloat16_and_back)
+    full = {rid: model.logits(t, **stored).numpy() for rid, t in reqs.items()}
+    with_4_bit_cache(monkeypatch)
+    held = {rid: model.logits(t, **stored).numpy() for rid, t in reqs.items()}
+    steps, places, peak = traces.mixed(reqs, **(dict(chunks=(2, 5, 24, 96, 150, 260, 40)) if name == "C" else {}))
+    rp = Replayer(folder, dtype, peak + 16 * len(reqs), page_size=16, kv_format="fp4")
+    off, moved = [], []
+    for s in steps:
+        got = rp.run_step(s)
+        rp.engine.cache.check_invariants()
+        for row, (rid, pos) in enumerate(places.get(s["step"], [])):
+            off.append(np.abs(got[row] - held[rid][pos]).mean())
+            moved.append(np.abs(held[rid][pos] - full[rid][pos]).mean())
+    # sums in another order flip a code here and there (in bfloat16, where rows are rounded elsewhere than in the plain model, many
+    # more); a wrong scale, row or key moves logits as far as the 4 bits themselves do
+    assert np.mean(off) < (0.05 if dtype == "float32" else 0.6) * np.mean(moved), (np.mean(off), np.mean(moved))
+
+
+def test_generation_is_the_same_however_requests_are_batched(tmp_path):
+    from helpers import TINY, tiny_folder
+    from torchllms_b200.inference import LLM
+    folder = tiny_folder(tmp_path, "C")
+    prompts = [[1, 2, 3], [5], [7 * i % 777 for i in range(150)], list(range(100, 164))]
+    kw = dict(precision="float32", max_len=256, page_size=16, kv_cache="fp4")
+    many = LLM(folder, max_bsz=4, max_num_batched_tokens=64, prefill_chunk=24, **kw)
+    few = LLM(folder, max_bsz=1, **kw)
+    a, b = (llm.generate(prompt_token_ids=prompts, max_new_tokens=8) for llm in (many, few))
+    # (float32: a code that flips where sums are taken in another order could change a token of a near tie; most must agree)
+    same = sum(x == y for r, s in zip(a, b) for x, y in zip(r.token_ids, s.token_ids))
+    assert same >= 28 and all(len(r.token_ids) == 8 and r.error is None for r in a + b)
+    many.engine.cache.check_invariants()

@@ -16,7 +16,9 @@ request also owns a dense *slot* that indexes fixed-size state rows and the
 engine's static per-request buffers.
 
 Page tensors are laid out ``[run, page, kv_head, slot_in_page, head_dim]`` so
-that one head's part of a page is one contiguous tile.
+that one head's part of a page is one contiguous tile; those of a 4-bit cache
+``[run, page, kv_head, page_size / 16, 9 * head_dim]`` bytes
+(:mod:`torchllms_b200.cache.fp4`).
 """
 
 from __future__ import annotations
@@ -28,6 +30,7 @@ import numpy as np
 import torch
 
 from ..parts.base import CacheNeed, StateNeed
+from . import fp4
 
 
 class OutOfPages(RuntimeError):
@@ -98,14 +101,15 @@ class _Request:
 class RunCacheView:
     """What one run of a mixer sees of the cache during a step."""
 
-    k_pages: Optional[torch.Tensor]      # [pages, kv_heads, page_size, head_dim]
-    v_pages: Optional[torch.Tensor]      # [pages, value_heads, page_size, value_dim]; None where only keys are stored
+    k_pages: Optional[torch.Tensor]      # [pages, kv_heads, page_size, head_dim]; 4-bit: [pages, kv_heads, page_size / 16, 9 * head_dim] bytes
+    v_pages: Optional[torch.Tensor]      # [pages, value_heads, page_size, value_dim] (4-bit: as k_pages); None where only keys are stored
     block_table: Optional[torch.Tensor]  # [n_seqs, max_blocks] int32, FREED where no page
     slot_mapping: Optional[torch.Tensor]  # [n_tokens] int32: page * page_size + offset
     page_size: int
     writes: bool                         # False for a run that reads another run's cache
     state: Optional[torch.Tensor]        # [max_num_seqs, *shape]; rows indexed by ctx.state_slot
     window: Optional[int] = None
+    format: str = "full"                 # how the pages hold keys and values (CacheNeed.format)
 
 
 class CacheGroup:
@@ -118,10 +122,15 @@ class CacheGroup:
         self.runs = list(runs)
         self.page_size = page_size
         self.allocator = PageAllocator(n_pages)
-        shape = (len(runs), n_pages, need.n_kv_heads, page_size)
-        self.k_pages = torch.zeros(shape + (need.head_dim,), dtype=dtype, device=device)
-        v_shape = (len(runs), n_pages, need.value_heads, page_size, need.value_dim)
-        self.v_pages = torch.zeros(v_shape, dtype=dtype, device=device) if need.value_dim else None
+        if need.format == "fp4":
+            shape = (len(runs), *fp4.page_shape(n_pages, need.n_kv_heads, page_size, need.head_dim))
+            self.k_pages = torch.zeros(shape, dtype=torch.uint8, device=device)
+            self.v_pages = torch.zeros(shape, dtype=torch.uint8, device=device)
+        else:
+            shape = (len(runs), n_pages, need.n_kv_heads, page_size)
+            self.k_pages = torch.zeros(shape + (need.head_dim,), dtype=dtype, device=device)
+            v_shape = (len(runs), n_pages, need.value_heads, page_size, need.value_dim)
+            self.v_pages = torch.zeros(v_shape, dtype=dtype, device=device) if need.value_dim else None
         self.run_index = {run: i for i, run in enumerate(self.runs)}
         self.gives_back = need.kind != "full"      # pages that no later query can read go back while the request lives
         # blocks that hold the first tokens a window keeps: never given back while the request lives
@@ -402,7 +411,7 @@ class CacheManager:
         owner = self._owner_of_run[run]
         i = g.run_index[owner]
         return RunCacheView(g.k_pages[i], None if g.v_pages is None else g.v_pages[i], block_tables[gi], slot_mappings[gi],
-                            self.page_size, owner == run, state, g.need.window)
+                            self.page_size, owner == run, state, g.need.window, g.need.format)
 
     # --------------------------------------------------------------- invariants
     def check_invariants(self) -> None:

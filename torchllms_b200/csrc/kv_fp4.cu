@@ -1,0 +1,257 @@
+// Writing a paged cache of 4-bit keys and values with the rotation on the way, and reading it back.
+//
+// rope_kv_write_fp4: a token's projected row is [q heads | k heads | v heads].  The first rot_dims coordinates of every q and
+// k head are rotated by the angles of the token's position, pairs (2i, 2i + 1) or (i, i + rot_dims / 2):
+//     y0 = x0 cos - x1 sin,  y1 = x1 cos + x0 sin
+// in float32, every product and sum rounded by itself (no fused multiply-add: what goes into the cache is then the same
+// number whichever kernel or program rotates, and a code does not flip).  q leaves rounded once; k and v are not
+// rounded before they become 4-bit numbers (fp4.cuh), which happens in the same registers: a thread has eight coordinates, a
+// pair of lanes the sixteen of a group.
+//
+// Bound by memory: a row is read once, q and 4.5 bits a number of k and v are written.
+#include "fp4.cuh"
+
+namespace {
+
+// eight consecutive elements as floats
+__device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+}
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&x)[8]) {
+    Vec16<__nv_bfloat16> v;
+    v.load(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = v.get(i);
+}
+__device__ __forceinline__ void store8(float* p, const float (&x)[8]) {
+    *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+    *reinterpret_cast<float4*>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
+}
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&x)[8]) {
+    Vec16<__nv_bfloat16> v;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v.set(i, x[i]);
+    v.store(p);
+}
+
+struct WriteParams {
+    const int* positions;
+    const float* table;            // [table_rows, rot_dims / 2, 2]
+    const int* slot_mapping;
+    unsigned char* k_pages;
+    unsigned char* v_pages;
+    long long plane, n_pages;
+    int splits, n_tokens, n_heads, n_kv_heads, head_dim, rot_dims, page_size, table_rows;
+    RowScale rs;
+};
+
+// eight coordinates of a row, its planes added up and scaled
+template <typename TI>
+__device__ __forceinline__ void fetch8(const TI* src, const WriteParams& p, float sc, float (&x)[8]) {
+    load8(src, x);
+    for (int sp = 1; sp < p.splits; ++sp) {
+        float y[8];
+        load8(src + sp * p.plane, y);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] += y[i];
+    }
+    if (p.rs.ssq != nullptr) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] *= sc;
+    }
+}
+template <typename TI>
+__device__ __forceinline__ float fetch1(const TI* src, const WriteParams& p, float sc) {
+    float x = to_float(*src);
+    for (int sp = 1; sp < p.splits; ++sp) x += to_float(src[sp * p.plane]);
+    return p.rs.ssq != nullptr ? x * sc : x;
+}
+
+// A CTA (or several, blockIdx.y) to a token, a thread to a run of eight coordinates at a time; a head has an even number of
+// runs and a CTA an even number of threads, so the two runs of a group are neighbouring lanes.
+template <typename TI, typename T, bool INTERLEAVED>
+__global__ void __launch_bounds__(128) rope_kv_write_fp4_kernel(const TI* __restrict__ qkv, T* __restrict__ q_out, const WriteParams p) {
+    grid_launch_dependents();
+    grid_dependency_wait();
+    const int t = blockIdx.x;
+    const float sc = warp_row_scale(p.rs, t);
+    const int per_head = p.head_dim >> 3, heads = p.n_heads + 2 * p.n_kv_heads, runs = heads * per_head;
+    int pos = p.positions[t];
+    (void)TL_CHECK(pos >= 0 && pos < p.table_rows, TL_DBG_POSITION);
+    pos = pos < 0 ? 0 : (pos >= p.table_rows ? p.table_rows - 1 : pos);   // the host keeps positions inside the table
+    const float* cs = p.table + (size_t)pos * p.rot_dims;
+    const TI* src = qkv + (size_t)t * heads * p.head_dim;
+    long long page = 0;
+    int slot = 0;
+    bool write = p.k_pages != nullptr;
+    if (write) {
+        const int sm = p.slot_mapping[t];
+        page = sm / p.page_size;
+        slot = sm - (int)page * p.page_size;
+        // (a slot outside the cache is not written; debug builds report it)
+        write = TL_CHECK(sm >= 0, TL_DBG_SLOT) && tl_check_page(page) && sm >= 0 && page < p.n_pages;
+    }
+    const int half = p.rot_dims >> 1;
+    // (whole warps go round together: the lanes of a group exchange their maxima)
+    for (int c0 = blockIdx.y * blockDim.x; c0 < runs; c0 += gridDim.y * blockDim.x) {
+        const int c = c0 + threadIdx.x;
+        const bool mine = c < runs;
+        const int head = mine ? c / per_head : 0;
+        const int off = mine ? (c - head * per_head) << 3 : 0;
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = 0.f;
+        if (mine) {
+            fetch8(src + head * p.head_dim + off, p, sc, x);
+            if (head < p.n_heads + p.n_kv_heads && off < p.rot_dims) {
+                if (INTERLEAVED) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (off + 2 * i < p.rot_dims) {
+                            const float2 r = *reinterpret_cast<const float2*>(cs + off + 2 * i);
+                            const float a = x[2 * i], b = x[2 * i + 1];
+                            x[2 * i] = __fsub_rn(__fmul_rn(a, r.x), __fmul_rn(b, r.y));
+                            x[2 * i + 1] = __fadd_rn(__fmul_rn(b, r.x), __fmul_rn(a, r.y));
+                        }
+                } else if ((half & 7) == 0) {
+                    // the partners are another whole run
+                    const bool first = off < half;
+                    float y[8];
+                    fetch8(src + head * p.head_dim + (first ? off + half : off - half), p, sc, y);
+                    const float* r = cs + 2 * (first ? off : off - half);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float2 a = *reinterpret_cast<const float2*>(r + 2 * i);
+                        const float u = __fmul_rn(x[i], a.x), v = __fmul_rn(y[i], a.y);
+                        x[i] = first ? __fsub_rn(u, v) : __fadd_rn(u, v);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int d = off + i;
+                        if (d < p.rot_dims) {
+                            const bool first = d < half;
+                            const float y = fetch1(src + head * p.head_dim + (first ? d + half : d - half), p, sc);
+                            const float2 a = *reinterpret_cast<const float2*>(cs + 2 * (first ? d : d - half));
+                            const float u = __fmul_rn(x[i], a.x), v = __fmul_rn(y, a.y);
+                            x[i] = first ? __fsub_rn(u, v) : __fadd_rn(u, v);
+                        }
+                    }
+                }
+            }
+        }
+        unsigned top = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        if (!mine) continue;
+        if (head < p.n_heads) {
+            store8(q_out + ((size_t)t * p.n_heads + head) * p.head_dim + off, x);
+        } else if (write) {
+            const bool is_k = head < p.n_heads + p.n_kv_heads;
+            const int kvh = is_k ? head - p.n_heads : head - p.n_heads - p.n_kv_heads;
+            unsigned char* base = is_k ? p.k_pages : p.v_pages;
+            const Fp4Place at = fp4_place(page, slot, kvh, p.n_kv_heads, p.page_size, p.head_dim);
+            const unsigned byte = fp4_scale_byte(top);
+            *reinterpret_cast<unsigned*>(base + at.codes + off / 2) = fp4_pack8(x, byte);
+            if ((off & 8) == 0) base[at.scales + off / FP4_GROUP] = (unsigned char)byte;
+        }
+    }
+}
+
+// The numbers of given slots: a thread to eight coordinates of a head of a slot; blockIdx.y: keys, values.
+template <typename T>
+__global__ void __launch_bounds__(128) kv_read_fp4_kernel(const unsigned char* __restrict__ k_pages, const unsigned char* __restrict__ v_pages,
+                                                          const int* __restrict__ slots, T* __restrict__ k_out, T* __restrict__ v_out,
+                                                          long long runs, long long n_pages, int n_kv_heads, int head_dim, int page_size) {
+    grid_launch_dependents();
+    grid_dependency_wait();
+    const unsigned char* pages = blockIdx.y ? v_pages : k_pages;
+    T* out = blockIdx.y ? v_out : k_out;
+    const int per_head = head_dim >> 3;
+    for (long long c = (long long)blockIdx.x * blockDim.x + threadIdx.x; c < runs; c += (long long)gridDim.x * blockDim.x) {
+        const long long row = c / per_head;
+        const int off = (int)(c - row * per_head) << 3;
+        const long long n = row / n_kv_heads;
+        const int head = (int)(row - n * n_kv_heads);
+        const int sm = slots[n];
+        const long long page = sm / page_size;
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = 0.f;
+        // (a slot outside the cache reads as zeros; debug builds report it)
+        if (TL_CHECK(sm >= 0, TL_DBG_SLOT) && tl_check_page(page) && sm >= 0 && page < n_pages) {
+            const Fp4Place at = fp4_place(page, sm - (int)page * page_size, head, n_kv_heads, page_size, head_dim);
+            __half2 r[4];
+            fp4_unpack(*reinterpret_cast<const unsigned*>(pages + at.codes + off / 2), r);
+            const __half2 s = fp4_scale2(pages[at.scales + off / FP4_GROUP]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 v = __half22float2(__hmul2(r[i], s));      // exact
+                x[2 * i] = v.x;
+                x[2 * i + 1] = v.y;
+            }
+        }
+        store8(out + c * 8, x);
+    }
+}
+
+bool takes(int n_kv_heads, int head_dim, int page_size) {
+    return n_kv_heads > 0 && head_dim >= FP4_GROUP && head_dim % FP4_GROUP == 0 && page_size >= FP4_RECORD && page_size % FP4_RECORD == 0;
+}
+
+}  // namespace
+
+// qkv: [splits, n_tokens, (n_heads + 2 n_kv_heads) head_dim] of in_dtype (splits > 1 only for float32 partial sums, `plane`
+// elements apart); q_out: [n_tokens, n_heads, head_dim] of dtype.  k_pages / v_pages may both be null: then only q is produced.
+// in_ssq may be null; else [n_tokens, in_parts] floats give every token's row scale (RowScale in common.cuh).
+extern "C" int tl_rope_kv_write_fp4(const void* qkv, int in_dtype, int splits, const int* positions, const float* table,
+                                    const int* slot_mapping, void* q_out, void* k_pages, void* v_pages, int dtype, int n_tokens,
+                                    int n_heads, int n_kv_heads, int head_dim, int rot_dims, int page_size, long long n_pages,
+                                    int table_rows, int interleaved, const float* in_ssq, int in_parts, float in_inv_dim, float in_eps,
+                                    void* stream) {
+    if (n_tokens <= 0) return TL_OK;
+    if (!takes(n_kv_heads, head_dim, page_size) || n_heads <= 0 || splits < 1 || table_rows <= 0) return TL_BAD_SIZE;
+    if (rot_dims < 2 || rot_dims > head_dim || (rot_dims & 1)) return TL_BAD_SIZE;
+    if ((k_pages == nullptr) != (v_pages == nullptr) || (in_ssq != nullptr && in_parts < 1)) return TL_BAD_SIZE;
+    if (!aligned16(qkv) || !aligned16(q_out) || !aligned16(table) || !aligned16(k_pages) || !aligned16(v_pages)) return TL_BAD_ALIGN;
+    WriteParams p;
+    p.positions = positions; p.table = table; p.slot_mapping = slot_mapping;
+    p.k_pages = (unsigned char*)k_pages; p.v_pages = (unsigned char*)v_pages;
+    const int heads = n_heads + 2 * n_kv_heads;
+    p.plane = (long long)n_tokens * heads * head_dim;
+    p.n_pages = n_pages; p.splits = splits; p.n_tokens = n_tokens; p.n_heads = n_heads; p.n_kv_heads = n_kv_heads;
+    p.head_dim = head_dim; p.rot_dims = rot_dims; p.page_size = page_size; p.table_rows = table_rows;
+    p.rs = {in_ssq, in_parts, in_inv_dim, in_eps};
+    const int runs = heads * (head_dim / 8);
+    const int by = n_tokens >= 256 ? 1 : (runs + 127) / 128;
+    cudaStream_t s = (cudaStream_t)stream;
+#define TL_WRITE(TI, T)                                                                                                         \
+    (interleaved ? tl_launch(rope_kv_write_fp4_kernel<TI, T, true>, dim3(n_tokens, by), dim3(128), 0, s, (const TI*)qkv, (T*)q_out, p) \
+                 : tl_launch(rope_kv_write_fp4_kernel<TI, T, false>, dim3(n_tokens, by), dim3(128), 0, s, (const TI*)qkv, (T*)q_out, p))
+    if (in_dtype == TL_F32 && dtype == TL_F32) return (int)TL_WRITE(float, float);
+    if (in_dtype == TL_BF16 && dtype == TL_BF16 && splits == 1) return (int)TL_WRITE(__nv_bfloat16, __nv_bfloat16);
+    if (in_dtype == TL_F32 && dtype == TL_BF16) return (int)TL_WRITE(float, __nv_bfloat16);
+#undef TL_WRITE
+    return TL_BAD_DTYPE;
+}
+
+// k_out, v_out: [n_slots, n_kv_heads, head_dim] of dtype.
+extern "C" int tl_kv_read_fp4(const void* k_pages, const void* v_pages, const int* slots, void* k_out, void* v_out, int dtype,
+                              int n_slots, long long n_pages, int n_kv_heads, int head_dim, int page_size, void* stream) {
+    if (n_slots <= 0) return TL_OK;
+    if (!takes(n_kv_heads, head_dim, page_size)) return TL_BAD_SIZE;
+    if (!aligned16(k_pages) || !aligned16(v_pages) || !aligned16(k_out) || !aligned16(v_out)) return TL_BAD_ALIGN;
+    const long long runs = (long long)n_slots * n_kv_heads * (head_dim / 8);
+    const unsigned bx = (unsigned)((runs + 127) / 128 < 148 * 8 ? (runs + 127) / 128 : 148 * 8);
+    cudaStream_t s = (cudaStream_t)stream;
+    const unsigned char *k = (const unsigned char*)k_pages, *v = (const unsigned char*)v_pages;
+    if (dtype == TL_BF16)
+        return (int)tl_launch(kv_read_fp4_kernel<__nv_bfloat16>, dim3(bx, 2), dim3(128), 0, s, k, v, slots, (__nv_bfloat16*)k_out,
+                              (__nv_bfloat16*)v_out, runs, n_pages, n_kv_heads, head_dim, page_size);
+    if (dtype == TL_F32)
+        return (int)tl_launch(kv_read_fp4_kernel<float>, dim3(bx, 2), dim3(128), 0, s, k, v, slots, (float*)k_out, (float*)v_out, runs,
+                              n_pages, n_kv_heads, head_dim, page_size);
+    return TL_BAD_DTYPE;
+}

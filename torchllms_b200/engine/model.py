@@ -21,7 +21,8 @@ from ..weights.loader import ExpectedTensor
 
 
 class Model:
-    def __init__(self, spec: ModelSpec, *, dtype: torch.dtype, device, ops, max_positions: Optional[int] = None):
+    def __init__(self, spec: ModelSpec, *, dtype: torch.dtype, device, ops, max_positions: Optional[int] = None,
+                 kv_format: str = "full"):
         if dtype not in (torch.float32, torch.bfloat16):
             raise ValueError(f"the engine computes in float32 or bfloat16, not {dtype}")
         self.spec = spec
@@ -33,8 +34,14 @@ class Model:
             # a learned position table ends where it ends: no request can grow past its last row
             self.max_positions = min(self.max_positions, spec.max_positions)
         self.env = BuildEnv(dim=spec.dim, dtype=dtype, device=self.device,
-                            max_positions=self.max_positions, ops=ops)
+                            max_positions=self.max_positions, ops=ops, kv_format=kv_format)
         self.blocks = [BLOCKS.build(layer.block, self.env) for layer in spec.layers]
+        self.kv_format = kv_format
+        for layer, blk in zip(spec.layers, self.blocks):
+            need = blk.cache_need()
+            if need is not None and need.format != kv_format:
+                raise ValueError(f"{layer.name} keeps its keys and values in format {need.format!r} only: "
+                                 f"this architecture has no cache of format {kv_format!r}")
         self.final_norm = NORMS.build(spec.final_norm, self.env)
         self.embedding_norm = None if spec.embedding_norm is None else NORMS.build(spec.embedding_norm, self.env)
         self.graph_safe = self.final_norm.graph_safe and all(b.graph_safe for b in self.blocks)

@@ -29,6 +29,7 @@ from typing import Dict, Optional
 import numpy as np
 import torch
 
+from ..cache.fp4 import CACHE_FORMATS
 from .loading import load_model
 from .step import Engine, StepEntry
 
@@ -39,14 +40,14 @@ def round_up(n: int, m: int) -> int:
 
 class Replayer:
     def __init__(self, model_dir, dtype: str, max_tokens: int, *, page_size: int = 16, device: str = "cuda",
-                 max_num_seqs: int = 16, ops=None):
+                 max_num_seqs: int = 16, ops=None, kv_format: str = "full"):
         from ..config.registry import load_config
         _arch, config = load_config(model_dir)
         # The pool is made for max_tokens, so the position table must reach as far as one
         # request could grow inside it, whatever the configuration's own limit says.
         max_positions = max(int(config.max_seq_len), round_up(max_tokens, page_size))
         _, self.config, model = load_model(model_dir, dtype=dtype, device=device, ops=ops,
-                                           max_positions=max_positions)
+                                           max_positions=max_positions, kv_format=kv_format)
         # (a model with a learned position table ends where its table ends, whatever was asked for)
         self.engine = Engine(model, page_size=page_size, pool_tokens=round_up(max_tokens, page_size),
                              max_num_seqs=max_num_seqs, max_len=model.max_positions,
@@ -86,10 +87,12 @@ def main(argv=None) -> int:
                     help="most tokens live requests hold at any time (each rounded up to 64)")
     ap.add_argument("--page-size", type=int, default=16)
     ap.add_argument("--max-requests", type=int, default=4, help="how many requests may be live at a time (state slots)")
+    ap.add_argument("--kv-cache", choices=CACHE_FORMATS, default="full", help="how keys and values are held")
     args = ap.parse_args(argv)
     out = Path(args.out)
     out.mkdir(parents=True, exist_ok=True)
-    replayer = Replayer(args.model, args.dtype, args.max_tokens, page_size=args.page_size, max_num_seqs=args.max_requests)
+    replayer = Replayer(args.model, args.dtype, args.max_tokens, page_size=args.page_size, max_num_seqs=args.max_requests,
+                        kv_format=args.kv_cache)
     for line in sys.stdin:
         line = line.strip()
         if not line:

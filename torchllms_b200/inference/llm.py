@@ -18,6 +18,7 @@ from typing import Any, Dict, List, Optional, Sequence, Union
 
 import torch
 
+from ..cache.fp4 import CACHE_FORMATS, check_page_size
 from ..engine.loading import load_model, model_dir_of, parse_dtype, random_model
 from ..engine.scheduler import Request, Scheduler
 from ..engine.step import Engine
@@ -64,6 +65,7 @@ class LLM:
         config=None,
         random_seed: Optional[int] = None,
         ops=None,
+        kv_cache: str = "full",
     ):
         """``ckpt_paths``: a model folder (``config.json`` + ``model.safetensors``), a file in
         one, or a list of them loaded in order, later tensors overriding earlier ones (the
@@ -73,24 +75,35 @@ class LLM:
         (a share of the device memory that is free once the weights are loaded) or ``kv_memory_gb``
         gives its size in GiB (torchllms/models/networks.py:872-884).  What a step needs besides comes out
         of the rest: its activations, and in float32 up to 6 bytes a number for the cut inputs of 4,096 rows
-        (50 to 350 MB at 2,048 to 14,336 numbers a row)."""
+        (50 to 350 MB at 2,048 to 14,336 numbers a row).  ``kv_cache`` is how keys and values are held: ``"full"`` (the
+        precision's own type) or ``"fp4"`` (4.5 bits a number: 3.6 times the tokens of bfloat16 in the same memory, and as
+        much less to read in a decode step; for architectures whose layers are rotary grouped-query attention, with pages
+        of a multiple of 16 tokens; others are refused)."""
+        if kv_cache not in CACHE_FORMATS:
+            raise ValueError(f"kv_cache must be one of {', '.join(CACHE_FORMATS)}, got {kv_cache!r}")
+        if kv_cache == "fp4":
+            check_page_size(int(page_size))
         if prefix_cache is not None:
             # the reference's argument at its place in the list; this engine keeps no cache of prefixes
             raise ValueError("prefix_cache: this engine has no prefix cache; leave it None")
         ops = ops or get_ops()
         precision = precision or "bfloat16"
         self.dtype = parse_dtype(precision)
-        ops.prepare(self.dtype)
+        if kv_cache == "full":
+            ops.prepare(self.dtype)
+        else:
+            ops.prepare(self.dtype, kv_format=kv_cache)
         if ckpt_paths is not None:
             paths = [ckpt_paths] if isinstance(ckpt_paths, (str, Path)) else list(ckpt_paths)
             self.model_dir: Optional[Path] = model_dir_of(paths[0])
             self.arch, self.config, self.model = load_model(
-                paths, dtype=self.dtype, device=device, overrides=model_kwargs, max_positions=max_len, ops=ops)
+                paths, dtype=self.dtype, device=device, overrides=model_kwargs, max_positions=max_len, ops=ops,
+                kv_format=kv_cache)
         elif config is not None:
             self.model_dir = None
             config = config.with_overrides(model_kwargs)
             self.arch, self.config, self.model = random_model(
-                config, random_seed or 0, dtype=self.dtype, device=device, max_positions=max_len, ops=ops)
+                config, random_seed or 0, dtype=self.dtype, device=device, max_positions=max_len, ops=ops, kv_format=kv_cache)
         else:
             raise ValueError("give ckpt_paths (a model folder) or config and random_seed")
         self.max_len = min(int(max_len), self.model.max_positions)     # (a learned position table ends where it ends)
@@ -98,9 +111,12 @@ class LLM:
         self.device = device
         self.seed = int(seed)
         self.batched = batched
-        bytes_per_token = sum(g_need.n_kv_heads * (g_need.head_dim + g_need.value_dim) * n_runs
-                              for g_need, n_runs in self._kv_layout())
-        bytes_per_token *= torch.empty((), dtype=self.dtype).element_size()
+        element_size = torch.empty((), dtype=self.dtype).element_size()
+        if kv_cache == "full":
+            bytes_per_token = element_size * sum(g_need.n_kv_heads * (g_need.head_dim + g_need.value_dim) * n_runs
+                                                 for g_need, n_runs in self._kv_layout())
+        else:
+            bytes_per_token = sum(g_need.bytes_per_token(element_size) * n_runs for g_need, n_runs in self._kv_layout())
         if kv_memory_gb is not None and kv_memory_fraction is not None:
             raise ValueError("give kv_memory_gb or kv_memory_fraction, not both")
         if kv_memory_fraction is not None:

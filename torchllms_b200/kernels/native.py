@@ -16,6 +16,7 @@ from typing import Dict, Optional, Tuple
 
 import torch
 
+from ..cache.fp4 import GROUP, MAX_HEAD_DIM, RECORD, record_bytes
 from .build import ALL_LIBRARIES, build_libraries, load_library
 from .lazy import PendingProduct, RowScaled
 
@@ -154,11 +155,13 @@ class NativeOps:
             _check(self._lib(lib_name).tl_debug_set_limit(which, ctypes.c_longlong(int(value)), _stream()), "debug limit")
 
     # ------------------------------------------------------------ libraries
-    def prepare(self, dtype: torch.dtype, sampling: bool = True) -> None:
-        """Compile, side by side, what a model of this dtype will call."""
+    def prepare(self, dtype: torch.dtype, sampling: bool = True, kv_format: str = "full") -> None:
+        """Compile, side by side, what a model of this dtype (and cache format) will call."""
         names = ["elementwise", "sublayer", "rope", "attention", "gemm_simt", "gemm_f32", "recurrent", "moe", "matrix_state", "stream_sum", "conv_mixers", "matrix_recurrence"]
         if dtype == torch.bfloat16:
             names += ["attention_mma", "attention_decode", "gemm_tcgen05"]
+        if kv_format == "fp4":
+            names += ["kv_fp4", "attention_fp4"]
         if sampling:
             names.append("sampling")
         build_libraries(names)
@@ -2025,6 +2028,130 @@ class NativeOps:
             1 if allow_split else 0, ctypes.byref(opt), _stream())
         _check(rc, "paged_attention")
         self.launches += 2 if n_splits.value > 1 else 1
+        return out
+
+    # ------------------------------------------------------------- keys and values in 4 bits
+    @staticmethod
+    def _fp4_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, n_kv_heads: int, head_dim: int, page_size: int) -> None:
+        _cuda_contig(k_pages, "k_pages", torch.uint8)
+        _cuda_contig(v_pages, "v_pages", torch.uint8)
+        _need(head_dim % GROUP == 0 and 0 < head_dim <= MAX_HEAD_DIM,
+              f"a 4-bit cache takes heads of a multiple of {GROUP} coordinates up to {MAX_HEAD_DIM}, got {head_dim}")
+        _need(page_size > 0 and page_size % RECORD == 0, f"a 4-bit cache takes pages of a multiple of {RECORD} tokens, got {page_size}")
+        _need(k_pages.shape == v_pages.shape and k_pages.dim() == 4
+              and k_pages.shape[1:] == (n_kv_heads, page_size // RECORD, record_bytes(head_dim)) and k_pages.shape[0] > 0,
+              "4-bit pages must be [pages, n_kv_heads, page_size / 16, 9 * head_dim] bytes, keys and values alike")
+
+    @_timed
+    def rope_kv_write_fp4(self, qkv, positions: torch.Tensor, table: torch.Tensor, *,
+                          n_heads: int, n_kv_heads: int, head_dim: int, interleaved: bool,
+                          k_pages: Optional[torch.Tensor], v_pages: Optional[torch.Tensor],
+                          slot_mapping: Optional[torch.Tensor], page_size: int,
+                          out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+        """:meth:`rope_kv_write` for pages that hold keys and values in 4 bits (``[pages, n_kv_heads, page_size / 16,
+        9 * head_dim]`` bytes, :mod:`torchllms_b200.cache.fp4`).  Keys (after rotation) and values become 4-bit numbers
+        from their float32 values.  The rotary table may cover the first coordinates of a head only
+        (``[positions, rotated / 2, 2]``); the others pass as they are."""
+        rs = qkv if isinstance(qkv, RowScaled) else None
+        if rs is not None:
+            qkv = rs.x
+        _cuda_contig(qkv, "qkv")
+        _cuda_contig(positions, "positions", torch.int32)
+        _cuda_contig(table, "rotary table", torch.float32)
+        splits = qkv.shape[0] if qkv.dim() == 3 else 1
+        T = qkv.shape[-2]
+        out_dtype = out_dtype or qkv.dtype
+        _need(n_heads > 0 and n_kv_heads > 0 and head_dim > 0 and head_dim % GROUP == 0,
+              f"a 4-bit cache takes heads of a multiple of {GROUP} coordinates, got {n_heads}, {n_kv_heads} heads of {head_dim}")
+        _need(qkv.dim() in (2, 3) and qkv.shape[-1] == (n_heads + 2 * n_kv_heads) * head_dim and qkv.dtype in _DT,
+              "qkv must be [tokens, (n_heads + 2 n_kv_heads) * head_dim]")
+        _need(splits == 1 or qkv.dtype == torch.float32, "partial sums must be float32")
+        _need(out_dtype in _DT and (out_dtype == qkv.dtype or qkv.dtype == torch.float32), "rope cannot widen bfloat16 input")
+        _need(table.dim() == 3 and 1 <= table.shape[1] <= head_dim // 2 and table.shape[2] == 2,
+              "rotary table must be [positions, pairs, 2] with at most head_dim / 2 pairs")
+        _need(positions.numel() == T, "one position per token")
+        n_pages = 0
+        if k_pages is not None:
+            _need(v_pages is not None and slot_mapping is not None, "k_pages, v_pages and slot_mapping go together")
+            self._fp4_pages(k_pages, v_pages, n_kv_heads, head_dim, page_size)
+            _cuda_contig(slot_mapping, "slot_mapping", torch.int32)
+            _need(slot_mapping.numel() == T, "one cache slot per token")
+            n_pages = k_pages.shape[0]
+            self._debug_limit("kv_fp4", 0, n_pages)
+        q = torch.empty((T, n_heads, head_dim), dtype=out_dtype, device=qkv.device)
+        rc = self._lib("kv_fp4").tl_rope_kv_write_fp4(
+            _ptr(qkv), _DT[qkv.dtype], splits, _ptr(positions), _ptr(table), _ptr(slot_mapping if k_pages is not None else None),
+            _ptr(q), _ptr(k_pages), _ptr(v_pages if k_pages is not None else None), _DT[out_dtype], T, n_heads, n_kv_heads, head_dim,
+            2 * table.shape[1], page_size, ctypes.c_longlong(n_pages), table.shape[0], 1 if interleaved else 0, *_scale_args(rs, T), _stream())
+        _check(rc, "rope_kv_write_fp4")
+        self.launches += 1
+        return q
+
+    @_timed
+    def kv_read_fp4(self, k_pages: torch.Tensor, v_pages: torch.Tensor, slots: torch.Tensor, *, head_dim: int, page_size: int,
+                    out_dtype: torch.dtype = torch.float32) -> Tuple[torch.Tensor, torch.Tensor]:
+        """The keys and values that a 4-bit cache holds in the given slots (int32, ``page * page_size + offset``):
+        two tensors ``[slots, n_kv_heads, head_dim]``.  Either dtype has every number exactly."""
+        _need(k_pages.dim() == 4, "4-bit pages must be [pages, n_kv_heads, page_size / 16, 9 * head_dim] bytes, keys and values alike")
+        KV = k_pages.shape[1]
+        self._fp4_pages(k_pages, v_pages, KV, head_dim, page_size)
+        _cuda_contig(slots, "slots", torch.int32)
+        _need(slots.dim() == 1 and out_dtype in _DT, "kv_read_fp4 takes a vector of slots and writes float32 or bfloat16")
+        n = slots.numel()
+        out = torch.empty((2, n, KV, head_dim), dtype=out_dtype, device=slots.device)
+        k, v = out.unbind(0)
+        self._debug_limit("kv_fp4", 0, k_pages.shape[0])
+        rc = self._lib("kv_fp4").tl_kv_read_fp4(_ptr(k_pages), _ptr(v_pages), _ptr(slots), _ptr(k), _ptr(v), _DT[out_dtype], n,
+                                               ctypes.c_longlong(k_pages.shape[0]), KV, head_dim, page_size, _stream())
+        _check(rc, "kv_read_fp4")
+        self.launches += 1
+        return k, v
+
+    @_timed
+    def paged_attention_fp4(self, q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                            block_table: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor, *,
+                            n_seqs: int, max_q_len: int, max_kv_len: int, scale: float,
+                            window: Optional[int], page_size: int, allow_split: bool = True,
+                            impl: str = "auto", n_tokens: Optional[int] = None,
+                            out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """:meth:`paged_attention` over pages that hold keys and values in 4 bits
+        (``[pages, n_kv_heads, page_size / 16, 9 * head_dim]`` bytes, :mod:`torchllms_b200.cache.fp4`): every token of
+        ``q`` ``[T, H, head_dim]`` attends to the keys of its request up to its own place, or to the last ``window`` of
+        them.  Keys and values are taken as the cache has them, nothing is rounded on the way; a row that sees no key is
+        zeros.  Arguments as there.  ``impl``: ``"general"`` (CUDA cores, heads of any multiple of 16 up to 256) or
+        ``"auto"``."""
+        _cuda_contig(q, "q")
+        _need(q.dim() == 3 and q.dtype in _DT, "q must be [tokens, heads, head_dim] in float32 or bfloat16")
+        _cuda_contig(q_start, "q_start", torch.int32)
+        _cuda_contig(kv_len, "kv_len", torch.int32)
+        _need(block_table.is_cuda and block_table.dtype == torch.int32 and block_table.dim() == 2
+              and block_table.stride(1) == 1, "block_table must be an int32 matrix with unit column stride")
+        T, n_heads, head_dim = q.shape
+        _need(k_pages.dim() == 4, "4-bit pages must be [pages, n_kv_heads, page_size / 16, 9 * head_dim] bytes, keys and values alike")
+        n_kv_heads = k_pages.shape[1]
+        self._fp4_pages(k_pages, v_pages, n_kv_heads, head_dim, page_size)
+        _need(n_heads > 0 and n_kv_heads > 0 and n_heads % n_kv_heads == 0,
+              f"n_heads ({n_heads}) must be a positive multiple of n_kv_heads ({n_kv_heads})")
+        if n_tokens is not None:
+            _need(0 < n_tokens <= T, "n_tokens must lie within q")
+            T = int(n_tokens)
+        if out is None:
+            out = torch.empty_like(q)
+        else:
+            _cuda_contig(out, "out", q.dtype)
+            _need(out.shape == q.shape, "out must have q's shape")
+        _need(window is None or window > 0, "a window holds at least one key")
+        _need(block_table.shape[0] >= n_seqs and q_start.numel() >= n_seqs + 1 and kv_len.numel() >= n_seqs,
+              "block_table, q_start and kv_len must cover every request of the step")
+        _need(block_table.shape[1] * page_size >= max_kv_len, "block_table is too narrow for max_kv_len")
+        _need(impl in ("auto", "general"), f"unknown attention implementation {impl!r}")
+        self._debug_limit("attention_fp4", 0, k_pages.shape[0])
+        rc = self._lib("attention_fp4").tl_attention_fp4_general(
+            _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(out), _ptr(block_table), block_table.stride(0), block_table.shape[1],
+            _ptr(q_start), _ptr(kv_len), _DT[q.dtype], n_seqs, n_heads, n_kv_heads, head_dim, page_size,
+            ctypes.c_longlong(k_pages.shape[0]), max_q_len, int(window or 0), ctypes.c_float(scale), _stream())
+        _check(rc, "paged_attention_fp4")
+        self.launches += 1
         return out
 
     # ---------------------------------------------------------------- sampling

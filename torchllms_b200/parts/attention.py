@@ -39,13 +39,16 @@ class PagedAttention(Mixer):
         # x only goes into the q/k/v product, whose result the position encoding's kernel may scale
         self.takes_row_scaled = self.position.takes_row_scaled
         env.ops.check_attention_sizes(self.n_heads, self.n_kv_heads, self.head_dim, env.dtype)
+        self.format = env.kv_format
+        if self.format not in self.position.cache_formats:
+            raise ValueError(f"position encoding {position.kind!r} cannot write a cache of format {self.format!r}")
         self.wqkv: Optional[torch.Tensor] = None
         self.wo: Optional[torch.Tensor] = None
 
     def cache_need(self) -> CacheNeed:
         if self.window is None:
-            return CacheNeed("full", self.n_kv_heads, self.head_dim)
-        return CacheNeed("window", self.n_kv_heads, self.head_dim, self.window)
+            return CacheNeed("full", self.n_kv_heads, self.head_dim, format=self.format)
+        return CacheNeed("window", self.n_kv_heads, self.head_dim, self.window, format=self.format)
 
     def expected_tensors(self) -> Dict[str, ExpectedTensor]:
         q, kv = self.n_heads * self.head_dim, self.n_kv_heads * self.head_dim
@@ -71,20 +74,21 @@ class PagedAttention(Mixer):
         qkv = ops.linear(x, self.wqkv, partials_ok=True)   # the encoding adds up split-K partial sums
         q = self.position.encode_and_store(qkv, ctx, cache, self.n_heads, self.n_kv_heads, self.head_dim)
         common = dict(scale=self.scale, window=self.window, page_size=cache.page_size)
+        attend = ops.paged_attention_fp4 if getattr(cache, "format", "full") == "fp4" else ops.paged_attention
         nd, B = getattr(ctx, "n_decode", 0), ctx.n_seqs
         if 0 < nd < B and ctx.max_q_len > 1:
             # decoded tokens beside prompt portions: the requests at the head of the batch bring one
             # token each and long histories, the rest bring portions; each kind goes to the kernel
             # shape made for it, both writing into one output
             o = torch.empty_like(q)
-            ops.paged_attention(q, cache.k_pages, cache.v_pages, cache.block_table[:nd], ctx.q_start[:nd + 1],
-                                ctx.kv_len[:nd], n_seqs=nd, max_q_len=1, max_kv_len=ctx.decode_kv_bound,
-                                n_tokens=nd, out=o, **common)
-            ops.paged_attention(q, cache.k_pages, cache.v_pages, cache.block_table[nd:], ctx.q_start[nd:],
-                                ctx.kv_len[nd:], n_seqs=B - nd, max_q_len=ctx.max_q_len, max_kv_len=ctx.max_kv_len,
-                                out=o, allow_split=False, **common)   # (a merge pass would run over the first call's rows too)
+            attend(q, cache.k_pages, cache.v_pages, cache.block_table[:nd], ctx.q_start[:nd + 1],
+                   ctx.kv_len[:nd], n_seqs=nd, max_q_len=1, max_kv_len=ctx.decode_kv_bound,
+                   n_tokens=nd, out=o, **common)
+            attend(q, cache.k_pages, cache.v_pages, cache.block_table[nd:], ctx.q_start[nd:],
+                   ctx.kv_len[nd:], n_seqs=B - nd, max_q_len=ctx.max_q_len, max_kv_len=ctx.max_kv_len,
+                   out=o, allow_split=False, **common)   # (a merge pass would run over the first call's rows too)
         else:
-            o = ops.paged_attention(
+            o = attend(
                 q, cache.k_pages, cache.v_pages, cache.block_table, ctx.q_start, ctx.kv_len,
                 n_seqs=B, max_q_len=ctx.max_q_len, max_kv_len=ctx.max_kv_len, **common)
         # the output projection is left to the norm that follows: it may add the product to the

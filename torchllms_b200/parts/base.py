@@ -28,6 +28,7 @@ from typing import Any, Callable, Dict, Mapping, Optional, Tuple
 
 import torch
 
+from ..cache.fp4 import CACHE_FORMATS, RECORD, check_head_dim, record_bytes
 from ..weights.loader import ExpectedTensor
 from .spec import PartSpec
 
@@ -41,6 +42,7 @@ class BuildEnv:
     device: torch.device
     max_positions: int       # the longest sequence the engine will hold
     ops: Any                 # the kernel library (see torchllms_b200.kernels)
+    kv_format: str = "full"  # how keys and values are to be kept (``CacheNeed.format``)
 
 
 @dataclass(frozen=True)
@@ -57,6 +59,8 @@ class CacheNeed:
     that derives keys and values from one stored vector).  ``n_v_heads`` is the number of value
     heads when it differs from the number of key heads (key head ``j`` then goes with value head
     ``j % n_v_heads``: several attention maps, each with keys of its own, over one set of values).
+    ``format`` is how a key and a value are held: ``"full"`` (the activation dtype) or ``"fp4"`` (4-bit numbers with an
+    8-bit scale for 16 of them, 4.5 bits a number; :mod:`torchllms_b200.cache.fp4`).
     Runs with equal needs share one group of pages and one block table.
     """
 
@@ -67,8 +71,11 @@ class CacheNeed:
     v_head_dim: Optional[int] = None
     keep_first: int = 0
     n_v_heads: Optional[int] = None
+    format: str = "full"
 
     def __post_init__(self):
+        if self.format not in CACHE_FORMATS:
+            raise ValueError(f"cache format must be one of {', '.join(CACHE_FORMATS)}, got {self.format!r}")
         if self.kind not in ("full", "window", "chunk"):
             raise ValueError(f"cache kind must be 'full', 'window' or 'chunk', got {self.kind!r}")
         if (self.kind != "full") != (self.window is not None):
@@ -82,6 +89,10 @@ class CacheNeed:
                 raise ValueError(f"n_v_heads ({self.n_v_heads}) must divide n_kv_heads ({self.n_kv_heads})")
             if self.n_v_heads == self.n_kv_heads:
                 object.__setattr__(self, "n_v_heads", None)
+        if self.format == "fp4":
+            if self.value_dim != self.head_dim or self.value_heads != self.n_kv_heads:
+                raise ValueError("a 4-bit cache holds keys and values of one size and head count")
+            check_head_dim(self.head_dim)
 
     @property
     def value_dim(self) -> int:
@@ -92,6 +103,12 @@ class CacheNeed:
     def value_heads(self) -> int:
         """How many heads a stored value has."""
         return self.n_kv_heads if self.n_v_heads is None else self.n_v_heads
+
+    def bytes_per_token(self, element_size: int) -> int:
+        """What one run of this need stores for a token, with activations of ``element_size`` bytes."""
+        if self.format == "fp4":
+            return 2 * self.n_kv_heads * record_bytes(self.head_dim) // RECORD
+        return (self.n_kv_heads * self.head_dim + self.value_heads * self.value_dim) * element_size
 
     def first_needed(self, position: int) -> int:
         """The first key that a query at ``position`` or any later place reads (apart from ``keep_first``)."""
@@ -104,16 +121,16 @@ class CacheNeed:
     def covering(self, other: "CacheNeed") -> "CacheNeed":
         """The need that keeps what both this one and ``other`` (a run that reads this run's cache
         through a mask of its own) will read."""
-        if (other.n_kv_heads, other.head_dim, other.value_dim, other.value_heads) != \
-                (self.n_kv_heads, self.head_dim, self.value_dim, self.value_heads):
+        if (other.n_kv_heads, other.head_dim, other.value_dim, other.value_heads, other.format) != \
+                (self.n_kv_heads, self.head_dim, self.value_dim, self.value_heads, self.format):
             raise ValueError("a run can read another run's cache only if both store the same vectors")
         if self.kind == "full" or other.kind == "full":
-            return CacheNeed("full", self.n_kv_heads, self.head_dim, None, self.v_head_dim, 0, self.n_v_heads)
+            return CacheNeed("full", self.n_kv_heads, self.head_dim, None, self.v_head_dim, 0, self.n_v_heads, self.format)
         if self == other:
             return self
         # (a chunk never reaches further back than a window of its size)
         return CacheNeed("window", self.n_kv_heads, self.head_dim, max(self.window, other.window), self.v_head_dim,
-                         max(self.keep_first, other.keep_first), self.n_v_heads)
+                         max(self.keep_first, other.keep_first), self.n_v_heads, self.format)
 
 
 @dataclass(frozen=True)
@@ -215,6 +232,8 @@ class PositionEncoding(Part):
     encoding sets ``takes_row_scaled``, a :class:`~torchllms_b200.kernels.lazy.RowScaled`."""
 
     takes_row_scaled = False
+    # the formats of a cache (``CacheNeed.format``) that ``encode_and_store`` can write; ``cache.format`` says which it meets
+    cache_formats: Tuple[str, ...] = ("full",)
 
     def encode_and_store(self, qkv, ctx, cache, n_heads: int, n_kv_heads: int, head_dim: int):
         raise NotImplementedError

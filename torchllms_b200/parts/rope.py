@@ -115,6 +115,7 @@ class RotaryEncoding(PositionEncoding):
 
     graph_safe = True
     takes_row_scaled = True      # the kernel scales every row before it rotates and stores it
+    cache_formats = ("full", "fp4")
 
     def __init__(self, env: BuildEnv, *, head_dim: int, theta: float,
                  scaling: Optional[Mapping[str, Any]] = None, pairing: str = "interleaved"):
@@ -130,7 +131,9 @@ class RotaryEncoding(PositionEncoding):
         return 0  # the table is gathered by rows, not streamed
 
     def encode_and_store(self, qkv, ctx, cache, n_heads: int, n_kv_heads: int, head_dim: int):
-        return self.env.ops.rope_kv_write(
+        ops = self.env.ops
+        write = ops.rope_kv_write_fp4 if cache.writes and getattr(cache, "format", "full") == "fp4" else ops.rope_kv_write
+        return write(
             qkv, ctx.positions, self.table,
             n_heads=n_heads, n_kv_heads=n_kv_heads, head_dim=head_dim,
             interleaved=(self.pairing == "interleaved"),

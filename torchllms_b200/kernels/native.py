@@ -121,6 +121,7 @@ class NativeOps:
         self.launches = 0          # kernels of this library launched so far (a bench counts with it)
         # (device, stream, inside a capture) -> ints that are zero between launches, and the capture they belong to
         self._counts: Dict[Tuple[int, int, bool], Tuple[int, torch.Tensor]] = {}
+        self._fp4_plans: Dict[tuple, Tuple[int, int]] = {}
         self.use_tcgen05 = True
         # SwiGLU in the epilogue of the gate/up product (TORCHLLMS_B200_NO_GATED=1 keeps the two kernels, for comparisons)
         self.use_gated = os.environ.get("TORCHLLMS_B200_NO_GATED", "") not in ("1", "true")
@@ -161,7 +162,7 @@ class NativeOps:
         if dtype == torch.bfloat16:
             names += ["attention_mma", "attention_decode", "gemm_tcgen05"]
         if kv_format == "fp4":
-            names += ["kv_fp4", "attention_fp4"]
+            names += ["kv_fp4", "attention_fp4", "attention_fp4_decode", "attention_decode"]
         if sampling:
             names.append("sampling")
         build_libraries(names)
@@ -2107,6 +2108,18 @@ class NativeOps:
         self.launches += 1
         return k, v
 
+    def _fp4_decode_plan(self, dtype: torch.dtype, *sizes: int) -> Tuple[int, int]:
+        """Floats of scratch and counters of a call of the decode kernel; the same sizes come back every layer."""
+        plan = self._fp4_plans.get((dtype, sizes))
+        if plan is None:
+            floats, counters = ctypes.c_longlong(0), ctypes.c_longlong(0)
+            _check(self._lib("attention_fp4_decode").tl_attention_fp4_decode_plan(_DT[dtype], *sizes, ctypes.byref(floats), ctypes.byref(counters)),
+                   "attention_fp4_decode_plan")
+            if len(self._fp4_plans) >= 4096:
+                self._fp4_plans.clear()
+            plan = self._fp4_plans[dtype, sizes] = (floats.value, counters.value)
+        return plan
+
     @_timed
     def paged_attention_fp4(self, q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                             block_table: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor, *,
@@ -2118,8 +2131,8 @@ class NativeOps:
         (``[pages, n_kv_heads, page_size / 16, 9 * head_dim]`` bytes, :mod:`torchllms_b200.cache.fp4`): every token of
         ``q`` ``[T, H, head_dim]`` attends to the keys of its request up to its own place, or to the last ``window`` of
         them.  Keys and values are taken as the cache has them, nothing is rounded on the way; a row that sees no key is
-        zeros.  Arguments as there.  ``impl``: ``"general"`` (CUDA cores, heads of any multiple of 16 up to 256) or
-        ``"auto"``."""
+        zeros.  Arguments as there.  ``impl``: ``"general"`` (CUDA cores, heads of any multiple of 16 up to 256),
+        ``"decode"`` (mma.sync tensor cores, head_dim 64 and 128) or ``"auto"`` (the most specialised kernel that applies)."""
         _cuda_contig(q, "q")
         _need(q.dim() == 3 and q.dtype in _DT, "q must be [tokens, heads, head_dim] in float32 or bfloat16")
         _cuda_contig(q_start, "q_start", torch.int32)
@@ -2144,7 +2157,21 @@ class NativeOps:
         _need(block_table.shape[0] >= n_seqs and q_start.numel() >= n_seqs + 1 and kv_len.numel() >= n_seqs,
               "block_table, q_start and kv_len must cover every request of the step")
         _need(block_table.shape[1] * page_size >= max_kv_len, "block_table is too narrow for max_kv_len")
-        _need(impl in ("auto", "general"), f"unknown attention implementation {impl!r}")
+        _need(impl in ("auto", "general", "decode"), f"unknown attention implementation {impl!r}")
+        decode_ok = head_dim in (64, 128)
+        _need(impl != "decode" or decode_ok, "the tensor-core kernels of the 4-bit cache take head_dim 64 or 128")
+        if decode_ok and impl != "general":
+            floats, counters = self._fp4_decode_plan(q.dtype, n_seqs, n_heads, n_kv_heads, head_dim, page_size, max_q_len, max_kv_len)
+            ws = torch.empty(floats, dtype=torch.float32, device=q.device)
+            self._debug_limit("attention_fp4_decode", 0, k_pages.shape[0])
+            rc = self._lib("attention_fp4_decode").tl_attention_fp4_decode(
+                _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(out), _ptr(block_table), block_table.stride(0), block_table.shape[1],
+                _ptr(q_start), _ptr(kv_len), _ptr(ws), _ptr(self._counters(q.device, counters)), ctypes.c_void_p(self._status.data_ptr()),
+                _DT[q.dtype], n_seqs, n_heads, n_kv_heads, head_dim, page_size, ctypes.c_longlong(k_pages.shape[0]), max_q_len, max_kv_len,
+                int(window or 0), ctypes.c_float(scale), _stream())
+            _check(rc, "paged_attention_fp4")
+            self.launches += 1
+            return out
         self._debug_limit("attention_fp4", 0, k_pages.shape[0])
         rc = self._lib("attention_fp4").tl_attention_fp4_general(
             _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(out), _ptr(block_table), block_table.stride(0), block_table.shape[1],

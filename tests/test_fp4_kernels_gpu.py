@@ -194,14 +194,17 @@ SHAPES = [
 ]
 
 
-@pytest.mark.parametrize("impl", ["general", "decode"])
+@pytest.mark.parametrize("impl", ["general", "decode", "prefill", "prefill in 3 pieces"])
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("H,KV,D,page,q_lens,kv_lens,window", SHAPES)
 def test_attention_is_the_formula(H, KV, D, page, q_lens, kv_lens, window, dtype, impl):
     if impl != "general" and D not in (64, 128):
         pytest.skip("the kernel takes heads of 64 and 128")
+    if impl.startswith("prefill") and dtype == "f32":
+        pytest.skip("the kernel takes bfloat16")
     a, kw = batch(H, KV, D, page, q_lens, kv_lens, window, dtype)
-    judge(ops().paged_attention_fp4(**a, **kw, impl=impl), a, kw)
+    pieces = dict(allow_split=3) if "pieces" in impl else {}
+    judge(ops().paged_attention_fp4(**a, **kw, impl=impl.split()[0], **pieces), a, kw)
     ops().check_status()
 
 
@@ -209,12 +212,15 @@ def test_attention_is_the_formula(H, KV, D, page, q_lens, kv_lens, window, dtype
 def test_large_and_tiny_queries(dtype):
     """Queries of 1e4 and of 1e-6 (scores that are one-hot, or all alike), and rows of zeros."""
     for sharp in (1e4, 1e-6, 0.0):
-        a, kw = batch(8, 2, 64, 16, [1, 3], [100, 230], None, dtype, sharp=sharp)
-        judge(ops().paged_attention_fp4(**a, **kw), a, kw)
+        for n in (3, 60):
+            a, kw = batch(8, 2, 64, 16, [1, n], [100, 230], None, dtype, sharp=sharp)
+            judge(ops().paged_attention_fp4(**a, **kw), a, kw)
 
 
-def test_a_number_that_is_none_shows_in_the_rows_that_see_it():
+@pytest.mark.parametrize("impl", ["general", "decode", "prefill"])
+def test_a_number_that_is_none_shows_in_the_rows_that_see_it(impl):
     a, kw = batch(4, 2, 64, 16, [1, 1, 4], [40, 40, 40])
+    kw["impl"] = impl
     v = fp4.rows_of(a["v_pages"], 64)[1]
     v[int(a["block_table"][0, 1]), 0, 0, 3, 1] = 255               # key 19 of the first request, head 0, coordinates 16 to 31
     k = fp4.rows_of(a["k_pages"], 64)[1]

@@ -42,7 +42,7 @@ NVCC_FLAGS += os.environ.get("TORCHLLMS_B200_NVCC_FLAGS", "").split()
 EXTRA_LINK: Dict[str, List[str]] = {}
 
 ALL_LIBRARIES = ("elementwise", "sublayer", "rope", "attention", "attention_mma", "attention_decode", "attention_prefill", "gemm_simt", "gemm_f32", "gemm_tcgen05", "sampling", "recurrent", "moe", "matrix_state", "stream_sum", "selective_scan", "conv_mixers", "matrix_recurrence",
-                 "kv_fp4", "attention_fp4", "attention_fp4_decode")
+                 "kv_fp4", "attention_fp4", "attention_fp4_decode", "attention_fp4_prefill")
 
 
 class KernelBuildError(RuntimeError):

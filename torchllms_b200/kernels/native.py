@@ -106,6 +106,7 @@ class NativeOps:
     """The kernels as methods.  Libraries are compiled and loaded on first use."""
 
     F32_ROWS = 4096         # rows of one float32 product
+    FP4_PREFILL_MIN_ROWS = 128   # rows (tokens x query heads of a key head) of a request from which the 4-bit cache's tcgen05 kernel is used
     PREFILL_MIN_Q = 96      # portions at least this long go to the tcgen05 prefill attention kernel
     FUSE_MAX_ROWS = 16      # steps of at most this many tokens let a product add itself to the residual stream and
                             # prepare the norm that follows in its own kernel; with more rows product + norm
@@ -162,7 +163,7 @@ class NativeOps:
         if dtype == torch.bfloat16:
             names += ["attention_mma", "attention_decode", "gemm_tcgen05"]
         if kv_format == "fp4":
-            names += ["kv_fp4", "attention_fp4", "attention_fp4_decode", "attention_decode"]
+            names += ["kv_fp4", "attention_fp4", "attention_fp4_decode", "attention_fp4_prefill", "attention_decode"]
         if sampling:
             names.append("sampling")
         build_libraries(names)
@@ -2132,7 +2133,9 @@ class NativeOps:
         ``q`` ``[T, H, head_dim]`` attends to the keys of its request up to its own place, or to the last ``window`` of
         them.  Keys and values are taken as the cache has them, nothing is rounded on the way; a row that sees no key is
         zeros.  Arguments as there.  ``impl``: ``"general"`` (CUDA cores, heads of any multiple of 16 up to 256),
-        ``"decode"`` (mma.sync tensor cores, head_dim 64 and 128) or ``"auto"`` (the most specialised kernel that applies)."""
+        ``"decode"`` (mma.sync tensor cores, head_dim 64 and 128), ``"prefill"`` (tcgen05 tensor cores, head_dim 64 and 128,
+        bfloat16, made for many tokens) or ``"auto"`` (the most specialised kernel that applies).  ``allow_split`` (of the
+        prefill kernel): False keeps every row's keys in one CTA, a number above 1 cuts them into so many pieces."""
         _cuda_contig(q, "q")
         _need(q.dim() == 3 and q.dtype in _DT, "q must be [tokens, heads, head_dim] in float32 or bfloat16")
         _cuda_contig(q_start, "q_start", torch.int32)
@@ -2157,9 +2160,26 @@ class NativeOps:
         _need(block_table.shape[0] >= n_seqs and q_start.numel() >= n_seqs + 1 and kv_len.numel() >= n_seqs,
               "block_table, q_start and kv_len must cover every request of the step")
         _need(block_table.shape[1] * page_size >= max_kv_len, "block_table is too narrow for max_kv_len")
-        _need(impl in ("auto", "general", "decode"), f"unknown attention implementation {impl!r}")
+        _need(impl in ("auto", "general", "decode", "prefill"), f"unknown attention implementation {impl!r}")
         decode_ok = head_dim in (64, 128)
-        _need(impl != "decode" or decode_ok, "the tensor-core kernels of the 4-bit cache take head_dim 64 or 128")
+        _need(impl not in ("decode", "prefill") or decode_ok, "the tensor-core kernels of the 4-bit cache take head_dim 64 or 128")
+        _need(impl != "prefill" or q.dtype == torch.bfloat16, "the tcgen05 kernel of the 4-bit cache takes bfloat16")
+        if impl == "prefill" or (impl == "auto" and decode_ok and q.dtype == torch.bfloat16
+                                 and max_q_len * (n_heads // n_kv_heads) >= self.FP4_PREFILL_MIN_ROWS):
+            lib = self._lib("attention_fp4_prefill")
+            pieces, floats = ctypes.c_int(0), ctypes.c_longlong(0)
+            _check(lib.tl_attention_fp4_prefill_plan(ctypes.c_longlong(q.shape[0]), n_seqs, n_heads, n_kv_heads, head_dim, max_q_len, max_kv_len,
+                                                     int(allow_split), ctypes.byref(pieces), ctypes.byref(floats)), "attention_fp4_prefill_plan")
+            ws = self._scratch(q.device, floats.value)
+            self._debug_limit("attention_fp4_prefill", 0, k_pages.shape[0])
+            rc = lib.tl_attention_fp4_prefill(
+                _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(out), _ptr(block_table), block_table.stride(0), block_table.shape[1],
+                _ptr(q_start), _ptr(kv_len), _ptr(ws), ctypes.c_void_p(self._status.data_ptr()), ctypes.c_longlong(q.shape[0]), n_seqs,
+                n_heads, n_kv_heads, head_dim, page_size, ctypes.c_longlong(k_pages.shape[0]), max_q_len, int(window or 0),
+                ctypes.c_float(scale), pieces, _stream())
+            _check(rc, "paged_attention_fp4")
+            self.launches += 1 if pieces.value == 1 else 2
+            return out
         if decode_ok and impl != "general":
             floats, counters = self._fp4_decode_plan(q.dtype, n_seqs, n_heads, n_kv_heads, head_dim, page_size, max_q_len, max_kv_len)
             ws = torch.empty(floats, dtype=torch.float32, device=q.device)

@@ -6,19 +6,19 @@
 // Bound by reading the cache once (144 bytes a key and head of 128, against 512 in bfloat16), and next to that by issuing the
 // instructions that unpack it: 16 keys and values of 128 numbers are 128 conversions and 128 products with scales a warp, beside
 // 16 products of the tensor cores.  So:
-//   - The cache comes in whole records of 16 tokens by cp.async.bulk, 64 keys a stage, into a ring that a producer warp keeps
-//     full across the borders of requests; four consumer warps take a record of keys and of values each.
+//   - The cache comes in whole records of 16 tokens by cp.async.bulk, 128 keys a stage, into a ring that a producer warp keeps
+//     full across the borders of requests; four consumer warps take two records of keys and of values each.
 //   - Nothing is unpacked into shared memory.  The products are taken transposed, scores^T = K Q^T and out^T = V^T P^T, so that
 //     keys and values are the left operands: a lane loads the coordinates that its fragments hold (any fixed order of the
-//     contraction's index will do, so they are neighbours in a row), converts them in registers, and for V pairs the numbers
-//     of two tokens by a byte permutation.  A cached number times its scale is a float16 exactly (fp4.cuh).
+//     contraction's index will do, so they are neighbours in a row), converts them in registers, and for V exchanges half bytes of two
+//     tokens first.  A cached number times its scale is a float16 exactly (fp4.cuh).
 //   - Queries are brought to float16 by a power of two for each row that puts its largest number just below 2^15: no rounding for
 //     bfloat16 (but of numbers 2^-31 of the largest).  float32 queries and the probabilities of float32 steps are two float16, value and remainder (22
 //     bits), and their products are added up in registers, tile by tile, rounded to nearest (the tensor cores cut).
 //   - Probabilities of bfloat16 steps are one float16 each (2^-12; the result's own rounding is 2^-9).
 //
 // Who does what: the rows of a request (token x query heads of a key head) are cut into blocks of 8 NT; the keys that a block sees, in
-// tiles of 64, are laid on one line, block after block and key head after key head, with the worth of WORTH tiles in front of each
+// tiles of 128, are laid on one line, block after block and key head after key head, with the worth of WORTH tiles in front of each
 // for what it costs to begin and end one, and every CTA takes an even stretch of the line, found on the device from the
 // requests' lengths.  Where a block is cut, each part leaves its sums, and the CTA that is last to finish adds them up in
 // order (a counter for each block and head): the result does not depend on who that is.
@@ -29,14 +29,17 @@
 
 namespace {
 
-constexpr int BN = 64;                  // keys of a tile: a record for each consumer warp
 constexpr int NCW = 4;                  // consumer warps
+constexpr int EACH = 2;                 // records that a consumer warp takes of a tile: one turn of the softmax for both
+constexpr int RECORDS = EACH * NCW;     // records of a tile
+constexpr int BN = RECORDS * FP4_RECORD;
 constexpr int NTHREADS = (NCW + 1) * 32;
-constexpr int WORTH = 2;                // what a block's beginning and end are worth, in tiles
+constexpr int WORTH = 1;                // what a block's beginning and end are worth, in tiles
 constexpr int MOST_PARTS = 64;          // parts of a block, at most
 constexpr int FAILED_PART = 1 << 16;    // what a CTA that gave up adds to a counter beside its 1
 constexpr int SMS = 148;
 constexpr float LOG2E = 1.4426950408889634f;
+constexpr float BIAS = 14.f;            // weights are multiplied as 2^14 times what they are: as float16, down to 2^-38 of the largest
 constexpr unsigned long long WAIT_NS = 2000ull * 1000ull * 1000ull;
 enum : int { ERR_PRODUCER_WAIT = 221, ERR_CONSUMER_WAIT = 222, ERR_COUNT = 223 };
 
@@ -314,95 +317,108 @@ struct Consumer {
         }
     }
 
-    // a record of keys and one of values; its first key is k0
-    __device__ __forceinline__ void record(const Params& p, const unsigned char* kr, const unsigned char* vr, int k0, int lo, int hi) {
+    // EACH records of keys and of values, records NCW apart; the first begins with key k0
+    __device__ __forceinline__ void records(const Params& p, const unsigned char* kr, const unsigned char* vr, int k0, int lo, int hi) {
         constexpr int CODES = FP4_RECORD * (HD / 2);            // where a record's scales begin
-        if (k0 > qmax || k0 + FP4_RECORD <= lo || k0 >= hi) return;
+        constexpr int RECORD = fp4_record_bytes(HD), STEP = NCW * FP4_RECORD, SPAN = (EACH - 1) * STEP + FP4_RECORD;
+        if (k0 > qmax || k0 + SPAN <= lo || k0 >= hi) return;
         // ---- scores
-        float sc[NT][4], low[NT][4];
+        float sc[EACH][NT][4];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int n = 0; n < EACH; ++n) {
+            const unsigned char* rec = kr + n * NCW * RECORD;
+            float low[NT][4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sc[nt][e] = low[nt][e] = 0.f;
-        unsigned wa[WORDS], wb[WORDS];
-        load_words(kr + g * (HD / 2) + t * (HD / 8), wa);
-        load_words(kr + (g + 8) * (HD / 2) + t * (HD / 8), wb);
-        __half2 sa[WORDS / 2], sb[WORDS / 2];                   // a scale for two words
-        if (HD == 128) {
-            const unsigned a = *reinterpret_cast<const unsigned short*>(kr + CODES + g * 8 + 2 * t);
-            const unsigned c = *reinterpret_cast<const unsigned short*>(kr + CODES + (g + 8) * 8 + 2 * t);
-            sa[0] = fp4_scale2(a & 255u); sa[WORDS / 2 - 1] = fp4_scale2(a >> 8);
-            sb[0] = fp4_scale2(c & 255u); sb[WORDS / 2 - 1] = fp4_scale2(c >> 8);
-        } else {
-            sa[0] = fp4_scale2(kr[CODES + g * 4 + t]);
-            sb[0] = fp4_scale2(kr[CODES + (g + 8) * 4 + t]);
-        }
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int j = 0; j < WORDS; ++j) {
-            __half2 a[4], c[4];
-            fp4_unpack(wa[j], a);
-            fp4_unpack(wb[j], c);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                a[i] = __hmul2(a[i], sa[j / 2]);
-                c[i] = __hmul2(c[i], sb[j / 2]);
+                for (int e = 0; e < 4; ++e) sc[n][nt][e] = low[nt][e] = 0.f;
+            unsigned wa[WORDS], wb[WORDS];
+            load_words(rec + g * (HD / 2) + t * (HD / 8), wa);
+            load_words(rec + (g + 8) * (HD / 2) + t * (HD / 8), wb);
+            __half2 sa[WORDS / 2], sb[WORDS / 2];                   // a scale for two words
+            if (HD == 128) {
+                const unsigned a = *reinterpret_cast<const unsigned short*>(rec + CODES + g * 8 + 2 * t);
+                const unsigned c = *reinterpret_cast<const unsigned short*>(rec + CODES + (g + 8) * 8 + 2 * t);
+                sa[0] = fp4_scale2(a & 255u); sa[WORDS / 2 - 1] = fp4_scale2(a >> 8);
+                sb[0] = fp4_scale2(c & 255u); sb[WORDS / 2 - 1] = fp4_scale2(c >> 8);
+            } else {
+                sa[0] = fp4_scale2(rec[CODES + g * 4 + t]);
+                sb[0] = fp4_scale2(rec[CODES + (g + 8) * 4 + t]);
             }
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const unsigned f[4] = {bits(a[2 * h]), bits(c[2 * h]), bits(a[2 * h + 1]), bits(c[2 * h + 1])};
+            for (int j = 0; j < WORDS; ++j) {
+                __half2 a[4], c[4];
+                fp4_unpack(wa[j], a);
+                fp4_unpack(wb[j], c);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    if (PARTS == 2) {
-                        float s[4] = {0.f, 0.f, 0.f, 0.f};
-                        mma_f16(s, f, qf[0][nt][2 * j + h][0], qf[0][nt][2 * j + h][1]);
-                        mma_f16(low[nt], f, qf[PARTS - 1][nt][2 * j + h][0], qf[PARTS - 1][nt][2 * j + h][1]);
+                for (int i = 0; i < 4; ++i) {
+                    a[i] = __hmul2(a[i], sa[j / 2]);
+                    c[i] = __hmul2(c[i], sb[j / 2]);
+                }
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) sc[nt][e] += s[e];
-                    } else {
-                        mma_f16(sc[nt], f, qf[0][nt][2 * j + h][0], qf[0][nt][2 * j + h][1]);
+                for (int h = 0; h < 2; ++h) {
+                    const unsigned f[4] = {bits(a[2 * h]), bits(c[2 * h]), bits(a[2 * h + 1]), bits(c[2 * h + 1])};
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        if (PARTS == 2) {
+                            float s[4] = {0.f, 0.f, 0.f, 0.f};
+                            mma_f16(s, f, qf[0][nt][2 * j + h][0], qf[0][nt][2 * j + h][1]);
+                            mma_f16(low[nt], f, qf[PARTS - 1][nt][2 * j + h][0], qf[PARTS - 1][nt][2 * j + h][1]);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) sc[n][nt][e] += s[e];
+                        } else {
+                            mma_f16(sc[n][nt], f, qf[0][nt][2 * j + h][0], qf[0][nt][2 * j + h][1]);
+                        }
                     }
                 }
             }
-        }
-        if (PARTS == 2) {
+            if (PARTS == 2) {
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sc[nt][e] += low[nt][e];
+                    for (int e = 0; e < 4; ++e) sc[n][nt][e] += low[nt][e];
+            }
         }
         // ---- masks
-        const bool inside = k0 >= lo && k0 + FP4_RECORD <= hi;
-        if (!(inside && k0 + FP4_RECORD - 1 <= qmin && (p.window <= 0 || k0 > qmax - p.window))) {
+        const bool inside = k0 >= lo && k0 + SPAN <= hi;
+        if (!(inside && k0 + SPAN - 1 <= qmin && (p.window <= 0 || k0 > qmax - p.window))) {
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int n = 0; n < EACH; ++n)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int qp = qpos[nt][e & 1], kpos = k0 + g + 8 * (e >> 1);
-                    if (!(kpos >= lo && kpos < hi && kpos <= qp && (p.window <= 0 || kpos > qp - p.window))) sc[nt][e] = -INFINITY;
-                }
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int qp = qpos[nt][e & 1], kpos = k0 + n * STEP + g + 8 * (e >> 1);
+                        if (!(kpos >= lo && kpos < hi && kpos <= qp && (p.window <= 0 || kpos > qp - p.window))) sc[n][nt][e] = -INFINITY;
+                    }
         }
         // ---- weights, moved from result layout [key g][rows 2t, 2t + 1] to operand layout [keys 2t, 2t + 1][row g]
-        unsigned ph[NT][2], pl[NT][2];
+        unsigned ph[EACH][NT][2], pl[EACH][NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             float safe[2], shrink[2];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                float mx = fmaxf(sc[nt][j], sc[nt][j + 2]);               // over the 16 keys: the lanes that share t
+                float mx = fmaxf(sc[0][nt][j], sc[0][nt][j + 2]);         // over the keys: the lanes that share t
+#pragma unroll
+                for (int n = 1; n < EACH; ++n) mx = fmaxf(mx, fmaxf(sc[n][nt][j], sc[n][nt][j + 2]));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
                 const float m_new = fmaxf(m[nt][j], mx * fit[nt][j]);     // maxima live on the base-2 scale
-                safe[j] = m_new == -INFINITY ? 0.f : m_new;               // no key seen yet: keep exponents finite
-                shrink[j] = ex2(m[nt][j] - safe[j]);
+                const float kept = m_new == -INFINITY ? 0.f : m_new;      // no key seen yet: keep exponents finite
+                shrink[j] = ex2(m[nt][j] - kept);
+                safe[j] = kept - BIAS;
                 m[nt][j] = m_new;
                 l[nt][j] *= shrink[j];
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                sc[nt][e] = ex2(fmaf(sc[nt][e], fit[nt][e & 1], -safe[e & 1]));
-                l[nt][e & 1] += sc[nt][e];
-            }
+            for (int n = 0; n < EACH; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    sc[n][nt][e] = ex2(fmaf(sc[n][nt][e], fit[nt][e & 1], -safe[e & 1]));
+                    l[nt][e & 1] += sc[n][nt][e];
+                }
             if (__any_sync(0xffffffffu, shrink[0] != 1.f || shrink[1] != 1.f)) {
 #pragma unroll
                 for (int d = 0; d < KSTEPS; ++d) {
@@ -411,62 +427,82 @@ struct Consumer {
                 }
             }
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                if (PARTS == 2) {
-                    unsigned hi2, lo2;
-                    split2(sc[nt][2 * h], sc[nt][2 * h + 1], hi2, lo2);
-                    ph[nt][h] = movmatrix_trans(hi2);
-                    pl[nt][h] = movmatrix_trans(lo2);
-                } else {
-                    ph[nt][h] = movmatrix_trans(bits(__floats2half2_rn(sc[nt][2 * h], sc[nt][2 * h + 1])));
+            for (int n = 0; n < EACH; ++n)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if (PARTS == 2) {
+                        unsigned hi2, lo2;
+                        split2(sc[n][nt][2 * h], sc[n][nt][2 * h + 1], hi2, lo2);
+                        ph[n][nt][h] = movmatrix_trans(hi2);
+                        pl[n][nt][h] = movmatrix_trans(lo2);
+                    } else {
+                        ph[n][nt][h] = movmatrix_trans(bits(__floats2half2_rn(sc[n][nt][2 * h], sc[n][nt][2 * h + 1])));
+                    }
                 }
-            }
         }
-        // ---- values: tokens 2t, 2t + 1, 2t + 8, 2t + 9, coordinates HD / 8 * g and the next; a token's numbers are words, the operand
-        // wants two tokens side by side
+        // ---- values: tokens 2t, 2t + 1, 2t + 8, 2t + 9, coordinates HD / 8 * g and the next.  A token's numbers are words, the operand
+        // wants a coordinate of two tokens side by side: the half bytes are exchanged before they are converted.
         constexpr int VW = HD / 64;                               // words of a token a lane has
-        unsigned vw[4][VW];
-        __half2 vs[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int key = 2 * t + (i & 1) + 8 * (i >> 1);
-            const unsigned char* at = vr + key * (HD / 2) + g * (HD / 16);
-            if (VW == 2) {
-                const uint2 v = *reinterpret_cast<const uint2*>(at);
-                vw[i][0] = v.x;
-                vw[i][VW - 1] = v.y;
-            } else {
-                vw[i][0] = *reinterpret_cast<const unsigned*>(at);
-            }
-            unsigned byte = vr[CODES + key * (HD / 16) + g * HD / 128];
-            // (what lies outside the keys in use may be anything: its weight is zero, and so is made what it is multiplied by)
-            if (!inside && (k0 + key < lo || k0 + key >= hi)) byte = 0;
-            vs[i] = fp4_scale2(byte);
-        }
-#pragma unroll
-        for (int w = 0; w < VW; ++w) {
-            __half2 r[4][4];
+        for (int n = 0; n < EACH; ++n) {
+            const unsigned char* rec = vr + n * NCW * RECORD;
+            unsigned vw[4][VW], byte[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                fp4_unpack(vw[i][w], r[i]);
+                const int key = 2 * t + (i & 1) + 8 * (i >> 1);
+                const unsigned char* at = rec + key * (HD / 2) + g * (HD / 16);
+                if (VW == 2) {
+                    const uint2 v = *reinterpret_cast<const uint2*>(at);
+                    vw[i][0] = v.x;
+                    vw[i][VW - 1] = v.y;
+                } else {
+                    vw[i][0] = *reinterpret_cast<const unsigned*>(at);
+                }
+                byte[i] = rec[CODES + key * (HD / 16) + g * HD / 128];
+            }
+            if (!inside) {
+                // (what lies outside the keys in use may be anything: its weight is zero, and so is made what it is multiplied by)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) r[i][e] = __hmul2(r[i][e], vs[i]);
+                for (int i = 0; i < 4; ++i) {
+                    const int kpos = k0 + n * STEP + 2 * t + (i & 1) + 8 * (i >> 1);
+                    if (kpos < lo || kpos >= hi) byte[i] = 0;
+                }
+            }
+            __half2 vs[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const unsigned u = (byte[2 * i] << 7) | (byte[2 * i + 1] << 23);
+                vs[i] = *reinterpret_cast<const __half2*>(&u);
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int d = 4 * w + e;
-                const unsigned f[4] = {__byte_perm(bits(r[0][e]), bits(r[1][e]), 0x5410), __byte_perm(bits(r[0][e]), bits(r[1][e]), 0x7632),
-                                       __byte_perm(bits(r[2][e]), bits(r[3][e]), 0x5410), __byte_perm(bits(r[2][e]), bits(r[3][e]), 0x7632)};
+            for (int w = 0; w < VW; ++w) {
+                __half2 even[2][4], odd[2][4];                    // coordinates 2e and 2e + 1 of the word, of tokens 2i and 2i + 1
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    if (PARTS == 2) {
-                        float s[4] = {0.f, 0.f, 0.f, 0.f};
-                        mma_f16(s, f, pl[nt][0], pl[nt][1]);
-                        mma_f16(s, f, ph[nt][0], ph[nt][1]);
+                for (int i = 0; i < 2; ++i) {
+                    const unsigned x = vw[2 * i][w], y = vw[2 * i + 1][w];
+                    fp4_unpack((x & 0x0f0f0f0fu) | ((y << 4) & 0xf0f0f0f0u), even[i]);
+                    fp4_unpack(((x >> 4) & 0x0f0f0f0fu) | (y & 0xf0f0f0f0u), odd[i]);
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) o[nt][d][x] += s[x];
-                    } else {
-                        mma_f16(o[nt][d], f, ph[nt][0], ph[nt][1]);
+                    for (int e = 0; e < 4; ++e) {
+                        even[i][e] = __hmul2(even[i][e], vs[i]);
+                        odd[i][e] = __hmul2(odd[i][e], vs[i]);
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int d = 4 * w + e;
+                    const unsigned f[4] = {bits(even[0][e]), bits(odd[0][e]), bits(even[1][e]), bits(odd[1][e])};
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        if (PARTS == 2) {
+                            float s[4] = {0.f, 0.f, 0.f, 0.f};
+                            mma_f16(s, f, pl[n][nt][0], pl[n][nt][1]);
+                            mma_f16(s, f, ph[n][nt][0], ph[n][nt][1]);
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) o[nt][d][x] += s[x];
+                        } else {
+                            mma_f16(o[nt][d], f, ph[n][nt][0], ph[n][nt][1]);
+                        }
                     }
                 }
             }
@@ -503,7 +539,7 @@ template <typename T, int HD, int STAGES, int NT>
 __global__ void __launch_bounds__(NTHREADS, (NT == 1 && sizeof(T) == 2) ? 3 : 2) attention_fp4_decode_kernel(const Params p) {
     using C = Consumer<T, HD, NT>;
     constexpr int ROWS = 8 * NT, RECORD = fp4_record_bytes(HD);
-    constexpr unsigned STAGE = 2 * NCW * RECORD;
+    constexpr unsigned STAGE = 2 * RECORDS * RECORD;
     extern __shared__ __align__(128) unsigned char smem[];        // the ring, then the warps' results and the weights of the parts
     float* Om = reinterpret_cast<float*>(smem + STAGES * STAGE);
     __shared__ float Mm[NCW * ROWS], Lm[NCW * ROWS];
@@ -529,18 +565,18 @@ __global__ void __launch_bounds__(NTHREADS, (NT == 1 && sizeof(T) == 2) ? 3 : 2)
     if (warp == NCW) {
         // ---- producer: lane = record of the tile (of keys, of values)
         asm volatile("fence.proxy.async.global;" ::: "memory");
-        int it = 0;
+        int it = 0, s = 0;
+        unsigned phase = 1;                             // (a barrier that nobody has waited for yet lets the wait for parity 1 pass)
         bool ok = true;
         do {
             const int* table = p.block_table + (size_t)w.k.b * p.table_stride;
             for (int i = w.t0; i < w.t1; ++i, ++it) {
-                const int s = it % STAGES;
-                if (it >= STAGES && !warp_wait(&empty_bar[s], ((it / STAGES) - 1) & 1, &failed_flag, p.status, ERR_PRODUCER_WAIT, lane)) {
+                if (!warp_wait(&empty_bar[s], phase, &failed_flag, p.status, ERR_PRODUCER_WAIT, lane)) {
                     ok = false;
                     break;
                 }
-                const int rec = (w.k.start + i * BN) / FP4_RECORD + (lane & (NCW - 1));
-                const bool mine = lane < 2 * NCW && rec * FP4_RECORD < w.k.hi;
+                const int rec = (w.k.start + i * BN) / FP4_RECORD + (lane & (RECORDS - 1));
+                const bool mine = lane < 2 * RECORDS && rec * FP4_RECORD < w.k.hi;
                 const unsigned there = __ballot_sync(0xffffffffu, mine);
                 if (lane == 0) mbar_expect_tx(&full_bar[s], __popc(there) * RECORD);
                 __syncwarp();
@@ -549,9 +585,13 @@ __global__ void __launch_bounds__(NTHREADS, (NT == 1 && sizeof(T) == 2) ? 3 : 2)
                     long long page = table[block];
                     if (!tl_check_page(page) || page < 0 || page >= p.n_pages) page = 0;       // (a bad page is not followed; debug builds report it)
                     const long long at = ((page * p.n_kv_heads + w.kvh) * p.page_records + rec - block * p.page_records) * RECORD;
-                    bulk_load(smem + s * STAGE + lane * RECORD, (lane < NCW ? p.k_pages : p.v_pages) + at, RECORD, &full_bar[s]);
+                    bulk_load(smem + s * STAGE + lane * RECORD, (lane < RECORDS ? p.k_pages : p.v_pages) + at, RECORD, &full_bar[s]);
                 }
                 __syncwarp();
+                if (++s == STAGES) {
+                    s = 0;
+                    phase ^= 1u;
+                }
             }
         } while (ok && walk_next<ROWS>(p, w));
         // (nothing that is still on its way may land in shared memory that is no longer this CTA's)
@@ -563,19 +603,23 @@ __global__ void __launch_bounds__(NTHREADS, (NT == 1 && sizeof(T) == 2) ? 3 : 2)
     // ---- consumers: all rows of the block, a record of every tile each
     C c;
     bool ok = true;
-    int it = 0;
+    int s = 0;
+    unsigned phase = 0;
     do {
         c.begin(p, w.k, w.kvh, lane);
-        for (int i = w.t0; i < w.t1; ++i, ++it) {
-            const int s = it % STAGES;
-            if (!ok || !warp_wait(&full_bar[s], (it / STAGES) & 1, &failed_flag, p.status, ERR_CONSUMER_WAIT, lane)) {
+        for (int i = w.t0; i < w.t1; ++i) {
+            if (!ok || !warp_wait(&full_bar[s], phase, &failed_flag, p.status, ERR_CONSUMER_WAIT, lane)) {
                 ok = false;
                 break;
             }
             const unsigned char* kr = smem + s * STAGE + warp * RECORD;
-            c.record(p, kr, kr + NCW * RECORD, w.k.start + i * BN + warp * FP4_RECORD, w.k.lo, w.k.hi);
+            c.records(p, kr, kr + RECORDS * RECORD, w.k.start + i * BN + warp * FP4_RECORD, w.k.lo, w.k.hi);
             __syncwarp();
             if (lane == 0) mbar_arrive(&empty_bar[s]);     // this warp is done with the stage
+            if (++s == STAGES) {
+                s = 0;
+                phase ^= 1u;
+            }
         }
         // ---- the four warps' results, through shared memory
         consumers_sync();
@@ -682,10 +726,10 @@ __global__ void __launch_bounds__(NTHREADS, (NT == 1 && sizeof(T) == 2) ? 3 : 2)
 
 // ---- host side ---------------------------------------------------------------------------------
 
-template <int HD> constexpr int stages_for() { return HD == 128 ? 5 : 8; }
+template <int HD> constexpr int stages_for() { return HD == 128 ? 3 : 5; }
 template <int HD> size_t smem_for(int rows) {
     const size_t results = (size_t)NCW * rows * (HD + 4) * 4, weights = (size_t)rows * MOST_PARTS * 4;
-    return (size_t)stages_for<HD>() * 2 * NCW * fp4_record_bytes(HD) + (results > weights ? results : weights);
+    return (size_t)stages_for<HD>() * 2 * RECORDS * fp4_record_bytes(HD) + (results > weights ? results : weights);
 }
 
 bool takes(int n_heads, int n_kv_heads, int head_dim, int page_size) {

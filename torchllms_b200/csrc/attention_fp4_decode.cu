@@ -56,6 +56,8 @@ struct Params {
     int* status;
     long long n_pages;
     int table_stride, table_cols, n_seqs, n_heads, n_kv_heads, group, page_records, blocks, rows, window;
+    unsigned per_group;         // 2^32 / group and one more (0 for a group of one head): row / group without a division
+    int page_shift;             // page_records is 1 << page_shift, or page_shift is negative
     float scale_log2;
 };
 
@@ -110,12 +112,20 @@ __device__ __forceinline__ float ex2(float x) {     // 2^x, one instruction; 2^-
     return y;
 }
 __device__ __forceinline__ unsigned bits(__half2 h) { return *reinterpret_cast<unsigned*>(&h); }
+__device__ __forceinline__ unsigned select_bits(unsigned mask, unsigned x, unsigned y) {      // x where mask is set, else y: one instruction
+    unsigned d;
+    asm("lop3.b32 %0, %1, %2, %3, 0xca;" : "=r"(d) : "r"(mask), "r"(x), "r"(y));
+    return d;
+}
 __device__ __forceinline__ unsigned movmatrix_trans(unsigned a) {     // 8 x 8 block of 16-bit numbers, transposed across the warp
     unsigned d;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
     return d;
 }
 __device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(NCW * 32) : "memory"); }
+
+// (exact for row * group < 2^32, which the host sees to)
+__device__ __forceinline__ int token_of(const Params& p, int row) { return p.per_group ? (int)__umulhi((unsigned)row, p.per_group) : row; }
 
 // ---- the line of tiles
 // What a block of a request's rows sees.
@@ -128,7 +138,7 @@ struct Block {
     int start, tiles;   // its tiles: the first begins at key `start`, on a record
 };
 template <int ROWS> __device__ __forceinline__ int block_at(const Params& p, int i, Block& k) {      // its worth of one key head, 0: there is no such block
-    k.b = i / p.blocks;
+    k.b = p.blocks == 1 ? i : i / p.blocks;
     k.number = i - k.b * p.blocks;
     k.first = p.q_start[k.b];
     const int ql = p.q_start[k.b + 1] - k.first;
@@ -136,7 +146,7 @@ template <int ROWS> __device__ __forceinline__ int block_at(const Params& p, int
     k.n_rows = min(ROWS, ql * p.group - k.row0);
     if (k.n_rows <= 0) return 0;
     k.base = p.kv_len[k.b] - ql;
-    const int t0 = k.row0 / p.group, t1 = (k.row0 + k.n_rows - 1) / p.group;
+    const int t0 = token_of(p, k.row0), t1 = token_of(p, k.row0 + k.n_rows - 1);
     k.lo = p.window > 0 ? max(0, k.base + t0 - p.window + 1) : 0;
     k.hi = min(k.base + t1 + 1, p.table_cols * p.page_records * FP4_RECORD);
     k.start = k.lo & ~(FP4_RECORD - 1);
@@ -156,7 +166,7 @@ template <int ROWS> __device__ __forceinline__ bool walk_here(const Params& p, W
     if (w.off + WORTH >= w.end) return false;
     w.t0 = max(0, w.begin - w.off - WORTH);
     w.t1 = min(w.k.tiles, w.end - w.off - WORTH);
-    w.parts = (w.off + WORTH + w.k.tiles - 1) / w.share - (w.off + WORTH) / w.share + 1;
+    w.parts = w.t1 - w.t0 == w.k.tiles ? 1 : (w.off + WORTH + w.k.tiles - 1) / w.share - (w.off + WORTH) / w.share + 1;
     return true;
 }
 template <int ROWS> __device__ __forceinline__ bool walk_next(const Params& p, Walk& w) {
@@ -171,12 +181,12 @@ template <int ROWS> __device__ __forceinline__ bool walk_next(const Params& p, W
 }
 template <int ROWS> __device__ __forceinline__ bool walk_first(const Params& p, Walk& w, int lane) {
     const int n = p.n_seqs * p.blocks;
-    int total = 0, longest = 0;
+    int total = 0, longest = 0, mine = 0;
     for (int i = lane; i < n; i += 32) {
         Block k;
-        const int worth = block_at<ROWS>(p, i, k);
-        total += worth;
-        longest = max(longest, worth);
+        mine = block_at<ROWS>(p, i, k);
+        total += mine;
+        longest = max(longest, mine);
     }
     total = __reduce_add_sync(0xffffffffu, total) * p.n_kv_heads;
     longest = __reduce_max_sync(0xffffffffu, longest);
@@ -186,9 +196,11 @@ template <int ROWS> __device__ __forceinline__ bool walk_first(const Params& p, 
     if (w.begin >= total) return false;
     int before = 0;                                     // worth (of all heads) of the blocks before these 32
     for (int i0 = 0; i0 < n; i0 += 32) {
-        Block k;
-        const int mine = i0 + lane < n ? block_at<ROWS>(p, i0 + lane, k) * p.n_kv_heads : 0;
-        int upto = mine;
+        if (n > 32) {                                   // (up to 32 blocks: each lane still has its own)
+            Block k;
+            mine = i0 + lane < n ? block_at<ROWS>(p, i0 + lane, k) : 0;
+        }
+        int upto = mine * p.n_kv_heads;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int v = __shfl_up_sync(0xffffffffu, upto, o);
@@ -199,7 +211,7 @@ template <int ROWS> __device__ __forceinline__ bool walk_first(const Params& p, 
             const int src = __ffs(here) - 1;            // the first block that reaches beyond the stretch's beginning
             w.i = i0 + src;
             const int worth = block_at<ROWS>(p, w.i, w.k);
-            const int at = before + __shfl_sync(0xffffffffu, upto - mine, src);
+            const int at = before + __shfl_sync(0xffffffffu, upto, src) - worth * p.n_kv_heads;
             w.kvh = (w.begin - at) / worth;
             w.off = at + w.kvh * worth;
             return walk_here<ROWS>(p, w);
@@ -259,7 +271,7 @@ struct Consumer {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const int r = nt * 8 + g;
-            const int row = k.row0 + r, token = row / p.group;
+            const int row = k.row0 + r, token = token_of(p, row);
             float x[WORDS][8];
             unsigned top = 0;
 #pragma unroll
@@ -293,7 +305,7 @@ struct Consumer {
             for (int j = 0; j < 2; ++j) {
                 fit[nt][j] = __shfl_sync(0xffffffffu, back, (2 * t + j) * 4);
                 const int rr = nt * 8 + 2 * t + j;
-                qpos[nt][j] = rr < k.n_rows ? k.base + (k.row0 + rr) / p.group : -1;
+                qpos[nt][j] = rr < k.n_rows ? k.base + token_of(p, k.row0 + rr) : -1;
                 top_pos = max(top_pos, qpos[nt][j]);
                 if (rr < k.n_rows) low_pos = min(low_pos, qpos[nt][j]);
                 m[nt][j] = -INFINITY;
@@ -339,8 +351,10 @@ struct Consumer {
             if (HD == 128) {
                 const unsigned a = *reinterpret_cast<const unsigned short*>(rec + CODES + g * 8 + 2 * t);
                 const unsigned c = *reinterpret_cast<const unsigned short*>(rec + CODES + (g + 8) * 8 + 2 * t);
-                sa[0] = fp4_scale2(a & 255u); sa[WORDS / 2 - 1] = fp4_scale2(a >> 8);
-                sb[0] = fp4_scale2(c & 255u); sb[WORDS / 2 - 1] = fp4_scale2(c >> 8);
+                auto scale2 = [](unsigned v) { v <<= 7; return *reinterpret_cast<const __half2*>(&v); };
+                // (bytes 2 and 3 of a 16-bit load are zero)
+                sa[0] = scale2(__byte_perm(a, a, 0x2020)); sa[WORDS / 2 - 1] = scale2(__byte_perm(a, a, 0x2121));
+                sb[0] = scale2(__byte_perm(c, c, 0x2020)); sb[WORDS / 2 - 1] = scale2(__byte_perm(c, c, 0x2121));
             } else {
                 sa[0] = fp4_scale2(rec[CODES + g * 4 + t]);
                 sb[0] = fp4_scale2(rec[CODES + (g + 8) * 4 + t]);
@@ -471,7 +485,7 @@ struct Consumer {
             __half2 vs[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const unsigned u = (byte[2 * i] << 7) | (byte[2 * i + 1] << 23);
+                const unsigned u = __byte_perm(byte[2 * i], byte[2 * i + 1], 0x5410) << 7;
                 vs[i] = *reinterpret_cast<const __half2*>(&u);
             }
 #pragma unroll
@@ -480,8 +494,8 @@ struct Consumer {
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const unsigned x = vw[2 * i][w], y = vw[2 * i + 1][w];
-                    fp4_unpack((x & 0x0f0f0f0fu) | ((y << 4) & 0xf0f0f0f0u), even[i]);
-                    fp4_unpack(((x >> 4) & 0x0f0f0f0fu) | (y & 0xf0f0f0f0u), odd[i]);
+                    fp4_unpack(select_bits(0x0f0f0f0fu, x, y << 4), even[i]);
+                    fp4_unpack(select_bits(0x0f0f0f0fu, x >> 4, y), odd[i]);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         even[i][e] = __hmul2(even[i][e], vs[i]);
@@ -540,7 +554,7 @@ __global__ void __launch_bounds__(NTHREADS, (NT == 1 && sizeof(T) == 2) ? 3 : 2)
     using C = Consumer<T, HD, NT>;
     constexpr int ROWS = 8 * NT, RECORD = fp4_record_bytes(HD);
     constexpr unsigned STAGE = 2 * RECORDS * RECORD;
-    extern __shared__ __align__(128) unsigned char smem[];        // the ring, then the warps' results and the weights of the parts
+    extern __shared__ __align__(128) unsigned char smem[];        // the ring, then the warps' results
     float* Om = reinterpret_cast<float*>(smem + STAGES * STAGE);
     __shared__ float Mm[NCW * ROWS], Lm[NCW * ROWS];
     __shared__ __align__(8) unsigned long long full_bar[STAGES];
@@ -581,7 +595,7 @@ __global__ void __launch_bounds__(NTHREADS, (NT == 1 && sizeof(T) == 2) ? 3 : 2)
                 if (lane == 0) mbar_expect_tx(&full_bar[s], __popc(there) * RECORD);
                 __syncwarp();
                 if (mine) {
-                    const int block = rec / p.page_records;
+                    const int block = p.page_shift >= 0 ? rec >> p.page_shift : rec / p.page_records;
                     long long page = table[block];
                     if (!tl_check_page(page) || page < 0 || page >= p.n_pages) page = 0;       // (a bad page is not followed; debug builds report it)
                     const long long at = ((page * p.n_kv_heads + w.kvh) * p.page_records + rec - block * p.page_records) * RECORD;
@@ -631,7 +645,7 @@ __global__ void __launch_bounds__(NTHREADS, (NT == 1 && sizeof(T) == 2) ? 3 : 2)
         const bool sound = gave_up == 0;
         const int n_rows = w.k.n_rows;
         auto out_row = [&](int rr) {
-            const int row = w.k.row0 + rr, token = row / p.group;
+            const int row = w.k.row0 + rr, token = token_of(p, row);
             return reinterpret_cast<T*>(p.out) + ((size_t)(w.k.first + token) * p.n_heads + w.kvh * p.group + row - token * p.group) * HD;
         };
         // where a part of this block lies: that with its first tile in its CTA's first place, others in the second
@@ -680,42 +694,42 @@ __global__ void __launch_bounds__(NTHREADS, (NT == 1 && sizeof(T) == 2) ? 3 : 2)
             }
             consumers_sync();
             if (arrived == w.parts) {
+                // (eight parts at a time are under way)
                 const int cta0 = (w.off + WORTH) / w.share;
-                float* weight = Om;                                          // [rows][MOST_PARTS]
-                for (int rr = warp; rr < n_rows; rr += NCW) {
-                    float2 ml[MOST_PARTS / 32];
-                    float M = -INFINITY, den = 0.f;
-#pragma unroll
-                    for (int i = 0; i < MOST_PARTS / 32; ++i) {
-                        const int c1 = i * 32 + lane;
-                        ml[i] = make_float2(-INFINITY, 0.f);
-                        if (c1 < w.parts) ml[i] = __ldcg(reinterpret_cast<const float2*>(part_of(cta0 + c1, c1 == 0) + p.rows * HD + 2 * rr));
-                        M = max_keep(M, ml[i].x);
-                    }
-#pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) M = max_keep(M, __shfl_xor_sync(0xffffffffu, M, o));
-#pragma unroll
-                    for (int i = 0; i < MOST_PARTS / 32; ++i) {
-                        const int c1 = i * 32 + lane;
-                        const float f = ml[i].x == -INFINITY ? 0.f : ex2(ml[i].x - M);
-                        if (c1 < w.parts) weight[rr * MOST_PARTS + c1] = f;
-                        den = fmaf(f, ml[i].y, den);
-                    }
-                    den = warp_sum(den);
-                    if (lane == 0) Lm[rr] = M == -INFINITY ? 0.f : 1.f / den;
-                }
-                consumers_sync();
                 for (int idx = tid; idx < n_rows * (HD / 4); idx += NCW * 32) {
                     const int rr = idx / (HD / 4), d = (idx - rr * (HD / 4)) * 4;
                     float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-                    for (int c1 = 0; c1 < w.parts; ++c1) {
-                        const float f = weight[rr * MOST_PARTS + c1];
-                        const float4 o4 = __ldcg(reinterpret_cast<const float4*>(part_of(cta0 + c1, c1 == 0) + rr * HD + d));
-                        num.x = fmaf(f, o4.x, num.x); num.y = fmaf(f, o4.y, num.y);
-                        num.z = fmaf(f, o4.z, num.z); num.w = fmaf(f, o4.w, num.w);
+                    float M = -INFINITY, den = 0.f;
+                    for (int c0 = 0; c0 < w.parts; c0 += 8) {
+                        float2 ml[8];
+                        float4 o4[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            ml[i] = make_float2(-INFINITY, 0.f);
+                            o4[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                            if (c0 + i < w.parts) {
+                                const float* part = part_of(cta0 + c0 + i, c0 + i == 0);
+                                ml[i] = __ldcg(reinterpret_cast<const float2*>(part + p.rows * HD + 2 * rr));
+                                o4[i] = __ldcg(reinterpret_cast<const float4*>(part + rr * HD + d));
+                            }
+                        }
+                        float top = M;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) top = max_keep(top, ml[i].x);
+                        const float old = M == -INFINITY ? 0.f : ex2(M - top);
+                        num.x *= old; num.y *= old; num.z *= old; num.w *= old;
+                        den *= old;
+                        M = top;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            if (ml[i].x == -INFINITY) continue;
+                            const float f = ex2(ml[i].x - M);
+                            num.x = fmaf(f, o4[i].x, num.x); num.y = fmaf(f, o4[i].y, num.y);
+                            num.z = fmaf(f, o4[i].z, num.z); num.w = fmaf(f, o4[i].w, num.w);
+                            den = fmaf(f, ml[i].y, den);
+                        }
                     }
-                    const float inv = Lm[rr];
+                    const float inv = M == -INFINITY ? 0.f : 1.f / den;
                     store4(out_row(rr) + d, make_float4(num.x * inv, num.y * inv, num.z * inv, num.w * inv));
                 }
             }
@@ -728,8 +742,7 @@ __global__ void __launch_bounds__(NTHREADS, (NT == 1 && sizeof(T) == 2) ? 3 : 2)
 
 template <int HD> constexpr int stages_for() { return HD == 128 ? 3 : 5; }
 template <int HD> size_t smem_for(int rows) {
-    const size_t results = (size_t)NCW * rows * (HD + 4) * 4, weights = (size_t)rows * MOST_PARTS * 4;
-    return (size_t)stages_for<HD>() * 2 * RECORDS * fp4_record_bytes(HD) + (results > weights ? results : weights);
+    return (size_t)stages_for<HD>() * 2 * RECORDS * fp4_record_bytes(HD) + (size_t)NCW * rows * (HD + 4) * 4;
 }
 
 bool takes(int n_heads, int n_kv_heads, int head_dim, int page_size) {
@@ -817,6 +830,11 @@ extern "C" int tl_attention_fp4_decode(const void* q, const void* k_pages, const
     p.part = workspace; p.counters = counters; p.status = status; p.n_pages = n_pages;
     p.table_stride = table_stride; p.table_cols = table_cols; p.n_seqs = n_seqs; p.n_heads = n_heads; p.n_kv_heads = n_kv_heads;
     p.group = n_heads / n_kv_heads; p.page_records = page_size / FP4_RECORD; p.blocks = pl.blocks; p.rows = pl.rows;
+    p.page_shift = -1;
+    for (int b = 0; b < 31; ++b)
+        if (p.page_records == 1 << b) p.page_shift = b;
+    p.per_group = p.group == 1 ? 0u : (unsigned)((1ull << 32) / (unsigned)p.group) + 1u;
+    if ((double)max_q_len * p.group * p.group >= 4294967296.0) return TL_BAD_SIZE;
     p.window = window > 0 ? window : 0;
     p.scale_log2 = scale * LOG2E;
     cudaStream_t s = (cudaStream_t)stream;

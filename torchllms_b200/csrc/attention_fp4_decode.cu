@@ -39,7 +39,9 @@ constexpr int MOST_PARTS = 64;          // parts of a block, at most
 constexpr int FAILED_PART = 1 << 16;    // what a CTA that gave up adds to a counter beside its 1
 constexpr int SMS = 148;
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr float BIAS = 14.f;            // weights are multiplied as 2^14 times what they are: as float16, down to 2^-38 of the largest
+// The maximum that exponents are taken against may lag behind by a factor of up to 2^LAG: then no lane asks another for its
+// maximum.  Weights are multiplied as 2^BIAS times what they are: as float16, down to 2^-34 of the largest.
+constexpr float LAG = 4.f, BIAS = 11.f;
 constexpr unsigned long long WAIT_NS = 2000ull * 1000ull * 1000ull;
 enum : int { ERR_PRODUCER_WAIT = 221, ERR_CONSUMER_WAIT = 222, ERR_COUNT = 223 };
 
@@ -111,10 +113,21 @@ __device__ __forceinline__ float ex2(float x) {     // 2^x, one instruction; 2^-
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 __device__ __forceinline__ unsigned bits(__half2 h) { return *reinterpret_cast<unsigned*>(&h); }
 __device__ __forceinline__ unsigned select_bits(unsigned mask, unsigned x, unsigned y) {      // x where mask is set, else y: one instruction
     unsigned d;
     asm("lop3.b32 %0, %1, %2, %3, 0xca;" : "=r"(d) : "r"(mask), "r"(x), "r"(y));
+    return d;
+}
+// (shifts as products: multiply-adds have a pipe of their own, shifts share the conversions')
+__device__ __forceinline__ unsigned mad(unsigned a, unsigned b, unsigned c) {
+    unsigned d;
+    asm("mad.lo.u32 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
     return d;
 }
 __device__ __forceinline__ unsigned movmatrix_trans(unsigned a) {     // 8 x 8 block of 16-bit numbers, transposed across the warp
@@ -349,12 +362,8 @@ struct Consumer {
             load_words(rec + (g + 8) * (HD / 2) + t * (HD / 8), wb);
             __half2 sa[WORDS / 2], sb[WORDS / 2];                   // a scale for two words
             if (HD == 128) {
-                const unsigned a = *reinterpret_cast<const unsigned short*>(rec + CODES + g * 8 + 2 * t);
-                const unsigned c = *reinterpret_cast<const unsigned short*>(rec + CODES + (g + 8) * 8 + 2 * t);
-                auto scale2 = [](unsigned v) { v <<= 7; return *reinterpret_cast<const __half2*>(&v); };
-                // (bytes 2 and 3 of a 16-bit load are zero)
-                sa[0] = scale2(__byte_perm(a, a, 0x2020)); sa[WORDS / 2 - 1] = scale2(__byte_perm(a, a, 0x2121));
-                sb[0] = scale2(__byte_perm(c, c, 0x2020)); sb[WORDS / 2 - 1] = scale2(__byte_perm(c, c, 0x2121));
+                sa[0] = fp4_scale2(rec[CODES + g * 8 + 2 * t]); sa[WORDS / 2 - 1] = fp4_scale2(rec[CODES + g * 8 + 2 * t + 1]);
+                sb[0] = fp4_scale2(rec[CODES + (g + 8) * 8 + 2 * t]); sb[WORDS / 2 - 1] = fp4_scale2(rec[CODES + (g + 8) * 8 + 2 * t + 1]);
             } else {
                 sa[0] = fp4_scale2(rec[CODES + g * 4 + t]);
                 sb[0] = fp4_scale2(rec[CODES + (g + 8) * 4 + t]);
@@ -410,22 +419,37 @@ struct Consumer {
         unsigned ph[EACH][NT][2], pl[EACH][NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            float safe[2], shrink[2];
+            float mx[2];
+            bool grown = false;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                float mx = fmaxf(sc[0][nt][j], sc[0][nt][j + 2]);         // over the keys: the lanes that share t
+                mx[j] = fmaxf(sc[0][nt][j], sc[0][nt][j + 2]);
 #pragma unroll
-                for (int n = 1; n < EACH; ++n) mx = fmaxf(mx, fmaxf(sc[n][nt][j], sc[n][nt][j + 2]));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                const float m_new = fmaxf(m[nt][j], mx * fit[nt][j]);     // maxima live on the base-2 scale
-                const float kept = m_new == -INFINITY ? 0.f : m_new;      // no key seen yet: keep exponents finite
-                shrink[j] = ex2(m[nt][j] - kept);
-                safe[j] = kept - BIAS;
-                m[nt][j] = m_new;
-                l[nt][j] *= shrink[j];
+                for (int n = 1; n < EACH; ++n) mx[j] = max3(mx[j], sc[n][nt][j], sc[n][nt][j + 2]);
+                mx[j] *= fit[nt][j];                                      // maxima live on the base-2 scale
+                grown = grown || mx[j] > m[nt][j] + LAG;                  // (also for the first key a row sees)
             }
+            if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {                             // over the keys: the lanes that share t
+                    float top = mx[j];
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                    const float m_new = fmaxf(m[nt][j], top);
+                    const float shrink = m_new == -INFINITY ? 1.f : ex2(m[nt][j] - m_new);
+                    m[nt][j] = m_new;
+                    l[nt][j] *= shrink;
+#pragma unroll
+                    for (int d = 0; d < KSTEPS; ++d) {
+                        o[nt][d][j] *= shrink;
+                        o[nt][d][j + 2] *= shrink;
+                    }
+                }
+            }
+            float safe[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) safe[j] = m[nt][j] == -INFINITY ? 0.f : m[nt][j] - BIAS;     // no key seen yet: keep exponents finite
 #pragma unroll
             for (int n = 0; n < EACH; ++n)
 #pragma unroll
@@ -433,13 +457,6 @@ struct Consumer {
                     sc[n][nt][e] = ex2(fmaf(sc[n][nt][e], fit[nt][e & 1], -safe[e & 1]));
                     l[nt][e & 1] += sc[n][nt][e];
                 }
-            if (__any_sync(0xffffffffu, shrink[0] != 1.f || shrink[1] != 1.f)) {
-#pragma unroll
-                for (int d = 0; d < KSTEPS; ++d) {
-                    o[nt][d][0] *= shrink[0]; o[nt][d][1] *= shrink[1];
-                    o[nt][d][2] *= shrink[0]; o[nt][d][3] *= shrink[1];
-                }
-            }
 #pragma unroll
             for (int n = 0; n < EACH; ++n)
 #pragma unroll
@@ -485,7 +502,7 @@ struct Consumer {
             __half2 vs[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const unsigned u = __byte_perm(byte[2 * i], byte[2 * i + 1], 0x5410) << 7;
+                const unsigned u = mad(byte[2 * i + 1], 1u << 23, mad(byte[2 * i], 1u << 7, 0u));
                 vs[i] = *reinterpret_cast<const __half2*>(&u);
             }
 #pragma unroll
@@ -494,7 +511,7 @@ struct Consumer {
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const unsigned x = vw[2 * i][w], y = vw[2 * i + 1][w];
-                    fp4_unpack(select_bits(0x0f0f0f0fu, x, y << 4), even[i]);
+                    fp4_unpack(select_bits(0x0f0f0f0fu, x, mad(y, 16u, 0u)), even[i]);
                     fp4_unpack(select_bits(0x0f0f0f0fu, x >> 4, y), odd[i]);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {

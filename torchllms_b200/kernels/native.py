@@ -123,11 +123,13 @@ class NativeOps:
         # (device, stream, inside a capture) -> ints that are zero between launches, and the capture they belong to
         self._counts: Dict[Tuple[int, int, bool], Tuple[int, torch.Tensor]] = {}
         self._fp4_plans: Dict[tuple, Tuple[int, int]] = {}
+        self._fp4_calls: Dict[str, object] = {}
         self.use_tcgen05 = True
         # SwiGLU in the epilogue of the gate/up product (TORCHLLMS_B200_NO_GATED=1 keeps the two kernels, for comparisons)
         self.use_gated = os.environ.get("TORCHLLMS_B200_NO_GATED", "") not in ("1", "true")
         # error word of kernels with bounded waits: pinned host memory the device writes to directly
         self._status = torch.zeros(4, dtype=torch.int32).pin_memory()
+        self._status_ptr = self._status.data_ptr()
         self._mm_out_dtype: Optional[bool] = None
         self._profile = None
         self._profile_depth = 0
@@ -1766,7 +1768,8 @@ class NativeOps:
         if n <= 0:
             return None
         stream, capture = _stream(), ctypes.c_ulonglong(0)
-        _check(self._lib("attention_decode").tl_stream_capture_id(stream, ctypes.byref(capture)), "stream_capture_id")
+        if torch.cuda.is_current_stream_capturing():
+            _check(self._lib("attention_decode").tl_stream_capture_id(stream, ctypes.byref(capture)), "stream_capture_id")
         key = (device.index or 0, stream.value or 0, capture.value != 0)
         of, buf = self._counts.get(key, (0, None))
         if buf is None or of != capture.value or buf.numel() < n:
@@ -2033,8 +2036,29 @@ class NativeOps:
         return out
 
     # ------------------------------------------------------------- keys and values in 4 bits
+    # These run once a layer and step, and a step of few tokens takes the device less time than the host needs for a call.  So a call
+    # looks its arguments over in one expression, and only one that does not pass is taken apart to say what is wrong.
+    _FP4_ARGS = {
+        "tl_rope_kv_write_fp4": ("kv_fp4", "piippppppiiiiiiiliipiffp"),
+        "tl_kv_read_fp4": ("kv_fp4", "pppppiiliiip"),
+        "tl_attention_fp4_general": ("attention_fp4", "ppppp" "iippiiiiiiliifp"),
+        "tl_attention_fp4_decode": ("attention_fp4_decode", "ppppp" "iippppp" "iiiiii" "liii" "fp"),
+        "tl_attention_fp4_prefill": ("attention_fp4_prefill", "ppppp" "iippppl" "iiiii" "lii" "fip"),
+    }
+    _FP4_TYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float}
+
+    def _fp4_call(self, name: str):
+        """A kernel's entry point, told its arguments' types (numbers then go through without objects around them)."""
+        fn = self._fp4_calls.get(name)
+        if fn is None:
+            lib, types = self._FP4_ARGS[name]
+            fn = getattr(self._lib(lib), name)
+            fn.argtypes = [self._FP4_TYPES[t] for t in types]
+            self._fp4_calls[name] = fn
+        return fn
+
     @staticmethod
-    def _fp4_pages(k_pages: torch.Tensor, v_pages: torch.Tensor, n_kv_heads: int, head_dim: int, page_size: int) -> None:
+    def _fp4_pages_explained(k_pages, v_pages, n_kv_heads: int, head_dim: int, page_size: int) -> None:
         _cuda_contig(k_pages, "k_pages", torch.uint8)
         _cuda_contig(v_pages, "v_pages", torch.uint8)
         _need(head_dim % GROUP == 0 and 0 < head_dim <= MAX_HEAD_DIM,
@@ -2043,6 +2067,35 @@ class NativeOps:
         _need(k_pages.shape == v_pages.shape and k_pages.dim() == 4
               and k_pages.shape[1:] == (n_kv_heads, page_size // RECORD, record_bytes(head_dim)) and k_pages.shape[0] > 0,
               "4-bit pages must be [pages, n_kv_heads, page_size / 16, 9 * head_dim] bytes, keys and values alike")
+
+    @staticmethod
+    def _fp4_pages_fit(k_pages, v_pages, n_kv_heads: int, head_dim: int, page_size: int) -> bool:
+        shape = k_pages.shape
+        return (k_pages.dtype is torch.uint8 and v_pages.dtype is torch.uint8 and k_pages.is_cuda and v_pages.is_cuda
+                and len(shape) == 4 and shape == v_pages.shape and shape[1] == n_kv_heads and page_size > 0 and head_dim > 0
+                and shape[2] * RECORD == page_size and shape[3] == 9 * head_dim and shape[0] > 0 and head_dim % GROUP == 0
+                and head_dim <= MAX_HEAD_DIM and k_pages.is_contiguous() and v_pages.is_contiguous())
+
+    def _rope_fp4_explained(self, qkv, positions, table, n_heads, n_kv_heads, head_dim, k_pages, v_pages, slot_mapping, page_size, out_dtype):
+        _cuda_contig(qkv, "qkv")
+        _cuda_contig(positions, "positions", torch.int32)
+        _cuda_contig(table, "rotary table", torch.float32)
+        _need(n_heads > 0 and n_kv_heads > 0 and head_dim > 0 and head_dim % GROUP == 0,
+              f"a 4-bit cache takes heads of a multiple of {GROUP} coordinates, got {n_heads}, {n_kv_heads} heads of {head_dim}")
+        _need(qkv.dim() in (2, 3) and qkv.shape[-1] == (n_heads + 2 * n_kv_heads) * head_dim and qkv.dtype in _DT,
+              "qkv must be [tokens, (n_heads + 2 n_kv_heads) * head_dim]")
+        _need(qkv.dim() == 2 or qkv.shape[0] == 1 or qkv.dtype == torch.float32, "partial sums must be float32")
+        _need(out_dtype in _DT and (out_dtype == qkv.dtype or qkv.dtype == torch.float32), "rope cannot widen bfloat16 input")
+        _need(table.dim() == 3 and 1 <= table.shape[1] <= head_dim // 2 and table.shape[2] == 2,
+              "rotary table must be [positions, pairs, 2] with at most head_dim / 2 pairs")
+        T = qkv.shape[-2]
+        _need(positions.numel() == T, "one position per token")
+        if k_pages is not None or v_pages is not None:
+            _need(k_pages is not None and v_pages is not None and slot_mapping is not None, "k_pages, v_pages and slot_mapping go together")
+            self._fp4_pages_explained(k_pages, v_pages, n_kv_heads, head_dim, page_size)
+            _cuda_contig(slot_mapping, "slot_mapping", torch.int32)
+            _need(slot_mapping.numel() == T, "one cache slot per token")
+        raise KernelError("rope_kv_write_fp4: arguments do not fit together")
 
     @_timed
     def rope_kv_write_fp4(self, qkv, positions: torch.Tensor, table: torch.Tensor, *,
@@ -2054,38 +2107,43 @@ class NativeOps:
         9 * head_dim]`` bytes, :mod:`torchllms_b200.cache.fp4`).  Keys (after rotation) and values become 4-bit numbers
         from their float32 values.  The rotary table may cover the first coordinates of a head only
         (``[positions, rotated / 2, 2]``); the others pass as they are."""
-        rs = qkv if isinstance(qkv, RowScaled) else None
-        if rs is not None:
-            qkv = rs.x
-        _cuda_contig(qkv, "qkv")
-        _cuda_contig(positions, "positions", torch.int32)
-        _cuda_contig(table, "rotary table", torch.float32)
-        splits = qkv.shape[0] if qkv.dim() == 3 else 1
-        T = qkv.shape[-2]
-        out_dtype = out_dtype or qkv.dtype
-        _need(n_heads > 0 and n_kv_heads > 0 and head_dim > 0 and head_dim % GROUP == 0,
-              f"a 4-bit cache takes heads of a multiple of {GROUP} coordinates, got {n_heads}, {n_kv_heads} heads of {head_dim}")
-        _need(qkv.dim() in (2, 3) and qkv.shape[-1] == (n_heads + 2 * n_kv_heads) * head_dim and qkv.dtype in _DT,
-              "qkv must be [tokens, (n_heads + 2 n_kv_heads) * head_dim]")
-        _need(splits == 1 or qkv.dtype == torch.float32, "partial sums must be float32")
-        _need(out_dtype in _DT and (out_dtype == qkv.dtype or qkv.dtype == torch.float32), "rope cannot widen bfloat16 input")
-        _need(table.dim() == 3 and 1 <= table.shape[1] <= head_dim // 2 and table.shape[2] == 2,
-              "rotary table must be [positions, pairs, 2] with at most head_dim / 2 pairs")
-        _need(positions.numel() == T, "one position per token")
+        rs = None
+        if isinstance(qkv, RowScaled):
+            rs, qkv = qkv, qkv.x
+        in_dtype = qkv.dtype
+        out_dtype = out_dtype or in_dtype
+        shape, turns = qkv.shape, table.shape
+        T = shape[-2]
+        splits = shape[0] if len(shape) == 3 else 1
+        writes = k_pages is not None
+        if not (qkv.is_cuda and qkv.is_contiguous() and positions.is_cuda and positions.dtype is torch.int32 and positions.is_contiguous()
+                and table.is_cuda and table.dtype is torch.float32 and table.is_contiguous() and n_heads > 0 and n_kv_heads > 0
+                and len(shape) <= 3 and shape[-1] == (n_heads + 2 * n_kv_heads) * head_dim and head_dim > 0 and head_dim % GROUP == 0
+                and in_dtype in _DT and out_dtype in _DT and (in_dtype is torch.float32 or (out_dtype is in_dtype and splits == 1))
+                and len(turns) == 3 and 1 <= turns[1] <= head_dim // 2 and turns[2] == 2 and positions.numel() == T
+                and (v_pages is None if not writes else
+                     (v_pages is not None and slot_mapping is not None and self._fp4_pages_fit(k_pages, v_pages, n_kv_heads, head_dim, page_size)
+                      and slot_mapping.is_cuda and slot_mapping.dtype is torch.int32 and slot_mapping.is_contiguous()
+                      and slot_mapping.numel() == T))):
+            self._rope_fp4_explained(qkv, positions, table, n_heads, n_kv_heads, head_dim, k_pages, v_pages, slot_mapping, page_size, out_dtype)
         n_pages = 0
-        if k_pages is not None:
-            _need(v_pages is not None and slot_mapping is not None, "k_pages, v_pages and slot_mapping go together")
-            self._fp4_pages(k_pages, v_pages, n_kv_heads, head_dim, page_size)
-            _cuda_contig(slot_mapping, "slot_mapping", torch.int32)
-            _need(slot_mapping.numel() == T, "one cache slot per token")
+        if writes:
             n_pages = k_pages.shape[0]
-            self._debug_limit("kv_fp4", 0, n_pages)
+            if self.debug:
+                self._debug_limit("kv_fp4", 0, n_pages)
         q = torch.empty((T, n_heads, head_dim), dtype=out_dtype, device=qkv.device)
-        rc = self._lib("kv_fp4").tl_rope_kv_write_fp4(
-            _ptr(qkv), _DT[qkv.dtype], splits, _ptr(positions), _ptr(table), _ptr(slot_mapping if k_pages is not None else None),
-            _ptr(q), _ptr(k_pages), _ptr(v_pages if k_pages is not None else None), _DT[out_dtype], T, n_heads, n_kv_heads, head_dim,
-            2 * table.shape[1], page_size, ctypes.c_longlong(n_pages), table.shape[0], 1 if interleaved else 0, *_scale_args(rs, T), _stream())
-        _check(rc, "rope_kv_write_fp4")
+        if rs is None:
+            ssq, parts, inv_dim, eps = 0, 0, 0.0, 0.0
+        else:
+            _scale_args(rs, T)             # (what it refuses)
+            ssq, parts, inv_dim, eps = rs.ssq.data_ptr(), rs.ssq.shape[1], 1.0 / rs.dim, rs.eps
+        rc = self._fp4_call("tl_rope_kv_write_fp4")(
+            qkv.data_ptr(), _DT[in_dtype], splits, positions.data_ptr(), table.data_ptr(), slot_mapping.data_ptr() if writes else 0,
+            q.data_ptr(), k_pages.data_ptr() if writes else 0, v_pages.data_ptr() if writes else 0, _DT[out_dtype], T, n_heads, n_kv_heads,
+            head_dim, 2 * turns[1], page_size if writes else RECORD, n_pages, turns[0], 1 if interleaved else 0, ssq, parts, inv_dim, eps,
+            _stream())
+        if rc:
+            _check(rc, "rope_kv_write_fp4")
         self.launches += 1
         return q
 
@@ -2095,17 +2153,20 @@ class NativeOps:
         """The keys and values that a 4-bit cache holds in the given slots (int32, ``page * page_size + offset``):
         two tensors ``[slots, n_kv_heads, head_dim]``.  Either dtype has every number exactly."""
         _need(k_pages.dim() == 4, "4-bit pages must be [pages, n_kv_heads, page_size / 16, 9 * head_dim] bytes, keys and values alike")
-        KV = k_pages.shape[1]
-        self._fp4_pages(k_pages, v_pages, KV, head_dim, page_size)
-        _cuda_contig(slots, "slots", torch.int32)
-        _need(slots.dim() == 1 and out_dtype in _DT, "kv_read_fp4 takes a vector of slots and writes float32 or bfloat16")
+        n_pages, KV = k_pages.shape[:2]
+        if not self._fp4_pages_fit(k_pages, v_pages, KV, head_dim, page_size):
+            self._fp4_pages_explained(k_pages, v_pages, KV, head_dim, page_size)
+        if not (slots.is_cuda and slots.dtype is torch.int32 and slots.is_contiguous() and slots.dim() == 1 and out_dtype in _DT):
+            _cuda_contig(slots, "slots", torch.int32)
+            _need(False, "kv_read_fp4 takes a vector of slots and writes float32 or bfloat16")
         n = slots.numel()
-        out = torch.empty((2, n, KV, head_dim), dtype=out_dtype, device=slots.device)
-        k, v = out.unbind(0)
-        self._debug_limit("kv_fp4", 0, k_pages.shape[0])
-        rc = self._lib("kv_fp4").tl_kv_read_fp4(_ptr(k_pages), _ptr(v_pages), _ptr(slots), _ptr(k), _ptr(v), _DT[out_dtype], n,
-                                               ctypes.c_longlong(k_pages.shape[0]), KV, head_dim, page_size, _stream())
-        _check(rc, "kv_read_fp4")
+        k, v = torch.empty((2, n, KV, head_dim), dtype=out_dtype, device=slots.device).unbind(0)
+        if self.debug:
+            self._debug_limit("kv_fp4", 0, n_pages)
+        rc = self._fp4_call("tl_kv_read_fp4")(k_pages.data_ptr(), v_pages.data_ptr(), slots.data_ptr(), k.data_ptr(), v.data_ptr(), _DT[out_dtype],
+                                             n, n_pages, KV, head_dim, page_size, _stream())
+        if rc:
+            _check(rc, "kv_read_fp4")
         self.launches += 1
         return k, v
 
@@ -2120,6 +2181,46 @@ class NativeOps:
                 self._fp4_plans.clear()
             plan = self._fp4_plans[dtype, sizes] = (floats.value, counters.value)
         return plan
+
+    def _fp4_prefill_plan(self, *sizes: int) -> Tuple[int, int]:
+        """Pieces that the keys are cut into and floats of scratch of a call of the prefill kernel."""
+        plan = self._fp4_plans.get(sizes)
+        if plan is None:
+            pieces, floats = ctypes.c_int(0), ctypes.c_longlong(0)
+            _check(self._lib("attention_fp4_prefill").tl_attention_fp4_prefill_plan(ctypes.c_longlong(sizes[0]), *sizes[1:], ctypes.byref(pieces),
+                                                                                   ctypes.byref(floats)), "attention_fp4_prefill_plan")
+            if len(self._fp4_plans) >= 4096:
+                self._fp4_plans.clear()
+            plan = self._fp4_plans[sizes] = (pieces.value, floats.value)
+        return plan
+
+    def _attention_fp4_explained(self, q, k_pages, v_pages, block_table, q_start, kv_len, n_seqs, max_kv_len, window, page_size, impl, n_tokens, out):
+        _cuda_contig(q, "q")
+        _need(q.dim() == 3 and q.dtype in _DT, "q must be [tokens, heads, head_dim] in float32 or bfloat16")
+        _cuda_contig(q_start, "q_start", torch.int32)
+        _cuda_contig(kv_len, "kv_len", torch.int32)
+        _need(block_table.is_cuda and block_table.dtype == torch.int32 and block_table.dim() == 2
+              and block_table.stride(1) == 1, "block_table must be an int32 matrix with unit column stride")
+        T, n_heads, head_dim = q.shape
+        _need(k_pages.dim() == 4, "4-bit pages must be [pages, n_kv_heads, page_size / 16, 9 * head_dim] bytes, keys and values alike")
+        n_kv_heads = k_pages.shape[1]
+        self._fp4_pages_explained(k_pages, v_pages, n_kv_heads, head_dim, page_size)
+        _need(n_heads > 0 and n_kv_heads > 0 and n_heads % n_kv_heads == 0,
+              f"n_heads ({n_heads}) must be a positive multiple of n_kv_heads ({n_kv_heads})")
+        _need(n_tokens is None or 0 < n_tokens <= T, "n_tokens must lie within q")
+        if out is not None:
+            _cuda_contig(out, "out", q.dtype)
+            _need(out.shape == q.shape, "out must have q's shape")
+        _need(window is None or window > 0, "a window holds at least one key")
+        _need(block_table.shape[0] >= n_seqs and q_start.numel() >= n_seqs + 1 and kv_len.numel() >= n_seqs,
+              "block_table, q_start and kv_len must cover every request of the step")
+        _need(block_table.shape[1] * page_size >= max_kv_len, "block_table is too narrow for max_kv_len")
+        _need(impl in self._FP4_IMPLS, f"unknown attention implementation {impl!r}")
+        _need(impl not in ("decode", "prefill") or head_dim in (64, 128), "the tensor-core kernels of the 4-bit cache take head_dim 64 or 128")
+        _need(impl != "prefill" or q.dtype == torch.bfloat16, "the tcgen05 kernel of the 4-bit cache takes bfloat16")
+        raise KernelError("paged_attention_fp4: arguments do not fit together")
+
+    _FP4_IMPLS = ("auto", "general", "decode", "prefill")
 
     @_timed
     def paged_attention_fp4(self, q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -2136,68 +2237,56 @@ class NativeOps:
         ``"decode"`` (mma.sync tensor cores, head_dim 64 and 128), ``"prefill"`` (tcgen05 tensor cores, head_dim 64 and 128,
         bfloat16, made for many tokens) or ``"auto"`` (the most specialised kernel that applies).  ``allow_split`` (of the
         prefill kernel): False keeps every row's keys in one CTA, a number above 1 cuts them into so many pieces."""
-        _cuda_contig(q, "q")
-        _need(q.dim() == 3 and q.dtype in _DT, "q must be [tokens, heads, head_dim] in float32 or bfloat16")
-        _cuda_contig(q_start, "q_start", torch.int32)
-        _cuda_contig(kv_len, "kv_len", torch.int32)
-        _need(block_table.is_cuda and block_table.dtype == torch.int32 and block_table.dim() == 2
-              and block_table.stride(1) == 1, "block_table must be an int32 matrix with unit column stride")
-        T, n_heads, head_dim = q.shape
-        _need(k_pages.dim() == 4, "4-bit pages must be [pages, n_kv_heads, page_size / 16, 9 * head_dim] bytes, keys and values alike")
-        n_kv_heads = k_pages.shape[1]
-        self._fp4_pages(k_pages, v_pages, n_kv_heads, head_dim, page_size)
-        _need(n_heads > 0 and n_kv_heads > 0 and n_heads % n_kv_heads == 0,
-              f"n_heads ({n_heads}) must be a positive multiple of n_kv_heads ({n_kv_heads})")
-        if n_tokens is not None:
-            _need(0 < n_tokens <= T, "n_tokens must lie within q")
-            T = int(n_tokens)
+        dtype, shape, columns = q.dtype, q.shape, block_table.shape
+        n_heads, head_dim = shape[-2:] if len(shape) == 3 else (0, 0)
+        n_kv_heads = k_pages.shape[1] if k_pages.dim() == 4 else 0
+        if not (dtype in _DT and n_heads and n_kv_heads and n_heads % n_kv_heads == 0 and q.is_cuda and q.is_contiguous()
+                and self._fp4_pages_fit(k_pages, v_pages, n_kv_heads, head_dim, page_size)
+                and q_start.dtype is torch.int32 and kv_len.dtype is torch.int32 and block_table.dtype is torch.int32 and q_start.is_cuda
+                and kv_len.is_cuda and block_table.is_cuda and q_start.is_contiguous() and kv_len.is_contiguous() and len(columns) == 2
+                and block_table.stride(1) == 1 and columns[0] >= n_seqs and columns[1] * page_size >= max_kv_len
+                and q_start.numel() > n_seqs and kv_len.numel() >= n_seqs and (window is None or window > 0)
+                and (n_tokens is None or 0 < n_tokens <= shape[0]) and impl in self._FP4_IMPLS
+                and (impl == "auto" or impl == "general" or (head_dim in (64, 128) and (impl == "decode" or dtype is torch.bfloat16)))
+                and (out is None or (out.is_cuda and out.dtype is dtype and out.is_contiguous() and out.shape == shape))):
+            self._attention_fp4_explained(q, k_pages, v_pages, block_table, q_start, kv_len, n_seqs, max_kv_len, window, page_size, impl, n_tokens, out)
         if out is None:
             out = torch.empty_like(q)
-        else:
-            _cuda_contig(out, "out", q.dtype)
-            _need(out.shape == q.shape, "out must have q's shape")
-        _need(window is None or window > 0, "a window holds at least one key")
-        _need(block_table.shape[0] >= n_seqs and q_start.numel() >= n_seqs + 1 and kv_len.numel() >= n_seqs,
-              "block_table, q_start and kv_len must cover every request of the step")
-        _need(block_table.shape[1] * page_size >= max_kv_len, "block_table is too narrow for max_kv_len")
-        _need(impl in ("auto", "general", "decode", "prefill"), f"unknown attention implementation {impl!r}")
-        decode_ok = head_dim in (64, 128)
-        _need(impl not in ("decode", "prefill") or decode_ok, "the tensor-core kernels of the 4-bit cache take head_dim 64 or 128")
-        _need(impl != "prefill" or q.dtype == torch.bfloat16, "the tcgen05 kernel of the 4-bit cache takes bfloat16")
-        if impl == "prefill" or (impl == "auto" and decode_ok and q.dtype == torch.bfloat16
-                                 and max_q_len * (n_heads // n_kv_heads) >= self.FP4_PREFILL_MIN_ROWS):
-            lib = self._lib("attention_fp4_prefill")
-            pieces, floats = ctypes.c_int(0), ctypes.c_longlong(0)
-            _check(lib.tl_attention_fp4_prefill_plan(ctypes.c_longlong(q.shape[0]), n_seqs, n_heads, n_kv_heads, head_dim, max_q_len, max_kv_len,
-                                                     int(allow_split), ctypes.byref(pieces), ctypes.byref(floats)), "attention_fp4_prefill_plan")
-            ws = self._scratch(q.device, floats.value)
-            self._debug_limit("attention_fp4_prefill", 0, k_pages.shape[0])
-            rc = lib.tl_attention_fp4_prefill(
-                _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(out), _ptr(block_table), block_table.stride(0), block_table.shape[1],
-                _ptr(q_start), _ptr(kv_len), _ptr(ws), ctypes.c_void_p(self._status.data_ptr()), ctypes.c_longlong(q.shape[0]), n_seqs,
-                n_heads, n_kv_heads, head_dim, page_size, ctypes.c_longlong(k_pages.shape[0]), max_q_len, int(window or 0),
-                ctypes.c_float(scale), pieces, _stream())
-            _check(rc, "paged_attention_fp4")
-            self.launches += 1 if pieces.value == 1 else 2
-            return out
-        if decode_ok and impl != "general":
-            floats, counters = self._fp4_decode_plan(q.dtype, n_seqs, n_heads, n_kv_heads, head_dim, page_size, max_q_len, max_kv_len)
+        if impl == "auto":
+            if head_dim != 64 and head_dim != 128:
+                impl = "general"
+            elif dtype is torch.bfloat16 and max_q_len * (n_heads // n_kv_heads) >= self.FP4_PREFILL_MIN_ROWS:
+                impl = "prefill"
+            else:
+                impl = "decode"
+        n_pages = k_pages.shape[0]
+        tensors = (q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), block_table.data_ptr(), block_table.stride(0), columns[1],
+                   q_start.data_ptr(), kv_len.data_ptr())
+        if impl == "decode":
+            floats, counters = self._fp4_decode_plan(dtype, n_seqs, n_heads, n_kv_heads, head_dim, page_size, max_q_len, max_kv_len)
             ws = torch.empty(floats, dtype=torch.float32, device=q.device)
-            self._debug_limit("attention_fp4_decode", 0, k_pages.shape[0])
-            rc = self._lib("attention_fp4_decode").tl_attention_fp4_decode(
-                _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(out), _ptr(block_table), block_table.stride(0), block_table.shape[1],
-                _ptr(q_start), _ptr(kv_len), _ptr(ws), _ptr(self._counters(q.device, counters)), ctypes.c_void_p(self._status.data_ptr()),
-                _DT[q.dtype], n_seqs, n_heads, n_kv_heads, head_dim, page_size, ctypes.c_longlong(k_pages.shape[0]), max_q_len, max_kv_len,
-                int(window or 0), ctypes.c_float(scale), _stream())
+            if self.debug:
+                self._debug_limit("attention_fp4_decode", 0, n_pages)
+            rc = self._fp4_call("tl_attention_fp4_decode")(
+                *tensors, ws.data_ptr(), self._counters(q.device, counters).data_ptr(), self._status_ptr, _DT[dtype], n_seqs, n_heads, n_kv_heads,
+                head_dim, page_size, n_pages, max_q_len, max_kv_len, window or 0, scale, _stream())
+        elif impl == "prefill":
+            pieces, floats = self._fp4_prefill_plan(shape[0], n_seqs, n_heads, n_kv_heads, head_dim, max_q_len, max_kv_len, int(allow_split))
+            ws = self._scratch(q.device, floats)
+            if self.debug:
+                self._debug_limit("attention_fp4_prefill", 0, n_pages)
+            rc = self._fp4_call("tl_attention_fp4_prefill")(
+                *tensors, 0 if ws is None else ws.data_ptr(), self._status_ptr, shape[0], n_seqs, n_heads, n_kv_heads, head_dim, page_size, n_pages,
+                max_q_len, window or 0, scale, pieces, _stream())
+            if pieces > 1:
+                self.launches += 1
+        else:
+            if self.debug:
+                self._debug_limit("attention_fp4", 0, n_pages)
+            rc = self._fp4_call("tl_attention_fp4_general")(
+                *tensors, _DT[dtype], n_seqs, n_heads, n_kv_heads, head_dim, page_size, n_pages, max_q_len, window or 0, scale, _stream())
+        if rc:
             _check(rc, "paged_attention_fp4")
-            self.launches += 1
-            return out
-        self._debug_limit("attention_fp4", 0, k_pages.shape[0])
-        rc = self._lib("attention_fp4").tl_attention_fp4_general(
-            _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(out), _ptr(block_table), block_table.stride(0), block_table.shape[1],
-            _ptr(q_start), _ptr(kv_len), _DT[q.dtype], n_seqs, n_heads, n_kv_heads, head_dim, page_size,
-            ctypes.c_longlong(k_pages.shape[0]), max_q_len, int(window or 0), ctypes.c_float(scale), _stream())
-        _check(rc, "paged_attention_fp4")
         self.launches += 1
         return out
 

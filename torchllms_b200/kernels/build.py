@@ -13,10 +13,13 @@ from __future__ import annotations
 
 import ctypes
 import hashlib
+import importlib.machinery
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 import tempfile
 import threading
 import time
@@ -42,7 +45,12 @@ NVCC_FLAGS += os.environ.get("TORCHLLMS_B200_NVCC_FLAGS", "").split()
 EXTRA_LINK: Dict[str, List[str]] = {}
 
 ALL_LIBRARIES = ("elementwise", "sublayer", "rope", "attention", "attention_mma", "attention_decode", "attention_prefill", "gemm_simt", "gemm_f32", "gemm_tcgen05", "sampling", "recurrent", "moe", "matrix_state", "stream_sum", "selective_scan", "conv_mixers", "matrix_recurrence",
-                 "kv_fp4", "attention_fp4", "attention_fp4_decode", "attention_fp4_prefill")
+                 "kv_fp4", "attention_fp4", "attention_fp4_decode", "attention_fp4_prefill", "fp4_calls")
+
+
+# Python modules (``csrc/<name>.cpp``, compiled with the host compiler against this Python's and this torch's headers): front ends of
+# operators whose calls cost more than their kernels
+EXTENSIONS = ("fp4_calls",)
 
 
 class KernelBuildError(RuntimeError):
@@ -51,6 +59,7 @@ class KernelBuildError(RuntimeError):
 
 _lock = threading.Lock()
 _loaded: Dict[str, ctypes.CDLL] = {}
+_extensions: Dict[str, object] = {}
 
 
 def _say(msg: str) -> None:
@@ -78,8 +87,26 @@ def _headers() -> List[Path]:
     return sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h"))
 
 
+def _extension_command(src: Path, out: Path) -> List[str]:
+    import torch
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(find_nvcc()).resolve().parent.parent
+    compiler = os.environ.get("CXX") or shutil.which("g++") or shutil.which("c++")
+    if not compiler:
+        raise KernelBuildError("no C++ compiler was found (looked at $CXX, g++ and c++)")
+    include = [sysconfig.get_paths()["include"], root / "include", root / "include" / "torch" / "csrc" / "api" / "include", cuda / "include"]
+    return [compiler, "-O2", "-std=c++17", "-shared", "-fPIC", "-w", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            *(f"-I{p}" for p in include), str(src), "-o", str(out), f"-L{root / 'lib'}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda",
+            "-lc10", "-lc10_cuda", f"-L{cuda / 'lib64'}", "-lcudart"]
+
+
 def _digest(name: str) -> str:
     h = hashlib.sha256()
+    if name in EXTENSIONS:
+        import torch
+        h.update(f"{torch.__version__} {sys.version} {torch._C._GLIBCXX_USE_CXX11_ABI}".encode())
+        h.update((CSRC / f"{name}.cpp").read_bytes())
+        return h.hexdigest()[:16]
     h.update(" ".join(NVCC_FLAGS + EXTRA_LINK.get(name, [])).encode())
     for p in [CSRC / f"{name}.cu"] + _headers():
         h.update(p.name.encode())
@@ -121,7 +148,7 @@ def library_path(name: str) -> Optional[Path]:
 
 
 def compile_library(name: str) -> Path:
-    src = CSRC / f"{name}.cu"
+    src = CSRC / (f"{name}.cpp" if name in EXTENSIONS else f"{name}.cu")
     if not src.is_file():
         raise KernelBuildError(f"no kernel source {src}")
     existing = library_path(name)
@@ -130,8 +157,11 @@ def compile_library(name: str) -> Path:
     out_dir = _writable_dir()
     out = out_dir / f"{name}.{_digest(name)}.so"
     tmp = out_dir / f".{out.name}.{os.getpid()}.{threading.get_ident()}.tmp"
-    cmd = [find_nvcc(), *NVCC_FLAGS, "-I", str(CSRC), str(src), "-o", str(tmp), *EXTRA_LINK.get(name, [])]
-    _say(f"compiling {src.name} for sm_100a ...")
+    if name in EXTENSIONS:
+        cmd = _extension_command(src, tmp)
+    else:
+        cmd = [find_nvcc(), *NVCC_FLAGS, "-I", str(CSRC), str(src), "-o", str(tmp), *EXTRA_LINK.get(name, [])]
+    _say(f"compiling {src.name}" + ("" if name in EXTENSIONS else " for sm_100a") + " ...")
     t0 = time.time()
     env = dict(os.environ)
     env.setdefault("TMPDIR", tempfile.gettempdir())
@@ -150,7 +180,7 @@ def compile_library(name: str) -> Path:
             tmp.unlink()
         except OSError:
             pass
-        raise KernelBuildError(f"nvcc failed on {src.name} (exit {proc.returncode}):\n{output}")
+        raise KernelBuildError(f"{Path(cmd[0]).name} failed on {src.name} (exit {proc.returncode}):\n{output}")
     os.replace(tmp, out)
     for stale in out_dir.glob(f"{name}.*.so"):        # libraries of earlier versions of this source
         if stale != out:
@@ -177,6 +207,25 @@ def load_library(name: str) -> ctypes.CDLL:
                 raise KernelBuildError(f"could not load {path}: {e}") from None
             _loaded[name] = lib
     return lib
+
+
+def load_extension(name: str):
+    """The Python module of ``csrc/<name>.cpp``, compiled first if need be."""
+    module = _extensions.get(name)
+    if module is None:
+        with _lock:
+            module = _extensions.get(name)
+            if module is None:
+                path = compile_library(name)
+                loader = importlib.machinery.ExtensionFileLoader(name, str(path))
+                spec = importlib.util.spec_from_loader(name, loader)
+                try:
+                    module = importlib.util.module_from_spec(spec)
+                    loader.exec_module(module)
+                except ImportError as e:
+                    raise KernelBuildError(f"could not load {path}: {e}") from None
+                _extensions[name] = module
+    return module
 
 
 def build_libraries(names: Iterable[str] = ALL_LIBRARIES, jobs: Optional[int] = None) -> List[Path]:

@@ -17,7 +17,7 @@ from typing import Dict, Optional, Tuple
 import torch
 
 from ..cache.fp4 import GROUP, MAX_HEAD_DIM, RECORD, record_bytes
-from .build import ALL_LIBRARIES, build_libraries, load_library
+from .build import ALL_LIBRARIES, build_libraries, load_extension, load_library
 from .lazy import PendingProduct, RowScaled
 
 _DT = {torch.float32: 0, torch.bfloat16: 1}
@@ -102,6 +102,15 @@ def _timed(fn):
     return wrapper
 
 
+_lean = []
+
+
+def _timed_when_asked(fn):
+    """As :func:`_timed`, for methods whose callers wait for the host: the wrapper is put in front while a profile is being taken only."""
+    _lean.append(fn)
+    return fn
+
+
 class NativeOps:
     """The kernels as methods.  Libraries are compiled and loaded on first use."""
 
@@ -122,14 +131,12 @@ class NativeOps:
         self.launches = 0          # kernels of this library launched so far (a bench counts with it)
         # (device, stream, inside a capture) -> ints that are zero between launches, and the capture they belong to
         self._counts: Dict[Tuple[int, int, bool], Tuple[int, torch.Tensor]] = {}
-        self._fp4_plans: Dict[tuple, Tuple[int, int]] = {}
-        self._fp4_calls: Dict[str, object] = {}
+        self._fp4 = None           # the front end of the 4-bit cache's operators, once it is loaded
         self.use_tcgen05 = True
         # SwiGLU in the epilogue of the gate/up product (TORCHLLMS_B200_NO_GATED=1 keeps the two kernels, for comparisons)
         self.use_gated = os.environ.get("TORCHLLMS_B200_NO_GATED", "") not in ("1", "true")
         # error word of kernels with bounded waits: pinned host memory the device writes to directly
         self._status = torch.zeros(4, dtype=torch.int32).pin_memory()
-        self._status_ptr = self._status.data_ptr()
         self._mm_out_dtype: Optional[bool] = None
         self._profile = None
         self._profile_depth = 0
@@ -165,7 +172,7 @@ class NativeOps:
         if dtype == torch.bfloat16:
             names += ["attention_mma", "attention_decode", "gemm_tcgen05"]
         if kv_format == "fp4":
-            names += ["kv_fp4", "attention_fp4", "attention_fp4_decode", "attention_fp4_prefill", "attention_decode"]
+            names += ["kv_fp4", "attention_fp4", "attention_fp4_decode", "attention_fp4_prefill", "fp4_calls"]
         if sampling:
             names.append("sampling")
         build_libraries(names)
@@ -179,10 +186,14 @@ class NativeOps:
         that is filled when the block ends (the stream is synchronised then)."""
         result: Dict[str, list] = {}
         self._profile = []
+        for fn in _lean:
+            setattr(self, fn.__name__, _timed(fn).__get__(self))
         try:
             yield result
         finally:
             records, self._profile = self._profile, None
+            for fn in _lean:
+                delattr(self, fn.__name__)
             torch.cuda.synchronize()
             inner: Dict[int, float] = {}            # time of finished calls by depth, not yet taken off their caller
             for name, a, b, depth in records:       # (a call made inside another finishes, and is listed, first)
@@ -1643,6 +1654,8 @@ class NativeOps:
             for capture, counts in list(self._counts.values()):
                 if not capture:
                     counts.zero_()               # (whatever happened, the next call counts from zero; a graph's replay does so itself)
+            if self._fp4 is not None:
+                self._fp4.reset()
             torch.cuda.synchronize()
             raise KernelError(f"a kernel gave up waiting (code {code}); its output is not valid")
         if self.debug:
@@ -1768,8 +1781,7 @@ class NativeOps:
         if n <= 0:
             return None
         stream, capture = _stream(), ctypes.c_ulonglong(0)
-        if torch.cuda.is_current_stream_capturing():
-            _check(self._lib("attention_decode").tl_stream_capture_id(stream, ctypes.byref(capture)), "stream_capture_id")
+        _check(self._lib("attention_decode").tl_stream_capture_id(stream, ctypes.byref(capture)), "stream_capture_id")
         key = (device.index or 0, stream.value or 0, capture.value != 0)
         of, buf = self._counts.get(key, (0, None))
         if buf is None or of != capture.value or buf.numel() < n:
@@ -2036,26 +2048,23 @@ class NativeOps:
         return out
 
     # ------------------------------------------------------------- keys and values in 4 bits
-    # These run once a layer and step, and a step of few tokens takes the device less time than the host needs for a call.  So a call
-    # looks its arguments over in one expression, and only one that does not pass is taken apart to say what is wrong.
-    _FP4_ARGS = {
-        "tl_rope_kv_write_fp4": ("kv_fp4", "piippppppiiiiiiiliipiffp"),
-        "tl_kv_read_fp4": ("kv_fp4", "pppppiiliiip"),
-        "tl_attention_fp4_general": ("attention_fp4", "ppppp" "iippiiiiiiliifp"),
-        "tl_attention_fp4_decode": ("attention_fp4_decode", "ppppp" "iippppp" "iiiiii" "liii" "fp"),
-        "tl_attention_fp4_prefill": ("attention_fp4_prefill", "ppppp" "iippppl" "iiiii" "lii" "fip"),
-    }
-    _FP4_TYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float}
+    # These run once a layer and step, and a step of few tokens takes the device less time than a front end in Python needs for a call: theirs
+    # is csrc/fp4_calls.cpp.  It returns None for arguments that do not fit, and the methods named _explained say what is wrong.
+    _FP4_CODES = {None: -1, torch.float32: 0, torch.bfloat16: 1}
+    _FP4_IMPLS = {"auto": 0, "general": 1, "decode": 2, "prefill": 3}
 
-    def _fp4_call(self, name: str):
-        """A kernel's entry point, told its arguments' types (numbers then go through without objects around them)."""
-        fn = self._fp4_calls.get(name)
-        if fn is None:
-            lib, types = self._FP4_ARGS[name]
-            fn = getattr(self._lib(lib), name)
-            fn.argtypes = [self._FP4_TYPES[t] for t in types]
-            self._fp4_calls[name] = fn
-        return fn
+    def _fp4_load(self):
+        calls = load_extension("fp4_calls")
+        names = (("kv_fp4", "tl_rope_kv_write_fp4"), ("kv_fp4", "tl_kv_read_fp4"), ("attention_fp4", "tl_attention_fp4_general"),
+                 ("attention_fp4_decode", "tl_attention_fp4_decode"), ("attention_fp4_decode", "tl_attention_fp4_decode_plan"),
+                 ("attention_fp4_prefill", "tl_attention_fp4_prefill"), ("attention_fp4_prefill", "tl_attention_fp4_prefill_plan"))
+        calls.bind(*(ctypes.cast(getattr(self._lib(lib), name), ctypes.c_void_p).value for lib, name in names), self._status.data_ptr())
+        self._fp4 = calls
+        return calls
+
+    def _fp4_debug(self, n_pages: int) -> None:
+        for lib in ("kv_fp4", "attention_fp4", "attention_fp4_decode", "attention_fp4_prefill"):
+            self._debug_limit(lib, 0, n_pages)
 
     @staticmethod
     def _fp4_pages_explained(k_pages, v_pages, n_kv_heads: int, head_dim: int, page_size: int) -> None:
@@ -2067,14 +2076,6 @@ class NativeOps:
         _need(k_pages.shape == v_pages.shape and k_pages.dim() == 4
               and k_pages.shape[1:] == (n_kv_heads, page_size // RECORD, record_bytes(head_dim)) and k_pages.shape[0] > 0,
               "4-bit pages must be [pages, n_kv_heads, page_size / 16, 9 * head_dim] bytes, keys and values alike")
-
-    @staticmethod
-    def _fp4_pages_fit(k_pages, v_pages, n_kv_heads: int, head_dim: int, page_size: int) -> bool:
-        shape = k_pages.shape
-        return (k_pages.dtype is torch.uint8 and v_pages.dtype is torch.uint8 and k_pages.is_cuda and v_pages.is_cuda
-                and len(shape) == 4 and shape == v_pages.shape and shape[1] == n_kv_heads and page_size > 0 and head_dim > 0
-                and shape[2] * RECORD == page_size and shape[3] == 9 * head_dim and shape[0] > 0 and head_dim % GROUP == 0
-                and head_dim <= MAX_HEAD_DIM and k_pages.is_contiguous() and v_pages.is_contiguous())
 
     def _rope_fp4_explained(self, qkv, positions, table, n_heads, n_kv_heads, head_dim, k_pages, v_pages, slot_mapping, page_size, out_dtype):
         _cuda_contig(qkv, "qkv")
@@ -2097,7 +2098,7 @@ class NativeOps:
             _need(slot_mapping.numel() == T, "one cache slot per token")
         raise KernelError("rope_kv_write_fp4: arguments do not fit together")
 
-    @_timed
+    @_timed_when_asked
     def rope_kv_write_fp4(self, qkv, positions: torch.Tensor, table: torch.Tensor, *,
                           n_heads: int, n_kv_heads: int, head_dim: int, interleaved: bool,
                           k_pages: Optional[torch.Tensor], v_pages: Optional[torch.Tensor],
@@ -2107,92 +2108,41 @@ class NativeOps:
         9 * head_dim]`` bytes, :mod:`torchllms_b200.cache.fp4`).  Keys (after rotation) and values become 4-bit numbers
         from their float32 values.  The rotary table may cover the first coordinates of a head only
         (``[positions, rotated / 2, 2]``); the others pass as they are."""
-        rs = None
+        ssq, inv_dim, eps = None, 0.0, 0.0
         if isinstance(qkv, RowScaled):
-            rs, qkv = qkv, qkv.x
-        in_dtype = qkv.dtype
-        out_dtype = out_dtype or in_dtype
-        shape, turns = qkv.shape, table.shape
-        T = shape[-2]
-        splits = shape[0] if len(shape) == 3 else 1
-        writes = k_pages is not None
-        if not (qkv.is_cuda and qkv.is_contiguous() and positions.is_cuda and positions.dtype is torch.int32 and positions.is_contiguous()
-                and table.is_cuda and table.dtype is torch.float32 and table.is_contiguous() and n_heads > 0 and n_kv_heads > 0
-                and len(shape) <= 3 and shape[-1] == (n_heads + 2 * n_kv_heads) * head_dim and head_dim > 0 and head_dim % GROUP == 0
-                and in_dtype in _DT and out_dtype in _DT and (in_dtype is torch.float32 or (out_dtype is in_dtype and splits == 1))
-                and len(turns) == 3 and 1 <= turns[1] <= head_dim // 2 and turns[2] == 2 and positions.numel() == T
-                and (v_pages is None if not writes else
-                     (v_pages is not None and slot_mapping is not None and self._fp4_pages_fit(k_pages, v_pages, n_kv_heads, head_dim, page_size)
-                      and slot_mapping.is_cuda and slot_mapping.dtype is torch.int32 and slot_mapping.is_contiguous()
-                      and slot_mapping.numel() == T))):
-            self._rope_fp4_explained(qkv, positions, table, n_heads, n_kv_heads, head_dim, k_pages, v_pages, slot_mapping, page_size, out_dtype)
-        n_pages = 0
-        if writes:
-            n_pages = k_pages.shape[0]
-            if self.debug:
-                self._debug_limit("kv_fp4", 0, n_pages)
-        q = torch.empty((T, n_heads, head_dim), dtype=out_dtype, device=qkv.device)
-        if rs is None:
-            ssq, parts, inv_dim, eps = 0, 0, 0.0, 0.0
-        else:
-            _scale_args(rs, T)             # (what it refuses)
-            ssq, parts, inv_dim, eps = rs.ssq.data_ptr(), rs.ssq.shape[1], 1.0 / rs.dim, rs.eps
-        rc = self._fp4_call("tl_rope_kv_write_fp4")(
-            qkv.data_ptr(), _DT[in_dtype], splits, positions.data_ptr(), table.data_ptr(), slot_mapping.data_ptr() if writes else 0,
-            q.data_ptr(), k_pages.data_ptr() if writes else 0, v_pages.data_ptr() if writes else 0, _DT[out_dtype], T, n_heads, n_kv_heads,
-            head_dim, 2 * turns[1], page_size if writes else RECORD, n_pages, turns[0], 1 if interleaved else 0, ssq, parts, inv_dim, eps,
-            _stream())
-        if rc:
-            _check(rc, "rope_kv_write_fp4")
+            _scale_args(qkv, qkv.x.shape[-2])             # (what it refuses)
+            ssq, inv_dim, eps, qkv = qkv.ssq, 1.0 / qkv.dim, qkv.eps, qkv.x
+        calls = self._fp4 or self._fp4_load()
+        if self.debug and k_pages is not None:
+            self._fp4_debug(k_pages.shape[0])
+        q = calls.write(qkv, positions, table, n_heads, n_kv_heads, head_dim, interleaved, k_pages, v_pages, slot_mapping, page_size,
+                        self._FP4_CODES.get(out_dtype, 9), ssq, inv_dim, eps)
+        if q is None:
+            self._rope_fp4_explained(qkv, positions, table, n_heads, n_kv_heads, head_dim, k_pages, v_pages, slot_mapping, page_size,
+                                     out_dtype or qkv.dtype)
+        if q.__class__ is int:
+            _check(q, "rope_kv_write_fp4")
         self.launches += 1
         return q
 
-    @_timed
+    @_timed_when_asked
     def kv_read_fp4(self, k_pages: torch.Tensor, v_pages: torch.Tensor, slots: torch.Tensor, *, head_dim: int, page_size: int,
                     out_dtype: torch.dtype = torch.float32) -> Tuple[torch.Tensor, torch.Tensor]:
         """The keys and values that a 4-bit cache holds in the given slots (int32, ``page * page_size + offset``):
         two tensors ``[slots, n_kv_heads, head_dim]``.  Either dtype has every number exactly."""
-        _need(k_pages.dim() == 4, "4-bit pages must be [pages, n_kv_heads, page_size / 16, 9 * head_dim] bytes, keys and values alike")
-        n_pages, KV = k_pages.shape[:2]
-        if not self._fp4_pages_fit(k_pages, v_pages, KV, head_dim, page_size):
-            self._fp4_pages_explained(k_pages, v_pages, KV, head_dim, page_size)
-        if not (slots.is_cuda and slots.dtype is torch.int32 and slots.is_contiguous() and slots.dim() == 1 and out_dtype in _DT):
-            _cuda_contig(slots, "slots", torch.int32)
-            _need(False, "kv_read_fp4 takes a vector of slots and writes float32 or bfloat16")
-        n = slots.numel()
-        k, v = torch.empty((2, n, KV, head_dim), dtype=out_dtype, device=slots.device).unbind(0)
+        calls = self._fp4 or self._fp4_load()
         if self.debug:
-            self._debug_limit("kv_fp4", 0, n_pages)
-        rc = self._fp4_call("tl_kv_read_fp4")(k_pages.data_ptr(), v_pages.data_ptr(), slots.data_ptr(), k.data_ptr(), v.data_ptr(), _DT[out_dtype],
-                                             n, n_pages, KV, head_dim, page_size, _stream())
-        if rc:
-            _check(rc, "kv_read_fp4")
+            self._fp4_debug(k_pages.shape[0])
+        got = calls.read(k_pages, v_pages, slots, head_dim, page_size, self._FP4_CODES.get(out_dtype, 9))
+        if got is None:
+            _need(k_pages.dim() == 4, "4-bit pages must be [pages, n_kv_heads, page_size / 16, 9 * head_dim] bytes, keys and values alike")
+            self._fp4_pages_explained(k_pages, v_pages, k_pages.shape[1], head_dim, page_size)
+            _cuda_contig(slots, "slots", torch.int32)
+            raise KernelError("kv_read_fp4 takes a vector of slots and writes float32 or bfloat16")
+        if got.__class__ is int:
+            _check(got, "kv_read_fp4")
         self.launches += 1
-        return k, v
-
-    def _fp4_decode_plan(self, dtype: torch.dtype, *sizes: int) -> Tuple[int, int]:
-        """Floats of scratch and counters of a call of the decode kernel; the same sizes come back every layer."""
-        plan = self._fp4_plans.get((dtype, sizes))
-        if plan is None:
-            floats, counters = ctypes.c_longlong(0), ctypes.c_longlong(0)
-            _check(self._lib("attention_fp4_decode").tl_attention_fp4_decode_plan(_DT[dtype], *sizes, ctypes.byref(floats), ctypes.byref(counters)),
-                   "attention_fp4_decode_plan")
-            if len(self._fp4_plans) >= 4096:
-                self._fp4_plans.clear()
-            plan = self._fp4_plans[dtype, sizes] = (floats.value, counters.value)
-        return plan
-
-    def _fp4_prefill_plan(self, *sizes: int) -> Tuple[int, int]:
-        """Pieces that the keys are cut into and floats of scratch of a call of the prefill kernel."""
-        plan = self._fp4_plans.get(sizes)
-        if plan is None:
-            pieces, floats = ctypes.c_int(0), ctypes.c_longlong(0)
-            _check(self._lib("attention_fp4_prefill").tl_attention_fp4_prefill_plan(ctypes.c_longlong(sizes[0]), *sizes[1:], ctypes.byref(pieces),
-                                                                                   ctypes.byref(floats)), "attention_fp4_prefill_plan")
-            if len(self._fp4_plans) >= 4096:
-                self._fp4_plans.clear()
-            plan = self._fp4_plans[sizes] = (pieces.value, floats.value)
-        return plan
+        return got
 
     def _attention_fp4_explained(self, q, k_pages, v_pages, block_table, q_start, kv_len, n_seqs, max_kv_len, window, page_size, impl, n_tokens, out):
         _cuda_contig(q, "q")
@@ -2220,9 +2170,7 @@ class NativeOps:
         _need(impl != "prefill" or q.dtype == torch.bfloat16, "the tcgen05 kernel of the 4-bit cache takes bfloat16")
         raise KernelError("paged_attention_fp4: arguments do not fit together")
 
-    _FP4_IMPLS = ("auto", "general", "decode", "prefill")
-
-    @_timed
+    @_timed_when_asked
     def paged_attention_fp4(self, q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                             block_table: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor, *,
                             n_seqs: int, max_q_len: int, max_kv_len: int, scale: float,
@@ -2237,58 +2185,17 @@ class NativeOps:
         ``"decode"`` (mma.sync tensor cores, head_dim 64 and 128), ``"prefill"`` (tcgen05 tensor cores, head_dim 64 and 128,
         bfloat16, made for many tokens) or ``"auto"`` (the most specialised kernel that applies).  ``allow_split`` (of the
         prefill kernel): False keeps every row's keys in one CTA, a number above 1 cuts them into so many pieces."""
-        dtype, shape, columns = q.dtype, q.shape, block_table.shape
-        n_heads, head_dim = shape[-2:] if len(shape) == 3 else (0, 0)
-        n_kv_heads = k_pages.shape[1] if k_pages.dim() == 4 else 0
-        if not (dtype in _DT and n_heads and n_kv_heads and n_heads % n_kv_heads == 0 and q.is_cuda and q.is_contiguous()
-                and self._fp4_pages_fit(k_pages, v_pages, n_kv_heads, head_dim, page_size)
-                and q_start.dtype is torch.int32 and kv_len.dtype is torch.int32 and block_table.dtype is torch.int32 and q_start.is_cuda
-                and kv_len.is_cuda and block_table.is_cuda and q_start.is_contiguous() and kv_len.is_contiguous() and len(columns) == 2
-                and block_table.stride(1) == 1 and columns[0] >= n_seqs and columns[1] * page_size >= max_kv_len
-                and q_start.numel() > n_seqs and kv_len.numel() >= n_seqs and (window is None or window > 0)
-                and (n_tokens is None or 0 < n_tokens <= shape[0]) and impl in self._FP4_IMPLS
-                and (impl == "auto" or impl == "general" or (head_dim in (64, 128) and (impl == "decode" or dtype is torch.bfloat16)))
-                and (out is None or (out.is_cuda and out.dtype is dtype and out.is_contiguous() and out.shape == shape))):
+        calls = self._fp4 or self._fp4_load()
+        if self.debug:
+            self._fp4_debug(k_pages.shape[0])
+        got = calls.attend(q, k_pages, v_pages, block_table, q_start, kv_len, n_seqs, max_q_len, max_kv_len, scale, window, page_size,
+                           allow_split, self._FP4_IMPLS.get(impl, -1), n_tokens, out, self.FP4_PREFILL_MIN_ROWS)
+        if got is None:
             self._attention_fp4_explained(q, k_pages, v_pages, block_table, q_start, kv_len, n_seqs, max_kv_len, window, page_size, impl, n_tokens, out)
-        if out is None:
-            out = torch.empty_like(q)
-        if impl == "auto":
-            if head_dim != 64 and head_dim != 128:
-                impl = "general"
-            elif dtype is torch.bfloat16 and max_q_len * (n_heads // n_kv_heads) >= self.FP4_PREFILL_MIN_ROWS:
-                impl = "prefill"
-            else:
-                impl = "decode"
-        n_pages = k_pages.shape[0]
-        tensors = (q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), block_table.data_ptr(), block_table.stride(0), columns[1],
-                   q_start.data_ptr(), kv_len.data_ptr())
-        if impl == "decode":
-            floats, counters = self._fp4_decode_plan(dtype, n_seqs, n_heads, n_kv_heads, head_dim, page_size, max_q_len, max_kv_len)
-            ws = torch.empty(floats, dtype=torch.float32, device=q.device)
-            if self.debug:
-                self._debug_limit("attention_fp4_decode", 0, n_pages)
-            rc = self._fp4_call("tl_attention_fp4_decode")(
-                *tensors, ws.data_ptr(), self._counters(q.device, counters).data_ptr(), self._status_ptr, _DT[dtype], n_seqs, n_heads, n_kv_heads,
-                head_dim, page_size, n_pages, max_q_len, max_kv_len, window or 0, scale, _stream())
-        elif impl == "prefill":
-            pieces, floats = self._fp4_prefill_plan(shape[0], n_seqs, n_heads, n_kv_heads, head_dim, max_q_len, max_kv_len, int(allow_split))
-            ws = self._scratch(q.device, floats)
-            if self.debug:
-                self._debug_limit("attention_fp4_prefill", 0, n_pages)
-            rc = self._fp4_call("tl_attention_fp4_prefill")(
-                *tensors, 0 if ws is None else ws.data_ptr(), self._status_ptr, shape[0], n_seqs, n_heads, n_kv_heads, head_dim, page_size, n_pages,
-                max_q_len, window or 0, scale, pieces, _stream())
-            if pieces > 1:
-                self.launches += 1
-        else:
-            if self.debug:
-                self._debug_limit("attention_fp4", 0, n_pages)
-            rc = self._fp4_call("tl_attention_fp4_general")(
-                *tensors, _DT[dtype], n_seqs, n_heads, n_kv_heads, head_dim, page_size, n_pages, max_q_len, window or 0, scale, _stream())
-        if rc:
-            _check(rc, "paged_attention_fp4")
-        self.launches += 1
-        return out
+        if got.__class__ is int:
+            _check(got, "paged_attention_fp4")
+        self.launches += got[1]
+        return got[0]
 
     # ---------------------------------------------------------------- sampling
     @_timed

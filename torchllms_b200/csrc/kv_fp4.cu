@@ -160,40 +160,167 @@ __global__ void __launch_bounds__(128) rope_kv_write_fp4_kernel(const TI* __rest
     }
 }
 
-// The numbers of given slots: a thread to eight coordinates of a head of a slot; blockIdx.y: keys, values.
+// The same for bfloat16 rows of one plane whose pairs are neighbours or halves of a multiple of 16, heads of a power of two up to 1,024 and
+// many tokens: a thread's runs lie a multiple of the head size apart, so that one run of the rotation table serves them all, heads
+// come by a shift, and the loads of a token (EACH runs a thread, and their partners) are under way together.
+//   7,586 tokens, 48 heads of 128: 57 us with the kernel above, WRITE_US here (see below for what is read and written)
+constexpr int EACH = 3;
+template <bool INTERLEAVED>
+__global__ void __launch_bounds__(128) rope_kv_write_fp4_rows_kernel(const __nv_bfloat16* __restrict__ qkv, __nv_bfloat16* __restrict__ q_out,
+                                                                    const int log_runs, const WriteParams p) {
+    grid_launch_dependents();
+    grid_dependency_wait();
+    const int t = blockIdx.x;
+    const int heads = p.n_heads + 2 * p.n_kv_heads, runs = heads << log_runs;
+    const int off = (threadIdx.x & ((1 << log_runs) - 1)) << 3;
+    const int half = p.rot_dims >> 1;
+    const bool turns = off < p.rot_dims, first = off < half;
+    const int partner = first ? half : -half;            // (halves: where the other numbers of the pairs lie)
+    const __nv_bfloat16* src = qkv + (size_t)t * heads * p.head_dim;
+    uint4 raw[EACH], other[EACH];
+    auto fetch = [&](int c0) {
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) {
+            const int c = c0 + e * 128;
+            if (c < runs) {
+                raw[e] = *reinterpret_cast<const uint4*>(src + (size_t)c * 8);
+                if (!INTERLEAVED && turns && (c >> log_runs) < p.n_heads + p.n_kv_heads) other[e] = *reinterpret_cast<const uint4*>(src + (size_t)c * 8 + partner);
+            }
+        }
+    };
+    fetch(threadIdx.x);
+    int pos = p.positions[t];
+    (void)TL_CHECK(pos >= 0 && pos < p.table_rows, TL_DBG_POSITION);
+    pos = pos < 0 ? 0 : (pos >= p.table_rows ? p.table_rows - 1 : pos);   // the host keeps positions inside the table
+    long long page = 0;
+    int slot = 0;
+    bool write = p.k_pages != nullptr;
+    if (write) {
+        const int sm = p.slot_mapping[t];
+        page = sm / p.page_size;
+        slot = sm - (int)page * p.page_size;
+        // (a slot outside the cache is not written; debug builds report it)
+        write = TL_CHECK(sm >= 0, TL_DBG_SLOT) && tl_check_page(page) && sm >= 0 && page < p.n_pages;
+    }
+    float cs[INTERLEAVED ? 8 : 16];
+    if (turns) {
+        const float* at = p.table + (size_t)pos * p.rot_dims + (INTERLEAVED ? off : 2 * (first ? off : off - half));
+#pragma unroll
+        for (int i = 0; i < (INTERLEAVED ? 2 : 4); ++i) {
+            const float4 v = *reinterpret_cast<const float4*>(at + 4 * i);
+            cs[4 * i] = v.x; cs[4 * i + 1] = v.y; cs[4 * i + 2] = v.z; cs[4 * i + 3] = v.w;
+        }
+    }
+    const float sc = warp_row_scale(p.rs, t);
+    // (whole warps go round together: the lanes of a group exchange their maxima)
+    for (int c0 = threadIdx.x; c0 - (int)threadIdx.x < runs; c0 += EACH * 128) {
+        if (c0 != (int)threadIdx.x) fetch(c0);
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) {
+            const int c = c0 + e * 128;
+            if (c - (int)threadIdx.x >= runs) break;
+            const bool mine = c < runs;
+            const int head = c >> log_runs;
+            float x[8];
+            const __nv_bfloat162* x2 = reinterpret_cast<const __nv_bfloat162*>(&raw[e]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 v = mine ? __bfloat1622float2(x2[i]) : make_float2(0.f, 0.f);
+                x[2 * i] = v.x;
+                x[2 * i + 1] = v.y;
+            }
+            if (p.rs.ssq != nullptr) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] *= sc;
+            }
+            if (turns && mine && head < p.n_heads + p.n_kv_heads) {
+                if (INTERLEAVED) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float a = x[2 * i], b = x[2 * i + 1];
+                        x[2 * i] = __fsub_rn(__fmul_rn(a, cs[2 * i]), __fmul_rn(b, cs[2 * i + 1]));
+                        x[2 * i + 1] = __fadd_rn(__fmul_rn(b, cs[2 * i]), __fmul_rn(a, cs[2 * i + 1]));
+                    }
+                } else {
+                    const __nv_bfloat162* y2 = reinterpret_cast<const __nv_bfloat162*>(&other[e]);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float2 both = __bfloat1622float2(y2[i / 2]);
+                        float y = i & 1 ? both.y : both.x;
+                        if (p.rs.ssq != nullptr) y *= sc;
+                        const float u = __fmul_rn(x[i], cs[(2 * i) % (INTERLEAVED ? 8 : 16)]), v = __fmul_rn(y, cs[(2 * i + 1) % (INTERLEAVED ? 8 : 16)]);
+                        x[i] = first ? __fsub_rn(u, v) : __fadd_rn(u, v);
+                    }
+                }
+            }
+            if (c - (int)threadIdx.x + 127 < (p.n_heads << log_runs)) {                // (the whole CTA has heads of q)
+                store8(q_out + ((size_t)t * p.n_heads << (log_runs + 3)) + (size_t)c * 8, x);
+                continue;
+            }
+            unsigned top = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            if (!mine) continue;
+            if (head < p.n_heads) {
+                store8(q_out + ((size_t)t * p.n_heads << (log_runs + 3)) + (size_t)c * 8, x);
+            } else if (write) {
+                const bool is_k = head < p.n_heads + p.n_kv_heads;
+                const int kvh = is_k ? head - p.n_heads : head - p.n_heads - p.n_kv_heads;
+                unsigned char* base = is_k ? p.k_pages : p.v_pages;
+                const Fp4Place at = fp4_place(page, slot, kvh, p.n_kv_heads, p.page_size, p.head_dim);
+                const unsigned byte = fp4_scale_byte(top);
+                *reinterpret_cast<unsigned*>(base + at.codes + off / 2) = fp4_pack8(x, byte);
+                if ((off & 8) == 0) base[at.scales + off / FP4_GROUP] = (unsigned char)byte;
+            }
+        }
+    }
+}
+
+// The numbers of given slots: a CTA to a slot at a time, blockIdx.y: keys, values; a thread to eight coordinates of a head, four slots
+// under way together.
+constexpr int SLOTS = 4;
 template <typename T>
 __global__ void __launch_bounds__(128) kv_read_fp4_kernel(const unsigned char* __restrict__ k_pages, const unsigned char* __restrict__ v_pages,
                                                           const int* __restrict__ slots, T* __restrict__ k_out, T* __restrict__ v_out,
-                                                          long long runs, long long n_pages, int n_kv_heads, int head_dim, int page_size) {
+                                                          int n_slots, long long n_pages, int n_kv_heads, int head_dim, int page_size) {
     grid_launch_dependents();
     grid_dependency_wait();
     const unsigned char* pages = blockIdx.y ? v_pages : k_pages;
     T* out = blockIdx.y ? v_out : k_out;
-    const int per_head = head_dim >> 3;
-    for (long long c = (long long)blockIdx.x * blockDim.x + threadIdx.x; c < runs; c += (long long)gridDim.x * blockDim.x) {
-        const long long row = c / per_head;
-        const int off = (int)(c - row * per_head) << 3;
-        const long long n = row / n_kv_heads;
-        const int head = (int)(row - n * n_kv_heads);
-        const int sm = slots[n];
-        const long long page = sm / page_size;
-        float x[8];
+    const int per_head = head_dim >> 3, runs = n_kv_heads * per_head;
+    for (int c = threadIdx.x; c < runs; c += blockDim.x) {
+        const int head = c / per_head, off = (c - head * per_head) << 3;
+        for (long long n0 = (long long)blockIdx.x * SLOTS; n0 < n_slots; n0 += (long long)gridDim.x * SLOTS) {
+            unsigned w[SLOTS], byte[SLOTS];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = 0.f;
-        // (a slot outside the cache reads as zeros; debug builds report it)
-        if (TL_CHECK(sm >= 0, TL_DBG_SLOT) && tl_check_page(page) && sm >= 0 && page < n_pages) {
-            const Fp4Place at = fp4_place(page, sm - (int)page * page_size, head, n_kv_heads, page_size, head_dim);
-            __half2 r[4];
-            fp4_unpack(*reinterpret_cast<const unsigned*>(pages + at.codes + off / 2), r);
-            const __half2 s = fp4_scale2(pages[at.scales + off / FP4_GROUP]);
+            for (int i = 0; i < SLOTS; ++i) {
+                w[i] = byte[i] = 0u;                    // (a slot outside the cache reads as zeros; debug builds report it)
+                if (n0 + i >= n_slots) continue;
+                const int sm = slots[n0 + i];
+                const int page = sm / page_size;
+                if (TL_CHECK(sm >= 0, TL_DBG_SLOT) && tl_check_page(page) && sm >= 0 && page < n_pages) {
+                    const Fp4Place at = fp4_place(page, sm - page * page_size, head, n_kv_heads, page_size, head_dim);
+                    w[i] = *reinterpret_cast<const unsigned*>(pages + at.codes + off / 2);
+                    byte[i] = pages[at.scales + off / FP4_GROUP];
+                }
+            }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float2 v = __half22float2(__hmul2(r[i], s));      // exact
-                x[2 * i] = v.x;
-                x[2 * i + 1] = v.y;
+            for (int i = 0; i < SLOTS; ++i) {
+                if (n0 + i >= n_slots) continue;
+                __half2 r[4];
+                fp4_unpack(w[i], r);
+                const __half2 s = fp4_scale2(byte[i]);
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float2 v = __half22float2(__hmul2(r[e], s));      // exact
+                    x[2 * e] = v.x;
+                    x[2 * e + 1] = v.y;
+                }
+                store8(out + ((size_t)(n0 + i) * runs + c) * 8, x);
             }
         }
-        store8(out + c * 8, x);
     }
 }
 
@@ -227,6 +354,14 @@ extern "C" int tl_rope_kv_write_fp4(const void* qkv, int in_dtype, int splits, c
     const int runs = heads * (head_dim / 8);
     const int by = n_tokens >= 256 ? 1 : (runs + 127) / 128;
     cudaStream_t s = (cudaStream_t)stream;
+    const int head_runs = head_dim / 8;
+    if (in_dtype == TL_BF16 && dtype == TL_BF16 && splits == 1 && n_tokens >= 148 && head_runs <= 128 && (head_runs & (head_runs - 1)) == 0 &&
+        rot_dims % (interleaved ? 8 : 16) == 0) {
+        int log_runs = 0;
+        while ((1 << log_runs) < head_runs) ++log_runs;
+        return (int)(interleaved ? tl_launch(rope_kv_write_fp4_rows_kernel<true>, dim3(n_tokens), dim3(128), 0, s, (const __nv_bfloat16*)qkv, (__nv_bfloat16*)q_out, log_runs, p)
+                                 : tl_launch(rope_kv_write_fp4_rows_kernel<false>, dim3(n_tokens), dim3(128), 0, s, (const __nv_bfloat16*)qkv, (__nv_bfloat16*)q_out, log_runs, p));
+    }
 #define TL_WRITE(TI, T)                                                                                                         \
     (interleaved ? tl_launch(rope_kv_write_fp4_kernel<TI, T, true>, dim3(n_tokens, by), dim3(128), 0, s, (const TI*)qkv, (T*)q_out, p) \
                  : tl_launch(rope_kv_write_fp4_kernel<TI, T, false>, dim3(n_tokens, by), dim3(128), 0, s, (const TI*)qkv, (T*)q_out, p))
@@ -243,15 +378,15 @@ extern "C" int tl_kv_read_fp4(const void* k_pages, const void* v_pages, const in
     if (n_slots <= 0) return TL_OK;
     if (!takes(n_kv_heads, head_dim, page_size)) return TL_BAD_SIZE;
     if (!aligned16(k_pages) || !aligned16(v_pages) || !aligned16(k_out) || !aligned16(v_out)) return TL_BAD_ALIGN;
-    const long long runs = (long long)n_slots * n_kv_heads * (head_dim / 8);
-    const unsigned bx = (unsigned)((runs + 127) / 128 < 148 * 8 ? (runs + 127) / 128 : 148 * 8);
+    const long long groups = ((long long)n_slots + SLOTS - 1) / SLOTS;
+    const unsigned bx = (unsigned)(groups < 148 * 16 ? groups : 148 * 16);
     cudaStream_t s = (cudaStream_t)stream;
     const unsigned char *k = (const unsigned char*)k_pages, *v = (const unsigned char*)v_pages;
     if (dtype == TL_BF16)
         return (int)tl_launch(kv_read_fp4_kernel<__nv_bfloat16>, dim3(bx, 2), dim3(128), 0, s, k, v, slots, (__nv_bfloat16*)k_out,
-                              (__nv_bfloat16*)v_out, runs, n_pages, n_kv_heads, head_dim, page_size);
+                              (__nv_bfloat16*)v_out, n_slots, n_pages, n_kv_heads, head_dim, page_size);
     if (dtype == TL_F32)
-        return (int)tl_launch(kv_read_fp4_kernel<float>, dim3(bx, 2), dim3(128), 0, s, k, v, slots, (float*)k_out, (float*)v_out, runs,
+        return (int)tl_launch(kv_read_fp4_kernel<float>, dim3(bx, 2), dim3(128), 0, s, k, v, slots, (float*)k_out, (float*)v_out, n_slots,
                               n_pages, n_kv_heads, head_dim, page_size);
     return TL_BAD_DTYPE;
 }

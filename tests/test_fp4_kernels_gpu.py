@@ -42,6 +42,12 @@ def turned(x, cs, interleaved):
     (300, 4, 4, 16, 10, 32, True, "bf16", 1),        # the rotated part ends inside a run of eight
     (515, 14, 2, 128, 64, 64, True, "bf16", 1),
     (70, 8, 2, 256, 128, 16, False, "bf16", 1),
+    (150, 5, 2, 128, 96, 16, False, "f32", 1),       # (from 148 tokens on a kernel of their own)
+    (201, 7, 1, 128, 128, 32, True, "f32", 1),
+    (163, 3, 1, 64, 64, 16, False, "bf16", 1),
+    (149, 4, 2, 32, 16, 16, False, "bf16", 1),
+    (180, 12, 2, 256, 8, 16, True, "bf16", 1),
+    (148, 1, 1, 16, 16, 16, False, "f32", 1),
     (5, 32, 8, 128, 128, 16, True, "bf16", 3),       # float32 partial sums
     (9, 4, 2, 64, 64, 16, False, "f32", 2),
 ])

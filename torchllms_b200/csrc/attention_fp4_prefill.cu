@@ -176,6 +176,11 @@ __device__ __forceinline__ unsigned pack_bf16(float lo, float hi) {
     __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<unsigned*>(&v);
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 __device__ __forceinline__ unsigned pack_half(float lo, float hi) {
     __half2 v = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<unsigned*>(&v);
@@ -466,11 +471,17 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_fp4_prefill_kernel(cons
         // the rows of q, as float16: 32 / CH rows at a time, 16 bytes a lane
         float back = 0.f;
         if (n_tiles > 0) {
-#pragma unroll 4
+            uint4 loaded[CH];                      // (all under way together)
+#pragma unroll
             for (int i = 0; i < CH; ++i) {
                 const int rr = sw * 32 + i * (32 / CH) + lane / CH, chunk = lane % CH;
-                uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-                if (rr < rows) raw = *reinterpret_cast<const uint4*>(p.q + row_of(rr) * HD + chunk * 8);
+                loaded[i] = make_uint4(0u, 0u, 0u, 0u);
+                if (rr < rows) loaded[i] = *reinterpret_cast<const uint4*>(p.q + row_of(rr) * HD + chunk * 8);
+            }
+#pragma unroll
+            for (int i = 0; i < CH; ++i) {
+                const int rr = sw * 32 + i * (32 / CH) + lane / CH, chunk = lane % CH;
+                const uint4 raw = loaded[i];
                 const unsigned w[4] = {raw.x, raw.y, raw.z, raw.w};
                 unsigned top = 0;
 #pragma unroll
@@ -520,14 +531,14 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_fp4_prefill_kernel(cons
                 for (int i = 0; i < BN; ++i)
                     if (k0 + i < from || k0 + i >= to) raw[i] = 0xff800000u;      // -inf
             }
-            float mx[8];
+            float mx[4];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) mx[i] = __uint_as_float(raw[i]);
+            for (int i = 0; i < 4; ++i) mx[i] = fmaxf(__uint_as_float(raw[i]), __uint_as_float(raw[i + 4]));
 #pragma unroll
             for (int i = 8; i < BN; i += 8)
 #pragma unroll
-                for (int k = 0; k < 8; ++k) mx[k] = fmaxf(mx[k], __uint_as_float(raw[i + k]));
-            const float m_new = fmaxf(m_used, fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7]))) * fit);
+                for (int k = 0; k < 4; ++k) mx[k] = max3(mx[k], __uint_as_float(raw[i + k]), __uint_as_float(raw[i + k + 4]));
+            const float m_new = fmaxf(m_used, fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * fit);
             const bool grow = m_new > m_used + LAG;      // also true for the first keys a row sees
             // (the weights of the key tile before have been read, and the accumulator may be touched, when its product is over)
             if (it > 0) {

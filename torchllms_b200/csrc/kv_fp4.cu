@@ -160,14 +160,24 @@ __global__ void __launch_bounds__(128) rope_kv_write_fp4_kernel(const TI* __rest
     }
 }
 
-// The same for bfloat16 rows of one plane whose pairs are neighbours or halves of a multiple of 16, heads of a power of two up to 1,024 and
-// many tokens: a thread's runs lie a multiple of the head size apart, so that one run of the rotation table serves them all, heads
-// come by a shift, and the loads of a token (EACH runs a thread, and their partners) are under way together.
-//   7,586 tokens, 48 heads of 128: 57 us with the kernel above, WRITE_US here (see below for what is read and written)
-constexpr int EACH = 3;
-template <bool INTERLEAVED>
-__global__ void __launch_bounds__(128) rope_kv_write_fp4_rows_kernel(const __nv_bfloat16* __restrict__ qkv, __nv_bfloat16* __restrict__ q_out,
-                                                                    const int log_runs, const WriteParams p) {
+// The same for rows of one plane and of the type that q leaves in, whose pairs are neighbours or halves of a multiple of 16, heads of a
+// power of two up to 1,024 and many tokens: a thread's runs lie a multiple of the head size apart, so that one run of the rotation table
+// serves them all, heads come by a shift, and the loads of a token (RUNS runs a thread, and their partners) are under way together.
+//   8,276 tokens, 48 heads of 128, bfloat16 (179 MB, 27 us of them): 36 us; with three runs at a time 40, with the kernel above
+//   and divisions 72.  Without the 4-bit numbers' arithmetic it would take 32: what bounds it next to memory.
+template <typename T> struct Runs { static constexpr int N = sizeof(T) == 2 ? 6 : 3; };
+template <typename T> struct Run8 {                     // eight numbers as they are stored
+    uint4 v[sizeof(T) / 2];
+    __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = reinterpret_cast<const uint4*>(p)[i];
+    }
+    __device__ __forceinline__ float get(int i) const { return to_float(reinterpret_cast<const T*>(v)[i]); }
+};
+template <typename T, bool INTERLEAVED>
+__global__ void __launch_bounds__(128, sizeof(T) == 2 && INTERLEAVED ? 8 : 5) rope_kv_write_fp4_rows_kernel(const T* __restrict__ qkv, T* __restrict__ q_out,
+                                                                                              const int log_runs, const WriteParams p) {
+    constexpr int EACH = Runs<T>::N;
     grid_launch_dependents();
     grid_dependency_wait();
     const int t = blockIdx.x;
@@ -176,15 +186,15 @@ __global__ void __launch_bounds__(128) rope_kv_write_fp4_rows_kernel(const __nv_
     const int half = p.rot_dims >> 1;
     const bool turns = off < p.rot_dims, first = off < half;
     const int partner = first ? half : -half;            // (halves: where the other numbers of the pairs lie)
-    const __nv_bfloat16* src = qkv + (size_t)t * heads * p.head_dim;
-    uint4 raw[EACH], other[EACH];
+    const T* src = qkv + (size_t)t * heads * p.head_dim;
+    Run8<T> raw[EACH], other[INTERLEAVED ? 1 : EACH];
     auto fetch = [&](int c0) {
 #pragma unroll
         for (int e = 0; e < EACH; ++e) {
             const int c = c0 + e * 128;
             if (c < runs) {
-                raw[e] = *reinterpret_cast<const uint4*>(src + (size_t)c * 8);
-                if (!INTERLEAVED && turns && (c >> log_runs) < p.n_heads + p.n_kv_heads) other[e] = *reinterpret_cast<const uint4*>(src + (size_t)c * 8 + partner);
+                raw[e].load(src + (size_t)c * 8);
+                if (!INTERLEAVED && turns && (c >> log_runs) < p.n_heads + p.n_kv_heads) other[INTERLEAVED ? 0 : e].load(src + (size_t)c * 8 + partner);
             }
         }
     };
@@ -222,13 +232,8 @@ __global__ void __launch_bounds__(128) rope_kv_write_fp4_rows_kernel(const __nv_
             const bool mine = c < runs;
             const int head = c >> log_runs;
             float x[8];
-            const __nv_bfloat162* x2 = reinterpret_cast<const __nv_bfloat162*>(&raw[e]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float2 v = mine ? __bfloat1622float2(x2[i]) : make_float2(0.f, 0.f);
-                x[2 * i] = v.x;
-                x[2 * i + 1] = v.y;
-            }
+            for (int i = 0; i < 8; ++i) x[i] = mine ? raw[e].get(i) : 0.f;
             if (p.rs.ssq != nullptr) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) x[i] *= sc;
@@ -242,11 +247,9 @@ __global__ void __launch_bounds__(128) rope_kv_write_fp4_rows_kernel(const __nv_
                         x[2 * i + 1] = __fadd_rn(__fmul_rn(b, cs[2 * i]), __fmul_rn(a, cs[2 * i + 1]));
                     }
                 } else {
-                    const __nv_bfloat162* y2 = reinterpret_cast<const __nv_bfloat162*>(&other[e]);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        const float2 both = __bfloat1622float2(y2[i / 2]);
-                        float y = i & 1 ? both.y : both.x;
+                        float y = other[INTERLEAVED ? 0 : e].get(i);
                         if (p.rs.ssq != nullptr) y *= sc;
                         const float u = __fmul_rn(x[i], cs[(2 * i) % (INTERLEAVED ? 8 : 16)]), v = __fmul_rn(y, cs[(2 * i + 1) % (INTERLEAVED ? 8 : 16)]);
                         x[i] = first ? __fsub_rn(u, v) : __fadd_rn(u, v);
@@ -355,12 +358,14 @@ extern "C" int tl_rope_kv_write_fp4(const void* qkv, int in_dtype, int splits, c
     const int by = n_tokens >= 256 ? 1 : (runs + 127) / 128;
     cudaStream_t s = (cudaStream_t)stream;
     const int head_runs = head_dim / 8;
-    if (in_dtype == TL_BF16 && dtype == TL_BF16 && splits == 1 && n_tokens >= 148 && head_runs <= 128 && (head_runs & (head_runs - 1)) == 0 &&
+    if (in_dtype == dtype && splits == 1 && n_tokens >= 148 && head_runs <= 128 && (head_runs & (head_runs - 1)) == 0 &&
         rot_dims % (interleaved ? 8 : 16) == 0) {
         int log_runs = 0;
         while ((1 << log_runs) < head_runs) ++log_runs;
-        return (int)(interleaved ? tl_launch(rope_kv_write_fp4_rows_kernel<true>, dim3(n_tokens), dim3(128), 0, s, (const __nv_bfloat16*)qkv, (__nv_bfloat16*)q_out, log_runs, p)
-                                 : tl_launch(rope_kv_write_fp4_rows_kernel<false>, dim3(n_tokens), dim3(128), 0, s, (const __nv_bfloat16*)qkv, (__nv_bfloat16*)q_out, log_runs, p));
+#define TL_WRITE_ROWS(T, I) tl_launch(rope_kv_write_fp4_rows_kernel<T, I>, dim3(n_tokens), dim3(128), 0, s, (const T*)qkv, (T*)q_out, log_runs, p)
+        if (dtype == TL_BF16) return (int)(interleaved ? TL_WRITE_ROWS(__nv_bfloat16, true) : TL_WRITE_ROWS(__nv_bfloat16, false));
+        if (dtype == TL_F32) return (int)(interleaved ? TL_WRITE_ROWS(float, true) : TL_WRITE_ROWS(float, false));
+#undef TL_WRITE_ROWS
     }
 #define TL_WRITE(TI, T)                                                                                                         \
     (interleaved ? tl_launch(rope_kv_write_fp4_kernel<TI, T, true>, dim3(n_tokens, by), dim3(128), 0, s, (const TI*)qkv, (T*)q_out, p) \

@@ -61,8 +61,11 @@ struct Params {
     int table_stride, table_cols;
     int n_heads, n_kv_heads, group, page_records;
     int n_blocks, pieces, window;
+    unsigned per_group;         // 2^32 / group and one more (0 for a group of one head): row / group without a division
     float scale_log2;
 };
+// (exact for row * group < 2^32, which the host sees to)
+__device__ __forceinline__ int token_of(const Params& p, int row) { return p.per_group ? (int)__umulhi((unsigned)row, p.per_group) : row; }
 
 __device__ __forceinline__ unsigned smem_u32(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void mbar_init(unsigned long long* bar, unsigned count) {
@@ -301,8 +304,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_fp4_prefill_kernel(cons
     const bool active = row0 < all_rows && *(volatile int*)failed == 0;
     const int last_row = min(row0 + QT * BM, all_rows) - 1;
     // keys lo .. hi - 1 of the block, and of this piece of them (whole tiles)
-    int lo = p.window > 0 ? max(0, base + row0 / p.group - p.window + 1) : 0;
-    int hi = min(base + (active ? last_row / p.group : 0) + 1, p.table_cols * p.page_records * FP4_RECORD);
+    int lo = p.window > 0 ? max(0, base + token_of(p, row0) - p.window + 1) : 0;
+    int hi = min(base + (active ? token_of(p, last_row) : 0) + 1, p.table_cols * p.page_records * FP4_RECORD);
     int k_start = lo & ~(BN - 1);
     if (p.pieces > 1) {
         const int tiles = hi > k_start ? (hi - k_start + BN - 1) / BN : 0, each = (tiles + p.pieces - 1) / p.pieces;
@@ -317,8 +320,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_fp4_prefill_kernel(cons
         const int r0 = row0 + t * BM;
         const int rows = active ? max(0, min(BM, all_rows - r0)) : 0;
         range[t].rows = rows;
-        range[t].low = base + r0 / p.group;
-        range[t].high = base + (rows > 0 ? (r0 + rows - 1) / p.group : 0);
+        range[t].low = base + token_of(p, r0);
+        range[t].high = base + (rows > 0 ? token_of(p, r0 + rows - 1) : 0);
         const int from = p.window > 0 ? max(lo, range[t].low - p.window + 1) : lo, to = min(hi, range[t].high + 1);
         const bool any = rows > 0 && to > from;
         range[t].first = any ? (from - k_start) / BN : 0;
@@ -465,7 +468,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_fp4_prefill_kernel(cons
         unsigned char* stage = Qs + t * KV_BYTES;
         constexpr int CH = HD / 8;                 // lanes that share a row in global memory
         auto row_of = [&](int rr) {                // the row of q (and out) of a row of the tile
-            const int token = (tile_row0 + rr) / p.group;
+            const int token = token_of(p, tile_row0 + rr);
             return (size_t)(first_token + token) * p.n_heads + kvh * p.group + tile_row0 + rr - token * p.group;
         };
         // the rows of q, as float16: 32 / CH rows at a time, 16 bytes a lane
@@ -509,7 +512,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_fp4_prefill_kernel(cons
         const unsigned col_s = COL_S + (NS == 1 ? 0 : t * BN), col_p = COL_P + t * (BN / 2), col_o = COL_O + t * HD;
         const float fit = back * p.scale_log2;
         float m_used = -INFINITY, l_sum = 0.f;
-        const int qpos = base + (tile_row0 + (r < rows ? r : max(rows - 1, 0))) / p.group;
+        const int qpos = base + token_of(p, tile_row0 + (r < rows ? r : max(rows - 1, 0)));
         const float2 sc2 = make_float2(fit, fit);
         bool ok = true;
         for (int j = first; j < last; ++j) {
@@ -797,6 +800,8 @@ extern "C" int tl_attention_fp4_prefill(const void* q, const void* k_pages, cons
     p.block_table = block_table; p.q_start = q_start; p.kv_len = kv_len; p.status = status; p.n_pages = n_pages;
     p.table_stride = table_stride; p.table_cols = table_cols; p.n_heads = n_heads; p.n_kv_heads = n_kv_heads; p.group = n_heads / n_kv_heads;
     p.page_records = page_size / FP4_RECORD; p.n_blocks = pl.blocks; p.pieces = pieces; p.window = window > 0 ? window : 0;
+    p.per_group = p.group == 1 ? 0u : (unsigned)((1ull << 32) / (unsigned)p.group) + 1u;
+    if ((double)pl.blocks * QT * BM * p.group >= 4294967296.0) return TL_BAD_SIZE;
     p.scale_log2 = scale * LOG2E;
     p.part_o = workspace;
     p.part_ml = pieces > 1 ? workspace + q_rows * n_heads * pieces * head_dim : nullptr;

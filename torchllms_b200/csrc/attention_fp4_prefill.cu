@@ -179,6 +179,21 @@ __device__ __forceinline__ unsigned pack_bf16(float lo, float hi) {
     __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<unsigned*>(&v);
 }
+// 16 bytes from global to shared memory, `bytes` of them from there and zeros for the rest
+__device__ __forceinline__ void copy16(void* to, const void* from, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(to)), "l"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+// 32 bytes, a whole sector (the address is a multiple of 32)
+__device__ __forceinline__ void store32(void* to, const unsigned (&w)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]),
+                 "r"(w[6]), "r"(w[7]) : "memory");
+}
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {      // the largest magnitude; not a number if one is none
+    float d;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -471,39 +486,40 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_fp4_prefill_kernel(cons
             const int token = token_of(p, tile_row0 + rr);
             return (size_t)(first_token + token) * p.n_heads + kvh * p.group + tile_row0 + rr - token * p.group;
         };
-        // the rows of q, as float16: 32 / CH rows at a time, 16 bytes a lane
+        // The warp's 32 rows of q come into shared memory, 16 bytes a lane, where the operand layout has them (zeros for rows that are
+        // none), and there every thread brings its own row to float16.  (Loops, and not unrolled: this runs once, and straight code
+        // would be fetched instruction by instruction; through registers and all unrolled a prompt
+        // of 2,048 took 51 us, so 46.)
         float back = 0.f;
         if (n_tiles > 0) {
-            uint4 loaded[CH];                      // (all under way together)
-#pragma unroll
+#pragma unroll 2
             for (int i = 0; i < CH; ++i) {
                 const int rr = sw * 32 + i * (32 / CH) + lane / CH, chunk = lane % CH;
-                loaded[i] = make_uint4(0u, 0u, 0u, 0u);
-                if (rr < rows) loaded[i] = *reinterpret_cast<const uint4*>(p.q + row_of(rr) * HD + chunk * 8);
+                copy16(stage + (chunk >> 3) * HALF_BYTES + rr * 128 + (((chunk & 7) ^ (rr & 7)) << 4), rr < rows ? p.q + row_of(rr) * HD + chunk * 8 : p.q,
+                       rr < rows ? 16 : 0);
             }
-#pragma unroll
-            for (int i = 0; i < CH; ++i) {
-                const int rr = sw * 32 + i * (32 / CH) + lane / CH, chunk = lane % CH;
-                const uint4 raw = loaded[i];
-                const unsigned w[4] = {raw.x, raw.y, raw.z, raw.w};
-                unsigned top = 0;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) top = max(top, max(w[e] & 0x7fff0000u, (w[e] << 16) & 0x7fff0000u));
-#pragma unroll
-                for (int o = 1; o < CH; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-                // the row's largest number goes to 2^14 .. 2^15 (exponents as float32 has them, 127 more than they mean)
-                const int up = min(268 - (int)(top >> 23), 253);
-                const float factor = __uint_as_float((unsigned)up << 23);
-                unsigned h[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const __half2 x = __floats2half2_rn(__uint_as_float(w[e] << 16) * factor, __uint_as_float(w[e] & 0xffff0000u) * factor);
-                    h[e] = *reinterpret_cast<const unsigned*>(&x);
-                }
-                *reinterpret_cast<uint4*>(stage + (chunk >> 3) * HALF_BYTES + rr * 128 + (((chunk & 7) ^ (rr & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
-                // (the lane whose own row this is keeps what undoes the factor)
-                const float undo = __shfl_sync(0xffffffffu, __uint_as_float((unsigned)(254 - up) << 23), (lane * CH) & 31);
-                if (lane / (32 / CH) == i) back = undo;
+            copies_wait();
+            __syncwarp();
+            auto at = [&](int c) { return reinterpret_cast<uint4*>(stage + (c >> 3) * HALF_BYTES + r * 128 + (((c & 7) ^ (r & 7)) << 4)); };
+            // (the upper number of a word is read with the lower one behind it: that changes no exponent)
+            float top = 0.f;
+#pragma unroll 4
+            for (int c = 0; c < CH; ++c) {
+                const uint4 x = *at(c);
+                top = max3_abs(top, __uint_as_float(x.x), __uint_as_float(x.x << 16));
+                top = max3_abs(top, __uint_as_float(x.y), __uint_as_float(x.y << 16));
+                top = max3_abs(top, __uint_as_float(x.z), __uint_as_float(x.z << 16));
+                top = max3_abs(top, __uint_as_float(x.w), __uint_as_float(x.w << 16));
+            }
+            // the row's largest number goes to 2^14 .. 2^15 (exponents as float32 has them, 127 more than they mean)
+            const int up = min(268 - (int)((__float_as_uint(top) & 0x7fffffffu) >> 23), 253);
+            const float factor = __uint_as_float((unsigned)up << 23);
+            back = __uint_as_float((unsigned)(254 - up) << 23);
+#pragma unroll 2
+            for (int c = 0; c < CH; ++c) {
+                const uint4 x = *at(c);
+                auto half2 = [&](unsigned w) { return pack_half(__uint_as_float(w << 16) * factor, __uint_as_float(w & 0xffff0000u) * factor); };
+                *at(c) = make_uint4(half2(x.x), half2(x.y), half2(x.z), half2(x.w));
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
@@ -606,35 +622,20 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_fp4_prefill_kernel(cons
         if (ok && rows > 0) {
             if (p.pieces == 1) {
                 const float inv = l_sum == 0.f ? 0.f : 1.f / l_sum;
-                // The rows leave through shared memory (the place of the row tile's queries: its last scores are made), in the
-                // swizzled layout the queries had, so that they are written to global memory a row at a time.
+                // (a thread its own row, whole sectors at a time: the rows of a group's heads lie side by side)
+                __nv_bfloat16* to = p.out + row_of(r < rows ? r : 0) * HD;
+#pragma unroll 1
+                for (int c = 0; c < HD / 16; ++c) {
+                    unsigned v[16], w[8];
 #pragma unroll
-                for (int c = 0; c < HD / 32; ++c) {
-                    unsigned v[32];
+                    for (int i = 0; i < 16; ++i) v[i] = 0u;
                     if (n > 0) {
-                        tmem_ld<32>(lane_addr + col_o + c * 32, v);
+                        tmem_ld16(lane_addr + col_o + c * 16, v);
                         tmem_wait_ld();
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] = 0u;
                     }
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        uint4 w;
-                        w.x = pack_bf16(__uint_as_float(v[8 * i]) * inv, __uint_as_float(v[8 * i + 1]) * inv);
-                        w.y = pack_bf16(__uint_as_float(v[8 * i + 2]) * inv, __uint_as_float(v[8 * i + 3]) * inv);
-                        w.z = pack_bf16(__uint_as_float(v[8 * i + 4]) * inv, __uint_as_float(v[8 * i + 5]) * inv);
-                        w.w = pack_bf16(__uint_as_float(v[8 * i + 6]) * inv, __uint_as_float(v[8 * i + 7]) * inv);
-                        const int chunk = c * 4 + i;
-                        *reinterpret_cast<uint4*>(stage + (chunk >> 3) * HALF_BYTES + r * 128 + (((chunk & 7) ^ (r & 7)) << 4)) = w;
-                    }
-                }
-                __syncwarp();                                // (a warp writes out the 32 rows it staged itself)
-#pragma unroll
-                for (int i = 0; i < CH; ++i) {
-                    const int rr = sw * 32 + i * (32 / CH) + lane / CH, chunk = lane % CH;
-                    const uint4 w = *reinterpret_cast<const uint4*>(stage + (chunk >> 3) * HALF_BYTES + rr * 128 + (((chunk & 7) ^ (rr & 7)) << 4));
-                    if (rr < rows) *reinterpret_cast<uint4*>(p.out + row_of(rr) * HD + chunk * 8) = w;
+                    for (int e = 0; e < 8; ++e) w[e] = pack_bf16(__uint_as_float(v[2 * e]) * inv, __uint_as_float(v[2 * e + 1]) * inv);
+                    if (r < rows) store32(to + c * 16, w);
                 }
             } else if (r < rows || n > 0) {
                 const size_t row = row_of(r < rows ? r : 0) * p.pieces + piece;
@@ -643,15 +644,14 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_fp4_prefill_kernel(cons
                     p.part_ml[2 * row + 1] = l_sum;
                 }
                 if (n > 0) {
-#pragma unroll
-                    for (int c = 0; c < HD / 32; ++c) {
-                        unsigned v[32];
-                        tmem_ld<32>(lane_addr + col_o + c * 32, v);
+#pragma unroll 1
+                    for (int c = 0; c < HD / 16; ++c) {
+                        unsigned v[16];
+                        tmem_ld16(lane_addr + col_o + c * 16, v);
                         tmem_wait_ld();
                         if (r < rows) {
-#pragma unroll
-                            for (int i = 0; i < 8; ++i)
-                                *reinterpret_cast<uint4*>(p.part_o + row * HD + c * 32 + i * 4) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                            store32(p.part_o + row * HD + c * 16, *reinterpret_cast<const unsigned(*)[8]>(&v[0]));
+                            store32(p.part_o + row * HD + c * 16 + 8, *reinterpret_cast<const unsigned(*)[8]>(&v[8]));
                         }
                     }
                 }
@@ -790,8 +790,10 @@ extern "C" int tl_attention_fp4_prefill(const void* q, const void* k_pages, cons
                                         int max_q_len, int window, float scale, int pieces, void* stream) {
     if (n_seqs <= 0 || max_q_len <= 0) return TL_OK;
     if (!takes(n_heads, n_kv_heads, head_dim, page_size) || n_pages <= 0 || pieces < 1 || pieces > MOST_PIECES) return TL_BAD_SIZE;
-    if (!aligned16(q) || !aligned16(out) || !aligned16(k_pages) || !aligned16(v_pages) || status == nullptr) return TL_BAD_ALIGN;
-    if (pieces > 1 && (workspace == nullptr || !aligned16(workspace))) return TL_BAD_SIZE;
+    // (results are stored 32 bytes at a time)
+    auto aligned32 = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 31u) == 0; };
+    if (!aligned16(q) || !aligned32(out) || !aligned16(k_pages) || !aligned16(v_pages) || status == nullptr) return TL_BAD_ALIGN;
+    if (pieces > 1 && (workspace == nullptr || !aligned32(workspace))) return TL_BAD_SIZE;
     const Plan pl = make_plan(n_seqs, n_heads, n_kv_heads, max_q_len, 1);
     if (n_seqs > 65535 || pl.blocks > 65535) return TL_BAD_SIZE;
     Params p;

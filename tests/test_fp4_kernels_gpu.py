@@ -214,6 +214,17 @@ def test_attention_is_the_formula(H, KV, D, page, q_lens, kv_lens, window, dtype
     ops().check_status()
 
 
+@pytest.mark.parametrize("group,D,q_lens,dtype", [(7, 128, [1] * 6, "bf16"), (1, 64, [1] * 5, "bf16"), (3, 128, [1, 1], "f32"), (5, 64, [1] * 4, "f32"),
+                                                  (1, 128, [3, 1, 2], "bf16"), (13, 128, [1, 1], "bf16"), (3, 64, [5, 4], "f32")])
+def test_requests_that_are_cut_and_have_an_odd_number_of_rows(group, D, q_lens, dtype):
+    """The sums that parts of a request leave lie on 16 bytes however many rows there are."""
+    kv_lens = [777 - 130 * i for i in range(len(q_lens))]
+    a, kw = batch(4 * group, 4, D, 16, q_lens, kv_lens, None, dtype)
+    got = ops().paged_attention_fp4(**a, **kw, impl="decode")
+    ops().check_status()
+    judge(got, a, kw)
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_large_and_tiny_queries(dtype):
     """Queries of 1e4 and of 1e-6 (scores that are one-hot, or all alike), and rows of zeros."""

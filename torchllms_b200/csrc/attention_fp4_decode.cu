@@ -53,7 +53,7 @@ struct Params {
     const int* block_table;
     const int* q_start;
     const int* kv_len;
-    float* part;                // [CTAs, 2, rows, HD + 2]: sums, then maximum (base 2) and sum of the weights
+    float* part;                // [CTAs, 2, part_floats]: rows x HD sums, then maximum (base 2) and sum of the weights of every row
     int* counters;              // [n_seqs, blocks, n_kv_heads], zero between launches
     int* status;
     long long n_pages;
@@ -62,6 +62,9 @@ struct Params {
     int page_shift;             // page_records is 1 << page_shift, or page_shift is negative
     float scale_log2;
 };
+
+// floats of a part: whole 16 bytes also for an odd number of rows, since sums are stored four at a time
+__host__ __device__ constexpr int part_floats(int rows, int head_dim) { return (rows * (head_dim + 2) + 3) / 4 * 4; }
 
 __device__ __forceinline__ unsigned smem_u32(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void mbar_init(unsigned long long* bar, unsigned count) {
@@ -666,7 +669,7 @@ __global__ void __launch_bounds__(NTHREADS, (NT == 1 && sizeof(T) == 2) ? 3 : 2)
             return reinterpret_cast<T*>(p.out) + ((size_t)(w.k.first + token) * p.n_heads + w.kvh * p.group + row - token * p.group) * HD;
         };
         // where a part of this block lies: that with its first tile in its CTA's first place, others in the second
-        const size_t place = (size_t)p.rows * (HD + 2);
+        const size_t place = part_floats(p.rows, HD);
         auto part_of = [&](int cta, bool first) { return p.part + ((size_t)cta * 2 + (first ? 0 : 1)) * place; };
         if (sound) {
             float* part = part_of(blockIdx.x, w.t0 == 0);
@@ -823,7 +826,7 @@ extern "C" int tl_attention_fp4_decode_plan(int dtype, int n_seqs, int n_heads, 
     if (!takes(n_heads, n_kv_heads, head_dim, page_size) || max_q_len < 1 || n_seqs < 1) return TL_BAD_SIZE;
     if (dtype != TL_BF16 && dtype != TL_F32) return TL_BAD_DTYPE;
     const Plan pl = make_plan(dtype, n_seqs, n_heads, n_kv_heads, head_dim, max_q_len, max_kv_len);
-    *workspace_floats = (long long)pl.ctas * 2 * pl.rows * (head_dim + 2);
+    *workspace_floats = (long long)pl.ctas * 2 * part_floats(pl.rows, head_dim);
     *n_counters = (long long)n_seqs * pl.blocks * n_kv_heads;
     return TL_OK;
 }

@@ -34,7 +34,7 @@ constexpr int EACH = 2;                 // records that a consumer warp takes of
 constexpr int RECORDS = EACH * NCW;     // records of a tile
 constexpr int BN = RECORDS * FP4_RECORD;
 constexpr int NTHREADS = (NCW + 1) * 32;
-constexpr int WORTH = 1;                // what a block's beginning and end are worth, in tiles
+constexpr int WORTH = 2;                // what a block's beginning and end are worth, in tiles
 constexpr int MOST_PARTS = 64;          // parts of a block, at most
 constexpr int FAILED_PART = 1 << 16;    // what a CTA that gave up adds to a counter beside its 1
 constexpr int SMS = 148;

@@ -187,6 +187,19 @@ PyObject* read(PyObject*, PyObject* const* args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// Whether a step is one for the tcgen05 kernel, whose CTA has 256 rows and an SM to itself, and not for the mma.sync kernel, which unpacks keys and
+// values again for every 16 rows.  `rows`: tokens x query heads of a key head; `units`: requests x key heads.  Measured (us, the mma.sync
+// kernel and the other; contexts of 200, 2,000 and 12,000 tokens):
+//   1 request, 32 / 8 heads of 128, 16 rows: 11.4  9.9   15.0 14.8   26.4 22.0     64: 12.3 10.2   17.0 16.0   34.0 22.9     256: 14.7 14.2   26.5 22.8   78 31
+//   8 requests                      16 rows: 12.6 10.6   18.8 22.5   48.6 97.6     64: 11.2 10.9   38.5 23.9   145 100       256: 39.0 14.8   116  36    530 118
+//   1 request,           of 64      32 rows:  9.0  8.1   12.0 14.7   17.7 20.3     64:  9.1  7.9   12.6 15.1   24.0 21.0     256: 11.0 12.0   18.9 18.6   57 28
+//   8 requests                      32 rows: 10.2  8.5   18.8 19.5   57.3 69.7     64:  8.7  8.8   27.6 20.0   105  71       256: 27.4 12.4   80.1 29.5  375 96
+// So it is one from `least` rows on, and with heads of 128 from 17 on where there are no more than 1,024 tiles of 128 keys (8 requests of 2,000
+// tokens: 32 rows 26.2 and 23.4 us; of 12,000 80.8 and 98.0).
+bool many_rows(long long rows, int head_dim, long long units, int max_kv, int least) {
+    return rows >= least || (head_dim == 128 && rows > 16 && units * ((max_kv + 127) / 128) <= 1024);
+}
+
 // q, k_pages, v_pages, block_table, q_start, kv_len, n_seqs, max_q_len, max_kv_len, scale, window, page_size, allow_split, impl (0 the kernel that fits,
 // 1 general, 2 decode, 3 prefill), n_tokens, out, rows of a request from which 3 fits -> (out, launches), an error code, or None
 PyObject* attend(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -214,8 +227,12 @@ PyObject* attend(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (given != nullptr ? (!given->is_cuda() || given->scalar_type() != q->scalar_type() || !given->is_contiguous() || given->sizes() != q->sizes())
                          : args[15] != Py_None)
         Py_RETURN_NONE;
-    if (impl == 0) impl = !tensor_cores ? 1 : code == 1 && (long long)max_q * (heads / kv_heads) >= min_rows ? 3 : 2;
     at::Tensor out = given != nullptr ? *given : at::empty_like(*q);
+    if (impl == 0) {        // (the tcgen05 kernel stores 32 bytes at a time)
+        const bool many = code == 1 && (uintptr_t)out.data_ptr() % 32 == 0 &&
+                          many_rows(max_q * (heads / kv_heads), (int)head_dim, n_seqs * kv_heads, max_kv, min_rows);
+        impl = !tensor_cores ? 1 : many ? 3 : 2;
+    }
     void* stream = stream_of(*q);
     const int* bt = table->data_ptr<int>();
     const int stride = (int)table->stride(0), columns = (int)table->size(1);

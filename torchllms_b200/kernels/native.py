@@ -115,7 +115,8 @@ class NativeOps:
     """The kernels as methods.  Libraries are compiled and loaded on first use."""
 
     F32_ROWS = 4096         # rows of one float32 product
-    FP4_PREFILL_MIN_ROWS = 128   # rows (tokens x query heads of a key head) of a request from which the 4-bit cache's tcgen05 kernel is used
+    FP4_PREFILL_MIN_ROWS = 64    # rows (tokens x query heads of a key head) of a request from which the 4-bit cache's tcgen05 kernel is used
+                                 # whatever the context (csrc/fp4_calls.cpp has the times of both sides)
     PREFILL_MIN_Q = 96      # portions at least this long go to the tcgen05 prefill attention kernel
     FUSE_MAX_ROWS = 16      # steps of at most this many tokens let a product add itself to the residual stream and
                             # prepare the norm that follows in its own kernel; with more rows product + norm

@@ -60,7 +60,8 @@ struct Params {
     long long n_pages;
     int table_stride, table_cols;
     int n_heads, n_kv_heads, group, page_records;
-    int n_blocks, pieces, window;
+    int n_seqs, pieces, window;
+    int most_blocks;            // of a request
     unsigned per_group;         // 2^32 / group and one more (0 for a group of one head): row / group without a division
     float scale_log2;
 };
@@ -310,13 +311,33 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_fp4_prefill_kernel(cons
     grid_launch_dependents();
     grid_dependency_wait();         // (lengths, tables, queries and the cache itself may come from the kernels before this one)
 
-    const int b = blockIdx.z, kvh = blockIdx.x / p.pieces, piece = blockIdx.x - kvh * p.pieces;
+    const int per_block = p.n_kv_heads * p.pieces, index = blockIdx.x / per_block, rest = blockIdx.x - index * per_block;
+    const int kvh = rest / p.pieces, piece = rest - kvh * p.pieces;
+    // The blocks of all requests are numbered through; the request's that this one is (every warp for itself, 32 requests at a time)
+    int b = 0, number = -1;
+    for (int b0 = 0, before = 0; b0 < p.n_seqs && number < 0; b0 += 32) {
+        const int mine = b0 + lane;
+        const int count = mine < p.n_seqs ? min(((p.q_start[mine + 1] - p.q_start[mine]) * p.group + QT * BM - 1) / (QT * BM), p.most_blocks) : 0;
+        int upto = count;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+        }
+        const unsigned here = __ballot_sync(0xffffffffu, before + upto > index);
+        if (here) {
+            const int src = __ffs(here) - 1;
+            b = b0 + src;
+            number = before + __shfl_sync(0xffffffffu, upto, src) - 1 - index;       // (the blocks that see most keys begin first)
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
+    }
     const int first_token = p.q_start[b];
     const int ql = p.q_start[b + 1] - first_token;
     const int base = p.kv_len[b] - ql;
-    const int row0 = (p.n_blocks - 1 - (int)blockIdx.y) * (QT * BM);      // (the blocks that see most keys begin first)
+    const int row0 = max(number, 0) * (QT * BM);
     const int all_rows = ql * p.group;
-    const bool active = row0 < all_rows && *(volatile int*)failed == 0;
+    const bool active = number >= 0 && *(volatile int*)failed == 0;
     const int last_row = min(row0 + QT * BM, all_rows) - 1;
     // keys lo .. hi - 1 of the block, and of this piece of them (whole tiles)
     int lo = p.window > 0 ? max(0, base + token_of(p, row0) - p.window + 1) : 0;
@@ -731,21 +752,24 @@ bool takes(int n_heads, int n_kv_heads, int head_dim, int page_size) {
 }
 
 struct Plan {
-    int blocks, pieces;
+    long long of_request, blocks;       // blocks of a request, of all: at most
+    int pieces;
 };
-Plan make_plan(int n_seqs, int n_heads, int n_kv_heads, int max_q_len, int max_kv_len) {
+Plan make_plan(long long q_rows, int n_seqs, int n_heads, int n_kv_heads, int max_q_len, int max_kv_len) {
     Plan pl;
-    const long long rows = (long long)max_q_len * (n_heads / n_kv_heads);
-    pl.blocks = (int)((rows + QT * BM - 1) / (QT * BM));
+    const long long group = n_heads / n_kv_heads, rows = max_q_len * group;
+    pl.of_request = (rows + QT * BM - 1) / (QT * BM);
+    pl.blocks = pl.of_request * n_seqs;
+    if (q_rows * group / (QT * BM) + n_seqs < pl.blocks) pl.blocks = q_rows * group / (QT * BM) + n_seqs;
     pl.pieces = 1;
     // CTAs run in waves of 148, one an SM.  A piece takes as long as its tiles and about five more (the queries, the first and
     // the last tile's way through the roles, the results); the sums of pieces cost writing and adding up.
-    const long long ctas = (long long)pl.blocks * n_kv_heads * n_seqs;
+    const long long ctas = pl.blocks * n_kv_heads;
     const int tiles = (max_kv_len + BN - 1) / BN;
     double best = 1e30;
     for (int s = 1; s <= MOST_PIECES && s <= tiles; ++s) {
         const double waves = (double)((ctas * s + 147) / 148);
-        const double cost = waves * ((tiles + s - 1) / s + 5) + (s > 1 ? 4 + 0.02 * s * rows * n_kv_heads * n_seqs / 148.0 / 16.0 : 0.0);
+        const double cost = waves * ((tiles + s - 1) / s + 5) + (s > 1 ? 4 + 0.02 * s * (double)(q_rows * group < rows * n_seqs ? q_rows * group : rows * n_seqs) * n_kv_heads / 148.0 / 16.0 : 0.0);
         if (cost < best - 1e-9) {
             best = cost;
             pl.pieces = s;
@@ -776,7 +800,7 @@ extern "C" int tl_attention_fp4_prefill_supports(int n_heads, int n_kv_heads, in
 extern "C" int tl_attention_fp4_prefill_plan(long long q_rows, int n_seqs, int n_heads, int n_kv_heads, int head_dim, int max_q_len, int max_kv_len,
                                              int allow_split, int* pieces, long long* workspace_floats) {
     if (!takes(n_heads, n_kv_heads, head_dim, FP4_RECORD) || max_q_len < 1 || n_seqs < 1) return TL_BAD_SIZE;
-    const Plan pl = make_plan(n_seqs, n_heads, n_kv_heads, max_q_len, max_kv_len);
+    const Plan pl = make_plan(q_rows, n_seqs, n_heads, n_kv_heads, max_q_len, max_kv_len);
     *pieces = allow_split > 1 ? (allow_split < MOST_PIECES ? allow_split : MOST_PIECES) : allow_split ? pl.pieces : 1;
     *workspace_floats = *pieces > 1 ? q_rows * n_heads * *pieces * (head_dim + 2) : 0;
     return TL_OK;
@@ -794,21 +818,21 @@ extern "C" int tl_attention_fp4_prefill(const void* q, const void* k_pages, cons
     auto aligned32 = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 31u) == 0; };
     if (!aligned16(q) || !aligned32(out) || !aligned16(k_pages) || !aligned16(v_pages) || status == nullptr) return TL_BAD_ALIGN;
     if (pieces > 1 && (workspace == nullptr || !aligned32(workspace))) return TL_BAD_SIZE;
-    const Plan pl = make_plan(n_seqs, n_heads, n_kv_heads, max_q_len, 1);
-    if (n_seqs > 65535 || pl.blocks > 65535) return TL_BAD_SIZE;
+    const Plan pl = make_plan(q_rows, n_seqs, n_heads, n_kv_heads, max_q_len, 1);
+    if ((double)pl.blocks * n_kv_heads * pieces >= 2147483647.0) return TL_BAD_SIZE;
     Params p;
     p.q = (const __nv_bfloat16*)q; p.out = (__nv_bfloat16*)out;
     p.k_pages = (const unsigned char*)k_pages; p.v_pages = (const unsigned char*)v_pages;
     p.block_table = block_table; p.q_start = q_start; p.kv_len = kv_len; p.status = status; p.n_pages = n_pages;
     p.table_stride = table_stride; p.table_cols = table_cols; p.n_heads = n_heads; p.n_kv_heads = n_kv_heads; p.group = n_heads / n_kv_heads;
-    p.page_records = page_size / FP4_RECORD; p.n_blocks = pl.blocks; p.pieces = pieces; p.window = window > 0 ? window : 0;
+    p.page_records = page_size / FP4_RECORD; p.n_seqs = n_seqs; p.most_blocks = (int)pl.of_request; p.pieces = pieces; p.window = window > 0 ? window : 0;
     p.per_group = p.group == 1 ? 0u : (unsigned)((1ull << 32) / (unsigned)p.group) + 1u;
-    if ((double)pl.blocks * QT * BM * p.group >= 4294967296.0) return TL_BAD_SIZE;
+    if ((double)pl.of_request * QT * BM * p.group >= 4294967296.0) return TL_BAD_SIZE;
     p.scale_log2 = scale * LOG2E;
     p.part_o = workspace;
     p.part_ml = pieces > 1 ? workspace + q_rows * n_heads * pieces * head_dim : nullptr;
     cudaStream_t s = (cudaStream_t)stream;
-    const dim3 grid(pieces * n_kv_heads, pl.blocks, n_seqs);
+    const dim3 grid((unsigned)(pl.blocks * n_kv_heads * pieces));
     const int rc = head_dim == 128 ? launch<128>(p, grid, s) : launch<64>(p, grid, s);
     if (rc != TL_OK || pieces == 1) return rc;
     const unsigned merge = (unsigned)((q_rows * n_heads + 3) / 4);

@@ -19,8 +19,7 @@
 // Weights are multiplied as one float16 (2^-12; the result's own rounding is 2^-9), 2^BIAS times as large as they are, so that
 // weights down to 2^-32 of the largest count; the row's sum carries the same factor.
 //
-// Scores, weights and accumulators have tensor memory of their own.  With head_dim 128 there is room for one score buffer, which the
-// row tiles use in turn.  Where rows are few and keys are many the keys are cut into pieces, which leave
+// Scores, weights and accumulators have tensor memory of their own; the row tiles use one score buffer in turn.  Where rows are few and keys are many the keys are cut into pieces, which leave
 // float32 sums that a second kernel adds up in order.
 //
 // Every mbarrier wait is bounded in time; on a time-out the CTA records a code in the status word, lets its products land, frees its
@@ -208,7 +207,7 @@ __device__ __forceinline__ unsigned pack_half(float lo, float hi) {
 template <int KSTAGES, int VSTAGES>
 struct Tail {                   // what lies behind the tiles in shared memory
     unsigned long long q_full, k_full[KSTAGES], k_empty[KSTAGES], v_full[VSTAGES], v_empty[VSTAGES];
-    unsigned long long s_full[QT], s_free[QT], p_half[QT], p_full[QT], pv_done[QT], settled[2];
+    unsigned long long s_full[QT], s_free, p_half[QT], p_full[QT], pv_done[QT], settled[2];
     unsigned tmem_base_slot;
     int failed_flag;
 };
@@ -264,9 +263,9 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_fp4_prefill_kernel(cons
     constexpr int HALVES = HD / 64;
     constexpr unsigned HALF_BYTES = BN * 128;
     constexpr unsigned KV_BYTES = HALVES * HALF_BYTES;
-    // Tensor memory.  With head_dim 64 every row tile has a score buffer, with 128 both use one in turn.
-    constexpr int NS = HD == 64 ? 2 : 1;
-    constexpr unsigned COL_S = 0, COL_P = NS * BN, COL_O = COL_P + QT * (BN / 2);
+    // Tensor memory: a score buffer, which the row tiles use in turn.  (With head_dim 64 there is room for two; but then both row tiles wait for the
+    // exponential unit together and leave it idle together: 3,290 cycles for 128 keys of both, so 3,080.)
+    constexpr unsigned COL_S = 0, COL_P = BN, COL_O = COL_P + QT * (BN / 2);
     static_assert(COL_O + QT * HD <= TMEM_COLS, "scores, weights and accumulators must fit the tensor memory of a CTA");
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* Qs = smem_raw;
@@ -277,6 +276,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_fp4_prefill_kernel(cons
     if (tid == 0) {
         tail.failed_flag = 0;
         mbar_init(&tail.q_full, 4 * QT);
+        mbar_init(&tail.s_free, 4);
         for (int s = 0; s < KSTAGES; ++s) {
             mbar_init(&tail.k_full[s], 4);
             mbar_init(&tail.k_empty[s], QT);
@@ -287,7 +287,6 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_fp4_prefill_kernel(cons
         }
         for (int t = 0; t < QT; ++t) {
             mbar_init(&tail.s_full[t], 1);
-            mbar_init(&tail.s_free[t], 4);
             mbar_init(&tail.p_half[t], 4);
             mbar_init(&tail.p_full[t], 4);
             mbar_init(&tail.pv_done[t], 1);
@@ -384,15 +383,14 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_fp4_prefill_kernel(cons
                     for (int t = 0; t < QT; ++t) {
                         if (!ok) break;
                         if (j >= range[t].first && j < range[t].last) {
-                            const int before = NS == 1 ? used : j - range[t].first;
-                            if (before > 0) ok = __all_sync(0xffffffffu, mbar_wait(&tail.s_free[NS == 1 ? 0 : t], (before - 1) & 1, failed));
+                            if (used > 0) ok = __all_sync(0xffffffffu, mbar_wait(&tail.s_free, (used - 1) & 1, failed));
                             if (!ok) break;
                             tc_fence_after();
                             const unsigned long long qd0 = desc_k_major(smem_u32(Qs + t * KV_BYTES));
 #pragma unroll
                             for (int kd = 0; kd < HD / 16; ++kd) {
                                 const unsigned off = ((kd / 4) * HALF_BYTES + (kd % 4) * 32) >> 4;
-                                umma_ss_elect(tmem + COL_S + (NS == 1 ? 0 : t * BN), qd0 + off, kd0 + off, id_s, kd > 0 ? 1u : 0u);
+                                umma_ss_elect(tmem + COL_S, qd0 + off, kd0 + off, id_s, kd > 0 ? 1u : 0u);
                             }
                             umma_commit_elect(&tail.s_full[t]);
                             umma_commit_elect(&tail.k_empty[s]);
@@ -546,7 +544,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_fp4_prefill_kernel(cons
             __syncwarp();
             if (lane == 0) mbar_arrive(&tail.q_full);
         }
-        const unsigned col_s = COL_S + (NS == 1 ? 0 : t * BN), col_p = COL_P + t * (BN / 2), col_o = COL_O + t * HD;
+        const unsigned col_s = COL_S, col_p = COL_P + t * (BN / 2), col_o = COL_O + t * HD;
         const float fit = back * p.scale_log2;
         float m_used = -INFINITY, l_sum = 0.f;
         const int qpos = base + token_of(p, tile_row0 + (r < rows ? r : max(rows - 1, 0)));
@@ -563,7 +561,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_fp4_prefill_kernel(cons
             tmem_wait_ld();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&tail.s_free[NS == 1 ? 0 : t]);      // the buffer may take the next scores
+            if (lane == 0) mbar_arrive(&tail.s_free);      // the buffer may take the next scores
             const bool clear = k0 >= lo && k0 + BN <= hi && k0 + BN - 1 <= low && (p.window <= 0 || k0 > high - p.window);
             if (!clear) {
                 const int from = max(lo, p.window > 0 ? qpos - p.window + 1 : 0), to = min(hi, qpos + 1);

@@ -225,6 +225,21 @@ def test_requests_that_are_cut_and_have_an_odd_number_of_rows(group, D, q_lens, 
     judge(got, a, kw)
 
 
+@pytest.mark.parametrize("H,KV,D,q_lens,kv_lens,window", [
+    (32, 8, 64, [65, 0, 200, 7], [65, 30, 777, 7], None),
+    (28, 4, 128, [130, 91], [130, 400], None),
+    (8, 8, 64, [301, 64, 515], [800, 64, 515], 70),
+    (16, 8, 128, [250, 33, 1], [450, 40, 1000], 129),
+])
+def test_float32_prompts(H, KV, D, q_lens, kv_lens, window):
+    """Many rows: every warp has some of its own."""
+    a, kw = batch(H, KV, D, 16, q_lens, kv_lens, window, "f32")
+    got = ops().paged_attention_fp4(**a, **kw)
+    ops().check_status()
+    judge(got, a, kw)
+    assert torch.equal(ops().paged_attention_fp4(**a, **kw), got)
+
+
 def test_an_output_on_16_bytes():
     """(the tcgen05 kernel stores 32 bytes at a time: another runs where the output does not lie so)"""
     a, kw = batch(8, 2, 64, 16, [70], [120])

@@ -18,7 +18,7 @@
 //   - Probabilities of bfloat16 steps are one float16 each (2^-12; the result's own rounding is 2^-9).
 //
 // Who does what: the rows of a request (token x query heads of a key head) are cut into blocks of 8 NT; the keys that a block sees, in
-// tiles of 128, are laid on one line, block after block and key head after key head, with the worth of WORTH tiles in front of each
+// tiles of 128, are laid on one line, block after block and key head after key head, with the worth of one or two tiles in front of each
 // for what it costs to begin and end one, and every CTA takes an even stretch of the line, found on the device from the
 // requests' lengths.  Where a block is cut, each part leaves its sums, and the CTA that is last to finish adds them up in
 // order (a counter for each block and head): the result does not depend on who that is.
@@ -34,7 +34,6 @@ constexpr int EACH = 2;                 // records that a consumer warp takes of
 constexpr int RECORDS = EACH * NCW;     // records of a tile
 constexpr int BN = RECORDS * FP4_RECORD;
 constexpr int NTHREADS = (NCW + 1) * 32;
-constexpr int WORTH = 2;                // what a block's beginning and end are worth, in tiles
 constexpr int MOST_PARTS = 64;          // parts of a block, at most
 constexpr int FAILED_PART = 1 << 16;    // what a CTA that gave up adds to a counter beside its 1
 constexpr int SMS = 148;
@@ -144,6 +143,9 @@ __device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;
 __device__ __forceinline__ int token_of(const Params& p, int row) { return p.per_group ? (int)__umulhi((unsigned)row, p.per_group) : row; }
 
 // ---- the line of tiles
+// What a block's beginning and end are worth, in tiles: a tile of 64 rows is four times the work of one of 16.  (8 requests of 32,000 tokens 37.0 us
+// with 1 and 35.9 with 2, a 32-bit prompt of 16 rows a block 79 and 73; with 64 rows a block 56.0 with 1 and 58.5 with 2.)
+__host__ __device__ constexpr int worth_of(int rows) { return rows > 16 ? 1 : 2; }
 // What a block of a request's rows sees.
 struct Block {
     int b, number;
@@ -167,7 +169,7 @@ template <int ROWS> __device__ __forceinline__ int block_at(const Params& p, int
     k.hi = min(k.base + t1 + 1, p.table_cols * p.page_records * FP4_RECORD);
     k.start = k.lo & ~(FP4_RECORD - 1);
     k.tiles = max((k.hi - k.start + BN - 1) / BN, 1);
-    return k.tiles + WORTH;
+    return k.tiles + worth_of(ROWS);
 }
 // A CTA's way along its stretch: parts of blocks, one after the other.
 struct Walk {
@@ -179,14 +181,14 @@ struct Walk {
     int parts;          // in how many parts the block is cut (for this head)
 };
 template <int ROWS> __device__ __forceinline__ bool walk_here(const Params& p, Walk& w) {      // the part of the place where w stands; false: beyond the stretch
-    if (w.off + WORTH >= w.end) return false;
-    w.t0 = max(0, w.begin - w.off - WORTH);
-    w.t1 = min(w.k.tiles, w.end - w.off - WORTH);
-    w.parts = w.t1 - w.t0 == w.k.tiles ? 1 : (w.off + WORTH + w.k.tiles - 1) / w.share - (w.off + WORTH) / w.share + 1;
+    if (w.off + worth_of(ROWS) >= w.end) return false;
+    w.t0 = max(0, w.begin - w.off - worth_of(ROWS));
+    w.t1 = min(w.k.tiles, w.end - w.off - worth_of(ROWS));
+    w.parts = w.t1 - w.t0 == w.k.tiles ? 1 : (w.off + worth_of(ROWS) + w.k.tiles - 1) / w.share - (w.off + worth_of(ROWS)) / w.share + 1;
     return true;
 }
 template <int ROWS> __device__ __forceinline__ bool walk_next(const Params& p, Walk& w) {
-    w.off += w.k.tiles + WORTH;
+    w.off += w.k.tiles + worth_of(ROWS);
     if (++w.kvh == p.n_kv_heads) {
         w.kvh = 0;
         do {
@@ -206,7 +208,7 @@ template <int ROWS> __device__ __forceinline__ bool walk_first(const Params& p, 
     }
     total = __reduce_add_sync(0xffffffffu, total) * p.n_kv_heads;
     longest = __reduce_max_sync(0xffffffffu, longest);
-    w.share = max(max((total + (int)gridDim.x - 1) / (int)gridDim.x, (longest + MOST_PARTS - 2) / (MOST_PARTS - 1)), 1 + WORTH);
+    w.share = max(max((total + (int)gridDim.x - 1) / (int)gridDim.x, (longest + MOST_PARTS - 2) / (MOST_PARTS - 1)), 1 + worth_of(ROWS));
     w.begin = blockIdx.x * w.share;
     w.end = w.begin + w.share;
     if (w.begin >= total) return false;
@@ -345,16 +347,17 @@ struct Consumer {
         }
     }
 
-    // EACH records of keys and of values, records NCW apart; the first begins with key k0
-    __device__ __forceinline__ void records(const Params& p, const unsigned char* kr, const unsigned char* vr, int k0, int lo, int hi) {
+    // EACH records of keys and of values, APART records apart; the first begins with key k0
+    template <int APART> __device__ __forceinline__ void records(const Params& p, const unsigned char* kr, const unsigned char* vr, int k0, int lo, int hi) {
         constexpr int CODES = FP4_RECORD * (HD / 2);            // where a record's scales begin
-        constexpr int RECORD = fp4_record_bytes(HD), STEP = NCW * FP4_RECORD, SPAN = (EACH - 1) * STEP + FP4_RECORD;
+        constexpr int RECORD = fp4_record_bytes(HD), STEP = APART * FP4_RECORD, SPAN = (EACH - 1) * STEP + FP4_RECORD;
         if (k0 > qmax || k0 + SPAN <= lo || k0 >= hi) return;
+        if (APART == 1 && p.window > 0 && k0 + SPAN - 1 <= qmin - p.window) return;     // (the first key of a block is the first row's)
         // ---- scores
         float sc[EACH][NT][4];
 #pragma unroll
         for (int n = 0; n < EACH; ++n) {
-            const unsigned char* rec = kr + n * NCW * RECORD;
+            const unsigned char* rec = kr + n * APART * RECORD;
             float low[NT][4];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
@@ -479,7 +482,7 @@ struct Consumer {
         constexpr int VW = HD / 64;                               // words of a token a lane has
 #pragma unroll
         for (int n = 0; n < EACH; ++n) {
-            const unsigned char* rec = vr + n * NCW * RECORD;
+            const unsigned char* rec = vr + n * APART * RECORD;
             unsigned vw[4][VW], byte[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -543,6 +546,32 @@ struct Consumer {
         }
     }
 
+    // Results of a warp that has rows of its own: into out, or a part's sums.  A lane's numbers of a row are neighbours.
+    template <typename Row> __device__ __forceinline__ void finish(float* part, int part_rows, int row_in_part, int n_rows, Row out_row) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                float sum = l[nt][j];
+                sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+                const int rr = nt * 8 + 2 * t + j;
+                if (rr < n_rows) {
+                    const float inv = part != nullptr ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+                    const int at = row_in_part + rr;
+#pragma unroll
+                    for (int d = 0; d < KSTEPS; d += 2) {
+                        const float4 v = make_float4(o[nt][d][j] * inv, o[nt][d][j + 2] * inv, o[nt][d + 1][j] * inv, o[nt][d + 1][j + 2] * inv);
+                        if (part != nullptr) __stcg(reinterpret_cast<float4*>(part + at * HD + g * (HD / 8) + 2 * d), v);
+                        else store4(out_row(at) + g * (HD / 8) + 2 * d, v);
+                    }
+                    if (part != nullptr && g == 0)      // (no maximum remembers a score that is not a number)
+                        __stcg(reinterpret_cast<float2*>(part + part_rows * HD + 2 * at), make_float2(sum != sum ? NAN : m[nt][j], sum));
+                }
+            }
+    }
+
     // the warp's results: Om [NCW][rows][OPITCH], Mm and Lm [NCW][ROWS]
     __device__ __forceinline__ void leave(float* Om, float* Mm, float* Lm, int warp, int rows, int n_rows) {
 #pragma unroll
@@ -569,14 +598,15 @@ struct Consumer {
 // (a maximum that is not a number is kept: the row is not a number)
 __device__ __forceinline__ float max_keep(float a, float b) { return (a != a || b != b) ? NAN : fmaxf(a, b); }
 
-template <typename T, int HD, int STAGES, int NT>
+// OWN: every consumer warp has 8 NT rows of its own and takes all records of a tile; else the warps share the rows, and a tile's records.
+template <typename T, int HD, int STAGES, int NT, bool OWN>
 __global__ void __launch_bounds__(NTHREADS, (NT == 1 && sizeof(T) == 2) ? 3 : 2) attention_fp4_decode_kernel(const Params p) {
     using C = Consumer<T, HD, NT>;
-    constexpr int ROWS = 8 * NT, RECORD = fp4_record_bytes(HD);
+    constexpr int ROWS = (OWN ? NCW : 1) * 8 * NT, RECORD = fp4_record_bytes(HD);
     constexpr unsigned STAGE = 2 * RECORDS * RECORD;
     extern __shared__ __align__(128) unsigned char smem[];        // the ring, then the warps' results
     float* Om = reinterpret_cast<float*>(smem + STAGES * STAGE);
-    __shared__ float Mm[NCW * ROWS], Lm[NCW * ROWS];
+    __shared__ float Mm[OWN ? 1 : NCW * ROWS], Lm[OWN ? 1 : NCW * ROWS];
     __shared__ __align__(8) unsigned long long full_bar[STAGES];
     __shared__ __align__(8) unsigned long long empty_bar[STAGES];
     __shared__ int failed_flag, arrived, gave_up;
@@ -640,14 +670,25 @@ __global__ void __launch_bounds__(NTHREADS, (NT == 1 && sizeof(T) == 2) ? 3 : 2)
     int s = 0;
     unsigned phase = 0;
     do {
-        c.begin(p, w.k, w.kvh, lane);
+        Block mine = w.k;
+        if (OWN) {
+            mine.row0 += warp * 8 * NT;
+            mine.n_rows = min(max(mine.n_rows - warp * 8 * NT, 0), 8 * NT);
+        }
+        c.begin(p, mine, w.kvh, lane);
         for (int i = w.t0; i < w.t1; ++i) {
             if (!ok || !warp_wait(&full_bar[s], phase, &failed_flag, p.status, ERR_CONSUMER_WAIT, lane)) {
                 ok = false;
                 break;
             }
-            const unsigned char* kr = smem + s * STAGE + warp * RECORD;
-            c.records(p, kr, kr + RECORDS * RECORD, w.k.start + i * BN + warp * FP4_RECORD, w.k.lo, w.k.hi);
+            const unsigned char* kr = smem + s * STAGE;
+            if (OWN) {
+#pragma unroll 1
+                for (int r = 0; r < RECORDS; r += EACH)
+                    c.template records<1>(p, kr + r * RECORD, kr + (RECORDS + r) * RECORD, w.k.start + i * BN + r * FP4_RECORD, w.k.lo, w.k.hi);
+            } else {
+                c.template records<NCW>(p, kr + warp * RECORD, kr + (RECORDS + warp) * RECORD, w.k.start + i * BN + warp * FP4_RECORD, w.k.lo, w.k.hi);
+            }
             __syncwarp();
             if (lane == 0) mbar_arrive(&empty_bar[s]);     // this warp is done with the stage
             if (++s == STAGES) {
@@ -655,15 +696,6 @@ __global__ void __launch_bounds__(NTHREADS, (NT == 1 && sizeof(T) == 2) ? 3 : 2)
                 phase ^= 1u;
             }
         }
-        // ---- the four warps' results, through shared memory
-        consumers_sync();
-        c.leave(Om, Mm, Lm, warp, p.rows, w.k.n_rows);
-        // (the producer may give up at any moment: one thread reads the flag for all, so that all take the same way
-        // through the barriers below; what this part is made of has arrived by now, or a consumer has set the flag)
-        if (tid == 0) gave_up = *(volatile int*)&failed_flag;
-        consumers_sync();
-        const bool sound = gave_up == 0;
-        const int n_rows = w.k.n_rows;
         auto out_row = [&](int rr) {
             const int row = w.k.row0 + rr, token = token_of(p, row);
             return reinterpret_cast<T*>(p.out) + ((size_t)(w.k.first + token) * p.n_heads + w.kvh * p.group + row - token * p.group) * HD;
@@ -671,7 +703,22 @@ __global__ void __launch_bounds__(NTHREADS, (NT == 1 && sizeof(T) == 2) ? 3 : 2)
         // where a part of this block lies: that with its first tile in its CTA's first place, others in the second
         const size_t place = part_floats(p.rows, HD);
         auto part_of = [&](int cta, bool first) { return p.part + ((size_t)cta * 2 + (first ? 0 : 1)) * place; };
-        if (sound) {
+        if (OWN && w.parts == 1) {
+            if (ok) c.finish(nullptr, 0, warp * 8 * NT, mine.n_rows, out_row);
+            continue;
+        }
+        // ---- the four warps' results, through shared memory
+        consumers_sync();
+        if (!OWN) c.leave(Om, Mm, Lm, warp, p.rows, w.k.n_rows);
+        // (the producer may give up at any moment: one thread reads the flag for all, so that all take the same way
+        // through the barriers below; what this part is made of has arrived by now, or a consumer has set the flag)
+        if (tid == 0) gave_up = *(volatile int*)&failed_flag;
+        consumers_sync();
+        const bool sound = gave_up == 0;
+        const int n_rows = w.k.n_rows;
+        if (OWN) {
+            if (sound) c.finish(part_of(blockIdx.x, w.t0 == 0), p.rows, warp * 8 * NT, mine.n_rows, out_row);
+        } else if (sound) {
             float* part = part_of(blockIdx.x, w.t0 == 0);
             for (int idx = tid; idx < n_rows * (HD / 4); idx += NCW * 32) {      // four columns of a row per turn
                 const int rr = idx / (HD / 4), d = (idx - rr * (HD / 4)) * 4;
@@ -715,7 +762,7 @@ __global__ void __launch_bounds__(NTHREADS, (NT == 1 && sizeof(T) == 2) ? 3 : 2)
             consumers_sync();
             if (arrived == w.parts) {
                 // (eight parts at a time are under way)
-                const int cta0 = (w.off + WORTH) / w.share;
+                const int cta0 = (w.off + worth_of(ROWS)) / w.share;
                 for (int idx = tid; idx < n_rows * (HD / 4); idx += NCW * 32) {
                     const int rr = idx / (HD / 4), d = (idx - rr * (HD / 4)) * 4;
                     float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -761,8 +808,8 @@ __global__ void __launch_bounds__(NTHREADS, (NT == 1 && sizeof(T) == 2) ? 3 : 2)
 // ---- host side ---------------------------------------------------------------------------------
 
 template <int HD> constexpr int stages_for() { return HD == 128 ? 3 : 5; }
-template <int HD> size_t smem_for(int rows) {
-    return (size_t)stages_for<HD>() * 2 * RECORDS * fp4_record_bytes(HD) + (size_t)NCW * rows * (HD + 4) * 4;
+template <int HD> size_t smem_for(int rows, bool own) {
+    return (size_t)stages_for<HD>() * 2 * RECORDS * fp4_record_bytes(HD) + (own ? 0 : (size_t)NCW * rows * (HD + 4) * 4);
 }
 
 bool takes(int n_heads, int n_kv_heads, int head_dim, int page_size) {
@@ -772,17 +819,18 @@ bool takes(int n_heads, int n_kv_heads, int head_dim, int page_size) {
 }
 
 struct Plan {
+    bool own;
     int nt, rows, blocks, ctas;
     size_t smem;
 };
 
-template <typename T, int HD, int NT> int ctas_per_sm(int rows) {
-    static int known[8 * NT + 1] = {};                     // (threads that come here at the same time write the same)
+template <typename T, int HD, int NT, bool OWN> int ctas_per_sm(int rows) {
+    static int known[8 * NT * NCW + 1] = {};               // (threads that come here at the same time write the same)
     if (known[rows] == 0) {
-        auto kern = attention_fp4_decode_kernel<T, HD, stages_for<HD>(), NT>;
+        auto kern = attention_fp4_decode_kernel<T, HD, stages_for<HD>(), NT, OWN>;
         int n = 0;
-        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_for<HD>(8 * NT)) != cudaSuccess ||
-            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, NTHREADS, smem_for<HD>(rows)) != cudaSuccess || n < 1) {
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_for<HD>(8 * NT, OWN)) != cudaSuccess ||
+            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, NTHREADS, smem_for<HD>(rows, OWN)) != cudaSuccess || n < 1) {
             cudaGetLastError();
             n = 1;
         }
@@ -790,27 +838,40 @@ template <typename T, int HD, int NT> int ctas_per_sm(int rows) {
     }
     return known[rows];
 }
-template <typename T, int HD> int ctas_per_sm(int nt, int rows) { return nt == 1 ? ctas_per_sm<T, HD, 1>(rows) : ctas_per_sm<T, HD, 2>(rows); }
+template <int HD> int ctas_per_sm(int dtype, const bool own, int nt, int rows) {
+    if (dtype == TL_F32)
+        return own ? ctas_per_sm<float, HD, 2, true>(rows) : nt == 1 ? ctas_per_sm<float, HD, 1, false>(rows) : ctas_per_sm<float, HD, 2, false>(rows);
+    return nt == 1 ? ctas_per_sm<__nv_bfloat16, HD, 1, false>(rows) : ctas_per_sm<__nv_bfloat16, HD, 2, false>(rows);
+}
 
 Plan make_plan(int dtype, int n_seqs, int n_heads, int n_kv_heads, int head_dim, int max_q_len, int max_kv_len) {
     Plan pl;
     const long long all = (long long)max_q_len * (n_heads / n_kv_heads);
+    // float32 steps of many rows: rows of its own for each warp, where that gives 96 blocks or more.  (us, shared rows and own: 32 / 8 heads of 64,
+    // 3 requests of 64 tokens behind 500, 96 blocks, 24.1 25.5; one of 128, 64 blocks, 19.4 25.5; one of 512, 256 blocks, 54.6 50.1; 8 of 512 behind 4,000
+    // 1,430 1,210; heads of 128: 52.6 46.3; 39.4 45.9; 136 94; 4,167 2,333.)
+    constexpr int OWN = NCW * 16;
+    pl.own = dtype == TL_F32 && all >= OWN && (double)n_seqs * ((all + OWN - 1) / OWN) * n_kv_heads >= 96.0;
     pl.nt = all <= 8 ? 1 : 2;
-    pl.rows = all < 8 * pl.nt ? (int)all : 8 * pl.nt;
-    pl.blocks = (int)((all + 8 * pl.nt - 1) / (8 * pl.nt));
-    pl.smem = head_dim == 128 ? smem_for<128>(pl.rows) : smem_for<64>(pl.rows);
-    const int fit = dtype == TL_F32 ? (head_dim == 128 ? ctas_per_sm<float, 128>(pl.nt, pl.rows) : ctas_per_sm<float, 64>(pl.nt, pl.rows))
-                                    : (head_dim == 128 ? ctas_per_sm<__nv_bfloat16, 128>(pl.nt, pl.rows) : ctas_per_sm<__nv_bfloat16, 64>(pl.nt, pl.rows));
+    const int most = 8 * pl.nt * (pl.own ? NCW : 1);
+    pl.rows = all < most ? (int)all : most;
+    pl.blocks = (int)((all + most - 1) / most);
+    pl.smem = head_dim == 128 ? smem_for<128>(pl.rows, pl.own) : smem_for<64>(pl.rows, pl.own);
+    const int fit = head_dim == 128 ? ctas_per_sm<128>(dtype, pl.own, pl.nt, pl.rows) : ctas_per_sm<64>(dtype, pl.own, pl.nt, pl.rows);
     // no more CTAs than there can be tiles
-    const double most = (double)n_seqs * pl.blocks * n_kv_heads * ((max_kv_len + BN - 1) / BN + 1);
-    pl.ctas = most < (double)SMS * fit ? (int)most : SMS * fit;
+    const double tiles = (double)n_seqs * pl.blocks * n_kv_heads * ((max_kv_len + BN - 1) / BN + 1);
+    pl.ctas = tiles < (double)SMS * fit ? (int)tiles : SMS * fit;
     if (pl.ctas < 1) pl.ctas = 1;
     return pl;
 }
 
-template <typename T, int HD> int launch(const Params& p, const Plan& pl, cudaStream_t s) {      // (ctas_per_sm has raised the limit on shared memory)
-    if (pl.nt == 1) return (int)tl_launch(attention_fp4_decode_kernel<T, HD, stages_for<HD>(), 1>, dim3(pl.ctas), dim3(NTHREADS), pl.smem, s, p);
-    return (int)tl_launch(attention_fp4_decode_kernel<T, HD, stages_for<HD>(), 2>, dim3(pl.ctas), dim3(NTHREADS), pl.smem, s, p);
+template <typename T, int HD, int NT, bool OWN> int launch(const Params& p, const Plan& pl, cudaStream_t s) {      // (ctas_per_sm has raised the limit on shared memory)
+    return (int)tl_launch(attention_fp4_decode_kernel<T, HD, stages_for<HD>(), NT, OWN>, dim3(pl.ctas), dim3(NTHREADS), pl.smem, s, p);
+}
+template <int HD> int launch(int dtype, const Params& p, const Plan& pl, cudaStream_t s) {
+    if (dtype == TL_F32)
+        return pl.own ? launch<float, HD, 2, true>(p, pl, s) : pl.nt == 1 ? launch<float, HD, 1, false>(p, pl, s) : launch<float, HD, 2, false>(p, pl, s);
+    return pl.nt == 1 ? launch<__nv_bfloat16, HD, 1, false>(p, pl, s) : launch<__nv_bfloat16, HD, 2, false>(p, pl, s);
 }
 
 }  // namespace
@@ -843,7 +904,7 @@ extern "C" int tl_attention_fp4_decode(const void* q, const void* k_pages, const
     if (!aligned16(q) || !aligned16(out) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(workspace)) return TL_BAD_ALIGN;
     if (workspace == nullptr || counters == nullptr || status == nullptr) return TL_BAD_SIZE;
     const Plan pl = make_plan(dtype, n_seqs, n_heads, n_kv_heads, head_dim, max_q_len, max_kv_len);
-    if ((double)n_seqs * pl.blocks * n_kv_heads * ((double)table_cols * page_size / BN + 1 + WORTH) >= 2147483647.0) return TL_BAD_SIZE;
+    if ((double)n_seqs * pl.blocks * n_kv_heads * ((double)table_cols * page_size / BN + 3) >= 2147483647.0) return TL_BAD_SIZE;
     Params p;
     p.q = q; p.out = out; p.k_pages = (const unsigned char*)k_pages; p.v_pages = (const unsigned char*)v_pages;
     p.block_table = block_table; p.q_start = q_start; p.kv_len = kv_len;
@@ -858,6 +919,5 @@ extern "C" int tl_attention_fp4_decode(const void* q, const void* k_pages, const
     p.window = window > 0 ? window : 0;
     p.scale_log2 = scale * LOG2E;
     cudaStream_t s = (cudaStream_t)stream;
-    if (dtype == TL_F32) return head_dim == 128 ? launch<float, 128>(p, pl, s) : launch<float, 64>(p, pl, s);
-    return head_dim == 128 ? launch<__nv_bfloat16, 128>(p, pl, s) : launch<__nv_bfloat16, 64>(p, pl, s);
+    return head_dim == 128 ? launch<128>(dtype, p, pl, s) : launch<64>(dtype, p, pl, s);
 }

@@ -48,6 +48,9 @@ def turned(x, cs, interleaved):
     (149, 4, 2, 32, 16, 16, False, "bf16", 1),
     (180, 12, 2, 256, 8, 16, True, "bf16", 1),
     (148, 1, 1, 16, 16, 16, False, "f32", 1),
+    (155, 3, 2, 32, 32, 16, False, "f32", 1),        # (halves: a run and its partners together)
+    (166, 9, 3, 128, 32, 48, False, "bf16", 1),
+    (150, 40, 8, 256, 256, 16, False, "f32", 1),
     (5, 32, 8, 128, 128, 16, True, "bf16", 3),       # float32 partial sums
     (9, 4, 2, 64, 64, 16, False, "f32", 2),
 ])

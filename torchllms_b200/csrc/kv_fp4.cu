@@ -160,12 +160,18 @@ __global__ void __launch_bounds__(128) rope_kv_write_fp4_kernel(const TI* __rest
     }
 }
 
-// The same for rows of one plane and of the type that q leaves in, whose pairs are neighbours or halves of a multiple of 16, heads of a
-// power of two up to 1,024 and many tokens: a thread's runs lie a multiple of the head size apart, so that one run of the rotation table
-// serves them all, heads come by a shift, and the loads of a token (RUNS runs a thread, and their partners) are under way together.
-//   8,276 tokens, 48 heads of 128, bfloat16 (179 MB, 27 us of them): 36 us; with three runs at a time 40, with the kernel above
-//   and divisions 72.  Without the 4-bit numbers' arithmetic it would take 32: what bounds it next to memory.
-template <typename T> struct Runs { static constexpr int N = sizeof(T) == 2 ? 6 : 3; };
+// The same for rows of one plane and of the type that q leaves in, heads of a power of two up to 1,024 and many tokens: a thread's runs lie a
+// multiple of the head size apart, so that one run of the rotation table serves them all, heads come by a shift, and a
+// token's loads (EACH a thread) are under way together.  Where pairs are halves a thread takes both: a run and the run of its partners
+// (of what is not turned, a run of its first and one of its second half), a multiple of 16 apart.
+//   8,276 tokens, 48 heads of 128, bfloat16 (179 MB, 27 us of them): 36.7 us (4.9 TB/s); with three runs at a time 40, with the kernel above
+//   and divisions 72.  Without the 4-bit numbers' arithmetic it would take 32: what bounds it next to memory.  CTAs an SM, 8,276 / 4,000 / 600 tokens:
+//   8 (spills) 36.4 / 17.8 / 6.0, 7 36.7 / 17.1 / 5.4, 6 38.8 / 17.6 / 4.9.
+//   Halves, 4,000 tokens, float32 (168 MB, 26 us): 32.4 us (5.2 TB/s), bfloat16 20.5 (4.2 TB/s); fetching the partners beside every run 43.0 and 27.3.
+template <typename T, bool INTERLEAVED> struct Runs {
+    static constexpr int EACH = sizeof(T) == 2 && INTERLEAVED ? 6 : 3, PER = INTERLEAVED ? 1 : 2;
+    static constexpr int CTAS = sizeof(T) == 2 ? (INTERLEAVED ? 7 : 5) : (INTERLEAVED ? 5 : 4);       // of an SM, at least: what its registers are cut to
+};
 template <typename T> struct Run8 {                     // eight numbers as they are stored
     uint4 v[sizeof(T) / 2];
     __device__ __forceinline__ void load(const T* p) {
@@ -175,26 +181,29 @@ template <typename T> struct Run8 {                     // eight numbers as they
     __device__ __forceinline__ float get(int i) const { return to_float(reinterpret_cast<const T*>(v)[i]); }
 };
 template <typename T, bool INTERLEAVED>
-__global__ void __launch_bounds__(128, sizeof(T) == 2 && INTERLEAVED ? 8 : 5) rope_kv_write_fp4_rows_kernel(const T* __restrict__ qkv, T* __restrict__ q_out,
+__global__ void __launch_bounds__(128, Runs<T, INTERLEAVED>::CTAS) rope_kv_write_fp4_rows_kernel(const T* __restrict__ qkv, T* __restrict__ q_out,
                                                                                               const int log_runs, const WriteParams p) {
-    constexpr int EACH = Runs<T>::N;
+    constexpr int EACH = Runs<T, INTERLEAVED>::EACH, PER = Runs<T, INTERLEAVED>::PER;      // a thread's turns at a time, runs of a turn
     grid_launch_dependents();
     grid_dependency_wait();
     const int t = blockIdx.x;
-    const int heads = p.n_heads + 2 * p.n_kv_heads, runs = heads << log_runs;
-    const int off = (threadIdx.x & ((1 << log_runs) - 1)) << 3;
-    const int half = p.rot_dims >> 1;
-    const bool turns = off < p.rot_dims, first = off < half;
-    const int partner = first ? half : -half;            // (halves: where the other numbers of the pairs lie)
-    const T* src = qkv + (size_t)t * heads * p.head_dim;
-    Run8<T> raw[EACH], other[INTERLEAVED ? 1 : EACH];
+    const int log_head = log_runs + 3, log_turns = log_runs - (PER - 1);
+    const int heads = p.n_heads + 2 * p.n_kv_heads, turns_all = heads << log_turns;
+    const int turn = threadIdx.x & ((1 << log_turns) - 1), turned = p.rot_dims / (8 * PER);
+    const bool turns = turn < turned;
+    const int off = PER == 1 || turns ? turn * 8 : p.rot_dims + (turn - turned) * 8;
+    const int apart = PER == 1 ? 0 : (turns ? p.rot_dims : p.head_dim - p.rot_dims) >> 1;
+    // (whole runs follow one another: a turn's numbers, where it is one run, begin at 8 c)
+    const T* src = qkv + (size_t)t * (heads << log_head);
+    auto place = [&](int c) { return PER == 1 ? (size_t)c * 8 : ((size_t)(c >> log_turns) << log_head) + off; };
+    Run8<T> raw[EACH][PER];
     auto fetch = [&](int c0) {
 #pragma unroll
         for (int e = 0; e < EACH; ++e) {
             const int c = c0 + e * 128;
-            if (c < runs) {
-                raw[e].load(src + (size_t)c * 8);
-                if (!INTERLEAVED && turns && (c >> log_runs) < p.n_heads + p.n_kv_heads) other[INTERLEAVED ? 0 : e].load(src + (size_t)c * 8 + partner);
+            if (c < turns_all) {
+#pragma unroll
+                for (int i = 0; i < PER; ++i) raw[e][i].load(src + place(c) + i * apart);
             }
         }
     };
@@ -212,69 +221,69 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 && INTERLEAVED ? 8 : 5) ro
         // (a slot outside the cache is not written; debug builds report it)
         write = TL_CHECK(sm >= 0, TL_DBG_SLOT) && tl_check_page(page) && sm >= 0 && page < p.n_pages;
     }
-    float cs[INTERLEAVED ? 8 : 16];
+    float cs[8 * PER];
     if (turns) {
-        const float* at = p.table + (size_t)pos * p.rot_dims + (INTERLEAVED ? off : 2 * (first ? off : off - half));
+        const float* at = p.table + (size_t)pos * p.rot_dims + off * PER;
 #pragma unroll
-        for (int i = 0; i < (INTERLEAVED ? 2 : 4); ++i) {
+        for (int i = 0; i < 2 * PER; ++i) {
             const float4 v = *reinterpret_cast<const float4*>(at + 4 * i);
             cs[4 * i] = v.x; cs[4 * i + 1] = v.y; cs[4 * i + 2] = v.z; cs[4 * i + 3] = v.w;
         }
     }
     const float sc = warp_row_scale(p.rs, t);
     // (whole warps go round together: the lanes of a group exchange their maxima)
-    for (int c0 = threadIdx.x; c0 - (int)threadIdx.x < runs; c0 += EACH * 128) {
+    for (int c0 = threadIdx.x; c0 - (int)threadIdx.x < turns_all; c0 += EACH * 128) {
         if (c0 != (int)threadIdx.x) fetch(c0);
 #pragma unroll
         for (int e = 0; e < EACH; ++e) {
             const int c = c0 + e * 128;
-            if (c - (int)threadIdx.x >= runs) break;
-            const bool mine = c < runs;
-            const int head = c >> log_runs;
-            float x[8];
+            if (c - (int)threadIdx.x >= turns_all) break;
+            const bool mine = c < turns_all;
+            const int head = c >> log_turns;
+            float x[PER][8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = mine ? raw[e].get(i) : 0.f;
+            for (int k = 0; k < PER; ++k)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[k][i] = mine ? raw[e][k].get(i) : 0.f;
             if (p.rs.ssq != nullptr) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] *= sc;
+                for (int k = 0; k < PER; ++k)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x[k][i] *= sc;
             }
             if (turns && mine && head < p.n_heads + p.n_kv_heads) {
-                if (INTERLEAVED) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float a = x[2 * i], b = x[2 * i + 1];
-                        x[2 * i] = __fsub_rn(__fmul_rn(a, cs[2 * i]), __fmul_rn(b, cs[2 * i + 1]));
-                        x[2 * i + 1] = __fadd_rn(__fmul_rn(b, cs[2 * i]), __fmul_rn(a, cs[2 * i + 1]));
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        float y = other[INTERLEAVED ? 0 : e].get(i);
-                        if (p.rs.ssq != nullptr) y *= sc;
-                        const float u = __fmul_rn(x[i], cs[(2 * i) % (INTERLEAVED ? 8 : 16)]), v = __fmul_rn(y, cs[(2 * i + 1) % (INTERLEAVED ? 8 : 16)]);
-                        x[i] = first ? __fsub_rn(u, v) : __fadd_rn(u, v);
-                    }
+                for (int i = 0; i < 4 * PER; ++i) {
+                    float& u = PER == 1 ? x[0][2 * i] : x[0][i];
+                    float& v = PER == 1 ? x[0][2 * i + 1] : x[PER - 1][i];
+                    const float a = u, b = v;
+                    u = __fsub_rn(__fmul_rn(a, cs[2 * i]), __fmul_rn(b, cs[2 * i + 1]));
+                    v = __fadd_rn(__fmul_rn(b, cs[2 * i]), __fmul_rn(a, cs[2 * i + 1]));
                 }
             }
-            if (c - (int)threadIdx.x + 127 < (p.n_heads << log_runs)) {                // (the whole CTA has heads of q)
-                store8(q_out + ((size_t)t * p.n_heads << (log_runs + 3)) + (size_t)c * 8, x);
+            if (c - (int)threadIdx.x + 127 < (p.n_heads << log_turns)) {                // (the whole CTA has heads of q)
+#pragma unroll
+                for (int k = 0; k < PER; ++k) store8(q_out + ((size_t)t * p.n_heads << log_head) + place(c) + k * apart, x[k]);
                 continue;
             }
-            unsigned top = 0;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            if (!mine) continue;
-            if (head < p.n_heads) {
-                store8(q_out + ((size_t)t * p.n_heads << (log_runs + 3)) + (size_t)c * 8, x);
-            } else if (write) {
-                const bool is_k = head < p.n_heads + p.n_kv_heads;
-                const int kvh = is_k ? head - p.n_heads : head - p.n_heads - p.n_kv_heads;
-                unsigned char* base = is_k ? p.k_pages : p.v_pages;
-                const Fp4Place at = fp4_place(page, slot, kvh, p.n_kv_heads, p.page_size, p.head_dim);
-                const unsigned byte = fp4_scale_byte(top);
-                *reinterpret_cast<unsigned*>(base + at.codes + off / 2) = fp4_pack8(x, byte);
-                if ((off & 8) == 0) base[at.scales + off / FP4_GROUP] = (unsigned char)byte;
+            for (int k = 0; k < PER; ++k) {
+                unsigned top = 0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[k][i]) & 0x7fffffffu);
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                if (!mine) continue;
+                if (head < p.n_heads) {
+                    store8(q_out + ((size_t)t * p.n_heads << log_head) + place(c) + k * apart, x[k]);
+                } else if (write) {
+                    const bool is_k = head < p.n_heads + p.n_kv_heads;
+                    const int kvh = is_k ? head - p.n_heads : head - p.n_heads - p.n_kv_heads, d = off + k * apart;
+                    unsigned char* base = is_k ? p.k_pages : p.v_pages;
+                    const Fp4Place at = fp4_place(page, slot, kvh, p.n_kv_heads, p.page_size, p.head_dim);
+                    const unsigned byte = fp4_scale_byte(top);
+                    *reinterpret_cast<unsigned*>(base + at.codes + d / 2) = fp4_pack8(x[k], byte);
+                    if ((d & 8) == 0) base[at.scales + d / FP4_GROUP] = (unsigned char)byte;
+                }
             }
         }
     }
@@ -359,7 +368,7 @@ extern "C" int tl_rope_kv_write_fp4(const void* qkv, int in_dtype, int splits, c
     cudaStream_t s = (cudaStream_t)stream;
     const int head_runs = head_dim / 8;
     if (in_dtype == dtype && splits == 1 && n_tokens >= 148 && head_runs <= 128 && (head_runs & (head_runs - 1)) == 0 &&
-        rot_dims % (interleaved ? 8 : 16) == 0) {
+        rot_dims % (interleaved ? 8 : 32) == 0 && (interleaved || head_dim >= 32)) {
         int log_runs = 0;
         while ((1 << log_runs) < head_runs) ++log_runs;
 #define TL_WRITE_ROWS(T, I) tl_launch(rope_kv_write_fp4_rows_kernel<T, I>, dim3(n_tokens), dim3(128), 0, s, (const T*)qkv, (T*)q_out, log_runs, p)

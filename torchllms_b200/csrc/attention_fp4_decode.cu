@@ -7,7 +7,7 @@
 // instructions that unpack it: 16 keys and values of 128 numbers are 128 conversions and 128 products with scales a warp, beside
 // 16 products of the tensor cores.  So:
 //   - The cache comes in whole records of 16 tokens by cp.async.bulk, 128 keys a stage, into a ring that a producer warp keeps
-//     full across the borders of requests; four consumer warps take two records of keys and of values each.
+//     full across the borders of requests; four consumer warps take two records of keys and of values each, with one turn of the softmax for both.
 //   - Nothing is unpacked into shared memory.  The products are taken transposed, scores^T = K Q^T and out^T = V^T P^T, so that
 //     keys and values are the left operands: a lane loads the coordinates that its fragments hold (any fixed order of the
 //     contraction's index will do, so they are neighbours in a row), converts them in registers, and for V exchanges half bytes of two
@@ -22,7 +22,16 @@
 // for what it costs to begin and end one, and every CTA takes an even stretch of the line, found on the device from the
 // requests' lengths.  Where a block is cut, each part leaves its sums, and the CTA that is last to finish adds them up in
 // order (a counter for each block and head): the result does not depend on who that is.
+// In float32 steps of many rows a block has 64 of them, 16 to a consumer warp, which then takes all records of a tile: nothing is exchanged
+// between the warps, and a copied tile serves four times the rows.
 // Every wait is bounded; a CTA whose wait runs out sets the status word and takes part in the counting only.
+//
+// Measured (32 / 8 heads, us; a record's arithmetic is 427 cycles of a scheduler, 12 consumer warps an SM):
+//   bfloat16, heads of 128: 8 requests of 2,049 tokens 11.9 (19 MB; of it finding the stretch and fetching queries 2, joining warps and parts 3); 64 of 200
+//   to 16,000 146 (651 MB, 4.5 TB/s; the copies alone 113); 4 of 27,001 to 32,767 36 (134 MB, 3.7 TB/s: DRAM at 37 %, unpacking bounds).
+//   One request of 333, heads of 64: 7.1, a launch and a chain of trips to memory.
+//   float32, heads of 64: 12 requests of 2 to 4 tokens in a window of 1,024 14.5; prompts of 500 to 901 tokens 56 (16 rows a block: 73, half
+//   of it beginning blocks and exchanging results).
 #include "fp4.cuh"
 #include <limits.h>
 #include <math.h>

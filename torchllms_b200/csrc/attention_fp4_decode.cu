@@ -29,7 +29,7 @@
 // Measured (32 / 8 heads, us; a record's arithmetic is 427 cycles of a scheduler, 12 consumer warps an SM):
 //   bfloat16, heads of 128: 8 requests of 2,049 tokens 11.9 (19 MB; of it finding the stretch and fetching queries 2, joining warps and parts 3); 64 of 200
 //   to 16,000 146 (651 MB, 4.5 TB/s; the copies alone 113); 4 of 27,001 to 32,767 36 (134 MB, 3.7 TB/s: DRAM at 42 %, unpacking bounds).
-//   One request of 333, heads of 64: 7.1, a launch and a chain of trips to memory.
+//   One request of 333, heads of 64: 7.4, a launch and a chain of trips to memory.
 //   float32, heads of 64: 12 requests of 2 to 4 tokens in a window of 1,024 14.5; prompts of 500 to 901 tokens 56 (16 rows a block: 73, half
 //   of it beginning blocks and exchanging results).
 #include "fp4.cuh"
@@ -44,6 +44,9 @@ constexpr int RECORDS = EACH * NCW;     // records of a tile
 constexpr int BN = RECORDS * FP4_RECORD;
 constexpr int NTHREADS = (NCW + 1) * 32;
 constexpr int MOST_PARTS = 64;          // parts of a block, at most
+// A CTA's stretch, at least.  (32 / 8 heads of 128, three and two, us: 1 request of 500 tokens 9.1 8.3, 2 of 1,000 9.5 8.8, 8 of 700 11.2 10.5, 16 of 400 11.6
+// 10.6; 1 of 333 with heads of 64 7.3 7.5; a single key head, whose parts are then many, 1 of 8,000 13.1 14.3.  One is as two.)
+constexpr int LEAST = 2;
 constexpr int FAILED_PART = 1 << 16;    // what a CTA that gave up adds to a counter beside its 1
 constexpr int SMS = 148;
 constexpr float LOG2E = 1.4426950408889634f;
@@ -217,7 +220,7 @@ template <int ROWS> __device__ __forceinline__ bool walk_first(const Params& p, 
     }
     total = __reduce_add_sync(0xffffffffu, total) * p.n_kv_heads;
     longest = __reduce_max_sync(0xffffffffu, longest);
-    w.share = max(max((total + (int)gridDim.x - 1) / (int)gridDim.x, (longest + MOST_PARTS - 2) / (MOST_PARTS - 1)), 1 + worth_of(ROWS));
+    w.share = max(max((total + (int)gridDim.x - 1) / (int)gridDim.x, (longest + MOST_PARTS - 2) / (MOST_PARTS - 1)), LEAST);
     w.begin = blockIdx.x * w.share;
     w.end = w.begin + w.share;
     if (w.begin >= total) return false;

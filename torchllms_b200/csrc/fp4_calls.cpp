@@ -195,14 +195,14 @@ PyObject* read(PyObject*, PyObject* const* args, Py_ssize_t n) {
 // Whether a step is one for the tcgen05 kernel, whose CTA has 256 rows and an SM to itself, and not for the mma.sync kernel, which unpacks keys and
 // values again for every 16 rows.  `rows`: tokens x query heads of a key head; `units`: requests x key heads.  Measured (us, the mma.sync
 // kernel and the other; contexts of 200, 2,000 and 12,000 tokens):
-//   1 request, 32 / 8 heads of 128, 16 rows: 11.4  9.9   15.0 14.8   26.4 22.0     64: 12.3 10.2   17.0 16.0   34.0 22.9     256: 14.7 14.2   26.5 22.8   78 31
-//   8 requests                      16 rows: 12.6 10.6   18.8 22.5   48.6 97.6     64: 11.2 10.9   38.5 23.9   145 100       256: 39.0 14.8   116  36    530 118
-//   1 request,           of 64      32 rows:  9.0  8.1   12.0 14.7   17.7 20.3     64:  9.1  7.9   12.6 15.1   24.0 21.0     256: 11.0 12.0   18.9 18.6   57 28
-//   8 requests                      32 rows: 10.2  8.5   18.8 19.5   57.3 69.7     64:  8.7  8.8   27.6 20.0   105  71       256: 27.4 12.4   80.1 29.5  375 96
-// So it is one from `least` rows on, and with heads of 128 from 17 on where there are no more than 1,024 tiles of 128 keys (8 requests of 2,000
-// tokens: 32 rows 26.2 and 23.4 us; of 12,000 80.8 and 98.0).
+//   1 request, 32 / 8 heads of 128, 16 rows:  9.5 10.3   14.5 15.5   26.7 22.0     64: 10.2 10.7   16.2 16.5   35.0 23.7     256: 14.8 14.7   27.2 23.8    80  33
+//   8 requests                      16 rows: 10.2 11.0   19.2 22.9   49.4 96.6     64: 11.4 11.5   39.4 24.2   147  99       256: 40.3 15.5   118  36     537 117
+//   1 request,           of 64      32 rows:  7.8  8.6   11.0 15.2   17.6 21.4     64:  8.0  8.6   11.9 15.7   24.1 22.2     256: 11.1 12.3   19.0 19.2    58  28
+//   8 requests                      32 rows:  8.8  9.4   19.0 20.6   57.5 71.0     64:  8.8  9.4   28.2 21.0   105  72       256: 27.5 13.0   80   30     374  91
+// So it is one from `least` rows on, and with heads of 128 from 17 on where the context is long and there are no more than 1,024 tiles of 128 keys
+// (32 rows: one request of 12,000 tokens 25.9 and 22.7, 8 of 2,000 27.0 and 23.7; but 8 of 12,000 82 and 98, one of 200 9.6 and 10.4).
 bool many_rows(long long rows, int head_dim, long long units, int max_kv, int least) {
-    return rows >= least || (head_dim == 128 && rows > 16 && units * ((max_kv + 127) / 128) <= 1024);
+    return rows >= least || (head_dim == 128 && rows > 16 && max_kv >= 1024 && units * ((max_kv + 127) / 128) <= 1024);
 }
 
 // q, k_pages, v_pages, block_table, q_start, kv_len, n_seqs, max_q_len, max_kv_len, scale, window, page_size, allow_split, impl (0 the kernel that fits,

@@ -1,0 +1,69 @@
+"""Attention over the 4-bit cache at its bounds: what a row does not see takes no part in it, whatever it is."""
+
+import pytest
+import torch
+
+from test_fp4_kernels_gpu import batch, ops
+from torchllms_b200.cache import fp4
+
+pytestmark = pytest.mark.gpu
+
+
+def attend(a, kw, impl):
+    """One call; ``impl`` may name a number of pieces."""
+    pieces = dict(allow_split=int(impl.split()[2])) if "pieces" in impl else {}
+    out = ops().paged_attention_fp4(**a, **kw, impl=impl.split()[0], **pieces)
+    ops().check_status()
+    return out
+
+
+def poisoned(a, kw, share, seed):
+    """The step with ``share`` of the value groups that requests hold made NaN, and where a result has to be NaN for it: in the
+    coordinates of a group that is one at a key which the row sees."""
+    g = torch.Generator().manual_seed(seed)
+    T, H, D = a["q"].shape
+    KV, page, window = a["k_pages"].shape[1], kw["page_size"], kw["window"]
+    v_pages, wanted = a["v_pages"].clone(), torch.zeros((T, H, D), dtype=torch.bool)
+    scales = fp4.rows_of(v_pages, D)[1]
+    q_start, table = a["q_start"].tolist(), a["block_table"].cpu()
+    for b, L in enumerate(a["kv_len"].tolist()):
+        n = q_start[b + 1] - q_start[b]
+        if L == 0 or n == 0:
+            continue
+        bad = torch.rand((L, KV, D // 16), generator=g) < share
+        bad[L - 1, 0, 0] = bad[max(0, L - n), KV - 1, D // 16 - 1] = True          # (the last token, and the first new one)
+        if window:
+            bad[:max(0, L - n - window + 1)] = False                               # (no page holds those)
+        for j, h, c in bad.nonzero().tolist():
+            scales[int(table[b, j // page]), h, j % page // 16, j % 16, c] = fp4.NAN_SCALE
+        for i in range(n):
+            pos = L - n + i
+            seen = bad[max(0, pos - window + 1) if window else 0:max(pos + 1, 0)].any(0)
+            wanted[q_start[b] + i] = seen.repeat_interleave(16, 1).repeat_interleave(H // KV, 0)
+    return dict(a, v_pages=v_pages), wanted
+
+
+@pytest.mark.parametrize("share", [0.0, 0.002, 0.03])
+@pytest.mark.parametrize("impl,dtype", [("general", "bf16"), ("general", "f32"), ("decode", "bf16"), ("decode", "f32"), ("prefill", "bf16"),
+                                        ("prefill in 3 pieces", "bf16"), ("prefill in 7 pieces", "bf16"), ("auto", "bf16"), ("auto", "f32")])
+@pytest.mark.parametrize("H,KV,D,page,q_lens,kv_lens,window", [
+    pytest.param(2, 2, 64, 16, [300], [420], None, id="a_token_a_row"),
+    pytest.param(9, 3, 128, 32, [40, 3, 1], [40, 200, 30], None, id="group_of_3"),
+    pytest.param(32, 4, 64, 16, [130, 17], [130, 460], None, id="group_of_8"),
+    pytest.param(12, 1, 128, 64, [4, 1, 2], [900, 333, 20], None, id="drafts"),
+    pytest.param(8, 2, 128, 16, [90, 5], [700, 300], 100, id="window_100"),
+    pytest.param(4, 4, 64, 16, [290], [800], 33, id="window_33"),
+    pytest.param(6, 2, 128, 48, [64, 64], [64, 129], 1, id="window_1"),
+    pytest.param(2, 2, 128, 16, [257], [600], 300, id="window_300"),
+    pytest.param(4, 2, 64, 16, [5, 9, 3], [2, 70, 3], None, id="rows_that_see_nothing"),
+    pytest.param(4, 2, 64, 16, [9, 70], [5, 30], 7, id="rows_that_see_nothing_in_a_window"),
+    pytest.param(32, 8, 64, 16, [65, 0, 200, 7], [65, 30, 777, 7], None, id="prompts"),
+])
+def test_values_that_are_no_numbers_reach_the_rows_that_see_them_only(H, KV, D, page, q_lens, kv_lens, window, impl, dtype, share):
+    a, kw = batch(H, KV, D, page, q_lens, kv_lens, window, dtype, seed=len(q_lens) + D)
+    before = attend(a, kw, impl)
+    b, wanted = poisoned(a, kw, share, seed=H + D)
+    got = attend(b, kw, impl)
+    assert torch.equal(got.isnan().cpu(), wanted)
+    # everything else keeps its bits
+    assert torch.equal(got[~wanted.cuda()], before[~wanted.cuda()])

@@ -149,6 +149,12 @@ __device__ __forceinline__ unsigned movmatrix_trans(unsigned a) {     // 8 x 8 b
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
     return d;
 }
+// ones in the lowest n places (none below 0, all from 32 on)
+__device__ __forceinline__ unsigned first_bits(int n) {
+    unsigned m;
+    asm("shr.u32 %0, 0xffffffff, %1;" : "=r"(m) : "r"(32 - min(max(n, 0), 32)));       // (a shift by 32 leaves nothing)
+    return m;
+}
 __device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(NCW * 32) : "memory"); }
 
 // (exact for row * group < 2^32, which the host sees to)
@@ -284,7 +290,7 @@ __device__ __forceinline__ void store4(float* p, float4 v) { *reinterpret_cast<f
 // What a consumer warp keeps of a block.  Lane (g, t) = (lane / 4, lane % 4).  Of the scores^T tile it holds keys g and g + 8 for rows
 // 2t and 2t + 1 of every eight, of the out^T tile coordinates HD / 8 * g + 2m and + 1 for the same rows.  Its part of a key or
 // query is coordinates HD / 4 * t and the HD / 4 - 1 after them.
-template <typename T, int HD, int NT>
+template <typename T, int HD, int NT, bool UNEVEN>
 struct Consumer {
     static constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;
     static constexpr int KSTEPS = HD / 16, WORDS = HD / 32, ROWS = 8 * NT, OPITCH = HD + 4;
@@ -293,10 +299,12 @@ struct Consumer {
     float m[NT][2], l[NT][2], o[NT][KSTEPS][4];
     int qpos[NT][2], qmax, qmin;
     int g, t;
+    unsigned spoilt;                    // rows (a bit each) that see a value of this lane's coordinates which is not a number and was hidden
 
     __device__ __forceinline__ void begin(const Params& p, const Block& k, int kvh, int lane) {
         g = lane >> 2;
         t = lane & 3;
+        spoilt = 0;
         int top_pos = -1, low_pos = INT_MAX;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -357,6 +365,40 @@ struct Consumer {
             const uint2 v = *reinterpret_cast<const uint2*>(at);
             w[0] = v.x; w[1] = v.y;
         }
+    }
+
+    // A value that is not a number would reach rows that do not see it (its weight is 0, and 0 times NaN is NaN).  So those of a record, whose first key
+    // is k, take part as zeros where some rows see a key and others do not, and the rows that see one are remembered.  byte: scales of this lane's
+    // coordinates of four keys; the lanes that share g have the same coordinates, for other rows, and the other keys.
+    __device__ __forceinline__ void hide_nan(const Params& p, unsigned (&byte)[4], int k) {
+        unsigned keys = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (byte[i] == FP4_NAN_SCALE) {
+                keys |= 1u << (2 * t + (i & 1) + 8 * (i >> 1));
+                byte[i] = 0;
+            }
+        keys |= __shfl_xor_sync(0xffffffffu, keys, 1);
+        keys |= __shfl_xor_sync(0xffffffffu, keys, 2);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int from = p.window > 0 ? qpos[nt][j] + 1 - p.window - k : 0;
+                if (keys & first_bits(qpos[nt][j] + 1 - k) & ~first_bits(from)) spoilt |= 1u << (2 * nt + j);
+            }
+    }
+    // When the keys are through: what was hidden of the rows that see it.
+    __device__ __forceinline__ void spoil() {
+        if (!__any_sync(0xffffffffu, spoilt != 0u)) return;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                if ((spoilt >> (2 * nt + j)) & 1u) {
+#pragma unroll
+                    for (int d = 0; d < KSTEPS; ++d) o[nt][d][j] = o[nt][d][j + 2] = NAN;
+                }
     }
 
     // EACH records of keys and of values, APART records apart; the first begins with key k0
@@ -422,7 +464,8 @@ struct Consumer {
         }
         // ---- masks
         const bool inside = k0 >= lo && k0 + SPAN <= hi;
-        if (!(inside && k0 + SPAN - 1 <= qmin && (p.window <= 0 || k0 > qmax - p.window))) {
+        const bool clear = inside && k0 + SPAN - 1 <= qmin && (p.window <= 0 || k0 > qmax - p.window);     // (every row sees every key)
+        if (!clear) {
 #pragma unroll
             for (int n = 0; n < EACH; ++n)
 #pragma unroll
@@ -517,6 +560,12 @@ struct Consumer {
                     if (kpos < lo || kpos >= hi) byte[i] = 0;
                 }
             }
+            if (UNEVEN && !clear) {
+                bool none = false;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) none = none || byte[i] == FP4_NAN_SCALE;
+                if (__any_sync(0xffffffffu, none)) hide_nan(p, byte, k0 + n * STEP);
+            }
             __half2 vs[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
@@ -610,10 +659,12 @@ struct Consumer {
 // (a maximum that is not a number is kept: the row is not a number)
 __device__ __forceinline__ float max_keep(float a, float b) { return (a != a || b != b) ? NAN : fmaxf(a, b); }
 
-// OWN: every consumer warp has 8 NT rows of its own and takes all records of a tile; else the warps share the rows, and a tile's records.
-template <typename T, int HD, int STAGES, int NT, bool OWN>
+// OWN: every consumer warp has 8 NT rows of its own and takes all records of a tile; else the warps share the rows, and a tile's records.  UNEVEN: requests
+// may bring several tokens, whose rows do not see the same keys (steps of single tokens are 1 to 4 % faster without what that takes:
+// 8 requests of 2,049 12.0 us and 12.3, 4 of 27,001 to 32,767 36.8 and 38.3).
+template <typename T, int HD, int STAGES, int NT, bool OWN, bool UNEVEN>
 __global__ void __launch_bounds__(NTHREADS, (NT == 1 && sizeof(T) == 2) ? 3 : 2) attention_fp4_decode_kernel(const Params p) {
-    using C = Consumer<T, HD, NT>;
+    using C = Consumer<T, HD, NT, UNEVEN>;
     constexpr int ROWS = (OWN ? NCW : 1) * 8 * NT, RECORD = fp4_record_bytes(HD);
     constexpr unsigned STAGE = 2 * RECORDS * RECORD;
     extern __shared__ __align__(128) unsigned char smem[];        // the ring, then the warps' results
@@ -708,6 +759,7 @@ __global__ void __launch_bounds__(NTHREADS, (NT == 1 && sizeof(T) == 2) ? 3 : 2)
                 phase ^= 1u;
             }
         }
+        if (UNEVEN) c.spoil();
         auto out_row = [&](int rr) {
             const int row = w.k.row0 + rr, token = token_of(p, row);
             return reinterpret_cast<T*>(p.out) + ((size_t)(w.k.first + token) * p.n_heads + w.kvh * p.group + row - token * p.group) * HD;
@@ -831,15 +883,15 @@ bool takes(int n_heads, int n_kv_heads, int head_dim, int page_size) {
 }
 
 struct Plan {
-    bool own;
+    bool own, uneven;
     int nt, rows, blocks, ctas;
     size_t smem;
 };
 
-template <typename T, int HD, int NT, bool OWN> int ctas_per_sm(int rows) {
+template <typename T, int HD, int NT, bool OWN, bool UNEVEN> int ctas_per_sm(int rows) {
     static int known[8 * NT * NCW + 1] = {};               // (threads that come here at the same time write the same)
     if (known[rows] == 0) {
-        auto kern = attention_fp4_decode_kernel<T, HD, stages_for<HD>(), NT, OWN>;
+        auto kern = attention_fp4_decode_kernel<T, HD, stages_for<HD>(), NT, OWN, UNEVEN>;
         int n = 0;
         if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_for<HD>(8 * NT, OWN)) != cudaSuccess ||
             cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, NTHREADS, smem_for<HD>(rows, OWN)) != cudaSuccess || n < 1) {
@@ -850,10 +902,13 @@ template <typename T, int HD, int NT, bool OWN> int ctas_per_sm(int rows) {
     }
     return known[rows];
 }
-template <int HD> int ctas_per_sm(int dtype, const bool own, int nt, int rows) {
-    if (dtype == TL_F32)
-        return own ? ctas_per_sm<float, HD, 2, true>(rows) : nt == 1 ? ctas_per_sm<float, HD, 1, false>(rows) : ctas_per_sm<float, HD, 2, false>(rows);
-    return nt == 1 ? ctas_per_sm<__nv_bfloat16, HD, 1, false>(rows) : ctas_per_sm<__nv_bfloat16, HD, 2, false>(rows);
+template <typename T, int HD, bool UNEVEN> int ctas_per_sm(int nt, int rows) {
+    return nt == 1 ? ctas_per_sm<T, HD, 1, false, UNEVEN>(rows) : ctas_per_sm<T, HD, 2, false, UNEVEN>(rows);
+}
+template <int HD> int ctas_per_sm(int dtype, const Plan& pl) {
+    if (pl.own) return ctas_per_sm<float, HD, 2, true, true>(pl.rows);
+    if (dtype == TL_F32) return pl.uneven ? ctas_per_sm<float, HD, true>(pl.nt, pl.rows) : ctas_per_sm<float, HD, false>(pl.nt, pl.rows);
+    return pl.uneven ? ctas_per_sm<__nv_bfloat16, HD, true>(pl.nt, pl.rows) : ctas_per_sm<__nv_bfloat16, HD, false>(pl.nt, pl.rows);
 }
 
 Plan make_plan(int dtype, int n_seqs, int n_heads, int n_kv_heads, int head_dim, int max_q_len, int max_kv_len) {
@@ -864,12 +919,13 @@ Plan make_plan(int dtype, int n_seqs, int n_heads, int n_kv_heads, int head_dim,
     // 1,430 1,210; heads of 128: 52.6 46.3; 39.4 45.9; 136 94; 4,167 2,333.)
     constexpr int OWN = NCW * 16;
     pl.own = dtype == TL_F32 && all >= OWN && (double)n_seqs * ((all + OWN - 1) / OWN) * n_kv_heads >= 96.0;
+    pl.uneven = max_q_len > 1;
     pl.nt = all <= 8 ? 1 : 2;
     const int most = 8 * pl.nt * (pl.own ? NCW : 1);
     pl.rows = all < most ? (int)all : most;
     pl.blocks = (int)((all + most - 1) / most);
     pl.smem = head_dim == 128 ? smem_for<128>(pl.rows, pl.own) : smem_for<64>(pl.rows, pl.own);
-    const int fit = head_dim == 128 ? ctas_per_sm<128>(dtype, pl.own, pl.nt, pl.rows) : ctas_per_sm<64>(dtype, pl.own, pl.nt, pl.rows);
+    const int fit = head_dim == 128 ? ctas_per_sm<128>(dtype, pl) : ctas_per_sm<64>(dtype, pl);
     // no more CTAs than there can be tiles
     const double tiles = (double)n_seqs * pl.blocks * n_kv_heads * ((max_kv_len + BN - 1) / BN + 1);
     pl.ctas = tiles < (double)SMS * fit ? (int)tiles : SMS * fit;
@@ -877,13 +933,17 @@ Plan make_plan(int dtype, int n_seqs, int n_heads, int n_kv_heads, int head_dim,
     return pl;
 }
 
-template <typename T, int HD, int NT, bool OWN> int launch(const Params& p, const Plan& pl, cudaStream_t s) {      // (ctas_per_sm has raised the limit on shared memory)
-    return (int)tl_launch(attention_fp4_decode_kernel<T, HD, stages_for<HD>(), NT, OWN>, dim3(pl.ctas), dim3(NTHREADS), pl.smem, s, p);
+// (ctas_per_sm has raised the limit on shared memory)
+template <typename T, int HD, int NT, bool OWN, bool UNEVEN> int launch(const Params& p, const Plan& pl, cudaStream_t s) {
+    return (int)tl_launch(attention_fp4_decode_kernel<T, HD, stages_for<HD>(), NT, OWN, UNEVEN>, dim3(pl.ctas), dim3(NTHREADS), pl.smem, s, p);
+}
+template <typename T, int HD, bool UNEVEN> int launch(const Params& p, const Plan& pl, cudaStream_t s) {
+    return pl.nt == 1 ? launch<T, HD, 1, false, UNEVEN>(p, pl, s) : launch<T, HD, 2, false, UNEVEN>(p, pl, s);
 }
 template <int HD> int launch(int dtype, const Params& p, const Plan& pl, cudaStream_t s) {
-    if (dtype == TL_F32)
-        return pl.own ? launch<float, HD, 2, true>(p, pl, s) : pl.nt == 1 ? launch<float, HD, 1, false>(p, pl, s) : launch<float, HD, 2, false>(p, pl, s);
-    return pl.nt == 1 ? launch<__nv_bfloat16, HD, 1, false>(p, pl, s) : launch<__nv_bfloat16, HD, 2, false>(p, pl, s);
+    if (pl.own) return launch<float, HD, 2, true, true>(p, pl, s);
+    if (dtype == TL_F32) return pl.uneven ? launch<float, HD, true>(p, pl, s) : launch<float, HD, false>(p, pl, s);
+    return pl.uneven ? launch<__nv_bfloat16, HD, true>(p, pl, s) : launch<__nv_bfloat16, HD, false>(p, pl, s);
 }
 
 }  // namespace

@@ -68,6 +68,7 @@ struct Params {
     int n_heads, n_kv_heads, group, page_records;
     int n_seqs, pieces, window;
     int most_blocks;            // of a request
+    int page_shift;             // page_records is 1 << page_shift, or page_shift is negative
     unsigned per_group;         // 2^32 / group and one more (0 for a group of one head): row / group without a division
     float scale_log2;
 };
@@ -182,6 +183,12 @@ __device__ __forceinline__ float ex2(float x) {     // 2^x, one instruction; 2^-
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// ones in the lowest n places (none below 0, all from 32 on)
+__device__ __forceinline__ unsigned first_bits(int n) {
+    unsigned m;
+    asm("shr.u32 %0, 0xffffffff, %1;" : "=r"(m) : "r"(32 - min(max(n, 0), 32)));       // (a shift by 32 leaves nothing)
+    return m;
+}
 __device__ __forceinline__ unsigned pack_bf16(float lo, float hi) {
     __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<unsigned*>(&v);
@@ -214,9 +221,13 @@ __device__ __forceinline__ unsigned pack_half(float lo, float hi) {
 template <int KSTAGES, int VSTAGES>
 struct Tail {                   // what lies behind the tiles in shared memory
     unsigned long long q_full, k_full[KSTAGES], k_empty[KSTAGES], v_full[VSTAGES], v_empty[VSTAGES];
-    unsigned long long s_full[QT], s_free, p_half[QT], p_full[QT], pv_done[QT], settled[2];
+    unsigned long long s_full[QT], s_free, p_half[QT], p_full[QT], pv_done[QT], noted, settled[2];
     unsigned tmem_base_slot;
     int failed_flag;
+    // Groups of values that are not numbers, a bit each, of the keys that some rows of the CTA see and others do not: those behind the first row's
+    // place, and those ahead of the last row's window.  Its rows lie within 256 places, so there are no more of either.
+    int any_nan;
+    unsigned char nan_late[QT * BM], nan_early[QT * BM];
 };
 
 // What a row tile has to do with the CTA's key tiles (counted from the piece's first): it works on tiles first .. last - 1.
@@ -243,6 +254,20 @@ struct Packed {
         const unsigned char* s = record + FP4_RECORD * (HD / 2) + row * (HD / FP4_GROUP);
         if (HD == 128) scales = __ldg(reinterpret_cast<const uint2*>(s));
         else scales.x = __ldg(reinterpret_cast<const unsigned*>(s));
+    }
+    // The groups that are not numbers, a bit each.
+    __device__ __forceinline__ unsigned nan_groups() const {
+        unsigned none = 0;
+#pragma unroll
+        for (int c = 0; c < HD / FP4_GROUP; ++c)
+            if ((((c < 4 ? scales.x : scales.y) >> (8 * (c & 3))) & 255u) == (unsigned)FP4_NAN_SCALE) none |= 1u << c;
+        return none;
+    }
+    // Zeros for some groups of what `unpack` has written.
+    static __device__ __forceinline__ void clear_groups(unsigned char* tile, int key, unsigned groups) {
+        for (int c = 0; c < HD / 8; ++c)
+            if ((groups >> (c / 2)) & 1u)
+                *reinterpret_cast<uint4*>(tile + key * 128 + (c >> 3) * (BN * 128) + (((c & 7) ^ (key & 7)) << 4)) = make_uint4(0u, 0u, 0u, 0u);
     }
     // float16 rows of 128 bytes (64 coordinates), 16-byte chunks exchanged as the 128-byte swizzle has them
     __device__ __forceinline__ void unpack(unsigned char* tile, int key) const {
@@ -282,8 +307,10 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_fp4_prefill_kernel(cons
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) {
         tail.failed_flag = 0;
+        tail.any_nan = 0;
         mbar_init(&tail.q_full, 4 * QT);
         mbar_init(&tail.s_free, 4);
+        mbar_init(&tail.noted, 4);
         for (int s = 0; s < KSTAGES; ++s) {
             mbar_init(&tail.k_full[s], 4);
             mbar_init(&tail.k_empty[s], QT);
@@ -305,6 +332,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_fp4_prefill_kernel(cons
             atomicExch(p.status, ERR_PLACE);
         }
     }
+    if (tid < QT * BM) tail.nan_late[tid] = tail.nan_early[tid] = 0;
     if (warp == W_SCORES) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tail.tmem_base_slot)), "r"(TMEM_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -370,6 +398,9 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_fp4_prefill_kernel(cons
         range[t].last = any ? (to - k_start + BN - 1) / BN : 0;
         n_tiles = max(n_tiles, range[t].last);
     }
+    // Keys behind `late` are not seen by the CTA's first row, those ahead of `early` not by its last.  A value there that is not a number would reach rows that
+    // do not see it (its weight is 0, and 0 times NaN is NaN): whoever unpacks it makes it zero and notes it, and the rows that see it get their NaN at the end.
+    const int late = base + token_of(p, row0), early = p.window > 0 ? base + token_of(p, active ? last_row : row0) - p.window + 1 : INT_MIN;
 
     if (warp >= W_SCORES) {
         regs_down<REGS_REST>();
@@ -458,42 +489,52 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_fp4_prefill_kernel(cons
         auto place = [&](int j) {
             const int kpos = k_start + j * BN + key;
             if (j >= n_tiles || kpos < lo || kpos >= hi) return -1ll;
-            const int rec = kpos / FP4_RECORD, block = rec / p.page_records;
+            const int rec = kpos / FP4_RECORD, block = p.page_shift >= 0 ? rec >> p.page_shift : rec / p.page_records;
             long long page = table[block];
             if (!tl_check_page(page) || page < 0 || page >= p.n_pages) page = 0;       // (a bad page is not followed; debug builds report it)
             return ((page * p.n_kv_heads + kvh) * p.page_records + rec - block * p.page_records) * RECORD;
         };
         const int row = key & (FP4_RECORD - 1);            // (k_start is a multiple of a record)
-        Packed<HD> k, v;
-        long long at = place(0);
-        k.clear();
-        if (at >= 0) k.load(p.k_pages + at, row);
+        Packed<HD> held, coming;
+        long long at = place(0), next = -1;
+        coming.clear();
+        if (at >= 0) coming.load(p.k_pages + at, row);
         bool ok = true;
-        for (int j = 0; j < n_tiles; ++j) {
-            const int ks = j % KSTAGES, vs = j % VSTAGES;
-            v.clear();
-            if (at >= 0) v.load(p.v_pages + at, row);
-            const long long next = place(j + 1);
-            if (j >= KSTAGES && !__all_sync(0xffffffffu, mbar_wait(&tail.k_empty[ks], (j / KSTAGES - 1) & 1, failed))) {
+        const int late_tile = max(late + 1 - k_start, 0) / BN, early_end = early > k_start ? (early - k_start + BN - 1) / BN : 0;
+        // Keys and values go through the same instructions: the roles' loops together just about fit the instruction cache.  (With a loop that has a body for
+        // each, what hides values cost 2,048 tokens behind 14,001 472 -> 505 us and a prompt of 2,048 45.6 -> 49, with none of it ever run;
+        // this way 478 and 46.4.)
+#pragma unroll 1
+        for (int i = 0; i < 2 * n_tiles; ++i) {
+            const int j = i >> 1;
+            const bool values = (i & 1) != 0;
+            if (values) at = next;
+            else next = place(j + 1);
+            const int stages = values ? VSTAGES : KSTAGES, turn = values ? j / VSTAGES : j / KSTAGES, s = j - turn * stages;
+            unsigned char* tile = (values ? Vs : Ks) + s * KV_BYTES;
+            if (turn > 0 && !__all_sync(0xffffffffu, mbar_wait((values ? tail.v_empty : tail.k_empty) + s, (turn - 1) & 1, failed))) {
                 ok = false;
                 break;
             }
-            k.unpack(Ks + ks * KV_BYTES, key);
+            held = coming;
+            coming.clear();
+            if (at >= 0) coming.load((values ? p.k_pages : p.v_pages) + at, row);
+            held.unpack(tile, key);
+            if (values && (j >= late_tile || j < early_end)) {
+                const int kpos = k_start + j * BN + key;
+                const unsigned none = held.nan_groups();
+                if (none != 0u && (kpos > late || kpos < early)) {
+                    held.clear_groups(tile, key, none);
+                    if (kpos > late) tail.nan_late[kpos - late - 1] = (unsigned char)none;
+                    else tail.nan_early[early - 1 - kpos] = (unsigned char)none;
+                    tail.any_nan = 1;
+                }
+            }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // (the tensor cores read what was stored)
             __syncwarp();
-            if (lane == 0) mbar_arrive(&tail.k_full[ks]);
-            k.clear();
-            if (next >= 0) k.load(p.k_pages + next, row);
-            if (j >= VSTAGES && !__all_sync(0xffffffffu, mbar_wait(&tail.v_empty[vs], (j / VSTAGES - 1) & 1, failed))) {
-                ok = false;
-                break;
-            }
-            v.unpack(Vs + vs * KV_BYTES, key);
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&tail.v_full[vs]);
-            at = next;
+            if (lane == 0) mbar_arrive((values ? tail.v_full : tail.k_full) + s);
         }
+        if (lane == 0) mbar_arrive(&tail.noted);
         if (!ok && lane == 0 && atomicExch(failed, 1) == 0) atomicExch(p.status, ERR_UNPACK_WAIT);
     } else {
         regs_up<REGS_SOFTMAX>();
@@ -571,10 +612,14 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_fp4_prefill_kernel(cons
             if (lane == 0) mbar_arrive(&tail.s_free);      // the buffer may take the next scores
             const bool clear = k0 >= lo && k0 + BN <= hi && k0 + BN - 1 <= low && (p.window <= 0 || k0 > high - p.window);
             if (!clear) {
-                const int from = max(lo, p.window > 0 ? qpos - p.window + 1 : 0), to = min(hi, qpos + 1);
+                const int from = max(lo, p.window > 0 ? qpos - p.window + 1 : 0) - k0, to = min(hi, qpos + 1) - k0;
 #pragma unroll
-                for (int i = 0; i < BN; ++i)
-                    if (k0 + i < from || k0 + i >= to) raw[i] = 0xff800000u;      // -inf
+                for (int w = 0; w < BN / 32; ++w) {
+                    const unsigned seen = first_bits(to - 32 * w) & ~first_bits(from - 32 * w);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if (((seen >> i) & 1u) == 0u) raw[32 * w + i] = 0xff800000u;      // -inf
+                }
             }
             float mx[4];
 #pragma unroll
@@ -645,6 +690,16 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_fp4_prefill_kernel(cons
             ok = __all_sync(0xffffffffu, mbar_wait(&tail.pv_done[t], (n - 1) & 1, failed));
             tc_fence_after();
         }
+        // the groups in which this row sees a value that was hidden
+        unsigned none = 0;
+        if (ok && n > 0) {
+            ok = __all_sync(0xffffffffu, mbar_wait(&tail.noted, 0, failed));
+            if (ok && *(volatile int*)&tail.any_nan != 0) {
+                const int from = max(lo, p.window > 0 ? qpos - p.window + 1 : 0), to = min(hi, qpos + 1);
+                for (int k = max(from, late + 1); k < to; ++k) none |= tail.nan_late[k - late - 1];
+                for (int k = from; k < min(min(to, early), late + 1); ++k) none |= tail.nan_early[early - 1 - k];
+            }
+        }
         if (ok && rows > 0) {
             if (p.pieces == 1) {
                 const float inv = l_sum == 0.f ? 0.f : 1.f / l_sum;
@@ -661,6 +716,10 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_fp4_prefill_kernel(cons
                     }
 #pragma unroll
                     for (int e = 0; e < 8; ++e) w[e] = pack_bf16(__uint_as_float(v[2 * e]) * inv, __uint_as_float(v[2 * e + 1]) * inv);
+                    if ((none >> c) & 1u) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) w[e] = 0x7fff7fffu;
+                    }
                     if (r < rows) store32(to + c * 16, w);
                 }
             } else if (r < rows || n > 0) {
@@ -675,6 +734,10 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_fp4_prefill_kernel(cons
                         unsigned v[16];
                         tmem_ld16(lane_addr + col_o + c * 16, v);
                         tmem_wait_ld();
+                        if ((none >> c) & 1u) {
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) v[i] = 0x7fffffffu;
+                        }
                         if (r < rows) {
                             store32(p.part_o + row * HD + c * 16, *reinterpret_cast<const unsigned(*)[8]>(&v[0]));
                             store32(p.part_o + row * HD + c * 16 + 8, *reinterpret_cast<const unsigned(*)[8]>(&v[8]));
@@ -831,6 +894,9 @@ extern "C" int tl_attention_fp4_prefill(const void* q, const void* k_pages, cons
     p.block_table = block_table; p.q_start = q_start; p.kv_len = kv_len; p.status = status; p.n_pages = n_pages;
     p.table_stride = table_stride; p.table_cols = table_cols; p.n_heads = n_heads; p.n_kv_heads = n_kv_heads; p.group = n_heads / n_kv_heads;
     p.page_records = page_size / FP4_RECORD; p.n_seqs = n_seqs; p.most_blocks = (int)pl.of_request; p.pieces = pieces; p.window = window > 0 ? window : 0;
+    p.page_shift = -1;
+    for (int i = 0; i < 31; ++i)
+        if (p.page_records == 1 << i) p.page_shift = i;
     p.per_group = p.group == 1 ? 0u : (unsigned)((1ull << 32) / (unsigned)p.group) + 1u;
     if ((double)pl.of_request * QT * BM * p.group >= 4294967296.0) return TL_BAD_SIZE;
     p.scale_log2 = scale * LOG2E;

@@ -5,7 +5,8 @@
 //     scale(E, M) = M 2^-17 for E = 0, else (8 + M) 2^(E - 18).
 // With a = max |x| of the group, scale = a / 6 rounded to nearest (ties to even) and at most 10240, a number is x / scale
 // rounded to nearest (ties to the even code), at most 6.  A group that holds a number which is not finite has the scale
-// byte 255 and reads as NaN throughout, so that such a number does not vanish.  A group below 6 * 2^-18 reads as zeros.
+// byte 255 and reads as NaN throughout, so that such a number does not vanish; attention gives it to the rows that see its token, and to
+// no others.  A group below 6 * 2^-18 reads as zeros.
 //
 // What that choice buys the readers: the scale's byte shifted left by 7 is the float16 with its value, and a number times
 // its scale has 2 + 4 significant bits and lies between 2^-18 and 61440, so it IS a float16.  Attention over the cache

@@ -67,3 +67,12 @@ def test_values_that_are_no_numbers_reach_the_rows_that_see_them_only(H, KV, D, 
     assert torch.equal(got.isnan().cpu(), wanted)
     # everything else keeps its bits
     assert torch.equal(got[~wanted.cuda()], before[~wanted.cuda()])
+
+
+@pytest.mark.parametrize("impl,dtype", [("general", "bf16"), ("decode", "bf16"), ("decode", "f32"), ("prefill", "bf16"), ("prefill in 3 pieces", "bf16")])
+def test_a_window_of_any_size(impl, dtype):
+    """A window that holds every key is no window, up to the largest number there is."""
+    a, kw = batch(4, 2, 64, 16, [9, 70, 1], [5, 30, 90], None, dtype)
+    whole = attend(a, kw, impl)
+    for window in (90, 2 ** 20, 2 ** 31 - 1):
+        assert torch.equal(attend(a, dict(kw, window=window), impl), whole)

@@ -158,9 +158,10 @@ extern "C" int tl_attention_fp4_general(const void* q, const void* k_pages, cons
     if (n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads != 0 || n_heads > 65535 || n_seqs > 65535 || n_pages <= 0) return TL_BAD_SIZE;
     if (head_dim < FP4_GROUP || head_dim > MAX_DIM || head_dim % FP4_GROUP != 0 || page_size < FP4_RECORD || page_size % FP4_RECORD != 0)
         return TL_BAD_SIZE;
+    if (!fp4_places_fit(table_cols, page_size, max_q_len)) return TL_BAD_SIZE;
     if (!aligned16(k_pages) || !aligned16(v_pages)) return TL_BAD_ALIGN;
     const GeneralParams p = {(const unsigned char*)k_pages, (const unsigned char*)v_pages, block_table, q_start, kv_len, n_pages, table_stride,
-                             table_cols, n_heads, n_kv_heads, head_dim, page_size, window > 0 ? window : 0, scale * LOG2E};
+                             table_cols, n_heads, n_kv_heads, head_dim, page_size, fp4_window(window, table_cols, page_size), scale * LOG2E};
     const dim3 grid((unsigned)max_q_len, (unsigned)n_heads, (unsigned)n_seqs);
     cudaStream_t s = (cudaStream_t)stream;
     if (dtype == TL_BF16)

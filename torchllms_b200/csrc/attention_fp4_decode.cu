@@ -971,7 +971,7 @@ extern "C" int tl_attention_fp4_decode(const void* q, const void* k_pages, const
                                        int* counters, int* status, int dtype, int n_seqs, int n_heads, int n_kv_heads, int head_dim,
                                        int page_size, long long n_pages, int max_q_len, int max_kv_len, int window, float scale, void* stream) {
     if (n_seqs <= 0 || max_q_len <= 0) return TL_OK;
-    if (!takes(n_heads, n_kv_heads, head_dim, page_size) || n_pages <= 0 || max_kv_len < 0) return TL_BAD_SIZE;
+    if (!takes(n_heads, n_kv_heads, head_dim, page_size) || n_pages <= 0 || max_kv_len < 0 || !fp4_places_fit(table_cols, page_size, max_q_len)) return TL_BAD_SIZE;
     if (dtype != TL_BF16 && dtype != TL_F32) return TL_BAD_DTYPE;
     if (!aligned16(q) || !aligned16(out) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(workspace)) return TL_BAD_ALIGN;
     if (workspace == nullptr || counters == nullptr || status == nullptr) return TL_BAD_SIZE;
@@ -988,7 +988,7 @@ extern "C" int tl_attention_fp4_decode(const void* q, const void* k_pages, const
         if (p.page_records == 1 << b) p.page_shift = b;
     p.per_group = p.group == 1 ? 0u : (unsigned)((1ull << 32) / (unsigned)p.group) + 1u;
     if ((double)max_q_len * p.group * p.group >= 4294967296.0) return TL_BAD_SIZE;
-    p.window = window > 0 ? window : 0;
+    p.window = fp4_window(window, table_cols, page_size);
     p.scale_log2 = scale * LOG2E;
     cudaStream_t s = (cudaStream_t)stream;
     return head_dim == 128 ? launch<128>(dtype, p, pl, s) : launch<64>(dtype, p, pl, s);

@@ -881,7 +881,8 @@ extern "C" int tl_attention_fp4_prefill(const void* q, const void* k_pages, cons
                                         long long q_rows, int n_seqs, int n_heads, int n_kv_heads, int head_dim, int page_size, long long n_pages,
                                         int max_q_len, int window, float scale, int pieces, void* stream) {
     if (n_seqs <= 0 || max_q_len <= 0) return TL_OK;
-    if (!takes(n_heads, n_kv_heads, head_dim, page_size) || n_pages <= 0 || pieces < 1 || pieces > MOST_PIECES) return TL_BAD_SIZE;
+    if (!takes(n_heads, n_kv_heads, head_dim, page_size) || n_pages <= 0 || pieces < 1 || pieces > MOST_PIECES || !fp4_places_fit(table_cols, page_size, max_q_len))
+        return TL_BAD_SIZE;
     // (results are stored 32 bytes at a time)
     auto aligned32 = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 31u) == 0; };
     if (!aligned16(q) || !aligned32(out) || !aligned16(k_pages) || !aligned16(v_pages) || status == nullptr) return TL_BAD_ALIGN;
@@ -893,7 +894,7 @@ extern "C" int tl_attention_fp4_prefill(const void* q, const void* k_pages, cons
     p.k_pages = (const unsigned char*)k_pages; p.v_pages = (const unsigned char*)v_pages;
     p.block_table = block_table; p.q_start = q_start; p.kv_len = kv_len; p.status = status; p.n_pages = n_pages;
     p.table_stride = table_stride; p.table_cols = table_cols; p.n_heads = n_heads; p.n_kv_heads = n_kv_heads; p.group = n_heads / n_kv_heads;
-    p.page_records = page_size / FP4_RECORD; p.n_seqs = n_seqs; p.most_blocks = (int)pl.of_request; p.pieces = pieces; p.window = window > 0 ? window : 0;
+    p.page_records = page_size / FP4_RECORD; p.n_seqs = n_seqs; p.most_blocks = (int)pl.of_request; p.pieces = pieces; p.window = fp4_window(window, table_cols, page_size);
     p.page_shift = -1;
     for (int i = 0; i < 31; ++i)
         if (p.page_records == 1 << i) p.page_shift = i;

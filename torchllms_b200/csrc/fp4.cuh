@@ -85,6 +85,16 @@ __device__ __forceinline__ unsigned fp4_pack8(const float (&x)[8], unsigned byte
     return w;
 }
 
+// Attention: whether all places of a step stay within 32 bits, also with a tile added or a window taken off.  (A row's place is below zero, down to
+// minus max_q_len, where a request is shorter than its new tokens.)
+static inline bool fp4_places_fit(int table_cols, int page_size, int max_q_len) {
+    return (double)table_cols * page_size + (double)max_q_len + 4096.0 < 2147483648.0;
+}
+// The window as the kernels take it, 0 for none: one that holds every key that a table can name is none.
+static inline int fp4_window(int window, int table_cols, int page_size) {
+    return window > 0 && (long long)window < (long long)table_cols * page_size ? window : 0;
+}
+
 // Where a token of a head lies: its row of numbers and its row of scales.
 struct Fp4Place {
     long long codes, scales;

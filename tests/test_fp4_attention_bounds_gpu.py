@@ -3,6 +3,7 @@
 import pytest
 import torch
 
+import fp4_plain
 from test_fp4_kernels_gpu import batch, ops
 from torchllms_b200.cache import fp4
 
@@ -76,3 +77,19 @@ def test_a_window_of_any_size(impl, dtype):
     whole = attend(a, kw, impl)
     for window in (90, 2 ** 20, 2 ** 31 - 1):
         assert torch.equal(attend(a, dict(kw, window=window), impl), whole)
+
+
+@pytest.mark.parametrize("impl,dtype", [("general", "bf16"), ("decode", "bf16"), ("decode", "f32")])
+@pytest.mark.parametrize("H,KV,D,most", [(4, 2, 64, 1), (7, 1, 128, 1), (7, 1, 64, 2), (3, 3, 128, 3)])
+def test_requests_with_more_tokens_than_the_step_says(H, KV, D, most, impl, dtype):
+    """Of a request that brings more than ``max_q_len`` tokens the first ones are computed, and nothing else is touched."""
+    a, kw = batch(H, KV, D, 16, [3, 1, 9, 2], [300, 20, 90, 2], None, dtype)
+    kw["max_q_len"] = most
+    out = torch.full_like(a["q"], 9.0)
+    got = ops().paged_attention_fp4(**a, **kw, impl=impl, out=out).double().cpu()
+    ops().check_status()
+    want, s, v = fp4_plain.attention(a["q"], a["k_pages"], a["v_pages"], a["block_table"], a["q_start"], a["kv_len"], 16, kw["scale"], None)
+    bound = v * (s + 4.0) * 2.0 ** -18 + (v * 2.0 ** -12 + want.abs() * 2.0 ** -8 if dtype == "bf16" else 0.0)
+    starts = a["q_start"].tolist()
+    computed = torch.tensor([t - lo < most for lo, hi in zip(starts, starts[1:]) for t in range(lo, hi)])
+    assert ((got - want).abs() <= bound)[computed].all() and (got[~computed] == 9.0).all()

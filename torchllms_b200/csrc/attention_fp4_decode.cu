@@ -179,7 +179,9 @@ template <int ROWS> __device__ __forceinline__ int block_at(const Params& p, int
     k.first = p.q_start[k.b];
     const int ql = p.q_start[k.b + 1] - k.first;
     k.row0 = k.number * ROWS;
-    k.n_rows = min(ROWS, ql * p.group - k.row0);
+    // (p.rows, fewer than ROWS where one block has all: a request that brings more tokens than the step's max_q_len must not have
+    // rows that the places of the warps' and parts' results were not made for)
+    k.n_rows = min(p.rows, ql * p.group - k.row0);
     if (k.n_rows <= 0) return 0;
     k.base = p.kv_len[k.b] - ql;
     const int t0 = token_of(p, k.row0), t1 = token_of(p, k.row0 + k.n_rows - 1);

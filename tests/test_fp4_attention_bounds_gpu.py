@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import fp4_plain
-from test_fp4_kernels_gpu import batch, ops
+from test_fp4_kernels_gpu import batch, judge, ops
 from torchllms_b200.cache import fp4
 
 pytestmark = pytest.mark.gpu
@@ -93,3 +93,21 @@ def test_requests_with_more_tokens_than_the_step_says(H, KV, D, most, impl, dtyp
     starts = a["q_start"].tolist()
     computed = torch.tensor([t - lo < most for lo, hi in zip(starts, starts[1:]) for t in range(lo, hi)])
     assert ((got - want).abs() <= bound)[computed].all() and (got[~computed] == 9.0).all()
+
+
+@pytest.mark.parametrize("impl,dtype", [("general", "f32"), ("decode", "bf16"), ("decode", "f32"), ("prefill", "bf16"), ("prefill in 3 pieces", "bf16")])
+@pytest.mark.parametrize("scale", [-0.125, 0.0, 1e-30, -1e-30])
+def test_scales_that_are_not_positive(impl, dtype, scale):
+    """The formula holds for any factor: negative ones, none at all, and ones that vanish beside small queries."""
+    for sharp in (1.0, 1e-30, 0.0):
+        a, kw = batch(8, 2, 64, 16, [1, 70, 3], [200, 150, 2], None, dtype, sharp=sharp)
+        kw["scale"] = scale
+        judge(attend(a, kw, impl), a, kw)
+
+
+def test_scales_that_are_no_numbers_are_refused():
+    from torchllms_b200.kernels.native import KernelError
+    a, kw = batch(4, 2, 64, 16, [1], [30])
+    for scale in (float("nan"), float("inf"), -float("inf"), 1e300):
+        with pytest.raises(KernelError, match="finite float32"):
+            ops().paged_attention_fp4(**a, **dict(kw, scale=scale))

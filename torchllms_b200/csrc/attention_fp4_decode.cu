@@ -328,7 +328,10 @@ struct Consumer {
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
             // the row's largest number goes to 2^14 .. 2^15 (exponents as float32 has them, 127 more than they mean)
             const int up = min(268 - (int)(top >> 23), 253);
-            const float factor = __uint_as_float((unsigned)up << 23), back = __uint_as_float((unsigned)(254 - up) << 23) * p.scale_log2;
+            // (the scale's sign goes with the queries, so that larger sums are larger scores; and what scores are multiplied by stays above
+            // zero, for -inf times it: where 2^-126 stands for less, scores are below 2^-80 either way)
+            const float factor = __uint_as_float((unsigned)up << 23 | (__float_as_uint(p.scale_log2) & 0x80000000u));
+            const float back = fmaxf(__uint_as_float((unsigned)(254 - up) << 23) * fabsf(p.scale_log2), 1.17549435e-38f);
 #pragma unroll
             for (int j = 0; j < WORDS; ++j)
 #pragma unroll

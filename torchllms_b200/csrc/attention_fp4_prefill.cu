@@ -580,7 +580,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_fp4_prefill_kernel(cons
             }
             // the row's largest number goes to 2^14 .. 2^15 (exponents as float32 has them, 127 more than they mean)
             const int up = min(268 - (int)((__float_as_uint(top) & 0x7fffffffu) >> 23), 253);
-            const float factor = __uint_as_float((unsigned)up << 23);
+            // (the scale's sign goes with the queries: larger sums are larger scores)
+            const float factor = __uint_as_float((unsigned)up << 23 | (__float_as_uint(p.scale_log2) & 0x80000000u));
             back = __uint_as_float((unsigned)(254 - up) << 23);
 #pragma unroll 2
             for (int c = 0; c < CH; ++c) {
@@ -593,7 +594,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_fp4_prefill_kernel(cons
             if (lane == 0) mbar_arrive(&tail.q_full);
         }
         const unsigned col_s = COL_S, col_p = COL_P + t * (BN / 2), col_o = COL_O + t * HD;
-        const float fit = back * p.scale_log2;
+        // (above zero, for -inf times it: where 2^-126 stands for less, scores are below 2^-80 either way)
+        const float fit = fmaxf(back * fabsf(p.scale_log2), 1.17549435e-38f);
         float m_used = -INFINITY, l_sum = 0.f;
         const int qpos = base + token_of(p, tile_row0 + (r < rows ? r : max(rows - 1, 0)));
         const float2 sc2 = make_float2(fit, fit);

@@ -15,6 +15,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cmath>
 #include <vector>
 
 namespace {
@@ -215,7 +216,7 @@ PyObject* attend(PyObject*, PyObject* const* args, Py_ssize_t n) {
     int n_seqs, max_q, max_kv, page_size, split, impl, min_rows, window = 0, n_tokens = 1;
     double scale;
     if (q == nullptr || k == nullptr || table == nullptr || q->dim() != 3 || k->dim() != 4 || !whole(args[6], n_seqs) || !whole(args[7], max_q) ||
-        !whole(args[8], max_kv) || !number(args[9], scale) || (args[10] != Py_None && (!whole(args[10], window) || window <= 0)) ||
+        !whole(args[8], max_kv) || !number(args[9], scale) || !std::isfinite((float)scale) || (args[10] != Py_None && (!whole(args[10], window) || window <= 0)) ||
         !whole(args[11], page_size) || !whole(args[12], split) || !whole(args[13], impl) || (args[14] != Py_None && !whole(args[14], n_tokens)) ||
         !whole(args[16], min_rows))
         Py_RETURN_NONE;

@@ -2145,7 +2145,8 @@ class NativeOps:
         self.launches += 1
         return got
 
-    def _attention_fp4_explained(self, q, k_pages, v_pages, block_table, q_start, kv_len, n_seqs, max_kv_len, window, page_size, impl, n_tokens, out):
+    def _attention_fp4_explained(self, q, k_pages, v_pages, block_table, q_start, kv_len, n_seqs, max_kv_len, scale, window, page_size, impl,
+                                 n_tokens, out):
         _cuda_contig(q, "q")
         _need(q.dim() == 3 and q.dtype in _DT, "q must be [tokens, heads, head_dim] in float32 or bfloat16")
         _cuda_contig(q_start, "q_start", torch.int32)
@@ -2163,6 +2164,7 @@ class NativeOps:
             _cuda_contig(out, "out", q.dtype)
             _need(out.shape == q.shape, "out must have q's shape")
         _need(window is None or window > 0, "a window holds at least one key")
+        _need(abs(scale) < 2.0 ** 128, f"scale must be a finite float32, got {scale}")
         _need(block_table.shape[0] >= n_seqs and q_start.numel() >= n_seqs + 1 and kv_len.numel() >= n_seqs,
               "block_table, q_start and kv_len must cover every request of the step")
         _need(block_table.shape[1] * page_size >= max_kv_len, "block_table is too narrow for max_kv_len")
@@ -2192,7 +2194,8 @@ class NativeOps:
         got = calls.attend(q, k_pages, v_pages, block_table, q_start, kv_len, n_seqs, max_q_len, max_kv_len, scale, window, page_size,
                            allow_split, self._FP4_IMPLS.get(impl, -1), n_tokens, out, self.FP4_PREFILL_MIN_ROWS)
         if got is None:
-            self._attention_fp4_explained(q, k_pages, v_pages, block_table, q_start, kv_len, n_seqs, max_kv_len, window, page_size, impl, n_tokens, out)
+            self._attention_fp4_explained(q, k_pages, v_pages, block_table, q_start, kv_len, n_seqs, max_kv_len, scale, window, page_size, impl,
+                                          n_tokens, out)
         if got.__class__ is int:
             _check(got, "paged_attention_fp4")
         self.launches += got[1]

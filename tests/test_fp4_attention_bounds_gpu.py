@@ -111,3 +111,33 @@ def test_scales_that_are_no_numbers_are_refused():
     for scale in (float("nan"), float("inf"), -float("inf"), 1e300):
         with pytest.raises(KernelError, match="finite float32"):
             ops().paged_attention_fp4(**a, **dict(kw, scale=scale))
+
+
+def test_every_instance_has_its_own_status_word():
+    """A call's bounded waits report to the instance that made the call, whichever instance made its first call last."""
+    import ctypes
+    from torchllms_b200.kernels.native import NativeOps
+    seen = []
+    signature = ctypes.CFUNCTYPE(ctypes.c_int, *[ctypes.c_void_p] * 4, ctypes.c_void_p, ctypes.c_int, ctypes.c_int, *[ctypes.c_void_p] * 5,
+                                 *[ctypes.c_int] * 6, ctypes.c_longlong, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_float, ctypes.c_void_p)
+    fake = signature(lambda *args: seen.append(args[11]) or 0)           # (the status word is the twelfth; nothing is launched)
+
+    class Library:
+        def __init__(self, real):
+            self.real = real
+
+        def __getattr__(self, name):
+            return fake if name == "tl_attention_fp4_decode" else getattr(self.real, name)
+
+    one, two = NativeOps(), NativeOps()
+    for o in (one, two):
+        load = o._lib
+        o._lib = lambda name, load=load: Library(load(name)) if name == "attention_fp4_decode" else load(name)
+    a, kw = batch(4, 2, 64, 16, [1], [30])
+    try:
+        for o in (one, two, one):
+            o.paged_attention_fp4(**a, **kw, impl="decode")
+    finally:
+        ops()._fp4_load()                                                # (the kernels themselves again)
+    assert seen == [o._status.data_ptr() for o in (one, two, one)]
+    judge(ops().paged_attention_fp4(**a, **kw, impl="decode"), a, kw)

@@ -33,7 +33,6 @@ struct Entries {
     int (*prefill)(const void*, const void*, const void*, void*, const int*, int, int, const int*, const int*, float*, int*, long long, int, int, int, int,
                    int, long long, int, int, float, int, void*);
     int (*prefill_plan)(long long, int, int, int, int, int, int, int, int*, long long*);
-    int* status;
 } entry;
 
 constexpr int GROUP = 16, RECORD = 16, MAX_HEAD_DIM = 256;
@@ -108,12 +107,12 @@ int* counters(const at::Tensor& like, void* stream, long long n) {
 }
 
 PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
-    if (n != 8) {
-        PyErr_SetString(PyExc_TypeError, "bind takes eight addresses");
+    if (n != 7) {
+        PyErr_SetString(PyExc_TypeError, "bind takes seven addresses");
         return nullptr;
     }
-    void* at[8];
-    for (int i = 0; i < 8; ++i) at[i] = PyLong_AsVoidPtr(args[i]);
+    void* at[7];
+    for (int i = 0; i < 7; ++i) at[i] = PyLong_AsVoidPtr(args[i]);
     if (PyErr_Occurred()) return nullptr;
     entry.write = (decltype(entry.write))at[0];
     entry.read = (decltype(entry.read))at[1];
@@ -122,7 +121,6 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
     entry.decode_plan = (decltype(entry.decode_plan))at[4];
     entry.prefill = (decltype(entry.prefill))at[5];
     entry.prefill_plan = (decltype(entry.prefill_plan))at[6];
-    entry.status = (int*)at[7];
     Py_RETURN_NONE;
 }
 
@@ -207,10 +205,11 @@ bool many_rows(long long rows, int head_dim, long long units, int max_kv, int le
 }
 
 // q, k_pages, v_pages, block_table, q_start, kv_len, n_seqs, max_q_len, max_kv_len, scale, window, page_size, allow_split, impl (0 the kernel that fits,
-// 1 general, 2 decode, 3 prefill), n_tokens, out, rows of a request from which 3 fits -> (out, launches), an error code, or None
+// 1 general, 2 decode, 3 prefill), n_tokens, out, rows of a request from which 3 fits, the caller's status word (its address) -> (out, launches), an
+// error code, or None
 PyObject* attend(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    if (n != 17) Py_RETURN_NONE;
+    if (n != 18) Py_RETURN_NONE;
     const at::Tensor *q = tensor(args[0]), *k = tensor(args[1]), *v = tensor(args[2]), *table = tensor(args[3]), *q_start = tensor(args[4]),
                      *kv_len = tensor(args[5]), *given = tensor(args[15]);
     int n_seqs, max_q, max_kv, page_size, split, impl, min_rows, window = 0, n_tokens = 1;
@@ -220,6 +219,11 @@ PyObject* attend(PyObject*, PyObject* const* args, Py_ssize_t n) {
         !whole(args[11], page_size) || !whole(args[12], split) || !whole(args[13], impl) || (args[14] != Py_None && !whole(args[14], n_tokens)) ||
         !whole(args[16], min_rows))
         Py_RETURN_NONE;
+    int* status = PyLong_Check(args[17]) ? (int*)PyLong_AsVoidPtr(args[17]) : nullptr;
+    if (status == nullptr) {
+        PyErr_Clear();
+        Py_RETURN_NONE;
+    }
     const int code = code_of(*q);
     const long long heads = q->size(1), head_dim = q->size(2), kv_heads = k->size(1), n_pages = k->size(0);
     if (!q->is_cuda() || code < 0 || !q->is_contiguous() || heads <= 0 || heads > INT32_MAX || kv_heads <= 0 || heads % kv_heads != 0 ||
@@ -251,7 +255,7 @@ PyObject* attend(PyObject*, PyObject* const* args, Py_ssize_t n) {
                 at::Tensor scratch = fresh({floats}, at::kFloat, *q);
                 int* counts = counters(*q, stream, count);
                 rc = entry.decode(q->data_ptr(), k->data_ptr(), v->data_ptr(), out.data_ptr(), bt, stride, columns, q_start->data_ptr<int>(),
-                                  kv_len->data_ptr<int>(), scratch.data_ptr<float>(), counts, entry.status, code, n_seqs, (int)heads, (int)kv_heads,
+                                  kv_len->data_ptr<int>(), scratch.data_ptr<float>(), counts, status, code, n_seqs, (int)heads, (int)kv_heads,
                                   (int)head_dim, page_size, n_pages, max_q, max_kv, window, (float)scale, stream);
             }
         } else if (impl == 3) {
@@ -262,7 +266,7 @@ PyObject* attend(PyObject*, PyObject* const* args, Py_ssize_t n) {
                 at::Tensor scratch;
                 if (floats > 0) scratch = fresh({floats}, at::kFloat, *q);
                 rc = entry.prefill(q->data_ptr(), k->data_ptr(), v->data_ptr(), out.data_ptr(), bt, stride, columns, q_start->data_ptr<int>(),
-                                   kv_len->data_ptr<int>(), floats > 0 ? scratch.data_ptr<float>() : nullptr, entry.status, q->size(0), n_seqs,
+                                   kv_len->data_ptr<int>(), floats > 0 ? scratch.data_ptr<float>() : nullptr, status, q->size(0), n_seqs,
                                    (int)heads, (int)kv_heads, (int)head_dim, page_size, n_pages, max_q, window, (float)scale, pieces, stream);
                 if (pieces > 1) launches = 2;
             }

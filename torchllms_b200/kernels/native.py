@@ -138,6 +138,7 @@ class NativeOps:
         self.use_gated = os.environ.get("TORCHLLMS_B200_NO_GATED", "") not in ("1", "true")
         # error word of kernels with bounded waits: pinned host memory the device writes to directly
         self._status = torch.zeros(4, dtype=torch.int32).pin_memory()
+        self._status_at = self._status.data_ptr()
         self._mm_out_dtype: Optional[bool] = None
         self._profile = None
         self._profile_depth = 0
@@ -2059,7 +2060,7 @@ class NativeOps:
         names = (("kv_fp4", "tl_rope_kv_write_fp4"), ("kv_fp4", "tl_kv_read_fp4"), ("attention_fp4", "tl_attention_fp4_general"),
                  ("attention_fp4_decode", "tl_attention_fp4_decode"), ("attention_fp4_decode", "tl_attention_fp4_decode_plan"),
                  ("attention_fp4_prefill", "tl_attention_fp4_prefill"), ("attention_fp4_prefill", "tl_attention_fp4_prefill_plan"))
-        calls.bind(*(ctypes.cast(getattr(self._lib(lib), name), ctypes.c_void_p).value for lib, name in names), self._status.data_ptr())
+        calls.bind(*(ctypes.cast(getattr(self._lib(lib), name), ctypes.c_void_p).value for lib, name in names))
         self._fp4 = calls
         return calls
 
@@ -2192,7 +2193,7 @@ class NativeOps:
         if self.debug:
             self._fp4_debug(k_pages.shape[0])
         got = calls.attend(q, k_pages, v_pages, block_table, q_start, kv_len, n_seqs, max_q_len, max_kv_len, scale, window, page_size,
-                           allow_split, self._FP4_IMPLS.get(impl, -1), n_tokens, out, self.FP4_PREFILL_MIN_ROWS)
+                           allow_split, self._FP4_IMPLS.get(impl, -1), n_tokens, out, self.FP4_PREFILL_MIN_ROWS, self._status_at)
         if got is None:
             self._attention_fp4_explained(q, k_pages, v_pages, block_table, q_start, kv_len, n_seqs, max_kv_len, scale, window, page_size, impl,
                                           n_tokens, out)

@@ -141,3 +141,25 @@ def test_every_instance_has_its_own_status_word():
         ops()._fp4_load()                                                # (the kernels themselves again)
     assert seen == [o._status.data_ptr() for o in (one, two, one)]
     judge(ops().paged_attention_fp4(**a, **kw, impl="decode"), a, kw)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("n,behind", [(4, 3000), (16, 2500), (64, 1900), (200, 700)])
+def test_a_portion_that_is_cut_leaves_the_rows_beside_it_alone(D, n, behind):
+    """Decoded tokens and a portion in one output: the portion's keys are cut and its pieces added up over its own rows."""
+    H, KV, page, nd = 8, 2, 16, 3
+    a, kw = batch(H, KV, D, page, [1] * nd + [n], [40, 700, 1300, behind + n], None, "bf16", seed=n)
+    part = lambda lo, hi: dict(a, block_table=a["block_table"][lo:hi], q_start=a["q_start"][lo:hi + 1], kv_len=a["kv_len"][lo:hi])  # noqa: E731
+    out = torch.full_like(a["q"], 9.0)
+    ops().paged_attention_fp4(**part(0, nd), **dict(kw, n_seqs=nd, max_q_len=1), n_tokens=nd, out=out)
+    decoded = out[:nd].clone()
+    for cut in (True, 5):
+        before = ops().launches
+        ops().paged_attention_fp4(**part(nd, nd + 1), **dict(kw, n_seqs=1), out=out, allow_split=cut, impl="prefill")
+        assert ops().launches - before == 2 and torch.equal(out[:nd], decoded)
+        judge(out, a, kw)
+        out[nd:] = 9.0
+    ops().paged_attention_fp4(**part(nd, nd + 1), **dict(kw, n_seqs=1), out=out)
+    ops().check_status()
+    assert torch.equal(out[:nd], decoded)
+    judge(out, a, kw)

@@ -74,7 +74,8 @@ class PagedAttention(Mixer):
         qkv = ops.linear(x, self.wqkv, partials_ok=True)   # the encoding adds up split-K partial sums
         q = self.position.encode_and_store(qkv, ctx, cache, self.n_heads, self.n_kv_heads, self.head_dim)
         common = dict(scale=self.scale, window=self.window, page_size=cache.page_size)
-        attend = ops.paged_attention_fp4 if getattr(cache, "format", "full") == "fp4" else ops.paged_attention
+        packed = getattr(cache, "format", "full") == "fp4"
+        attend = ops.paged_attention_fp4 if packed else ops.paged_attention
         nd, B = getattr(ctx, "n_decode", 0), ctx.n_seqs
         if 0 < nd < B and ctx.max_q_len > 1:
             # decoded tokens beside prompt portions: the requests at the head of the batch bring one
@@ -84,9 +85,11 @@ class PagedAttention(Mixer):
             attend(q, cache.k_pages, cache.v_pages, cache.block_table[:nd], ctx.q_start[:nd + 1],
                    ctx.kv_len[:nd], n_seqs=nd, max_q_len=1, max_kv_len=ctx.decode_kv_bound,
                    n_tokens=nd, out=o, **common)
+            # (keys cut into pieces: the merge pass of the cache in the compute type would run over the first call's rows
+            # too; that of the 4-bit cache has its own call's rows only)
             attend(q, cache.k_pages, cache.v_pages, cache.block_table[nd:], ctx.q_start[nd:],
                    ctx.kv_len[nd:], n_seqs=B - nd, max_q_len=ctx.max_q_len, max_kv_len=ctx.max_kv_len,
-                   out=o, allow_split=False, **common)   # (a merge pass would run over the first call's rows too)
+                   out=o, allow_split=packed, **common)
         else:
             o = attend(
                 q, cache.k_pages, cache.v_pages, cache.block_table, ctx.q_start, ctx.kv_len,

@@ -163,3 +163,13 @@ def test_a_portion_that_is_cut_leaves_the_rows_beside_it_alone(D, n, behind):
     ops().check_status()
     assert torch.equal(out[:nd], decoded)
     judge(out, a, kw)
+
+
+def test_keys_that_may_not_be_cut_go_to_the_kernel_that_is_faster_so():
+    """(64 rows behind 12,000 keys: 8 CTAs of the tcgen05 kernel would walk all of them)"""
+    a, kw = batch(8, 2, 64, 16, [16], [3000], None, "bf16")
+    whole = ops().paged_attention_fp4(**a, **kw, allow_split=False)
+    assert torch.equal(whole, ops().paged_attention_fp4(**a, **kw, impl="decode"))
+    assert not torch.equal(whole, ops().paged_attention_fp4(**a, **kw, allow_split=False, impl="prefill"))
+    a, kw = batch(8, 8, 64, 16, [300] * 4, [400] * 4, None, "bf16")                      # 300 rows of 32 units
+    assert torch.equal(ops().paged_attention_fp4(**a, **kw, allow_split=False), ops().paged_attention_fp4(**a, **kw, allow_split=False, impl="prefill"))

@@ -200,7 +200,12 @@ PyObject* read(PyObject*, PyObject* const* args, Py_ssize_t n) {
 //   8 requests                      32 rows:  8.8  9.4   19.0 20.6   57.5 71.0     64:  8.8  9.4   28.2 21.0   105  72       256: 27.5 13.0   80   30     374  91
 // So it is one from `least` rows on, and with heads of 128 from 17 on where the context is long and there are no more than 1,024 tiles of 128 keys
 // (32 rows: one request of 12,000 tokens 25.9 and 22.7, 8 of 2,000 27.0 and 23.7; but 8 of 12,000 82 and 98, one of 200 9.6 and 10.4).
-bool many_rows(long long rows, int head_dim, long long units, int max_kv, int least) {
+// Those are times with keys that the tcgen05 kernel may cut into pieces.  Where it may not (`cut`), a CTA walks all keys of its rows, and more than two tiles of
+// them are for it only where rows are many: the mma.sync kernel, which cuts them as it likes, and the tcgen05 kernel without pieces, contexts of 2,000 and 12,000:
+//   rows x units     512 (1 request, 64 rows):  of 64: 11.6  27.8   24.4 131   of 128: 16.1  33.5   36.0 149       2,048 (4 requests): 19.4 28.3  59.8 163   27.7 34.1  86 192
+//                  4,096 (2 requests, 256 rows):       28.6  37.0    107 168           41.7  43.9    155 201       8,192 (4 requests): 47.9 37.2   204 174   70.6 44.2 294 208
+bool many_rows(long long rows, int head_dim, long long units, int max_kv, int least, bool cut) {
+    if (!cut && max_kv > 256) return rows >= least && rows * units >= 8192;
     return rows >= least || (head_dim == 128 && rows > 16 && max_kv >= 1024 && units * ((max_kv + 127) / 128) <= 1024);
 }
 
@@ -240,7 +245,7 @@ PyObject* attend(PyObject*, PyObject* const* args, Py_ssize_t n) {
     at::Tensor out = given != nullptr ? *given : fresh(q->sizes(), q->scalar_type(), *q);
     if (impl == 0) {        // (the tcgen05 kernel stores 32 bytes at a time)
         const bool many = code == 1 && (uintptr_t)out.data_ptr() % 32 == 0 &&
-                          many_rows(max_q * (heads / kv_heads), (int)head_dim, n_seqs * kv_heads, max_kv, min_rows);
+                          many_rows(max_q * (heads / kv_heads), (int)head_dim, n_seqs * kv_heads, max_kv, min_rows, split != 0);
         impl = !tensor_cores ? 1 : many ? 3 : 2;
     }
     void* stream = stream_of(*q);

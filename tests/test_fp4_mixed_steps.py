@@ -1,10 +1,12 @@
-"""Steps that have decoded tokens beside portions, over a 4-bit cache: which calls of the attention they make (on the host)."""
+"""Steps over a 4-bit cache that bring portions: what their calls of the attention are told, and recorded steps beside others."""
 
 import pytest
+import torch
 
-from helpers import tiny_folder
+from helpers import TINY_C, make_tensors, tiny_folder, write_model_folder
 from test_fp4_cache import Fp4TorchOps
 from torchllms_b200.engine.replay import Replayer
+from torchllms_b200.engine.step import StepEntry
 
 
 class Recording(Fp4TorchOps):
@@ -12,9 +14,10 @@ class Recording(Fp4TorchOps):
 
     def __init__(self):
         super().__init__()
-        self.calls = []
+        self.calls, self.bounds = [], []
 
     def paged_attention(self, q, *args, **kw):
+        self.bounds.append(kw["max_kv_len"])
         self.calls.append(("full", kw["n_seqs"], kw["max_q_len"], kw.get("allow_split", True)))
         return super().paged_attention(q, *args, **kw)
 
@@ -31,9 +34,42 @@ def test_keys_of_portions_beside_decoded_tokens_may_be_cut(tmp_path, kv_format, 
     ops = Recording()
     rp = Replayer(tiny_folder(tmp_path, "A"), "float32", 256, page_size=16, device="cpu", ops=ops, kv_format=kv_format)
     engine = rp.engine
-    from torchllms_b200.engine.step import StepEntry
     a, b = engine.claim(), engine.claim()
     engine.step([StepEntry(a, [1, 2, 3])])
     ops.calls.clear()
     engine.step([StepEntry(a, [4]), StepEntry(b, [5, 6, 7, 8, 9])])
     assert set(ops.calls) == {(kv_format, 1, 1, True), (kv_format, 1, 5, cut)}
+
+
+@pytest.mark.parametrize("kv_format,bounds", [("full", {30, 42, 60}), ("fp4", {128})])
+def test_portions_over_a_4_bit_cache_plan_for_a_bound(tmp_path, kv_format, bounds):
+    """Recorded steps are told apart by what their launches were planned for: with a cache whose keys are cut for long portions,
+    too, that is a bound of the context, not the length that the first such step happened to have."""
+    ops = Recording()
+    engine = Replayer(tiny_folder(tmp_path, "A"), "float32", 128, page_size=16, device="cpu", ops=ops, kv_format=kv_format).engine
+    a = engine.claim()
+    for n in (30, 12, 18):
+        ops.bounds.clear()
+        engine.step([StepEntry(a, [1 + i for i in range(n)])])
+        if n > 16:
+            assert set(ops.bounds) <= bounds, ops.bounds
+
+
+@pytest.mark.gpu
+def test_a_step_recorded_at_a_short_context_is_not_the_one_of_a_long_one(tmp_path):
+    """Portions of 48 tokens, one behind the other: recorded steps give the bits and make the launches of eager ones all the way."""
+    folder = write_model_folder(tmp_path / "long", dict(TINY_C, max_position_embeddings=8192), make_tensors(TINY_C, 2), torch.bfloat16)
+    runs = []
+    for graphs in (False, True):
+        engine = Replayer(folder, "bfloat16", 8192, page_size=16, kv_format="fp4").engine
+        engine.use_graphs = engine.use_graphs and graphs
+        assert engine.use_graphs == graphs
+        a, run = engine.claim(), []
+        for step in range(100):
+            before = engine.model.ops.launches
+            logits = engine.step([StepEntry(a, [(7 * step + i) % 777 for i in range(48)])]).clone()
+            run.append((logits, engine.model.ops.launches - before))
+        assert (engine.graph_replays > 50) == graphs
+        runs.append(run)
+    for (eager, launches), (recorded, as_many) in zip(*runs):
+        assert launches == as_many and torch.equal(eager, recorded)

@@ -173,10 +173,12 @@ class Engine:
         # A step's launch shapes depend only on (tokens, requests, wanted rows, longest portion) and, for
         # steps of short portions, on a coarse bound of the longest context (a power of two: it decides
         # over how many CTAs the keys are split), never on the exact lengths: the kernels read lengths
-        # and tables from the uploaded buffers.  So a shape that keeps coming back (every decode step
+        # and tables from the uploaded buffers.  (The attention over a 4-bit cache splits the keys of long
+        # portions, too: with such a cache every step plans for the bound.)  So a shape that keeps coming back (every decode step
         # with the same number of requests; every full prompt chunk) is recorded once into a CUDA graph
         # and replayed.
         ops = model.ops
+        self._bounds_portions = getattr(model, "kv_format", "full") == "fp4"
         self.use_graphs = bool(use_graphs and self.device.type == "cuda" and model.graph_safe
                                and getattr(ops, "graph_capturable", lambda d: False)(model.dtype))
         self._graphs = {}          # shape key -> (graph, logits buffer, launches)
@@ -203,7 +205,7 @@ class Engine:
         (while fewer than ``max_prompt_graphs`` of those exist); later steps replay.  The logits
         buffer of a shape is reused: its contents hold until the next step of that shape."""
         key = self._shape_key(ctx.n_tokens, ctx.n_seqs, ctx.n_want, ctx.max_q_len, ctx.n_decode,
-                              ctx.max_kv_len if ctx.max_q_len <= 16 else 0, ctx.decode_kv_bound)
+                              ctx.max_kv_len if self._plans_for_bound(ctx.max_q_len) else 0, ctx.decode_kv_bound)
         entry = self._graphs.get(key)
         if entry is None:
             seen = self._graph_seen.get(key, 0)
@@ -230,6 +232,10 @@ class Engine:
     def _shape_key(n_tokens: int, n_seqs: int, n_want: int, max_q_len: int, n_decode: int, kv_bound: int,
                    decode_bound: int = 0):
         return (n_tokens, n_seqs, n_want, max_q_len, n_decode, kv_bound, decode_bound)
+
+    def _plans_for_bound(self, max_q_len: int) -> bool:
+        """Whether a step's launches are planned for ``kv_bound`` of its longest context (and its shape has that for a part)."""
+        return max_q_len <= 16 or self._bounds_portions
 
     BOUND_BELOW = 16     # steps of fewer requests plan for a bound of their longest context, others for max_len
 
@@ -465,10 +471,10 @@ class Engine:
             n_decode = 0
             while n_decode < B and q_lens[n_decode] == 1:
                 n_decode += 1
-            # steps of short portions (where keys may be split over CTAs) plan for a coarse bound of the
-            # longest context, so that their launch shapes change only when a request outgrows it
-            short = max_q <= 16
-            bound = (self._forced_bound or self.kv_bound(max(kv_lens), B)) if short else 0
+            # steps whose keys may be split over CTAs (those of short portions; with a 4-bit cache all) plan for a coarse
+            # bound of the longest context, so that their launch shapes change only when a request outgrows it
+            bounded = self._plans_for_bound(max_q)
+            bound = (self._forced_bound or self.kv_bound(max(kv_lens), B)) if bounded else 0
             # a mixed step's one-token rows go to the decode kernel apart from the portions: their own bound
             decode_bound = self.kv_bound(max(kv_lens[:n_decode]), n_decode) if 0 < n_decode < B else 0
             recorded = (self._graphs.get(self._shape_key(T, B, n_want, max_q, n_decode, bound, decode_bound))
@@ -479,7 +485,7 @@ class Engine:
             else:
                 ctx = StepContext(
                     n_tokens=T, n_seqs=B, n_want=n_want, max_q_len=max_q, n_decode=n_decode,
-                    max_kv_len=bound if short else max(kv_lens), decode_kv_bound=decode_bound,
+                    max_kv_len=bound if bounded else max(kv_lens), decode_kv_bound=decode_bound,
                     token_ids=buf.dev_view("token_ids", T), positions=buf.dev_view("positions", T),
                     seq_of_token=buf.dev_view("seq_of_token", T), q_start=buf.dev_view("q_start", B + 1),
                     kv_len=buf.dev_view("kv_len", B), state_slot=buf.dev_view("state_slot", B),

@@ -173,3 +173,17 @@ def test_keys_that_may_not_be_cut_go_to_the_kernel_that_is_faster_so():
     assert not torch.equal(whole, ops().paged_attention_fp4(**a, **kw, allow_split=False, impl="prefill"))
     a, kw = batch(8, 8, 64, 16, [300] * 4, [400] * 4, None, "bf16")                      # 300 rows of 32 units
     assert torch.equal(ops().paged_attention_fp4(**a, **kw, allow_split=False), ops().paged_attention_fp4(**a, **kw, allow_split=False, impl="prefill"))
+
+
+@pytest.mark.parametrize("D,n,most_kv,kernel", [(128, 8, 200, "decode"), (128, 8, 1024, "decode"), (128, 8, 1025, "prefill"), (128, 8, 4096, "prefill"),
+                                                (128, 15, 1024, "decode"), (128, 4, 4096, "decode"), (128, 16, 1024, "prefill"), (64, 15, 4096, "decode"),
+                                                (64, 16, 1024, "prefill")])
+def test_the_kernel_goes_by_rows_and_the_planned_context(D, n, most_kv, kernel):
+    """(groups of four; a step may plan for more keys than its requests have)"""
+    a, kw = batch(8, 2, D, 16, [n, n], [200, 150], None, "bf16", seed=n)
+    a["block_table"] = torch.nn.functional.pad(a["block_table"], (0, 256), value=-1)
+    kw["max_kv_len"] = most_kv
+    got = {impl: ops().paged_attention_fp4(**a, **kw, impl=impl) for impl in ("auto", "decode", "prefill")}
+    ops().check_status()
+    judge(got["auto"], a, kw)
+    assert not torch.equal(got["decode"], got["prefill"]) and torch.equal(got["auto"], got[kernel])

@@ -198,7 +198,8 @@ PyObject* read(PyObject*, PyObject* const* args, Py_ssize_t n) {
 //   8 requests                      16 rows: 10.2 11.0   19.2 22.9   49.4 96.6     64: 11.4 11.5   39.4 24.2   147  99       256: 40.3 15.5   118  36     537 117
 //   1 request,           of 64      32 rows:  7.8  8.6   11.0 15.2   17.6 21.4     64:  8.0  8.6   11.9 15.7   24.1 22.2     256: 11.1 12.3   19.0 19.2    58  28
 //   8 requests                      32 rows:  8.8  9.4   19.0 20.6   57.5 71.0     64:  8.8  9.4   28.2 21.0   105  72       256: 27.5 13.0   80   30     374  91
-// So it is one from `least` rows on, and with heads of 128 from 17 on where the context is long and there are no more than 1,024 tiles of 128 keys
+// So it is one from `least` rows on, and with heads of 128 from 17 on where the context is long (beyond 1,024: the engine's steps plan for a power of two
+// that is no less, so that all shorter contexts come as 1,024) and there are no more than 1,024 tiles of 128 keys
 // (32 rows: one request of 12,000 tokens 25.9 and 22.7, 8 of 2,000 27.0 and 23.7; but 8 of 12,000 82 and 98, one of 200 9.6 and 10.4).
 // Those are times with keys that the tcgen05 kernel may cut into pieces.  Where it may not (`cut`), a CTA walks all keys of its rows, and more than two tiles of
 // them are for it only where rows are many: the mma.sync kernel, which cuts them as it likes, and the tcgen05 kernel without pieces, contexts of 2,000 and 12,000:
@@ -206,7 +207,7 @@ PyObject* read(PyObject*, PyObject* const* args, Py_ssize_t n) {
 //                  4,096 (2 requests, 256 rows):       28.6  37.0    107 168           41.7  43.9    155 201       8,192 (4 requests): 47.9 37.2   204 174   70.6 44.2 294 208
 bool many_rows(long long rows, int head_dim, long long units, int max_kv, int least, bool cut) {
     if (!cut && max_kv > 256) return rows >= least && rows * units >= 8192;
-    return rows >= least || (head_dim == 128 && rows > 16 && max_kv >= 1024 && units * ((max_kv + 127) / 128) <= 1024);
+    return rows >= least || (head_dim == 128 && rows > 16 && max_kv > 1024 && units * ((max_kv + 127) / 128) <= 1024);
 }
 
 // q, k_pages, v_pages, block_table, q_start, kv_len, n_seqs, max_q_len, max_kv_len, scale, window, page_size, allow_split, impl (0 the kernel that fits,

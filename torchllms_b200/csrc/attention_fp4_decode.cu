@@ -953,10 +953,6 @@ template <int HD> int launch(int dtype, const Params& p, const Plan& pl, cudaStr
 
 }  // namespace
 
-extern "C" int tl_attention_fp4_decode_supports(int n_heads, int n_kv_heads, int head_dim, int page_size) {
-    return takes(n_heads, n_kv_heads, head_dim, page_size) ? 1 : 0;
-}
-
 // What a call needs beside its operands: workspace_floats of scratch, and n_counters ints that are zero (and are zero again when
 // the call has run); no call that may run at the same time may have either.
 extern "C" int tl_attention_fp4_decode_plan(int dtype, int n_seqs, int n_heads, int n_kv_heads, int head_dim, int page_size, int max_q_len,

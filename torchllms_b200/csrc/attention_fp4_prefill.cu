@@ -862,10 +862,6 @@ template <int HD> int launch(const Params& p, dim3 grid, cudaStream_t s) {
 
 }  // namespace
 
-extern "C" int tl_attention_fp4_prefill_supports(int n_heads, int n_kv_heads, int head_dim, int page_size) {
-    return takes(n_heads, n_kv_heads, head_dim, page_size) ? 1 : 0;
-}
-
 // workspace_floats: scratch of a call (0: none); q_rows: rows of q, all of them.
 extern "C" int tl_attention_fp4_prefill_plan(long long q_rows, int n_seqs, int n_heads, int n_kv_heads, int head_dim, int max_q_len, int max_kv_len,
                                              int allow_split, int* pieces, long long* workspace_floats) {

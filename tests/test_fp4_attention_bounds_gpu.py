@@ -187,3 +187,26 @@ def test_the_kernel_goes_by_rows_and_the_planned_context(D, n, most_kv, kernel):
     ops().check_status()
     judge(got["auto"], a, kw)
     assert not torch.equal(got["decode"], got["prefill"]) and torch.equal(got["auto"], got[kernel])
+
+
+@pytest.mark.parametrize("impl,dtype", [("general", "bf16"), ("general", "f32"), ("decode", "bf16"), ("decode", "f32"), ("prefill", "bf16"), ("prefill in 3 pieces", "bf16")])
+@pytest.mark.parametrize("H,KV,q_lens,kv_lens,window", [(4, 2, [1, 1, 1], [1, 300, 17], None), (4, 2, [5, 70, 9], [2, 70, 400], None),
+                                                       (4, 2, [20, 3], [20, 90], 1), (32, 8, [65, 1, 200], [65, 30, 220], None)])
+@pytest.mark.parametrize("value", ["nan", "inf", "-inf"])
+def test_queries_that_are_not_finite(impl, dtype, H, KV, q_lens, kv_lens, window, value):
+    """They give what softmax gives (NaN, also where every score is -inf; a row without a key is zeros) and leave the other rows' bits alone."""
+    a, kw = batch(H, KV, 64, 16, q_lens, kv_lens, window, dtype, seed=len(q_lens))
+    before = attend(a, kw, impl)
+    g = torch.Generator().manual_seed(7)
+    T = a["q"].shape[0]
+    hit = torch.rand((T, H), generator=g) < 0.4
+    hit[0, 1] = hit[-1, 2] = True
+    where = torch.randint(0, 64, (T, H, 1), generator=g)
+    q = a["q"].cpu().scatter(2, where, torch.where(hit[..., None], float(value), a["q"].cpu().gather(2, where).float()).to(a["q"].dtype))
+    got = attend(dict(a, q=q.cuda()), kw, impl)
+    position = []
+    for b, L in enumerate(kv_lens):
+        position += list(range(L - q_lens[b], L))
+    wanted = hit & (torch.tensor(position) >= 0)[:, None]
+    assert torch.equal(got.isnan().cpu(), wanted[..., None].expand(-1, -1, 64))
+    assert torch.equal(got[~wanted.cuda()], before[~wanted.cuda()])

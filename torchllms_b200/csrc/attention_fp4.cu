@@ -137,7 +137,8 @@ __global__ void __launch_bounds__(WARPS * 32) attention_fp4_general_kernel(const
         f[w] = m_s[w] == -INFINITY ? 0.f : exp2f(m_s[w] - M);
         den = fmaf(f[w], l_s[w], den);
     }
-    const float inv = M == -INFINITY ? 0.f : 1.f / den;
+    // (no sum: zeros for a row without a key; where all scores are -inf, from a query that is not finite, there is no softmax)
+    const float inv = M == -INFINITY ? (pos >= 0 ? NAN : 0.f) : 1.f / den;
     for (int d = threadIdx.x; d < D; d += blockDim.x) {
         float num = 0.f;
 #pragma unroll

@@ -624,6 +624,8 @@ struct Consumer {
                 sum += __shfl_xor_sync(0xffffffffu, sum, 16);
                 const int rr = nt * 8 + 2 * t + j;
                 if (rr < n_rows) {
+                    // (no sum: a row without a key.  Rows of a warp's own are float32: a query there that is not finite has a remainder that is no
+                    // number, so that its sum is none either, also where every score is -inf)
                     const float inv = part != nullptr ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
                     const int at = row_in_part + rr;
 #pragma unroll
@@ -769,6 +771,8 @@ __global__ void __launch_bounds__(NTHREADS, (NT == 1 && sizeof(T) == 2) ? 3 : 2)
             const int row = w.k.row0 + rr, token = token_of(p, row);
             return reinterpret_cast<T*>(p.out) + ((size_t)(w.k.first + token) * p.n_heads + w.kvh * p.group + row - token * p.group) * HD;
         };
+        // what a row without a sum is multiplied by: zeros for one without a key; where all scores are -inf, from a query that is not finite, there is no softmax
+        auto unsummed = [&](int rr) { return w.k.base + token_of(p, w.k.row0 + rr) >= 0 ? NAN : 0.f; };
         // where a part of this block lies: that with its first tile in its CTA's first place, others in the second
         const size_t place = part_floats(p.rows, HD);
         auto part_of = [&](int cta, bool first) { return p.part + ((size_t)cta * 2 + (first ? 0 : 1)) * place; };
@@ -806,7 +810,7 @@ __global__ void __launch_bounds__(NTHREADS, (NT == 1 && sizeof(T) == 2) ? 3 : 2)
                     den = fmaf(f, Lm[v * ROWS + rr], den);
                 }
                 if (w.parts == 1) {
-                    const float inv = M == -INFINITY ? 0.f : 1.f / den;
+                    const float inv = M == -INFINITY ? unsummed(rr) : 1.f / den;
                     store4(out_row(rr) + d, make_float4(num.x * inv, num.y * inv, num.z * inv, num.w * inv));
                 } else {
                     __stcg(reinterpret_cast<float4*>(part + rr * HD + d), num);
@@ -865,7 +869,7 @@ __global__ void __launch_bounds__(NTHREADS, (NT == 1 && sizeof(T) == 2) ? 3 : 2)
                             den = fmaf(f, ml[i].y, den);
                         }
                     }
-                    const float inv = M == -INFINITY ? 0.f : 1.f / den;
+                    const float inv = M == -INFINITY ? unsummed(rr) : 1.f / den;
                     store4(out_row(rr) + d, make_float4(num.x * inv, num.y * inv, num.z * inv, num.w * inv));
                 }
             }

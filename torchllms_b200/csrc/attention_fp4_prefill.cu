@@ -704,7 +704,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_fp4_prefill_kernel(cons
         }
         if (ok && rows > 0) {
             if (p.pieces == 1) {
-                const float inv = l_sum == 0.f ? 0.f : 1.f / l_sum;
+                // (no sum: zeros for a row without a key; where all scores are -inf, from a query that is not finite, there is no softmax)
+                const float inv = l_sum == 0.f ? (qpos >= 0 ? NAN : 0.f) : 1.f / l_sum;
                 // (a thread its own row, whole sectors at a time: the rows of a group's heads lie side by side)
                 __nv_bfloat16* to = p.out + row_of(r < rows ? r : 0) * HD;
 #pragma unroll 1
@@ -728,7 +729,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_fp4_prefill_kernel(cons
                 const size_t row = row_of(r < rows ? r : 0) * p.pieces + piece;
                 if (r < rows) {
                     p.part_ml[2 * row] = l_sum != l_sum ? NAN : n > 0 ? m_used : -INFINITY;    // (no maximum remembers a score that is not a number)
-                    p.part_ml[2 * row + 1] = l_sum;
+                    p.part_ml[2 * row + 1] = l_sum == 0.f && qpos >= 0 ? -1.f : l_sum;         // (a row that sees keys, here or in other pieces, but has no sum)
                 }
                 if (n > 0) {
 #pragma unroll 1
@@ -785,7 +786,7 @@ __global__ void __launch_bounds__(128) merge_pieces_kernel(const float* __restri
     }
     const float f = m == -INFINITY ? 0.f : exp2f(m - M);
     const float den = warp_sum(f * l);
-    const float inv = M == -INFINITY ? 0.f : 1.f / den;
+    const float inv = M == -INFINITY ? (__any_sync(0xffffffffu, l < 0.f) ? NAN : 0.f) : 1.f / den;        // (zeros for a row without a key)
     constexpr int N = HD / 32;
     float num[N];
 #pragma unroll

@@ -502,7 +502,7 @@ struct Consumer {
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                    const float m_new = fmaxf(m[nt][j], top);
+                    const float m_new = top > m[nt][j] + LAG ? top : m[nt][j];        // (by this row alone, whatever the rows beside it)
                     const float shrink = m_new == -INFINITY ? 1.f : ex2(m[nt][j] - m_new);
                     m[nt][j] = m_new;
                     l[nt][j] *= shrink;

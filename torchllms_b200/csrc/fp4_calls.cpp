@@ -146,6 +146,10 @@ PyObject* write(PyObject*, PyObject* const* args, Py_ssize_t n) {
         !whole(args[11], out_code) || !number(args[13], inv_dim) || !number(args[14], eps))
         Py_RETURN_NONE;
     const int in_code = code_of(*qkv), interleaved = PyObject_IsTrue(args[6]);
+    if (interleaved < 0) {
+        PyErr_Clear();
+        Py_RETURN_NONE;
+    }
     if (out_code < 0) out_code = in_code;
     const long long dims = qkv->dim(), splits = dims == 3 ? qkv->size(0) : 1;
     if (!qkv->is_cuda() || in_code < 0 || out_code > 1 || dims < 2 || dims > 3 || !qkv->is_contiguous() || heads <= 0 || kv_heads <= 0 || head_dim <= 0 ||

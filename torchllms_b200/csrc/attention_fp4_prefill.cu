@@ -12,7 +12,7 @@
 //                    the largest) into shared memory in the operand layout.  Per key tile a thread reads its 128 scores, takes the
 //                    maximum, rescales the row's accumulator in the rare case that the maximum in use lags by more than 2^LAG,
 //                    and writes the weights into tensor memory; at the end it divides by their sum and stores the row.
-//   warps 8-11     : unpack.  A thread has a key of the tile: it fetches the key's 72 bytes a tile ahead, converts them to
+//   warps 8-11     : unpack.  A thread has a key of the tile: it converts the key's 72 bytes, fetched while it did what came before, to
 //                    float16 (exact: fp4.cuh) and writes them where the products read them (128-byte-swizzled rows), then
 //                    does the same with the value.
 //   warp 12        : issues the scores of both row tiles, warp 13 their products with V (one elected lane each).
@@ -22,10 +22,11 @@
 // Scores, weights and accumulators have tensor memory of their own; the row tiles use one score buffer in turn.  Where rows are few and keys are many the keys are cut into pieces, which leave
 // float32 sums that a second kernel adds up in order.
 //
-// Measured (32 / 8 heads, us): heads of 128: a prompt of 2,048 tokens 45.7 (752 TFLOP/s; some 6 us a CTA before its first and after its last key tile, 256
-// CTAs on 148 SMs), 2,048 tokens behind 14,001 431 (1,170 TFLOP/s, at the power cap's clock); heads of 64: six portions of 70 to 1,063 tokens 90
-// (460 TFLOP/s).  128 keys of both row tiles take 3,640 cycles with heads of 128, where the products want 2,100 and the exponentials 2,050, and 3,080
-// with 64.  Without the softmax it would be 3,500 (128), without unpacking 2,840, without exponentials 2,280 (64): the three wait for one another.
+// Measured (32 / 8 heads, us): heads of 128: a prompt of 2,048 tokens 47.0 (730 TFLOP/s; some 6 us a CTA before its first and after its last key tile, 256
+// CTAs on 148 SMs), 2,048 tokens behind 14,001 480 to 490 in a long loop (1,050 TFLOP/s, at the power cap's clock); heads of 64: six portions of 70 to
+// 1,063 tokens 89 (460 TFLOP/s).  128 keys of both row tiles take 3,800 cycles with heads of 128, where the products want 2,100 and the exponentials 2,050, and 3,150
+// with 64.  In copies with work taken out (of a kernel with a body for keys and one for values, 3,640 and 3,080): without the softmax 3,500 (128), without
+// unpacking 2,840, without exponentials 2,280 (64): the three wait for one another.
 // Measured and left out: exponentials by a polynomial on the multiply-add pipes for an eighth to a half of the scores (47 to 57 for 45.8), weights against the
 // maximum in use while the new one is found (46.5; 464 for 431), a row tile held back at the start (47.3), records fetched a tile further ahead (47.7; 491).
 //
@@ -265,6 +266,7 @@ struct Packed {
     }
     // Zeros for some groups of what `unpack` has written.
     static __device__ __forceinline__ void clear_groups(unsigned char* tile, int key, unsigned groups) {
+#pragma unroll 1
         for (int c = 0; c < HD / 8; ++c)
             if ((groups >> (c / 2)) & 1u)
                 *reinterpret_cast<uint4*>(tile + key * 128 + (c >> 3) * (BN * 128) + (((c & 7) ^ (key & 7)) << 4)) = make_uint4(0u, 0u, 0u, 0u);
@@ -501,9 +503,9 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_fp4_prefill_kernel(cons
         if (at >= 0) coming.load(p.k_pages + at, row);
         bool ok = true;
         const int late_tile = max(late + 1 - k_start, 0) / BN, early_end = early > k_start ? (early - k_start + BN - 1) / BN : 0;
-        // Keys and values go through the same instructions: the roles' loops together just about fit the instruction cache.  (With a loop that has a body for
-        // each, what hides values cost 2,048 tokens behind 14,001 472 -> 505 us and a prompt of 2,048 45.6 -> 49, with none of it ever run;
-        // this way 478 and 46.4.)
+        // Keys and values go through the same instructions, and what runs rarely stands apart from the loops: together they just about fit the instruction
+        // cache.  (With a loop that has a body for each, what hides values cost 2,048 tokens behind 14,001 472 -> 505 us and a prompt of 2,048
+        // 45.6 -> 49, with none of it ever run; this way 480 and 47.)
 #pragma unroll 1
         for (int i = 0; i < 2 * n_tiles; ++i) {
             const int j = i >> 1;
@@ -520,10 +522,10 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_fp4_prefill_kernel(cons
             coming.clear();
             if (at >= 0) coming.load((values ? p.k_pages : p.v_pages) + at, row);
             held.unpack(tile, key);
-            if (values && (j >= late_tile || j < early_end)) {
+            if (__builtin_expect(values && (j >= late_tile || j < early_end), 0)) {
                 const int kpos = k_start + j * BN + key;
                 const unsigned none = held.nan_groups();
-                if (none != 0u && (kpos > late || kpos < early)) {
+                if (__builtin_expect(none != 0u && (kpos > late || kpos < early), 0)) {
                     held.clear_groups(tile, key, none);
                     if (kpos > late) tail.nan_late[kpos - late - 1] = (unsigned char)none;
                     else tail.nan_early[early - 1 - kpos] = (unsigned char)none;
@@ -613,7 +615,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) attention_fp4_prefill_kernel(cons
             __syncwarp();
             if (lane == 0) mbar_arrive(&tail.s_free);      // the buffer may take the next scores
             const bool clear = k0 >= lo && k0 + BN <= hi && k0 + BN - 1 <= low && (p.window <= 0 || k0 > high - p.window);
-            if (!clear) {
+            if (__builtin_expect(!clear, 0)) {
                 const int from = max(lo, p.window > 0 ? qpos - p.window + 1 : 0) - k0, to = min(hi, qpos + 1) - k0;
 #pragma unroll
                 for (int w = 0; w < BN / 32; ++w) {

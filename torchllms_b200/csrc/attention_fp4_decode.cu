@@ -4,7 +4,7 @@
 //     o[t, h] = sum_j w_j v_j / sum_j w_j,  w_j = exp(scale q[t, h] . k_j),  j <= pos(t), j > pos(t) - window
 //
 // Bound by reading the cache once (144 bytes a key and head of 128, against 512 in bfloat16), and next to that by issuing the
-// instructions that unpack it: 16 keys and values of 128 numbers are 128 conversions and 128 products with scales a warp, beside
+// instructions that unpack it: 16 keys and values of 128 numbers are 64 conversions and 64 products with scales a warp, beside
 // 16 products of the tensor cores.  So:
 //   - The cache comes in whole records of 16 tokens by cp.async.bulk, 128 keys a stage, into a ring that a producer warp keeps
 //     full across the borders of requests; four consumer warps take two records of keys and of values each, with one turn of the softmax for both.
@@ -27,11 +27,13 @@
 // Every wait is bounded; a CTA whose wait runs out sets the status word and takes part in the counting only.
 //
 // Measured (32 / 8 heads, us; a record's arithmetic is 427 cycles of a scheduler, 12 consumer warps an SM):
-//   bfloat16, heads of 128: 8 requests of 2,049 tokens 11.9 (19 MB; of it finding the stretch and fetching queries 2, joining warps and parts 3); 64 of 200
-//   to 16,000 146 (651 MB, 4.5 TB/s; the copies alone 113); 4 of 27,001 to 32,767 36 (134 MB, 3.7 TB/s: DRAM at 42 %, unpacking bounds).
-//   One request of 333, heads of 64: 7.4, a launch and a chain of trips to memory.
-//   float32, heads of 64: 12 requests of 2 to 4 tokens in a window of 1,024 14.5; prompts of 500 to 901 tokens 56 (16 rows a block: 73, half
-//   of it beginning blocks and exchanging results).
+//   bfloat16, heads of 128: 8 requests of 2,049 tokens 12.0 (19 MB; of it finding the stretch and fetching queries 2, joining warps and parts 3); 64 of 200
+//   to 16,000 147 to 158 from box to box (651 MB, 4.1 to 4.4 TB/s; the copies alone 113, unpacking alone some 104); 4 of 27,001 to 32,767 36.9 (134 MB, 3.6
+//   TB/s: DRAM at 42 %, unpacking alone some 22 us).  Neither copies nor unpacking bound these two by themselves: they do not hide each other.
+//   One request of 333, heads of 64: 7.6, a launch and a chain of trips to memory.
+//   float32, heads of 64: 12 requests of 2 to 4 tokens in a window of 1,024 15.3; prompts of 500 to 901 tokens 58.3 (16 rows a block: 73, half
+//   of it beginning blocks and exchanging results).  float32 blocks of 16 rows and more with heads of 128 want more than the 168 registers that two CTAs
+//   an SM leave a thread: some 600 bytes of spills (8 requests of 512 tokens behind 4,000: 2.3 ms).
 #include "fp4.cuh"
 #include <limits.h>
 #include <math.h>
@@ -180,8 +182,8 @@ template <int ROWS> __device__ __forceinline__ int block_at(const Params& p, int
     const int ql = p.q_start[k.b + 1] - k.first;
     k.row0 = k.number * ROWS;
     // (p.rows, fewer than ROWS where one block has all: a request that brings more tokens than the step's max_q_len must not have
-    // rows that the places of the warps' and parts' results were not made for)
-    k.n_rows = min(p.rows, ql * p.group - k.row0);
+    // rows that the places of the warps' and parts' results were not made for.  With ROWS beside it the compiler knows a bound: one token 7.66 -> 7.54 us)
+    k.n_rows = min(min(ROWS, ql * p.group - k.row0), p.rows);
     if (k.n_rows <= 0) return 0;
     k.base = p.kv_len[k.b] - ql;
     const int t0 = token_of(p, k.row0), t1 = token_of(p, k.row0 + k.n_rows - 1);
@@ -734,7 +736,7 @@ __global__ void __launch_bounds__(NTHREADS, (NT == 1 && sizeof(T) == 2) ? 3 : 2)
         return;
     }
 
-    // ---- consumers: all rows of the block, a record of every tile each
+    // ---- consumers: all rows of the block and two records of every tile each, or rows of a warp's own and all records
     C c;
     bool ok = true;
     int s = 0;

@@ -12,7 +12,7 @@ low half of byte ``i``), then 16 rows of ``head_dim / 16`` scales.  Page tensors
 ``[pages, kv_heads, page_size / 16, 9 * head_dim]`` uint8.
 
 The reference keeps keys and values in the model's dtype (torchllms/models/paged_kv.py:186-222); this format is an addition:
-a cache of a third of bfloat16's size, a quarter with 3.5 times the tokens to spare, and as much less to read in a decode step.
+4.5 bits a number, so that the memory of a bfloat16 cache holds 3.6 times the tokens, and a decode step reads as much less.
 ``csrc/fp4.cuh`` has the kernels' side.  The functions below are for tools and tests; the engine does not call them.
 """
 

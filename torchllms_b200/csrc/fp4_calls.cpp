@@ -205,6 +205,8 @@ PyObject* read(PyObject*, PyObject* const* args, Py_ssize_t n) {
 // So it is one from `least` rows on, and with heads of 128 from 17 on where the context is long (beyond 1,024: the engine's steps plan for a power of two
 // that is no less, so that all shorter contexts come as 1,024) and there are no more than 1,024 tiles of 128 keys
 // (32 rows: one request of 12,000 tokens 25.9 and 22.7, 8 of 2,000 27.0 and 23.7; but 8 of 12,000 82 and 98, one of 200 9.6 and 10.4).
+// The rule is one line for rows and one for tiles, and takes the slower side here and there: the tcgen05 kernel for one request and heads of 64 (64 rows behind 2,000 a
+// third slower, 256 up to a tenth), the other for 16 rows of heads of 128 behind 12,000 (a fifth).
 // Those are times with keys that the tcgen05 kernel may cut into pieces.  Where it may not (`cut`), a CTA walks all keys of its rows, and more than two tiles of
 // them are for it only where rows are many: the mma.sync kernel, which cuts them as it likes, and the tcgen05 kernel without pieces, contexts of 2,000 and 12,000:
 //   rows x units     512 (1 request, 64 rows):  of 64: 11.6  27.8   24.4 131   of 128: 16.1  33.5   36.0 149       2,048 (4 requests): 19.4 28.3  59.8 163   27.7 34.1  86 192

@@ -116,7 +116,7 @@ class NativeOps:
 
     F32_ROWS = 4096         # rows of one float32 product
     FP4_PREFILL_MIN_ROWS = 64    # rows (tokens x query heads of a key head) of a request from which the 4-bit cache's tcgen05 kernel is used
-                                 # whatever the context (csrc/fp4_calls.cpp has the times of both sides)
+                                 # whatever the context, if keys may be cut (csrc/fp4_calls.cpp has the times of both sides)
     PREFILL_MIN_Q = 96      # portions at least this long go to the tcgen05 prefill attention kernel
     FUSE_MAX_ROWS = 16      # steps of at most this many tokens let a product add itself to the residual stream and
                             # prepare the norm that follows in its own kernel; with more rows product + norm
@@ -2185,10 +2185,11 @@ class NativeOps:
         (``[pages, n_kv_heads, page_size / 16, 9 * head_dim]`` bytes, :mod:`torchllms_b200.cache.fp4`): every token of
         ``q`` ``[T, H, head_dim]`` attends to the keys of its request up to its own place, or to the last ``window`` of
         them.  Keys and values are taken as the cache has them, nothing is rounded on the way; a row that sees no key is
-        zeros.  Arguments as there.  ``impl``: ``"general"`` (CUDA cores, heads of any multiple of 16 up to 256),
+        zeros, and a value that is not a number reaches the rows that see it only.  Arguments as there (``scale``: any finite number).  ``impl``: ``"general"`` (CUDA cores, heads of any multiple of 16 up to 256),
         ``"decode"`` (mma.sync tensor cores, head_dim 64 and 128), ``"prefill"`` (tcgen05 tensor cores, head_dim 64 and 128,
         bfloat16, made for many tokens) or ``"auto"`` (the most specialised kernel that applies).  ``allow_split`` (of the
-        prefill kernel): False keeps every row's keys in one CTA, a number above 1 cuts them into so many pieces."""
+        prefill kernel): False keeps every row's keys in one CTA (and ``"auto"`` then takes that kernel for many rows only), a number above
+        1 cuts them into so many pieces."""
         calls = self._fp4 or self._fp4_load()
         if self.debug:
             self._fp4_debug(k_pages.shape[0])

@@ -55,6 +55,19 @@ def test_portions_over_a_4_bit_cache_plan_for_a_bound(tmp_path, kv_format, bound
             assert set(ops.bounds) <= bounds, ops.bounds
 
 
+def test_portions_beside_many_requests_plan_for_their_own_bound(tmp_path):
+    """Short portions of many requests plan for the longest context there may be; a long one plans for what there is."""
+    folder = write_model_folder(tmp_path / "long", dict(TINY_C, max_position_embeddings=4096), make_tensors(TINY_C, 2), torch.float32)
+    ops = Recording()
+    engine = Replayer(folder, "float32", 4096, page_size=16, device="cpu", ops=ops, kv_format="fp4", max_num_seqs=20).engine
+    handles = [engine.claim() for _ in range(17)]
+    for n, bound in ((3, 4096), (20, 1024)):
+        ops.bounds.clear()
+        engine.step([StepEntry(h, [1]) for h in handles[:-1]] + [StepEntry(handles[-1], list(range(1, n + 1)))])
+        # (the one-token rows' own call plans for all of them either way)
+        assert sorted(set(ops.bounds)) == sorted({4096, bound})
+
+
 @pytest.mark.gpu
 def test_a_step_recorded_at_a_short_context_is_not_the_one_of_a_long_one(tmp_path):
     """Portions of 48 tokens, one behind the other: recorded steps give the bits and make the launches of eager ones all the way."""

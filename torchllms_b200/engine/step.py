@@ -474,7 +474,8 @@ class Engine:
             # steps whose keys may be split over CTAs (those of short portions; with a 4-bit cache all) plan for a coarse
             # bound of the longest context, so that their launch shapes change only when a request outgrows it
             bounded = self._plans_for_bound(max_q)
-            bound = (self._forced_bound or self.kv_bound(max(kv_lens), B)) if bounded else 0
+            # (however many requests there are beside it, a long portion's keys are cut by how long they are)
+            bound = (self._forced_bound or self.kv_bound(max(kv_lens), B if max_q <= 16 else 1)) if bounded else 0
             # a mixed step's one-token rows go to the decode kernel apart from the portions: their own bound
             decode_bound = self.kv_bound(max(kv_lens[:n_decode]), n_decode) if 0 < n_decode < B else 0
             recorded = (self._graphs.get(self._shape_key(T, B, n_want, max_q, n_decode, bound, decode_bound))

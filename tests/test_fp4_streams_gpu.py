@@ -78,6 +78,40 @@ def test_the_same_call_gives_the_same_bits(H, KV, D, q_lens, kv_lens, window, im
     ops().check_status()
 
 
+@pytest.mark.parametrize("T,H,KV,D", [(1, 4, 2, 64), (17, 32, 8, 128), (200, 16, 4, 64), (600, 8, 8, 128)])
+def test_what_is_written_is_what_the_next_calls_read(T, H, KV, D):
+    """The same slots written again and again, each time read back and attended over at once, by kernels that start while the one
+    before them still runs; eagerly and recorded."""
+    page = 16
+    g = torch.Generator(device="cuda").manual_seed(T)
+    rows = [torch.randn((T, (H + 2 * KV) * D), generator=g, device="cuda").to(torch.bfloat16) for _ in range(8)]
+    pages = [torch.zeros(fp4.page_shape(-(-T // page), KV, page, D), dtype=torch.uint8, device="cuda") for _ in range(2)]
+    table, places = torch.randn((T, D // 2, 2), generator=g, device="cuda"), torch.arange(T, dtype=torch.int32, device="cuda")
+    a = dict(block_table=torch.arange(pages[0].shape[0], dtype=torch.int32, device="cuda")[None], q_start=torch.tensor([0, T], dtype=torch.int32).cuda(),
+             kv_len=torch.tensor([T], dtype=torch.int32).cuda(), n_seqs=1, max_q_len=T, max_kv_len=T, scale=D ** -0.5, window=None, page_size=page)
+
+    def step(x):
+        q = ops().rope_kv_write_fp4(x, places, table, n_heads=H, n_kv_heads=KV, head_dim=D, interleaved=True, k_pages=pages[0], v_pages=pages[1],
+                                    slot_mapping=places, page_size=page)
+        return [*ops().kv_read_fp4(pages[0], pages[1], places, head_dim=D, page_size=page, out_dtype=torch.bfloat16),
+                *(ops().paged_attention_fp4(q, pages[0], pages[1], **a, impl=impl) for impl in ("general", "decode", "prefill"))]
+
+    want = []
+    for x in rows:
+        torch.cuda.synchronize()
+        want.append(step(x))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        recorded = [step(x) for x in rows]
+    for _ in range(10):
+        graph.replay()
+        torch.cuda.synchronize()
+        for got in ([step(x) for x in rows], recorded):
+            torch.cuda.synchronize()
+            assert all(torch.equal(x, y) for some, all_of in zip(got, want) for x, y in zip(some, all_of))
+    ops().check_status()
+
+
 def everything():
     """One call of each kernel of the operators, on sound input: what they give."""
     given = []

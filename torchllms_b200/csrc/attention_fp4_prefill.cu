@@ -239,7 +239,8 @@ struct TileRange {
 template <int N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
-// A key's (or value's) numbers and scales: HD / 32 pieces of 16 bytes, HD / 16 bytes of scales.
+// A key's (or value's) numbers and scales: HD / 32 pieces of 16 bytes, HD / 16 bytes of scales.  (Plain loads: the kernel before this one may write
+// the pages while a CTA is already resident, so they are not memory that nobody writes as long as this kernel runs.)
 template <int HD>
 struct Packed {
     uint4 codes[HD / 32];
@@ -251,10 +252,10 @@ struct Packed {
     }
     __device__ __forceinline__ void load(const unsigned char* record, int row) {
 #pragma unroll
-        for (int i = 0; i < HD / 32; ++i) codes[i] = __ldg(reinterpret_cast<const uint4*>(record + row * (HD / 2) + i * 16));
+        for (int i = 0; i < HD / 32; ++i) codes[i] = *reinterpret_cast<const uint4*>(record + row * (HD / 2) + i * 16);
         const unsigned char* s = record + FP4_RECORD * (HD / 2) + row * (HD / FP4_GROUP);
-        if (HD == 128) scales = __ldg(reinterpret_cast<const uint2*>(s));
-        else scales.x = __ldg(reinterpret_cast<const unsigned*>(s));
+        if (HD == 128) scales = *reinterpret_cast<const uint2*>(s);
+        else scales.x = *reinterpret_cast<const unsigned*>(s);
     }
     // The groups that are not numbers, a bit each.
     __device__ __forceinline__ unsigned nan_groups() const {

@@ -293,10 +293,12 @@ __global__ void __launch_bounds__(128, Runs<T, INTERLEAVED>::CTAS) rope_kv_write
 // The numbers of given slots: a CTA to a slot at a time, blockIdx.y: keys, values; a thread to eight coordinates of a head, four slots
 // under way together.  8,356 slots of 8 heads of 128 in bfloat16 (44 MB, 6.7 us of them): 8.6 us (5.1 TB/s; with the place of every slot and run worked out anew, a
 // division and 64-bit products, 11.2), 17 slots 2.0 (2.6); eight slots at a time 11.5 and 3.4.
+// (The pages are not declared free of aliases: a CTA may be resident while the kernel before this one writes them, and loads that count
+// on memory nobody writes are not for them.)
 constexpr int SLOTS = 4;
 template <typename T>
-__global__ void __launch_bounds__(128) kv_read_fp4_kernel(const unsigned char* __restrict__ k_pages, const unsigned char* __restrict__ v_pages,
-                                                          const int* __restrict__ slots, T* __restrict__ k_out, T* __restrict__ v_out,
+__global__ void __launch_bounds__(128) kv_read_fp4_kernel(const unsigned char* k_pages, const unsigned char* v_pages,
+                                                          const int* __restrict__ slots, T* k_out, T* v_out,
                                                           int n_slots, long long n_pages, int n_kv_heads, int head_dim, int page_size, int page_shift) {
     grid_launch_dependents();
     grid_dependency_wait();

@@ -1,0 +1,69 @@
+"""The 8-bit rows and what is done with them, from the definitions, in 64 bits: what the kernels are held to."""
+
+import math
+
+import torch
+
+BLOCK = 128
+
+
+def pitch(width):
+    return 4 * -(-width // 512)
+
+
+def hold(x):
+    """64-bit ``[rows, K]`` -> the numbers that are held (before their scale) and the exponents ``[rows, ceil(K / 128)]``."""
+    R, K = x.shape
+    g = torch.zeros((R, -(-K // BLOCK) * BLOCK), dtype=torch.float64, device=x.device)
+    g[:, :K] = x.double()
+    g = g.reshape(R, g.shape[1] // BLOCK, BLOCK)
+    fine = torch.isfinite(g)
+    a = torch.where(fine, g.abs(), torch.zeros_like(g)).amax(-1, keepdim=True)
+    e = torch.ceil(torch.log2((a / 448.0).clamp(min=2.0 ** -126)))
+    e = torch.where(a > 448.0 * torch.exp2(e), e + 1, torch.where((a <= 448.0 * torch.exp2(e - 1)) & (e > -126), e - 1, e))
+    v = torch.where(fine, g, torch.zeros_like(g)) / torch.exp2(e)
+    quantum = torch.exp2(torch.floor(torch.log2(v.abs().clamp(min=2.0 ** -6))) - 3)
+    held = torch.where(fine, (v / quantum).round() * quantum, torch.full_like(g, math.nan))
+    return held.flatten(1)[:, :K], e[..., 0]
+
+
+def value(rows):
+    """What an ``Fp8Rows`` stands for, 64 bits."""
+    K = rows.codes.shape[-1]
+    return rows.codes.double() * rows.scales.double().repeat_interleave(BLOCK, -1)[..., :K]
+
+
+def stands_for(x):
+    held, e = hold(x)
+    return held * torch.exp2(e).repeat_interleave(BLOCK, -1)[:, :x.shape[1]]
+
+
+def act(u, kind, gated=False, params=None):
+    """Activations of the feed-forwards in 64 bits."""
+    if gated:
+        g, up = u.chunk(2, -1)
+        if kind == "clamped_swish":
+            limit, alpha, offset = params
+            g, up = g.clamp(max=limit), up.clamp(-limit, limit)
+            return g * torch.sigmoid(alpha * g) * (up + offset)
+        return act(g, kind) * up
+    if kind == "silu":
+        return u * torch.sigmoid(u)
+    if kind == "gelu_tanh":
+        return 0.5 * u * (1.0 + torch.tanh(math.sqrt(2.0 / math.pi) * (u + 0.044715 * u ** 3)))
+    if kind == "gelu":
+        return 0.5 * u * (1.0 + torch.erf(u / math.sqrt(2.0)))
+    assert kind == "relu2"
+    return u.clamp(min=0) ** 2
+
+
+def experts(x, chosen, weights, up, down, kind, gated=False, params=None):
+    """``sum_k weights * down(act(up x))`` with the rows held in 8 bits on the way, 64 bits; ``up`` and ``down`` 64-bit ``[E, ..]``."""
+    rows = stands_for(x.double())
+    out = torch.zeros_like(rows)
+    for e in range(up.shape[0]):
+        token, choice = torch.nonzero(chosen == e, as_tuple=True)
+        if token.numel():
+            y = stands_for(act(rows[token] @ up[e].T, kind, gated, params)) @ down[e].T
+            out.index_add_(0, token, y * weights[token, choice].double()[:, None])
+    return out

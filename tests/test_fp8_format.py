@@ -1,0 +1,82 @@
+"""The 8-bit rows' format in PyTorch against its definition in 64 bits, and what the calls refuse (on the host)."""
+
+import math
+
+import pytest
+import torch
+
+import fp8_plain as plain
+from torchllms_b200.weights.fp8 import CODES, SCALES, Fp8Rows, check_width, decode, encode, scale_pitch
+
+
+def rows(T, K, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randn((T, K), generator=g) * torch.exp(1.5 * torch.randn((K,), generator=g))
+
+
+@pytest.mark.parametrize("K", [16, 112, 128, 144, 512, 528, 2064])
+def test_encode_holds_what_the_definition_says(K):
+    x = rows(20, K, K)
+    x[1] = 0.0
+    x[2, 0], x[3, 5], x[4, K - 1] = math.inf, math.nan, -math.inf
+    x[5] *= 1e-38
+    x[6] = (x[6].double() * 1e37).clamp(-3e38, 3e38).float()
+    codes, scales = encode(x)
+    assert codes.dtype == CODES and scales.dtype == SCALES and codes.shape == x.shape and scales.shape == (20, plain.pitch(K)) == (20, scale_pitch(K))
+    held, e = plain.hold(x)
+    assert torch.equal(codes.double().nan_to_num(777.0), held.nan_to_num(777.0))
+    byte = torch.zeros(scales.shape, dtype=torch.uint8)
+    byte[:, :e.shape[1]] = (e + 127).to(torch.uint8)
+    assert torch.equal(scales.view(torch.uint8), byte)
+    assert torch.equal(decode(codes, scales).double().nan_to_num(7.0), plain.value(Fp8Rows(codes, scales)).float().double().nan_to_num(7.0))
+
+
+def test_a_second_encoding_changes_nothing():
+    x = Fp8Rows(*encode(rows(8, 640, 3))).dequantize()
+    codes, scales = encode(x)
+    assert torch.equal(decode(codes, scales), x)
+
+
+def test_error_is_half_a_step():
+    x = rows(50, 1024, 4)
+    r = Fp8Rows(*encode(x))
+    scale = r.scales.float().repeat_interleave(128, -1)
+    assert bool(((r.dequantize() - x).abs() <= torch.maximum(x.abs() * 2.0 ** -4, scale * 2.0 ** -10)).all())
+
+
+def test_experts_and_views():
+    x = rows(24, 272, 5).reshape(4, 6, 272)
+    r = Fp8Rows(*encode(x))
+    assert r.shape == (4, 6, 272) and r.scales.shape == (4, 6, 4) and r.nbytes() == 4 * 6 * 276
+    part = r[1:3]
+    assert torch.equal(part.dequantize(), r.dequantize()[1:3]) and part.codes.data_ptr() == r.codes[1:].data_ptr()
+
+
+@pytest.mark.parametrize("K", [0, 8, 100, 130])
+def test_widths_that_are_refused(K):
+    with pytest.raises(ValueError):
+        check_width(K)
+
+
+def bare_ops():
+    """The front end without a GPU behind it: what it refuses, it refuses before anything is launched."""
+    from torchllms_b200.kernels.native import NativeOps
+    ops = object.__new__(NativeOps)
+    ops._profile, ops.launches = None, 0
+    return ops
+
+
+def test_calls_refuse_the_host():
+    from torchllms_b200.kernels.native import KernelError
+    ops, x = bare_ops(), rows(4, 256)
+    w = Fp8Rows(*encode(rows(32, 256)))
+    for call in (lambda: ops.quantize_fp8(x), lambda: ops.activation_fp8(x, "silu"), lambda: ops.rmsnorm_fp8(x, None, x[0], 1e-5),
+                 lambda: ops.linear_fp8(x, w), lambda: ops.linear_fp8(w, w), lambda: ops.linear_fp8(w, x),
+                 lambda: ops.moe_experts_fp8(x, torch.zeros((4, 1), dtype=torch.int32), torch.ones((4, 1)), w, w, activation="silu")):
+        with pytest.raises(KernelError):
+            call()
+    with pytest.raises(KernelError, match="unknown activation"):
+        ops.activation_fp8(x, "swish")
+    with pytest.raises(KernelError, match="clamped"):
+        ops.activation_fp8(x, "clamped_swish")
+    assert ops.launches == 0

@@ -1,0 +1,82 @@
+// Rows of numbers in 8 bits, the kernels' side (the format in PyTorch: weights/fp8.py).
+//
+// 128 neighbouring numbers of a row share a scale 2^e, e the least integer with a <= 448 * 2^e where a is their largest finite
+// magnitude, at least -126 and at most 120; a number is held as E4M3 of x * 2^-e, rounded to nearest (ties to even).  The scale is
+// a power of two, so the division is exact and the only rounding is that to E4M3's four significant bits; and it is the
+// E8M0 byte e + 127 that the block-scaled tensor-core instructions multiply by.  What is not finite is held as NaN.
+#pragma once
+#include "common.cuh"
+#include <math.h>
+
+constexpr int FP8_BLOCK = 128;       // numbers that share a scale
+
+// bytes of scales a row of K numbers has: one for every 128, in whole words (the places behind the last are 0)
+__host__ __device__ __forceinline__ int fp8_scale_pitch(int K) { return 4 * ((K + 511) / 512); }
+
+// the exponent for a largest magnitude given by its bits (finite, sign cleared): 448 = 1.75 * 2^8
+__device__ __forceinline__ int fp8_exponent(unsigned top_bits) {
+    const int e = (int)(top_bits >> 23) - 135 + ((top_bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return e < -126 ? -126 : e;
+}
+__device__ __forceinline__ float fp8_inverse(int e) { return __int_as_float((127 - e) << 23); }
+
+// two numbers, already divided by their scale, as two bytes (the first one low); infinities must not get here
+__device__ __forceinline__ unsigned fp8_pack2(float lo, float hi) {
+    unsigned short r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+// Eight numbers of a 128-number block that lies on 16 lanes (the other half warp has a block of its own): the scale's exponent
+// (the same on all 16 lanes) and the eight bytes.  Lanes behind the end of the row bring zeros.  Whole warps call it.
+__device__ __forceinline__ int fp8_encode8(const float (&v)[8], uint2& bytes) {
+    unsigned top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const bool odd = top >= 0x7f800000u;                  // (16 lanes alike) something is not finite
+    if (__any_sync(0xffffffffu, odd)) {
+        unsigned fine = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const unsigned b = __float_as_uint(v[i]) & 0x7fffffffu;
+            if (b < 0x7f800000u) fine = max(fine, b);
+        }
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) fine = max(fine, __shfl_xor_sync(0xffffffffu, fine, o));
+        top = fine;
+    }
+    const int e = fp8_exponent(top);
+    const float inv = fp8_inverse(e);
+    float t[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = v[i] * inv;
+    if (odd) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if ((__float_as_uint(v[i]) & 0x7f800000u) == 0x7f800000u) t[i] = __int_as_float(0x7fffffff);
+    }
+    bytes.x = fp8_pack2(t[0], t[1]) | (fp8_pack2(t[2], t[3]) << 16);
+    bytes.y = fp8_pack2(t[4], t[5]) | (fp8_pack2(t[6], t[7]) << 16);
+    return e;
+}
+
+// ---- activations of feed-forwards: the codes and the arithmetic of csrc/moe.cu
+enum : int { FP8_SILU = 0, FP8_GELU_TANH = 1, FP8_RELU2 = 2, FP8_CLAMPED_SWISH = 3, FP8_GELU = 4 };
+struct Fp8Gate { float limit, alpha, up_offset; };
+
+__device__ __forceinline__ float fp8_act(float x, int act) {
+    if (act == FP8_SILU) return x / (1.f + __expf(-x));
+    if (act == FP8_GELU_TANH) return 0.5f * x * (1.f + tanhf(0.7978845608028654f * (x + 0.044715f * x * x * x)));
+    if (act == FP8_GELU) return 0.5f * x * (1.f + erff(0.7071067811865476f * x));
+    const float r = x < 0.f ? 0.f : x;           // (comparisons, not fmaxf: what is not a number stays so)
+    return r * r;
+}
+__device__ __forceinline__ float fp8_gated(float gate, float up, int act, const Fp8Gate& p) {
+    if (act == FP8_CLAMPED_SWISH) {
+        const float g = gate > p.limit ? p.limit : gate, u = up > p.limit ? p.limit : (up < -p.limit ? -p.limit : up);
+        return g / (1.f + __expf(-p.alpha * g)) * (u + p.up_offset);
+    }
+    return fp8_act(gate, act) * up;
+}

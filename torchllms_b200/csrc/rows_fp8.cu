@@ -1,0 +1,222 @@
+// Rows into 8 bits (format: fp8.cuh): as they are, behind a residual sum and an RMS norm, behind an activation.
+//
+// rows:  codes, scales of x.
+// norm:  x = h + delta, h <- x;  y = x * rsqrt(mean(x^2) + eps) * w, all in float32;  codes, scales of y.
+//        (RMSNorm, torchllms/models/networks.py:195-200: the rows go straight to 8 bits, rounded once.)
+// act:   y = act(u), or act(g) * u of the halves of a row, in float32;  codes, scales of y.
+//
+// All three read every number once and write a byte for it: bandwidth is what bounds them, or the launch where rows are few.
+// A block of 128 numbers lies on 16 lanes, eight numbers each: 16 bytes a load in bfloat16, 128 contiguous bytes of codes
+// a half warp, its largest magnitude in four exchanges.
+#include "fp8.cuh"
+
+namespace {
+
+constexpr int ROWS_THREADS = 256;
+
+__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&v)[8]) {
+    const uint4 r = *reinterpret_cast<const uint4*>(p);
+    const unsigned w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+}
+
+// codes of the eight numbers at column d of a row and, from the first lane of a block, its scale byte; the last block of a
+// row also clears the places behind it
+__device__ __forceinline__ void keep8(const uint2& bytes, int e, unsigned char* codes, unsigned char* scales, int d, int K) {
+    if (d < K) {
+        *reinterpret_cast<uint2*>(codes + d) = bytes;
+        if (d % FP8_BLOCK == 0) {
+            scales[d / FP8_BLOCK] = (unsigned char)(e + 127);
+            if (d + FP8_BLOCK >= K)
+                for (int j = d / FP8_BLOCK + 1; j < fp8_scale_pitch(K); ++j) scales[j] = 0;
+        }
+    }
+}
+__device__ __forceinline__ void leave8(const float (&v)[8], unsigned char* codes, unsigned char* scales, int d, int K) {
+    uint2 bytes;
+    const int e = fp8_encode8(v, bytes);
+    keep8(bytes, e, codes, scales, d, K);
+}
+
+// FORM 0: the rows; 1: act(x); 2: gated act of the row's halves (x has 2 K columns); 3: the rows, each left at `top` places
+// (the rows that a token's choices of experts have in the sorted order).  grid (rows, chunks of 2,048 columns).
+template <typename T, int FORM>
+__global__ void __launch_bounds__(ROWS_THREADS) rows_kernel(const T* __restrict__ x, unsigned char* __restrict__ codes,
+                                                            unsigned char* __restrict__ scales, int K, int act, Fp8Gate gp,
+                                                            const int* __restrict__ place, int top) {
+    grid_launch_dependents();
+    grid_dependency_wait();
+    const size_t row = blockIdx.x;
+    const int d = (blockIdx.y * ROWS_THREADS + threadIdx.x) * 8;
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (d < K) {
+        if (FORM == 2) {
+            float u[8];
+            load8(x + row * 2 * K + d, v);
+            load8(x + row * 2 * K + K + d, u);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = fp8_gated(v[i], u[i], act, gp);
+        } else {
+            load8(x + row * K + d, v);
+            if (FORM == 1)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = fp8_act(v[i], act);
+        }
+    }
+    if (FORM == 3) {
+        uint2 bytes;
+        const int e = fp8_encode8(v, bytes);
+        for (int k = 0; k < top; ++k) {
+            const size_t to = place[row * top + k];
+            keep8(bytes, e, codes + to * K, scales + to * fp8_scale_pitch(K), d, K);
+        }
+        return;
+    }
+    leave8(v, codes + row * K, scales + row * fp8_scale_pitch(K), d, K);
+}
+
+// A CTA to a row, which stays in registers: SLOTS times eight numbers a thread.  delta: splits planes `plane` elements apart
+// (partial sums, added in order), or null.
+template <typename TD, int SLOTS>
+__global__ void __launch_bounds__(1024) norm_kernel(float* __restrict__ h, const TD* __restrict__ delta, int splits, long long plane,
+                                                    const float* __restrict__ weight, unsigned char* __restrict__ codes,
+                                                    unsigned char* __restrict__ scales, int K, float eps) {
+    __shared__ double part[32];
+    grid_launch_dependents();
+    grid_dependency_wait();
+    const size_t row = blockIdx.x;
+    float* hr = h + row * K;
+    float x[SLOTS][8];
+    float ss = 0.f;              // (of at most 32 squares; beyond a warp, 64 bits)
+#pragma unroll
+    for (int s = 0; s < SLOTS; ++s) {
+        const int d = (s * blockDim.x + threadIdx.x) * 8;
+        if (d < K) {
+            load8(hr + d, x[s]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[s][i] = 0.f;
+        }
+    }
+    if (delta != nullptr) {
+#pragma unroll
+        for (int s = 0; s < SLOTS; ++s) {
+            const int d = (s * blockDim.x + threadIdx.x) * 8;
+            if (d < K) {
+                float y[8];
+                load8(delta + row * K + d, y);
+                for (int sp = 1; sp < splits; ++sp) {
+                    float z[8];
+                    load8(delta + sp * plane + row * K + d, z);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) y[i] += z[i];
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[s][i] += y[i];
+                *reinterpret_cast<float4*>(hr + d) = make_float4(x[s][0], x[s][1], x[s][2], x[s][3]);
+                *reinterpret_cast<float4*>(hr + d + 4) = make_float4(x[s][4], x[s][5], x[s][6], x[s][7]);
+            }
+        }
+    }
+#pragma unroll
+    for (int s = 0; s < SLOTS; ++s) {
+        float q[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) q[i] = x[s][i] * x[s][i];
+        ss += ((q[0] + q[1]) + (q[2] + q[3])) + ((q[4] + q[5]) + (q[6] + q[7]));
+    }
+    ss = warp_sum(ss);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n_warps = blockDim.x >> 5;
+    if (lane == 0) part[warp] = ss;
+    __syncthreads();
+    double total = 0.0;
+    for (int i = 0; i < n_warps; ++i) total += part[i];
+    // (an error of the factor moves a whole row against E4M3's borders: 64 bits here, once a row)
+    const float factor = (float)(1.0 / sqrt(total / (double)K + (double)eps));
+#pragma unroll
+    for (int s = 0; s < SLOTS; ++s) {
+        const int d = (s * blockDim.x + threadIdx.x) * 8;
+        if (s * (int)blockDim.x * 8 >= K) break;
+        if (d < K) {
+            float w[8];
+            load8(weight + d, w);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[s][i] = x[s][i] * factor * w[i];
+        }
+        leave8(x[s], codes + row * K, scales + row * fp8_scale_pitch(K), d, K);
+    }
+}
+
+template <typename T>
+int launch_rows(const void* x, void* codes, void* scales, int rows, int K, int form, int act, const Fp8Gate& gp, const int* place, int top,
+                cudaStream_t s) {
+    const dim3 grid(rows, (K + 8 * ROWS_THREADS - 1) / (8 * ROWS_THREADS));
+    unsigned char *c = (unsigned char*)codes, *b = (unsigned char*)scales;
+    if (form == 0) return (int)tl_launch(rows_kernel<T, 0>, grid, dim3(ROWS_THREADS), 0, s, (const T*)x, c, b, K, act, gp, place, top);
+    if (form == 1) return (int)tl_launch(rows_kernel<T, 1>, grid, dim3(ROWS_THREADS), 0, s, (const T*)x, c, b, K, act, gp, place, top);
+    if (form == 3) return (int)tl_launch(rows_kernel<T, 3>, grid, dim3(ROWS_THREADS), 0, s, (const T*)x, c, b, K, act, gp, place, top);
+    return (int)tl_launch(rows_kernel<T, 2>, grid, dim3(ROWS_THREADS), 0, s, (const T*)x, c, b, K, act, gp, place, top);
+}
+
+template <typename TD>
+int launch_norm(float* h, const void* delta, int splits, long long plane, const float* weight, void* codes, void* scales, int rows, int K,
+                float eps, cudaStream_t s) {
+    const int lanes = (K + FP8_BLOCK - 1) / FP8_BLOCK * 16;        // whole blocks
+    auto threads = [&](int slots) { return ((lanes + slots - 1) / slots + 31) / 32 * 32; };
+    unsigned char *c = (unsigned char*)codes, *b = (unsigned char*)scales;
+#define TL_NORM(S) return (int)tl_launch(norm_kernel<TD, S>, dim3(rows), dim3(threads(S)), 0, s, h, (const TD*)delta, splits, plane, weight, c, b, K, eps)
+    if (lanes <= 1024) TL_NORM(1);
+    if (lanes <= 2048) TL_NORM(2);
+    TL_NORM(4);
+#undef TL_NORM
+}
+
+}  // namespace
+
+constexpr int FP8_MOST_NORM_WIDTH = 32768;
+
+namespace {
+int rows_of(const void* x, int dtype, void* codes, void* scales, int rows, int K, int form, int act, const Fp8Gate& gp, const int* place, int top,
+            cudaStream_t s) {
+    if (rows <= 0) return TL_OK;
+    if (K <= 0 || K % 16 != 0 || K > (1 << 26)) return TL_BAD_SIZE;
+    if (!aligned16(x) || !aligned16(codes) || (reinterpret_cast<uintptr_t>(scales) & 3u) != 0) return TL_BAD_ALIGN;
+    if (dtype == TL_F32) return launch_rows<float>(x, codes, scales, rows, K, form, act, gp, place, top, s);
+    if (dtype == TL_BF16) return launch_rows<__nv_bfloat16>(x, codes, scales, rows, K, form, act, gp, place, top, s);
+    return TL_BAD_DTYPE;
+}
+}  // namespace
+
+// x: [rows, K] of dtype (form 2: [rows, 2 K]); codes [rows, K]; scales [rows, fp8_scale_pitch(K)]; all 16-byte aligned (scales: 4).
+// form 0: the rows, 1: act(x), 2: act(first half) * second half; act as in fp8.cuh.
+extern "C" int tl_fp8_rows(const void* x, int dtype, void* codes, void* scales, int rows, int K, int form, int act, float limit, float alpha,
+                           float up_offset, void* stream) {
+    if (form < 0 || form > 2 || act < 0 || act > 4 || (act == FP8_CLAMPED_SWISH && form == 1)) return TL_BAD_SIZE;
+    return rows_of(x, dtype, codes, scales, rows, K, form, act, Fp8Gate{limit, alpha, up_offset}, nullptr, 1, (cudaStream_t)stream);
+}
+
+// x: [tokens, K]; codes, scales: [tokens * top] rows, token t's at place[t * top], .. place[t * top + top - 1].
+extern "C" int tl_fp8_rows_placed(const void* x, int dtype, void* codes, void* scales, int tokens, int K, const int* place, int top, void* stream) {
+    if (top < 1 || place == nullptr) return TL_BAD_SIZE;
+    return rows_of(x, dtype, codes, scales, tokens, K, 3, 0, Fp8Gate{0.f, 0.f, 0.f}, place, top, (cudaStream_t)stream);
+}
+
+// h [rows, K] float32, updated in place when delta is not null; delta [splits, rows, K] of delta_dtype, planes `plane` elements apart.
+extern "C" int tl_fp8_norm(float* h, const void* delta, int delta_dtype, int splits, long long plane, const float* weight, void* codes,
+                           void* scales, int rows, int K, float eps, void* stream) {
+    if (rows <= 0) return TL_OK;
+    if (K <= 0 || K % 16 != 0 || K > FP8_MOST_NORM_WIDTH || splits < 1 || plane % 8 != 0) return TL_BAD_SIZE;
+    if (!aligned16(h) || !aligned16(delta) || !aligned16(weight) || !aligned16(codes) || (reinterpret_cast<uintptr_t>(scales) & 3u) != 0)
+        return TL_BAD_ALIGN;
+    if (delta_dtype == TL_F32) return launch_norm<float>(h, delta, splits, plane, weight, codes, scales, rows, K, eps, (cudaStream_t)stream);
+    if (delta_dtype == TL_BF16) return launch_norm<__nv_bfloat16>(h, delta, splits, plane, weight, codes, scales, rows, K, eps, (cudaStream_t)stream);
+    return TL_BAD_DTYPE;
+}

@@ -17,6 +17,7 @@ from typing import Dict, Optional, Tuple
 import torch
 
 from ..cache.fp4 import GROUP, MAX_HEAD_DIM, RECORD, record_bytes
+from ..weights.fp8 import ALIGN as FP8_ALIGN, CODES as FP8_CODES, MAX_NORM_WIDTH as FP8_MAX_NORM_WIDTH, SCALES as FP8_SCALES, Fp8Rows, scale_pitch
 from .build import ALL_LIBRARIES, build_libraries, load_extension, load_library
 from .lazy import PendingProduct, RowScaled
 
@@ -1481,6 +1482,177 @@ class NativeOps:
                                               ctypes.c_float(alpha), ctypes.c_float(up_offset), ctypes.c_float(extra_limit), _stream())
         _check(rc, "moe_scale_act")
         self.launches += 1
+        return out
+
+    # ------------------------------------------------------------- rows and weights in 8 bits
+    @staticmethod
+    def _fp8_empty(rows: int, width: int, device) -> Fp8Rows:
+        return Fp8Rows(torch.empty((rows, width), dtype=FP8_CODES, device=device),
+                       torch.empty((rows, scale_pitch(width)), dtype=FP8_SCALES, device=device))
+
+    @staticmethod
+    def _fp8_need(t, name: str, dims: int = 2) -> None:
+        _need(isinstance(t, Fp8Rows), f"{name} must be 8-bit rows (Fp8Rows), got {type(t).__name__}")
+        _cuda_contig(t.codes, f"{name}: codes", FP8_CODES)
+        _cuda_contig(t.scales, f"{name}: scales", FP8_SCALES)
+        _need(t.codes.dim() == dims and t.codes.shape[-1] % FP8_ALIGN == 0 and t.codes.shape[-1] > 0,
+              f"{name}: codes must have {dims} axes and a multiple of {FP8_ALIGN} numbers a row")
+        _need(t.scales.shape == (*t.codes.shape[:-1], scale_pitch(t.codes.shape[-1])) and t.scales.device == t.codes.device,
+              f"{name}: scales must be [.., rows, {scale_pitch(t.codes.shape[-1])}] beside codes {tuple(t.codes.shape)}")
+
+    @staticmethod
+    def _fp8_here(*tensors) -> None:
+        """Launches go to the current device: everything has to lie there."""
+        at = torch.cuda.current_device()
+        for t in tensors:
+            _need(t is None or t.device.index == at, f"all tensors must lie on the current device (cuda:{at})")
+
+    def _fp8_width(self, x: torch.Tensor, name: str, parts: int = 1) -> int:
+        _cuda_contig(x, name)
+        _need(x.dtype in _DT and x.dim() == 2, f"{name} must be a float32/bfloat16 matrix")
+        _need(x.shape[1] > 0 and x.shape[1] % (parts * FP8_ALIGN) == 0, f"{name}: 8-bit rows take a multiple of {FP8_ALIGN} numbers, got {x.shape[1] // parts}")
+        _need(x.data_ptr() % 16 == 0, f"{name} must start on 16 bytes")
+        return x.shape[1] // parts
+
+    @_timed
+    def quantize_fp8(self, x: torch.Tensor) -> Fp8Rows:
+        """The rows of ``x`` (``[T, K]`` float32/bfloat16, ``K % 16 == 0``) in 8 bits: E4M3 numbers and a scale of a power of two for
+        every 128 of them (:mod:`torchllms_b200.weights.fp8` has the format; what is not finite becomes NaN)."""
+        K = self._fp8_width(x, "quantize_fp8: x")
+        self._fp8_here(x)
+        out = self._fp8_empty(x.shape[0], K, x.device)
+        rc = self._lib("rows_fp8").tl_fp8_rows(_ptr(x), _DT[x.dtype], _ptr(out.codes), _ptr(out.scales), x.shape[0], K, 0, 0, ctypes.c_float(0.0),
+                                              ctypes.c_float(0.0), ctypes.c_float(0.0), _stream())
+        _check(rc, "quantize_fp8")
+        self.launches += x.shape[0] > 0
+        return out
+
+    @_timed
+    def activation_fp8(self, u: torch.Tensor, activation: str, *, gated: bool = False, act_params=None) -> Fp8Rows:
+        """``act(u)``, or with ``gated`` ``act(g) * v`` of the halves ``[g | v]`` of ``u``'s rows, in 8 bits (as :meth:`quantize_fp8`); the
+        activation is taken in float32 and rounded once.  Activations and ``act_params`` as in :meth:`moe_experts`."""
+        _need(activation in self._ACTS, f"unknown activation {activation!r}; known: {', '.join(self._ACTS)}")
+        clamped = activation == "clamped_swish"
+        _need(not clamped or (gated and act_params is not None and len(act_params) == 3 and act_params[0] > 0),
+              "the clamped activation is a gated one and goes with (limit, alpha, up_offset), the limit positive")
+        K = self._fp8_width(u, "activation_fp8: u", 2 if gated else 1)
+        self._fp8_here(u)
+        limit, alpha, offset = act_params if clamped else (0.0, 0.0, 0.0)
+        out = self._fp8_empty(u.shape[0], K, u.device)
+        rc = self._lib("rows_fp8").tl_fp8_rows(_ptr(u), _DT[u.dtype], _ptr(out.codes), _ptr(out.scales), u.shape[0], K, 2 if gated else 1,
+                                              self._ACTS[activation], ctypes.c_float(limit), ctypes.c_float(alpha), ctypes.c_float(offset), _stream())
+        _check(rc, "activation_fp8")
+        self.launches += u.shape[0] > 0
+        return out
+
+    @_timed
+    def rmsnorm_fp8(self, h: torch.Tensor, delta, weight: torch.Tensor, eps: float) -> Fp8Rows:
+        """:meth:`rmsnorm` whose rows leave in 8 bits: ``h += delta`` in place (float32), then the rows of
+        ``h / sqrt(mean(h^2) + eps) * weight``, taken in float32 and rounded once.  ``delta``: ``[T, dim]`` float32/bfloat16, float32 partial
+        sums ``[splits, T, dim]``, a :class:`PendingProduct`, or ``None``."""
+        if isinstance(delta, PendingProduct):
+            delta = delta.take(self)
+        _cuda_contig(h, "residual stream", torch.float32)
+        K = self._fp8_width(h, "residual stream")
+        _cuda_contig(weight, "norm weight", torch.float32)
+        _need(weight.numel() == K, "norm weight must match the stream's width")
+        _need(K <= FP8_MAX_NORM_WIDTH, f"rmsnorm_fp8 keeps a row in registers: width {K} exceeds {FP8_MAX_NORM_WIDTH}")
+        splits, plane = 1, 0
+        if delta is not None:
+            _cuda_contig(delta, "delta")
+            _need(delta.dtype in _DT, "delta must be float32 or bfloat16")
+            if delta.dim() == 3:
+                _need(delta.shape[1:] == h.shape and delta.dtype == torch.float32 and delta.shape[0] >= 1,
+                      "partial sums must be float32 [splits, tokens, width]")
+                splits, plane = delta.shape[0], delta.stride(0)
+            else:
+                _need(delta.shape == h.shape, "delta must have the stream's shape")
+        self._fp8_here(h, delta, weight)
+        out = self._fp8_empty(h.shape[0], K, h.device)
+        rc = self._lib("rows_fp8").tl_fp8_norm(_ptr(h), _ptr(delta), 0 if delta is None else _DT[delta.dtype], splits, ctypes.c_longlong(plane),
+                                              _ptr(weight), _ptr(out.codes), _ptr(out.scales), h.shape[0], K, ctypes.c_float(eps), _stream())
+        _check(rc, "rmsnorm_fp8")
+        self.launches += h.shape[0] > 0
+        return out
+
+    @_timed
+    def linear_fp8(self, x, w: Fp8Rows, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+        """``x [M, K] @ w[N, K]^T`` of 8-bit rows, summed in float32.  ``x`` may be float32/bfloat16 rows, which are brought to 8 bits
+        first (:meth:`quantize_fp8`).  The result is bfloat16 or float32 ``[M, N]``."""
+        if not isinstance(x, Fp8Rows):
+            x = self.quantize_fp8(x)
+        self._fp8_need(x, "linear_fp8: x")
+        self._fp8_need(w, "linear_fp8: w")
+        (M, K), N = x.codes.shape, w.codes.shape[0]
+        _need(w.codes.shape[1] == K, f"linear_fp8: inner sizes differ ({K} and {w.codes.shape[1]})")
+        _need(out_dtype in _DT, f"linear_fp8: output dtype {out_dtype} unsupported")
+        self._fp8_here(x.codes, w.codes)
+        out = torch.empty((M, N), dtype=out_dtype, device=x.codes.device)
+        if M == 0 or N == 0:
+            return out
+        rc = self._lib("gemm_fp8").tl_gemm_fp8(_ptr(x.codes), _ptr(x.scales), _ptr(w.codes), _ptr(w.scales), _ptr(out),
+                                              1 if out_dtype == torch.float32 else 0, M, N, K, ctypes.c_void_p(self._status_at), _stream())
+        _check(rc, "linear_fp8")
+        self.launches += 1
+        return out
+
+    @_timed
+    def moe_experts_fp8(self, x: torch.Tensor, chosen: torch.Tensor, weights: torch.Tensor, w_up: Fp8Rows, w_down: Fp8Rows, *, activation: str,
+                        shared: Optional[torch.Tensor] = None, shared_gate: Optional[torch.Tensor] = None, gated: bool = False,
+                        act_params=None) -> torch.Tensor:
+        """:meth:`moe_experts` with weights in 8 bits: ``w_up`` ``[E, hidden, dim]`` (``gated``: ``[E, 2 * hidden, dim]``, rows ``[gate; up]``) and
+        ``w_down`` ``[E, dim, hidden]``.  A token's row is brought to 8 bits once, the hidden rows behind the activation again (taken in
+        float32, rounded once); both products run over the rows sorted by expert.  Experts that nobody chose are not read."""
+        _cuda_contig(x, "experts' input")
+        _cuda_contig(chosen, "chosen", torch.int32)
+        _cuda_contig(weights, "weights", torch.float32)
+        self._fp8_need(w_up, "experts' up weights", 3)
+        self._fp8_need(w_down, "experts' down weights", 3)
+        _need(activation in self._ACTS, f"unknown activation {activation!r}; known: {', '.join(self._ACTS)}")
+        dim = self._fp8_width(x, "experts' input")
+        _need(chosen.dim() == 2 and chosen.shape == weights.shape and chosen.shape[0] == x.shape[0], "experts: x [T, dim], chosen and weights [T, top]")
+        T, top = chosen.shape
+        _need(1 <= top <= 64, f"a token may use between 1 and 64 experts, got {top}")
+        E, up_rows = w_up.codes.shape[:2]
+        hidden = up_rows // 2 if gated else up_rows
+        _need((not gated or up_rows % 2 == 0) and w_up.codes.shape[2] == dim and w_down.codes.shape == (E, dim, hidden),
+              "experts: w_up [E, hidden, dim] (gated: 2 * hidden), w_down [E, dim, hidden]")
+        _need(1 <= E <= 4096, f"between 1 and 4096 experts, got {E}")
+        splits, plane = 1, 0
+        if shared is not None:
+            _cuda_contig(shared, "shared expert's output")
+            _need(shared.shape[-2:] == (T, dim) and (shared.dtype == x.dtype or shared.dtype == torch.float32), "shared must be [T, dim] or float32 partial sums of it")
+            if shared.dim() == 3:
+                _need(shared.dtype == torch.float32, "partial sums must be float32")
+                splits, plane = shared.shape[0], shared.stride(0)
+        if shared_gate is not None:
+            _cuda_contig(shared_gate, "shared gate", torch.float32)
+            _need(shared is not None and shared_gate.numel() == T, "one gate value per token, with a shared expert")
+        self._fp8_here(x, chosen, weights, w_up.codes, w_down.codes, shared, shared_gate)
+        out = torch.empty((T, dim), dtype=x.dtype, device=x.device)
+        if T == 0:
+            return out
+        pairs = T * top
+        moe, rows_lib, gemm = self._lib("moe"), self._lib("rows_fp8"), self._lib("gemm_fp8")
+        tile_rows = gemm.tl_gemm_fp8_tile_rows(pairs, E)
+        most = min(pairs, -(-pairs // tile_rows) + E)
+        index = torch.empty(2 * pairs + 1 + 3 * most, dtype=torch.int32, device=x.device)
+        order, place, tiles = index[:pairs], index[pairs:2 * pairs], index[2 * pairs:]
+        _check(moe.tl_moe_plan_tiles(_ptr(chosen), pairs, E, tile_rows, _ptr(order), _ptr(place), _ptr(tiles), _stream()), "moe_plan")
+        rows = self._fp8_empty(pairs, dim, x.device)
+        _check(rows_lib.tl_fp8_rows_placed(_ptr(x), _DT[x.dtype], _ptr(rows.codes), _ptr(rows.scales), T, dim, _ptr(place), top, _stream()), "experts' rows")
+        u = torch.empty((pairs, up_rows), dtype=torch.float32, device=x.device)
+        status = ctypes.c_void_p(self._status_at)
+        _check(gemm.tl_gemm_fp8_experts(_ptr(rows.codes), _ptr(rows.scales), _ptr(w_up.codes), _ptr(w_up.scales), _ptr(u), 1, pairs, up_rows, dim, E,
+                                        _ptr(tiles), most, status, _stream()), "experts' products (up)")
+        hid = self.activation_fp8(u, activation, gated=gated, act_params=act_params)
+        y = torch.empty((pairs, dim), dtype=x.dtype, device=x.device)
+        _check(gemm.tl_gemm_fp8_experts(_ptr(hid.codes), _ptr(hid.scales), _ptr(w_down.codes), _ptr(w_down.scales), _ptr(y),
+                                        1 if x.dtype == torch.float32 else 0, pairs, dim, hidden, E, _ptr(tiles), most, status, _stream()),
+               "experts' products (down)")
+        _check(moe.tl_moe_combine(_ptr(y), _DT[x.dtype], _ptr(place), _ptr(weights), _ptr(shared), _DT[shared.dtype] if shared is not None else 0,
+                                  splits, ctypes.c_longlong(plane), _ptr(shared_gate), _ptr(out), T, dim, top, _stream()), "moe_combine")
+        self.launches += 5
         return out
 
     def can_fuse_residual(self, pending, h: torch.Tensor) -> bool:

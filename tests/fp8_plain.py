@@ -67,3 +67,46 @@ def experts(x, chosen, weights, up, down, kind, gated=False, params=None):
             y = stands_for(act(rows[token] @ up[e].T, kind, gated, params)) @ down[e].T
             out.index_add_(0, token, y * weights[token, choice].double()[:, None])
     return out
+
+
+def moved(y, d):
+    """How far what ``y`` is held as may move when ``y`` moves by ``d`` (both 64-bit ``[rows, K]``): a number next to a border of E4M3 falls to
+    its other side, and where a block's largest number stands next to the border of its scale, the small ones get another step."""
+    at = stands_for(y)
+    reach = torch.maximum((stands_for(y + d) - at).abs(), (stands_for(y - d) - at).abs())
+    e = torch.exp2(hold(y)[1])
+    pad = lambda v: torch.nn.functional.pad(v, (0, -v.shape[1] % BLOCK)).reshape(v.shape[0], -1, BLOCK).amax(-1)  # noqa: E731
+    top, slack = pad(y.abs()), pad(d)
+    border = (top + slack > 448.0 * e) | ((top - slack) <= 224.0 * e)
+    return reach + (border * e * 2.0 ** -8).repeat_interleave(BLOCK, -1)[:, :y.shape[1]]
+
+
+def experts_bound(x, chosen, weights, up, down, kind, gated=False, params=None, result_eps=0.0):
+    """How far a result of float32 arithmetic may be from :func:`experts`, for every number of it: the first product's sums are off by 2^-24 of
+    their magnitudes for every 32 terms (and 4 more); the activation by what that does to it, at the corners, and by 2^-20 of itself and 2^-21
+    of its argument's size; a hidden number is then held as it is, or as its neighbour where the error reaches a border; the second
+    product's sums as the first one's; ``result_eps`` for the rounding of every expert's result, and of the sum."""
+    rows = stands_for(x.double())
+    out = torch.zeros_like(rows)
+    total = torch.zeros_like(rows)
+    for e in range(up.shape[0]):
+        token, choice = torch.nonzero(chosen == e, as_tuple=True)
+        if not token.numel():
+            continue
+        u = rows[token] @ up[e].T
+        du = (rows[token].abs() @ up[e].abs().T) * (rows.shape[1] / 32 + 4) * 2.0 ** -24
+        y = act(u, kind, gated, params)
+        if gated:
+            half = u.shape[1] // 2
+            sides = [torch.cat([a * du[:, :half], b * du[:, half:]], 1) for a in (-1, 1) for b in (-1, 1)]
+            size = u[:, :half].abs() * (u[:, half:].abs() + 1.0)
+        else:
+            sides, size = [-du, du], u.abs()
+        dy = torch.stack([(act(u + s, kind, gated, params) - y).abs() for s in sides]).amax(0) + y.abs() * 2.0 ** -20 + size * 2.0 ** -21
+        held, off = stands_for(y), moved(y, dy)
+        z = held @ down[e].T
+        dz = off @ down[e].abs().T + ((held.abs() + off) @ down[e].abs().T) * (y.shape[1] / 32 + 4) * 2.0 ** -24
+        share = weights[token, choice].double()[:, None]
+        out.index_add_(0, token, share * (dz + (z.abs() + dz) * result_eps))
+        total.index_add_(0, token, share * z.abs())
+    return out + total * 2.0 ** -22 + (total + out) * result_eps

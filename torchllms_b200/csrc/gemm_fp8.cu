@@ -11,9 +11,11 @@
 //
 // A persistent CTA per SM walks units (a slab of 128 rows of W, a tile of rows of x), tiles fastest, so that a slab of W comes from
 // memory once and the rows of x, which are fewer, from L2.  Inside a CTA (256 threads):
-//   warp 0    TMA: a [128 x 128] box of W and a [width x 128] box of x a stage, 128-byte swizzle
+//   warp 0    TMA: two [128 x 128] boxes of W and two [width x 128] boxes of x a stage, 128-byte swizzle
 //   warp 1    tcgen05.cp of scales (a word a row: four blocks of 128) and tcgen05.mma, four of K 32 a stage
-//   warp 2    scales from memory to shared memory, in the order that tcgen05.cp wants: row r of a chunk of 128 at 16 (r % 32) + 4 (r / 32)
+//   warps 2, 3  scales from memory to shared memory, four words a row and turn (2,048 of K), in turns; in the order that
+//             tcgen05.cp wants: row r of a chunk of 128 at 16 (r % 32) + 4 (r / 32).  (The fence behind them waits for all loads
+//             under way: a word a turn, copied ahead, kept the products waiting - 620 cycles of every 880 a stage.)
 //   warps 4-7 results: tcgen05.ld, through shared memory to rows of C; two accumulators, so that the next unit's products run meanwhile
 // Every wait is bounded: on a time-out the CTA records a code, lets its copies land, frees its tensor memory and returns.
 #include "fp8.cuh"
@@ -22,13 +24,15 @@
 namespace {
 
 constexpr int BM = 128;              // rows of W a CTA
-constexpr int BK = 128;              // bytes of K a stage: a swizzle row, and a block of numbers that share a scale
+constexpr int BK = 128;              // bytes of K a box: a swizzle row, and a block of numbers that share a scale
+constexpr int BOXES = 2;             // boxes of W (and of x) a stage: what a stage costs its issuer (a wait, a fence, a commit) is as much as
+                                     // four products of 240 rows take
 constexpr int MAX_WIDTH = 240;       // rows of x a tile: two accumulators and two sets of scales fill 512 columns
 constexpr int MAX_STAGES = 12;
-constexpr int SCALE_BUFS = 4;        // words of scales (512 of K) under way
-constexpr int SCALE_BYTES = 512 + 1024;
-constexpr int SCALE_LAG = 2;
+constexpr int SCALE_BUFS = 3;        // turns of scales under way
+constexpr int TURN = 16;             // blocks of 128 of a turn: four words a row
 constexpr int NTHREADS = 256;
+
 constexpr int STAGING = 4 * 2048;    // 32 x 32 results a warp
 constexpr unsigned TMEM_COLS = 512;
 constexpr unsigned SCALE_COL = 240;  // scales of set s at columns 256 s + 240: 4 of W, 8 of x
@@ -42,6 +46,8 @@ __device__ __forceinline__ void mbar_init(unsigned bar, unsigned count) {
 }
 __device__ __forceinline__ bool mbar_try_wait(unsigned bar, unsigned parity) {
     unsigned ok;
+    // (what a wait guards is read by the tensor cores and the copy engine, not by the waiting thread: an acquire at the scope of the
+    // cluster, which empties L1, cost a quarter of a decode step's product)
     asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
                  : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     return ok != 0;
@@ -51,35 +57,59 @@ __device__ __forceinline__ unsigned long long global_ns() {
     asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
     return t;
 }
-// false once the limit has passed, or as soon as another role has given up; a whole warp waits together
-__device__ __forceinline__ bool mbar_wait(unsigned bar, unsigned parity, volatile int* aborted) {
+// false once the limit has passed, or as soon as another role has given up
+__device__ __forceinline__ bool wait_one(unsigned bar, unsigned parity, volatile int* aborted) {
     bool ok = mbar_try_wait(bar, parity);
-    if (!ok) {
-        const unsigned long long t0 = global_ns();
-        for (unsigned i = 1; !ok; ++i) {
-            ok = mbar_try_wait(bar, parity);
-            if (!ok && (i & 255u) == 0u && (*aborted || global_ns() - t0 > WAIT_LIMIT_NS)) break;
+    unsigned long long t0 = 0;
+    // (the timer is read rarely: a read takes as long as a stage's products)
+    for (unsigned i = 1; !ok; ++i) {
+        ok = mbar_try_wait(bar, parity);
+        if (!ok && (i & 255u) == 0u) {
+            if (t0 == 0) t0 = global_ns();
+            if (*aborted || global_ns() - t0 > WAIT_LIMIT_NS) break;
         }
     }
-    return __all_sync(0xffffffffu, ok);
+    return ok;
+}
+// the same for a whole warp that waits together
+__device__ __forceinline__ bool mbar_wait(unsigned bar, unsigned parity, volatile int* aborted) {
+    return __all_sync(0xffffffffu, wait_one(bar, parity, aborted));
 }
 __device__ __forceinline__ void give_up(volatile int* aborted, int* status, int code) {
-    if ((threadIdx.x & 31) == 0) {
-        *aborted = 1;
-        atomicExch(status, code);
-    }
+    *aborted = 1;
+    atomicExch(status, code);
 }
-// one elected lane of a warp in step arrives
+// One elected lane of a warp in step arrives.  PAIR: at a barrier that may be the other CTA's.  (Neither form orders more than this CTA
+// sees: what it guards has gone through a proxy fence or has been read from tensor memory.  With release at the cluster's scope,
+// which waits for everything the warp has stored, a decode step's product took a quarter longer.)
+template <bool PAIR>
 __device__ __forceinline__ void arrive_elect(unsigned bar) {
-    asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t@e mbarrier.arrive.shared::cta.b64 _, [%0];\n\t}" ::"r"(bar) : "memory");
+    if (!PAIR) {
+        asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t@e mbarrier.arrive.shared::cta.b64 _, [%0];\n\t}" ::"r"(bar) : "memory");
+        return;
+    }
+    asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t@e mbarrier.arrive.shared::cluster.b64 _, [%0];\n\t}" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ void expect_tx_elect(unsigned bar, unsigned bytes) {
-    asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
-                 "@e mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar), "r"(bytes) : "memory");
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// the address of the pair's first CTA's variable of the same place
+__device__ __forceinline__ unsigned in_leader(unsigned addr) {
+    unsigned r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+    return r;
+}
+__device__ __forceinline__ void expect_tx(unsigned bar, unsigned bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+template <bool PAIR>
 __device__ __forceinline__ void tma_load(unsigned dst, const CUtensorMap* map, unsigned bar, int x, int y) {
-    asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
-                 "@e cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n\t}"
+    if (PAIR) {        // (the barrier that counts the bytes is the first CTA's)
+        asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                     ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+        return;
+    }
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
                  ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
 }
 
@@ -95,18 +125,38 @@ __device__ __forceinline__ unsigned long long scale_desc(unsigned addr) {
 __device__ __forceinline__ unsigned instruction(int M, int N, int byte) {
     return (1u << 23) | ((unsigned)(N >> 3) << 17) | ((unsigned)(M >> 4) << 24) | ((unsigned)byte << 29) | ((unsigned)byte << 4);
 }
+__device__ __forceinline__ bool elect_one() {
+    unsigned e;
+    asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\tselp.u32 %0, 1, 0, e;\n\t}" : "=r"(e));
+    return e != 0;
+}
+// One lane issues, always the same.  PAIR: for both CTAs, the first one issues; commits arrive at both CTAs' barriers.
+template <bool PAIR>
 __device__ __forceinline__ void mma(unsigned d, unsigned long long a, unsigned long long b, unsigned idesc, unsigned sa, unsigned sb, unsigned accumulate) {
-    asm volatile("{\n\t.reg .pred p, e;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-                 "@e tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate) : "memory");
+#define TL_MMA(G) \
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t" \
+                 "tcgen05.mma.cta_group::" #G ".kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" \
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate) : "memory")
+    if (PAIR) TL_MMA(2);
+    else TL_MMA(1);
+#undef TL_MMA
 }
+template <bool PAIR>
 __device__ __forceinline__ void copy_scales(unsigned taddr, unsigned long long desc) {
-    asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t@e tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n\t}"
-                 ::"r"(taddr), "l"(desc) : "memory");
+#define TL_COPY(G) \
+    asm volatile("tcgen05.cp.cta_group::" #G ".32x128b.warpx4 [%0], %1;" \
+                 ::"r"(taddr), "l"(desc) : "memory")
+    if (PAIR) TL_COPY(2);
+    else TL_COPY(1);
+#undef TL_COPY
 }
+template <bool PAIR>
 __device__ __forceinline__ void commit(unsigned bar) {
-    asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
-                 "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar) : "memory");
+    if (PAIR)
+        asm volatile("{\n\t.reg .b16 m;\n\tmov.b16 m, 3;\n\t"
+                     "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], m;\n\t}" ::"r"(bar) : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void tmem_load32(unsigned taddr, unsigned (&r)[32]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
@@ -117,9 +167,15 @@ __device__ __forceinline__ void tmem_load32(unsigned taddr, unsigned (&r)[32]) {
                    "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
                  : "r"(taddr));
 }
-// four bytes from memory, zeros where there is no row
-__device__ __forceinline__ void copy_word(unsigned dst, const unsigned char* src, bool there) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(there ? 4 : 0) : "memory");
+// up to four words of a row's scales, zeros where there is no row (null)
+__device__ __forceinline__ void load_words(const unsigned char* at, int words, bool whole, unsigned (&v)[4]) {
+    if (at != nullptr && whole) {        // (every turn of every row starts on 16 bytes and has 16)
+        const uint4 r = *reinterpret_cast<const uint4*>(at);
+        v[0] = r.x; v[1] = r.y; v[2] = r.z; v[3] = r.w;
+        return;
+    }
+#pragma unroll
+    for (int w = 0; w < 4; ++w) v[w] = at != nullptr && w < words ? *reinterpret_cast<const unsigned*>(at + 4 * w) : 0u;
 }
 
 struct Params {
@@ -132,7 +188,11 @@ struct Params {
     int width;                       // rows of x a tile, a multiple of 16
     int slabs, n_tiles, stages;
     int out_is_f32;
+    bool w_whole, x_whole;           // scales: rows are a multiple of 16 bytes and start on 16
 };
+
+// shared memory of a word of scales: 512 bytes for the rows of W and for every 128 rows of x
+__host__ __device__ constexpr int scale_bytes(int width) { return 512 * (1 + (width + 127) / 128); }
 
 struct Unit { int expert, row0, rows, slab; };
 
@@ -152,36 +212,49 @@ __device__ __forceinline__ Unit unit_of(const Params& p, int u, int n_tiles) {
     return r;
 }
 
+template <bool PAIR>
 __global__ void __launch_bounds__(NTHREADS, 1) gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                                                                const Params p) {
     extern __shared__ unsigned char smem_raw[];
     const unsigned smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u;            // tiles want 1,024-byte alignment for the swizzle
     unsigned char* const smem_at = smem_raw + (smem0 - smem_u32(smem_raw));
-    const unsigned w_bytes = BM * BK, stage_bytes = w_bytes + p.width * BK;
-    const unsigned scales_at = smem0 + p.stages * stage_bytes;
-    unsigned char* const staging = smem_at + p.stages * stage_bytes + SCALE_BUFS * SCALE_BYTES;
+    // a pair shares a unit of 256 rows of W: each CTA has 128 of them and half of the tile's rows of x
+    constexpr int SIDES = PAIR ? 2 : 1;
+    const int rank = PAIR ? (int)(blockIdx.x & 1) : 0;
+    const int first_unit = blockIdx.x / SIDES, step = gridDim.x / SIDES;
+    const unsigned w_bytes = BM * BK, x_bytes = p.width / SIDES * BK, stage_bytes = BOXES * (w_bytes + x_bytes);
+    const unsigned scales_at = smem0 + p.stages * stage_bytes, word_bytes = scale_bytes(p.width), turn_bytes = 4 * word_bytes;
+    unsigned char* const staging = smem_at + p.stages * stage_bytes + SCALE_BUFS * turn_bytes;
     __shared__ __align__(8) unsigned long long bars[2 * MAX_STAGES + 2 * SCALE_BUFS + 5];
     __shared__ unsigned tmem_slot;
     __shared__ int abort_flag;
     const unsigned bar0 = smem_u32(bars);
     const unsigned full = bar0, empty = bar0 + 8 * MAX_STAGES, sc_full = bar0 + 16 * MAX_STAGES, sc_empty = sc_full + 8 * SCALE_BUFS;
     const unsigned acc_full = sc_empty + 8 * SCALE_BUFS, acc_empty = acc_full + 16, drained = acc_empty + 16;
+    // (what the first CTA's issuing warp waits for counts arrivals of both)
+    auto leader = [&](unsigned bar) { return PAIR ? in_leader(bar) : bar; };
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         abort_flag = 0;
         for (int s = 0; s < MAX_STAGES; ++s) { mbar_init(full + 8 * s, 1); mbar_init(empty + 8 * s, 1); }
-        for (int s = 0; s < SCALE_BUFS; ++s) { mbar_init(sc_full + 8 * s, 1); mbar_init(sc_empty + 8 * s, 1); }
-        for (int s = 0; s < 2; ++s) { mbar_init(acc_full + 8 * s, 1); mbar_init(acc_empty + 8 * s, 4); }
+        for (int s = 0; s < SCALE_BUFS; ++s) { mbar_init(sc_full + 8 * s, SIDES); mbar_init(sc_empty + 8 * s, 1); }
+        for (int s = 0; s < 2; ++s) { mbar_init(acc_full + 8 * s, 1); mbar_init(acc_empty + 8 * s, 4 * SIDES); }
         mbar_init(drained, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(TMEM_COLS) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(TMEM_COLS) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(TMEM_COLS) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    if (PAIR) cluster_sync();          // both CTAs' barriers are set up and both have their tensor memory
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const unsigned tmem = tmem_slot;
     volatile int* aborted = &abort_flag;
@@ -192,130 +265,155 @@ __global__ void __launch_bounds__(NTHREADS, 1) gemm_fp8_kernel(const __grid_cons
     const int units = n_tiles * p.slabs;
 
     if (warp == 0) {
-        int it = 0, stage = 0;
-        bool ok = true;
-        for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
-            const Unit t = unit_of(p, u, n_tiles);
-            for (int kb = 0; kb < p.k_blocks; ++kb, ++it) {
-                if (it >= p.stages && !mbar_wait(empty + 8 * stage, (it / p.stages - 1) & 1, aborted)) {
-                    give_up(aborted, p.status, ERR_TMA_WAIT);
-                    ok = false;
-                    break;
+        if (elect_one()) {
+            int stage = 0, issued = 0;
+            unsigned phase = 1;                // (a barrier that has completed nothing counts as having completed phase 1)
+            bool ok = true;
+            for (int u = first_unit; u < units && ok; u += step) {
+                const Unit t = unit_of(p, u, n_tiles);
+                const int w_row = t.expert * p.N + (t.slab * SIDES + rank) * BM, x_row = t.row0 + rank * (((t.rows + 15) & ~15) / 2);
+                for (int kb = 0; kb < p.k_blocks; kb += BOXES) {
+                    if (!wait_one(empty + 8 * stage, phase, aborted)) {
+                        give_up(aborted, p.status, ERR_TMA_WAIT);
+                        ok = false;
+                        break;
+                    }
+                    const unsigned at = smem0 + stage * stage_bytes, bar = leader(full + 8 * stage);
+                    const int boxes = min(BOXES, p.k_blocks - kb);
+                    if (rank == 0) expect_tx(full + 8 * stage, SIDES * boxes * (w_bytes + x_bytes));
+#pragma unroll
+                    for (int i = 0; i < BOXES; ++i) {
+                        if (i < boxes) {
+                            tma_load<PAIR>(at + i * w_bytes, &map_w, bar, (kb + i) * BK, w_row);
+                            tma_load<PAIR>(at + BOXES * w_bytes + i * x_bytes, &map_x, bar, (kb + i) * BK, x_row);
+                        }
+                    }
+                    if (issued < p.stages) ++issued;
+                    if (++stage == p.stages) { stage = 0; phase ^= 1; }
                 }
-                const unsigned at = smem0 + stage * stage_bytes;
-                expect_tx_elect(full + 8 * stage, stage_bytes);
-                tma_load(at, &map_w, full + 8 * stage, kb * BK, t.expert * p.N + t.slab * BM);
-                tma_load(at + w_bytes, &map_x, full + 8 * stage, kb * BK, t.row0);
-                if (++stage == p.stages) stage = 0;
+            }
+            // whatever happened to the others, the copies under way land before the CTA ends (a pair ends together, and the first
+            // CTA's barriers count for both)
+            int none = 0;
+            for (int i = 0; i < issued && rank == 0; ++i) {
+                if (--stage < 0) { stage = p.stages - 1; phase ^= 1; }
+                wait_one(full + 8 * stage, phase ^ 1, &none);
             }
         }
-        // whatever happened to the others, the copies under way land before the CTA ends
-        int none = 0;
-        for (int i = it > p.stages ? it - p.stages : 0; i < it; ++i) mbar_wait(full + 8 * (i % p.stages), (i / p.stages) & 1, &none);
-    } else if (warp == 1) {
-        int it = 0, stage = 0, group = 0, n = 0;
-        bool ok = true;
-        for (int u = blockIdx.x; u < units && ok; u += gridDim.x, ++n) {
-            const Unit t = unit_of(p, u, n_tiles);
-            const int acc = n & 1, N = (t.rows + 15) & ~15;
-            const unsigned d = tmem + acc * 256;
-            if (n >= 2 && !mbar_wait(acc_empty + 8 * acc, (n / 2 - 1) & 1, aborted)) {
-                give_up(aborted, p.status, ERR_MMA_WAIT);
-                break;
-            }
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            for (int kb = 0; kb < p.k_blocks; ++kb, ++it) {
-                const int buf = group % SCALE_BUFS;
-                const unsigned set = tmem + (group & 1) * 256 + SCALE_COL;
-                if ((kb & 3) == 0) {
-                    if (!mbar_wait(sc_full + 8 * buf, (group / SCALE_BUFS) & 1, aborted)) {
+        __syncwarp();
+    } else if (warp == 1 && rank == 0) {
+        if (elect_one()) {
+            int stage = 0, buf = 0, n = 0;
+            unsigned phase = 0, sc_phase = 0, word = 0;
+            bool ok = true;
+            for (int u = first_unit; u < units && ok; u += step, ++n) {
+                const Unit t = unit_of(p, u, n_tiles);
+                const int acc = n & 1, N = (t.rows + 15) & ~15;
+                const unsigned d = tmem + acc * 256;
+                if (!wait_one(acc_empty + 8 * acc, ((n >> 1) & 1) ^ 1, aborted)) {
+                    give_up(aborted, p.status, ERR_MMA_WAIT);
+                    break;
+                }
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                for (int kb = 0; kb < p.k_blocks; kb += BOXES) {
+                    if (kb % TURN == 0 && !wait_one(sc_full + 8 * buf, sc_phase, aborted)) {
                         give_up(aborted, p.status, ERR_MMA_WAIT);
                         ok = false;
                         break;
                     }
-                    const unsigned at = scales_at + buf * SCALE_BYTES;
-                    copy_scales(set, scale_desc(at));
-                    copy_scales(set + 4, scale_desc(at + 512));
-                    if (N > 128) copy_scales(set + 8, scale_desc(at + 1024));
-                }
-                if (!mbar_wait(full + 8 * stage, (it / p.stages) & 1, aborted)) {
-                    give_up(aborted, p.status, ERR_MMA_WAIT);
-                    ok = false;
-                    break;
-                }
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const unsigned at = smem0 + stage * stage_bytes;
-                const unsigned idesc = instruction(BM, N, kb & 3);
-                const unsigned long long a = operand_desc(at), b = operand_desc(at + w_bytes);
+                    if (kb % 4 == 0) {
+                        // (two sets in turn: copies and products are carried out in the order of their issue)
+                        word ^= 1;
+                        const unsigned at = scales_at + buf * turn_bytes + kb / 4 % 4 * word_bytes, to = tmem + word * 256 + SCALE_COL;
+                        copy_scales<PAIR>(to, scale_desc(at));
+                        copy_scales<PAIR>(to + 4, scale_desc(at + 512));
+                        if (N > 128) copy_scales<PAIR>(to + 8, scale_desc(at + 1024));
+                    }
+                    const unsigned set = tmem + word * 256 + SCALE_COL;
+                    if (!wait_one(full + 8 * stage, phase, aborted)) {
+                        give_up(aborted, p.status, ERR_MMA_WAIT);
+                        ok = false;
+                        break;
+                    }
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const unsigned at = smem0 + stage * stage_bytes;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) mma(d, a + 2 * k, b + 2 * k, idesc, set, set + 4, (kb > 0 || k > 0) ? 1u : 0u);
-                commit(empty + 8 * stage);
-                if (++stage == p.stages) stage = 0;
-                if ((kb & 3) == 3 || kb == p.k_blocks - 1) {
-                    commit(sc_empty + 8 * buf);
-                    ++group;
+                    for (int i = 0; i < BOXES; ++i) {
+                        if (kb + i < p.k_blocks) {
+                            const unsigned idesc = instruction(SIDES * BM, N, (kb + i) & 3);
+                            const unsigned long long a = operand_desc(at + i * w_bytes), b = operand_desc(at + BOXES * w_bytes + i * x_bytes);
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) mma<PAIR>(d, a + 2 * k, b + 2 * k, idesc, set, set + 4, (kb > 0 || i > 0 || k > 0) ? 1u : 0u);
+                        }
+                    }
+                    commit<PAIR>(empty + 8 * stage);
+                    if (++stage == p.stages) { stage = 0; phase ^= 1; }
+                    if (kb % TURN == TURN - BOXES || kb + BOXES >= p.k_blocks) {
+                        commit<PAIR>(sc_empty + 8 * buf);
+                        if (++buf == SCALE_BUFS) { buf = 0; sc_phase ^= 1; }
+                    }
                 }
+                if (ok) commit<PAIR>(acc_full + 8 * acc);
             }
-            if (ok) commit(acc_full + 8 * acc);
+            // (the products read shared memory and their commits write barriers: all of it ends before the CTA does)
+            int none = 0;
+            commit<PAIR>(drained);
+            wait_one(drained, 0, &none);
         }
-        // (the products read shared memory: they end before the CTA does)
-        int none = 0;
-        commit(drained);
-        mbar_wait(drained, 0, &none);
-    } else if (warp == 2) {
-        int group = 0;
+        __syncwarp();
+    } else if (warp == 2 || warp == 3) {
+        int turn = 0, buf = 0;
+        unsigned phase = 1;
         bool ok = true;
-        auto publish = [&](int g) {
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            arrive_elect(sc_full + 8 * (g % SCALE_BUFS));
-        };
-        for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+        for (int u = first_unit; u < units && ok; u += step) {
             const Unit t = unit_of(p, u, n_tiles);
             const long long first = (long long)t.expert * p.N;
-            for (int g = 0; g * 4 < p.k_blocks; ++g, ++group) {
-                const int buf = group % SCALE_BUFS;
-                if (group >= SCALE_BUFS && !mbar_wait(sc_empty + 8 * buf, (group / SCALE_BUFS - 1) & 1, aborted)) {
-                    give_up(aborted, p.status, ERR_SCALE_WAIT);
-                    ok = false;
-                    break;
-                }
-                const unsigned at = scales_at + buf * SCALE_BYTES + 16 * lane;
+            for (int kb = 0; kb < p.k_blocks; kb += TURN, ++turn) {
+                if ((turn & 1) == warp - 2) {
+                    if (!mbar_wait(sc_empty + 8 * buf, phase, aborted)) {
+                        if (lane == 0) give_up(aborted, p.status, ERR_SCALE_WAIT);
+                        ok = false;
+                        break;
+                    }
+                    const unsigned at = scales_at + buf * turn_bytes + 16 * lane;
+                    const int words = min(4, (p.k_blocks - kb + 3) / 4);
+                    unsigned v[12][4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int r = t.slab * BM + 32 * j + lane;
-                    const bool there = r < p.N;
-                    copy_word(at + 4 * j, p.w_scales + (first + (there ? r : 0)) * p.pitch + 4 * g, there);
-                }
+                    for (int j = 0; j < 12; ++j) {
+                        const int r = j < 4 ? (t.slab * SIDES + rank) * BM + 32 * j + lane : 32 * (j - 4) + lane;
+                        const bool there = j < 4 ? r < p.N : r < t.rows;
+                        const unsigned char* row = j < 4 ? p.w_scales + (first + r) * p.pitch : p.x_scales + (long long)(t.row0 + r) * p.pitch;
+                        load_words(there ? row + kb : nullptr, words, j < 4 ? p.w_whole : p.x_whole, v[j]);
+                    }
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    if (32 * j >= t.rows) break;
-                    const bool there = 32 * j + lane < t.rows;
-                    copy_word(at + 512 + (j / 4) * 512 + 4 * (j % 4), p.x_scales + (long long)(t.row0 + (there ? 32 * j + lane : 0)) * p.pitch + 4 * g, there);
+                    for (int j = 0; j < 12; ++j) {
+                        if (j >= 4 && 32 * (j - 4) >= t.rows) break;
+                        const unsigned to = at + (j < 4 ? 4 * j : 512 + (j - 4) / 4 * 512 + 4 * (j % 4));
+#pragma unroll
+                        for (int w = 0; w < 4; ++w)
+                            if (w < words) asm volatile("st.shared.b32 [%0], %1;" ::"r"(to + w * word_bytes), "r"(v[j][w]) : "memory");
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    arrive_elect<PAIR>(leader(sc_full + 8 * buf));
                 }
-                asm volatile("cp.async.commit_group;" ::: "memory");
-                if (group >= SCALE_LAG) {
-                    asm volatile("cp.async.wait_group %0;" ::"n"(SCALE_LAG) : "memory");
-                    publish(group - SCALE_LAG);
-                }
+                if (++buf == SCALE_BUFS) { buf = 0; phase ^= 1; }
             }
         }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        for (int g = group > SCALE_LAG ? group - SCALE_LAG : 0; g < group; ++g) publish(g);
     } else if (warp >= 4) {
         const int quarter = warp & 3;
         unsigned char* const mine = staging + quarter * 2048;
         const bool wide = !p.out_is_f32 && p.N % 8 == 0;
         int n = 0;
-        for (int u = blockIdx.x; u < units; u += gridDim.x, ++n) {
+        for (int u = first_unit; u < units; u += step, ++n) {
             const Unit t = unit_of(p, u, n_tiles);
             const int acc = n & 1;
             if (!mbar_wait(acc_full + 8 * acc, (n / 2) & 1, aborted)) {
-                give_up(aborted, p.status, ERR_EPI_WAIT);
+                if (lane == 0) give_up(aborted, p.status, ERR_EPI_WAIT);
                 break;
             }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const int first = t.slab * BM + quarter * 32;          // this warp's first row of W
+            const int first = (t.slab * SIDES + rank) * BM + quarter * 32;          // this warp's first row of W
             for (int c0 = 0; c0 < t.rows; c0 += 32) {
                 unsigned r[32];
                 // (a load of 32 columns may reach into the scales' columns behind the accumulator: read, not used)
@@ -347,15 +445,28 @@ __global__ void __launch_bounds__(NTHREADS, 1) gemm_fp8_kernel(const __grid_cons
                 }
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            arrive_elect(acc_empty + 8 * acc);
+            arrive_elect<PAIR>(leader(acc_empty + 8 * acc));
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    if (PAIR && rank == 1 && warp == 1) {
+        // the second CTA issues nothing, but commits arrive at its barriers too, the last of them perhaps later than at the
+        // first CTA's: it must not end before they have
+        int none = 0;
+        mbar_wait(drained, 0, &none);
+    }
+    __syncwarp();
+    if (PAIR) cluster_sync();          // nothing of one CTA is used by the other from here on
     if (warp == 1) {
         __syncwarp();
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+        if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+    }
+    if (PAIR) {                        // the pair gives its tensor memory back together, and ends together
+        __syncthreads();
+        cluster_sync();
     }
 }
 
@@ -399,43 +510,74 @@ int even_width(int M) {
     return ((M + tiles - 1) / tiles + 15) / 16 * 16;
 }
 
+template <bool PAIR>
+int launch(Params& p, const void* x, const void* w, int experts, int K, cudaStream_t s) {
+    constexpr int SIDES = PAIR ? 2 : 1;
+    p.slabs = (p.N + SIDES * BM - 1) / (SIDES * BM);
+    if ((long long)p.slabs * p.n_tiles > 0x7fffffffll) return TL_BAD_SIZE;
+    const int stage_bytes = BOXES * (BM * BK + p.width / SIDES * BK);
+    const int most = 227 * 1024 - 1024 - 1024 - SCALE_BUFS * 4 * scale_bytes(p.width) - STAGING;       // (a kilobyte for barriers, one to align)
+    p.stages = most / stage_bytes;
+    if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
+    CUtensorMap mw, mx;
+    int rc = make_map(&mw, w, (long long)experts * p.N, K, BM);
+    if (rc != TL_OK) return rc;
+    rc = make_map(&mx, x, p.M, K, p.width / SIDES);
+    if (rc != TL_OK) return rc;
+    const size_t smem = 1024 + (size_t)p.stages * stage_bytes + SCALE_BUFS * 4 * scale_bytes(p.width) + STAGING;
+    auto kern = gemm_fp8_kernel<PAIR>;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024);
+    if (e != cudaSuccess) return (int)e;
+    const int units = p.slabs * p.n_tiles, most_units = sm_count() / SIDES;
+    const dim3 grid(SIDES * (units < most_units ? units : most_units));
+    if (!PAIR) return (int)tl_launch(kern, grid, dim3(NTHREADS), smem, s, mw, mx, p);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(NTHREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = SIDES;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return (int)cudaLaunchKernelEx(&cfg, kern, mw, mx, p);
+}
+
 int launch(const void* x, const void* x_scales, const void* w, const void* w_scales, void* out, int out_is_f32, int M, int N, int K, int experts,
-           const int* tiles, int most_tiles, int width, int* status, cudaStream_t s) {
+           const int* tiles, int most_tiles, int width, int form, int* status, cudaStream_t s) {
     if (N <= 0 || K <= 0 || K % 16 != 0 || experts <= 0 || (long long)experts * N > 0x7fffff00ll) return TL_BAD_SIZE;
     if (!aligned16(x) || !aligned16(w) || !aligned16(out) || status == nullptr || ((uintptr_t)x_scales & 3u) != 0 || ((uintptr_t)w_scales & 3u) != 0)
         return TL_BAD_ALIGN;
     Params p = {};
     p.out = out; p.status = status; p.out_is_f32 = out_is_f32;
     p.w_scales = (const unsigned char*)w_scales; p.x_scales = (const unsigned char*)x_scales;
+    p.w_whole = fp8_scale_pitch(K) % 16 == 0 && aligned16(w_scales);
+    p.x_whole = fp8_scale_pitch(K) % 16 == 0 && aligned16(x_scales);
     p.tiles = tiles;
     p.M = M; p.N = N; p.k_blocks = (K + BK - 1) / BK; p.pitch = fp8_scale_pitch(K);
     p.width = width;
-    p.slabs = (N + BM - 1) / BM;
     p.n_tiles = most_tiles;
-    if ((long long)p.slabs * most_tiles > 0x7fffffffll) return TL_BAD_SIZE;
-    const int most = 227 * 1024 - 1024 - 1024 - SCALE_BUFS * SCALE_BYTES - STAGING;       // (a kilobyte for barriers, one to align)
-    p.stages = most / (BM * BK + width * BK);
-    if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
-    CUtensorMap mw, mx;
-    int rc = make_map(&mw, w, (long long)experts * N, K, BM);
-    if (rc != TL_OK) return rc;
-    rc = make_map(&mx, x, M, K, width);
-    if (rc != TL_OK) return rc;
-    const size_t smem = 1024 + (size_t)p.stages * (BM * BK + width * BK) + SCALE_BUFS * SCALE_BYTES + STAGING;
-    cudaError_t e = cudaFuncSetAttribute(gemm_fp8_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024);
-    if (e != cudaSuccess) return (int)e;
-    const int units = p.slabs * most_tiles, sms = sm_count();
-    return (int)tl_launch(gemm_fp8_kernel, dim3(units < sms ? units : sms), dim3(NTHREADS), smem, s, mw, mx, p);
+    if (form < 0 || form > 2) return TL_BAD_SIZE;
+    // Pairs halve what a tile of x costs in copies, and that is what wide tiles wait for (2,048 rows of 28,672 x 4,096: 222 us
+    // alone, 186 in pairs); narrow ones stream W, which nobody shares (8 rows: 22.3 and 22.4)
+    const bool pair = form == 0 ? width > 64 : form == 2;
+    return pair ? launch<true>(p, x, w, experts, K, s) : launch<false>(p, x, w, experts, K, s);
 }
 
 }  // namespace
 
-// out[M, N] (float32 or bfloat16) = x . w^T for 8-bit rows x [M, K] and w [N, K] with their scales.
+// out[M, N] (float32 or bfloat16) = x . w^T for 8-bit rows x [M, K] and w [N, K] with their scales.  form: 0 the one that fits, 1 a CTA
+// to a unit, 2 a pair of CTAs.
 extern "C" int tl_gemm_fp8(const void* x, const void* x_scales, const void* w, const void* w_scales, void* out, int out_is_f32, int M, int N, int K,
-                           int* status, void* stream) {
+                           int form, int* status, void* stream) {
     if (M <= 0) return TL_OK;
     const int width = even_width(M);
-    return launch(x, x_scales, w, w_scales, out, out_is_f32, M, N, K, 1, nullptr, (M + width - 1) / width, width, status, (cudaStream_t)stream);
+    return launch(x, x_scales, w, w_scales, out, out_is_f32, M, N, K, 1, nullptr, (M + width - 1) / width, width, form, status, (cudaStream_t)stream);
 }
 
 // Rows of a tile of the experts' products, and how many tiles there can be.
@@ -449,9 +591,9 @@ extern "C" int tl_gemm_fp8_tile_rows(int pairs, int experts) {
 // The experts' products: x [pairs, K] sorted by expert, w [experts, N, K], out [pairs, N]; tiles as moe_plan leaves them, with
 // tl_gemm_fp8_tile_rows(pairs, experts) rows at most and most_tiles of them at most.
 extern "C" int tl_gemm_fp8_experts(const void* x, const void* x_scales, const void* w, const void* w_scales, void* out, int out_is_f32, int pairs,
-                                   int N, int K, int experts, const int* tiles, int most_tiles, int* status, void* stream) {
+                                   int N, int K, int experts, const int* tiles, int most_tiles, int form, int* status, void* stream) {
     if (pairs <= 0) return TL_OK;
     if (tiles == nullptr || most_tiles <= 0) return TL_BAD_SIZE;
-    return launch(x, x_scales, w, w_scales, out, out_is_f32, pairs, N, K, experts, tiles, most_tiles, tl_gemm_fp8_tile_rows(pairs, experts), status,
+    return launch(x, x_scales, w, w_scales, out, out_is_f32, pairs, N, K, experts, tiles, most_tiles, tl_gemm_fp8_tile_rows(pairs, experts), form, status,
                   (cudaStream_t)stream);
 }

@@ -1575,10 +1575,12 @@ class NativeOps:
         self.launches += h.shape[0] > 0
         return out
 
+    _FP8_FORMS = {"auto": 0, "single": 1, "pair": 2}
+
     @_timed
-    def linear_fp8(self, x, w: Fp8Rows, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    def linear_fp8(self, x, w: Fp8Rows, out_dtype: torch.dtype = torch.bfloat16, impl: str = "auto") -> torch.Tensor:
         """``x [M, K] @ w[N, K]^T`` of 8-bit rows, summed in float32.  ``x`` may be float32/bfloat16 rows, which are brought to 8 bits
-        first (:meth:`quantize_fp8`).  The result is bfloat16 or float32 ``[M, N]``."""
+        first (:meth:`quantize_fp8`).  The result is bfloat16 or float32 ``[M, N]``.  ``impl`` forces a form of the kernel (tests)."""
         if not isinstance(x, Fp8Rows):
             x = self.quantize_fp8(x)
         self._fp8_need(x, "linear_fp8: x")
@@ -1586,12 +1588,13 @@ class NativeOps:
         (M, K), N = x.codes.shape, w.codes.shape[0]
         _need(w.codes.shape[1] == K, f"linear_fp8: inner sizes differ ({K} and {w.codes.shape[1]})")
         _need(out_dtype in _DT, f"linear_fp8: output dtype {out_dtype} unsupported")
+        _need(impl in self._FP8_FORMS, f"linear_fp8: impl must be one of {', '.join(self._FP8_FORMS)}, got {impl!r}")
         self._fp8_here(x.codes, w.codes)
         out = torch.empty((M, N), dtype=out_dtype, device=x.codes.device)
         if M == 0 or N == 0:
             return out
         rc = self._lib("gemm_fp8").tl_gemm_fp8(_ptr(x.codes), _ptr(x.scales), _ptr(w.codes), _ptr(w.scales), _ptr(out),
-                                              1 if out_dtype == torch.float32 else 0, M, N, K, ctypes.c_void_p(self._status_at), _stream())
+                                              1 if out_dtype == torch.float32 else 0, M, N, K, self._FP8_FORMS[impl], ctypes.c_void_p(self._status_at), _stream())
         _check(rc, "linear_fp8")
         self.launches += 1
         return out
@@ -1599,7 +1602,7 @@ class NativeOps:
     @_timed
     def moe_experts_fp8(self, x: torch.Tensor, chosen: torch.Tensor, weights: torch.Tensor, w_up: Fp8Rows, w_down: Fp8Rows, *, activation: str,
                         shared: Optional[torch.Tensor] = None, shared_gate: Optional[torch.Tensor] = None, gated: bool = False,
-                        act_params=None) -> torch.Tensor:
+                        act_params=None, impl: str = "auto") -> torch.Tensor:
         """:meth:`moe_experts` with weights in 8 bits: ``w_up`` ``[E, hidden, dim]`` (``gated``: ``[E, 2 * hidden, dim]``, rows ``[gate; up]``) and
         ``w_down`` ``[E, dim, hidden]``.  A token's row is brought to 8 bits once, the hidden rows behind the activation again (taken in
         float32, rounded once); both products run over the rows sorted by expert.  Experts that nobody chose are not read."""
@@ -1609,6 +1612,8 @@ class NativeOps:
         self._fp8_need(w_up, "experts' up weights", 3)
         self._fp8_need(w_down, "experts' down weights", 3)
         _need(activation in self._ACTS, f"unknown activation {activation!r}; known: {', '.join(self._ACTS)}")
+        _need(impl in self._FP8_FORMS, f"experts: impl must be one of {', '.join(self._FP8_FORMS)}, got {impl!r}")
+        form = self._FP8_FORMS[impl]
         dim = self._fp8_width(x, "experts' input")
         _need(chosen.dim() == 2 and chosen.shape == weights.shape and chosen.shape[0] == x.shape[0], "experts: x [T, dim], chosen and weights [T, top]")
         T, top = chosen.shape
@@ -1644,11 +1649,11 @@ class NativeOps:
         u = torch.empty((pairs, up_rows), dtype=torch.float32, device=x.device)
         status = ctypes.c_void_p(self._status_at)
         _check(gemm.tl_gemm_fp8_experts(_ptr(rows.codes), _ptr(rows.scales), _ptr(w_up.codes), _ptr(w_up.scales), _ptr(u), 1, pairs, up_rows, dim, E,
-                                        _ptr(tiles), most, status, _stream()), "experts' products (up)")
+                                        _ptr(tiles), most, form, status, _stream()), "experts' products (up)")
         hid = self.activation_fp8(u, activation, gated=gated, act_params=act_params)
         y = torch.empty((pairs, dim), dtype=x.dtype, device=x.device)
         _check(gemm.tl_gemm_fp8_experts(_ptr(hid.codes), _ptr(hid.scales), _ptr(w_down.codes), _ptr(w_down.scales), _ptr(y),
-                                        1 if x.dtype == torch.float32 else 0, pairs, dim, hidden, E, _ptr(tiles), most, status, _stream()),
+                                        1 if x.dtype == torch.float32 else 0, pairs, dim, hidden, E, _ptr(tiles), most, form, status, _stream()),
                "experts' products (down)")
         _check(moe.tl_moe_combine(_ptr(y), _DT[x.dtype], _ptr(place), _ptr(weights), _ptr(shared), _DT[shared.dtype] if shared is not None else 0,
                                   splits, ctypes.c_longlong(plane), _ptr(shared_gate), _ptr(out), T, dim, top, _stream()), "moe_combine")

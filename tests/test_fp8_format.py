@@ -61,8 +61,10 @@ def test_widths_that_are_refused(K):
 def bare_ops():
     """The front end without a GPU behind it: what it refuses, it refuses before anything is launched."""
     from torchllms_b200.kernels.native import NativeOps
+    class Nothing:                       # (the C++ front end answers so where something does not fit)
+        rows = norm = product = experts = staticmethod(lambda *args: None)
     ops = object.__new__(NativeOps)
-    ops._profile, ops.launches = None, 0
+    ops._profile, ops.launches, ops._status_at, ops._fp8 = None, 0, 1, Nothing
     return ops
 
 

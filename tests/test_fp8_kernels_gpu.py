@@ -158,7 +158,7 @@ SIZES = [(1, 128, 128), (16, 128, 512), (3, 16, 16), (5, 130, 144), (17, 200, 64
          (128, 256, 2048), (129, 257, 528), (240, 512, 512), (241, 384, 528), (300, 1000, 4112), (3, 512, 2064), (500, 2048, 8192), (2048, 640, 512), (77, 1, 256), (33, 7, 14336)]
 
 
-@pytest.mark.parametrize("impl", ["single", "pair"])
+@pytest.mark.parametrize("impl", ["single", "pair", "split", "auto"])
 @pytest.mark.parametrize("M,N,K", SIZES)
 def test_product(ops, M, N, K, impl):
     x, w = held(uneven(M, K, seed=M)), held(rand((N, K), seed=N + 1, scale=K ** -0.5))

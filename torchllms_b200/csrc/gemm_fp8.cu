@@ -25,17 +25,15 @@ namespace {
 
 constexpr int BM = 128;              // rows of W a CTA
 constexpr int BK = 128;              // bytes of K a box: a swizzle row, and a block of numbers that share a scale
-constexpr int BOXES = 2;             // boxes of W (and of x) a stage: what a stage costs its issuer (a wait, a fence, a commit) is as much as
-                                     // four products of 240 rows take
 constexpr int MAX_WIDTH = 240;       // rows of x a tile: two accumulators and two sets of scales fill 512 columns
+constexpr int MAX_SPLIT_WIDTH = 224; // the same with one accumulator in 256 columns
 constexpr int MAX_STAGES = 12;
-constexpr int SCALE_BUFS = 3;        // turns of scales under way
+constexpr int MAX_SCALE_BUFS = 3;    // turns of scales under way
 constexpr int TURN = 16;             // blocks of 128 of a turn: four words a row
 constexpr int NTHREADS = 256;
 
 constexpr int STAGING = 4 * 2048;    // 32 x 32 results a warp
-constexpr unsigned TMEM_COLS = 512;
-constexpr unsigned SCALE_COL = 240;  // scales of set s at columns 256 s + 240: 4 of W, 8 of x
+constexpr unsigned ACC_COLS = 256;   // a second accumulator lies so many columns behind the first
 constexpr unsigned long long WAIT_LIMIT_NS = 2000ull * 1000ull * 1000ull;   // two seconds, then give up
 
 enum : int { ERR_TMA_WAIT = 601, ERR_MMA_WAIT = 602, ERR_SCALE_WAIT = 603, ERR_EPI_WAIT = 604 };
@@ -92,6 +90,14 @@ __device__ __forceinline__ void arrive_elect(unsigned bar) {
 }
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// 16 bytes of another CTA's shared memory
+__device__ __forceinline__ float4 load_from(unsigned addr, int cta) {
+    unsigned at;
+    float4 v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(addr), "r"(cta));
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+    return v;
 }
 // the address of the pair's first CTA's variable of the same place
 __device__ __forceinline__ unsigned in_leader(unsigned addr) {
@@ -186,13 +192,20 @@ struct Params {
     const int* tiles;                // experts: count, then (expert, first row, rows) of every tile; null: one weight, tiles of `width` rows
     int M, N, k_blocks, pitch;
     int width;                       // rows of x a tile, a multiple of 16
-    int slabs, n_tiles, stages;
+    int slabs, n_tiles, stages, scale_bufs;
     int out_is_f32;
     bool w_whole, x_whole;           // scales: rows are a multiple of 16 bytes and start on 16
+    int splits, split_blocks;        // SPLIT: CTAs of a cluster, and blocks of K of each (a multiple of 4)
+    unsigned tmem_cols, scale_col, set_cols;     // columns of tensor memory; where the first set of scales lies, and how far the second is behind it
 };
 
 // shared memory of a word of scales: 512 bytes for the rows of W and for every 128 rows of x
 __host__ __device__ constexpr int scale_bytes(int width) { return 512 * (1 + (width + 127) / 128); }
+
+enum : int { SINGLE = 1, PAIRS = 2, SPLIT = 3 };
+// Boxes of W (and of x) a stage: what a stage costs its issuer (a wait, a fence, a commit) is as much as four products of 240 rows
+// take.  Split: one, the few blocks of a CTA would be a stage or two otherwise.
+__host__ __device__ constexpr int boxes_of(int form) { return form == SPLIT ? 1 : 2; }
 
 struct Unit { int expert, row0, rows, slab; };
 
@@ -212,25 +225,31 @@ __device__ __forceinline__ Unit unit_of(const Params& p, int u, int n_tiles) {
     return r;
 }
 
-template <bool PAIR>
-__global__ void __launch_bounds__(NTHREADS, 1) gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
+template <int FORM>
+__global__ void __launch_bounds__(NTHREADS, FORM == SPLIT ? 2 : 1) gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                                                                const Params p) {
     extern __shared__ unsigned char smem_raw[];
     const unsigned smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u;            // tiles want 1,024-byte alignment for the swizzle
     unsigned char* const smem_at = smem_raw + (smem0 - smem_u32(smem_raw));
     // a pair shares a unit of 256 rows of W: each CTA has 128 of them and half of the tile's rows of x
+    constexpr bool PAIR = FORM == PAIRS;
+    constexpr int BOXES = boxes_of(FORM);
     constexpr int SIDES = PAIR ? 2 : 1;
     const int rank = PAIR ? (int)(blockIdx.x & 1) : 0;
-    const int first_unit = blockIdx.x / SIDES, step = gridDim.x / SIDES;
+    // split: a cluster to a unit, every CTA with a run of its blocks of K
+    const int cut = FORM == SPLIT ? (int)(blockIdx.x % (unsigned)p.splits) : 0;
+    const int first_unit = FORM == SPLIT ? (int)(blockIdx.x / (unsigned)p.splits) : (int)blockIdx.x / SIDES;
+    const int step = FORM == SPLIT ? p.n_tiles * p.slabs : (int)gridDim.x / SIDES;
+    const int kb0 = cut * p.split_blocks, kb1 = FORM == SPLIT ? min(kb0 + p.split_blocks, p.k_blocks) : p.k_blocks;
     const unsigned w_bytes = BM * BK, x_bytes = p.width / SIDES * BK, stage_bytes = BOXES * (w_bytes + x_bytes);
     const unsigned scales_at = smem0 + p.stages * stage_bytes, word_bytes = scale_bytes(p.width), turn_bytes = 4 * word_bytes;
-    unsigned char* const staging = smem_at + p.stages * stage_bytes + SCALE_BUFS * turn_bytes;
-    __shared__ __align__(8) unsigned long long bars[2 * MAX_STAGES + 2 * SCALE_BUFS + 5];
+    unsigned char* const staging = smem_at + p.stages * stage_bytes + p.scale_bufs * turn_bytes;
+    __shared__ __align__(8) unsigned long long bars[2 * MAX_STAGES + 2 * MAX_SCALE_BUFS + 5];
     __shared__ unsigned tmem_slot;
     __shared__ int abort_flag;
     const unsigned bar0 = smem_u32(bars);
-    const unsigned full = bar0, empty = bar0 + 8 * MAX_STAGES, sc_full = bar0 + 16 * MAX_STAGES, sc_empty = sc_full + 8 * SCALE_BUFS;
-    const unsigned acc_full = sc_empty + 8 * SCALE_BUFS, acc_empty = acc_full + 16, drained = acc_empty + 16;
+    const unsigned full = bar0, empty = bar0 + 8 * MAX_STAGES, sc_full = bar0 + 16 * MAX_STAGES, sc_empty = sc_full + 8 * MAX_SCALE_BUFS;
+    const unsigned acc_full = sc_empty + 8 * MAX_SCALE_BUFS, acc_empty = acc_full + 16, drained = acc_empty + 16;
     // (what the first CTA's issuing warp waits for counts arrivals of both)
     auto leader = [&](unsigned bar) { return PAIR ? in_leader(bar) : bar; };
 
@@ -238,17 +257,17 @@ __global__ void __launch_bounds__(NTHREADS, 1) gemm_fp8_kernel(const __grid_cons
     if (threadIdx.x == 0) {
         abort_flag = 0;
         for (int s = 0; s < MAX_STAGES; ++s) { mbar_init(full + 8 * s, 1); mbar_init(empty + 8 * s, 1); }
-        for (int s = 0; s < SCALE_BUFS; ++s) { mbar_init(sc_full + 8 * s, SIDES); mbar_init(sc_empty + 8 * s, 1); }
+        for (int s = 0; s < MAX_SCALE_BUFS; ++s) { mbar_init(sc_full + 8 * s, SIDES); mbar_init(sc_empty + 8 * s, 1); }
         for (int s = 0; s < 2; ++s) { mbar_init(acc_full + 8 * s, 1); mbar_init(acc_empty + 8 * s, 4 * SIDES); }
         mbar_init(drained, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
         if (PAIR) {
-            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(TMEM_COLS) : "memory");
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(p.tmem_cols) : "memory");
             asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
         } else {
-            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(TMEM_COLS) : "memory");
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(p.tmem_cols) : "memory");
             asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
         }
     }
@@ -259,32 +278,48 @@ __global__ void __launch_bounds__(NTHREADS, 1) gemm_fp8_kernel(const __grid_cons
     const unsigned tmem = tmem_slot;
     volatile int* aborted = &abort_flag;
     grid_launch_dependents();
-    grid_dependency_wait();
+    // W and its scales depend on no earlier kernel: the first boxes of a product without a list of tiles are asked for ahead
+    const bool ahead = p.tiles == nullptr;
+    if (!(ahead && (warp == 0 || warp == 2 || warp == 3))) grid_dependency_wait();
 
     const int n_tiles = p.tiles != nullptr ? p.tiles[0] : p.n_tiles;
     const int units = n_tiles * p.slabs;
 
     if (warp == 0) {
         if (elect_one()) {
-            int stage = 0, issued = 0;
+            int stage = 0, issued = 0, early = 0;
             unsigned phase = 1;                // (a barrier that has completed nothing counts as having completed phase 1)
             bool ok = true;
+            if (ahead) {
+                if (first_unit < units) {
+                    const int w_row = (first_unit / n_tiles * SIDES + rank) * BM;
+                    for (int kb = kb0; kb < kb1 && early < p.stages; kb += BOXES, ++early) {
+                        const unsigned at = smem0 + early * stage_bytes, bar = leader(full + 8 * early);
+                        const int boxes = min(BOXES, kb1 - kb);
+                        if (rank == 0) expect_tx(full + 8 * early, SIDES * boxes * (w_bytes + x_bytes));
+                        for (int i = 0; i < boxes; ++i) tma_load<PAIR>(at + i * w_bytes, &map_w, bar, (kb + i) * BK, w_row);
+                    }
+                }
+                grid_dependency_wait();
+            }
             for (int u = first_unit; u < units && ok; u += step) {
                 const Unit t = unit_of(p, u, n_tiles);
                 const int w_row = t.expert * p.N + (t.slab * SIDES + rank) * BM, x_row = t.row0 + rank * (((t.rows + 15) & ~15) / 2);
-                for (int kb = 0; kb < p.k_blocks; kb += BOXES) {
+                for (int kb = kb0; kb < kb1; kb += BOXES) {
                     if (!wait_one(empty + 8 * stage, phase, aborted)) {
                         give_up(aborted, p.status, ERR_TMA_WAIT);
                         ok = false;
                         break;
                     }
                     const unsigned at = smem0 + stage * stage_bytes, bar = leader(full + 8 * stage);
-                    const int boxes = min(BOXES, p.k_blocks - kb);
-                    if (rank == 0) expect_tx(full + 8 * stage, SIDES * boxes * (w_bytes + x_bytes));
+                    const int boxes = min(BOXES, kb1 - kb);
+                    const bool fresh = early == 0;             // (else W's boxes are under way already)
+                    if (!fresh) --early;
+                    if (fresh && rank == 0) expect_tx(full + 8 * stage, SIDES * boxes * (w_bytes + x_bytes));
 #pragma unroll
                     for (int i = 0; i < BOXES; ++i) {
                         if (i < boxes) {
-                            tma_load<PAIR>(at + i * w_bytes, &map_w, bar, (kb + i) * BK, w_row);
+                            if (fresh) tma_load<PAIR>(at + i * w_bytes, &map_w, bar, (kb + i) * BK, w_row);
                             tma_load<PAIR>(at + BOXES * w_bytes + i * x_bytes, &map_x, bar, (kb + i) * BK, x_row);
                         }
                     }
@@ -309,14 +344,14 @@ __global__ void __launch_bounds__(NTHREADS, 1) gemm_fp8_kernel(const __grid_cons
             for (int u = first_unit; u < units && ok; u += step, ++n) {
                 const Unit t = unit_of(p, u, n_tiles);
                 const int acc = n & 1, N = (t.rows + 15) & ~15;
-                const unsigned d = tmem + acc * 256;
+                const unsigned d = tmem + acc * ACC_COLS;
                 if (!wait_one(acc_empty + 8 * acc, ((n >> 1) & 1) ^ 1, aborted)) {
                     give_up(aborted, p.status, ERR_MMA_WAIT);
                     break;
                 }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                for (int kb = 0; kb < p.k_blocks; kb += BOXES) {
-                    if (kb % TURN == 0 && !wait_one(sc_full + 8 * buf, sc_phase, aborted)) {
+                for (int kb = kb0; kb < kb1; kb += BOXES) {
+                    if ((kb - kb0) % TURN == 0 && !wait_one(sc_full + 8 * buf, sc_phase, aborted)) {
                         give_up(aborted, p.status, ERR_MMA_WAIT);
                         ok = false;
                         break;
@@ -324,12 +359,12 @@ __global__ void __launch_bounds__(NTHREADS, 1) gemm_fp8_kernel(const __grid_cons
                     if (kb % 4 == 0) {
                         // (two sets in turn: copies and products are carried out in the order of their issue)
                         word ^= 1;
-                        const unsigned at = scales_at + buf * turn_bytes + kb / 4 % 4 * word_bytes, to = tmem + word * 256 + SCALE_COL;
+                        const unsigned at = scales_at + buf * turn_bytes + (kb - kb0) / 4 % 4 * word_bytes, to = tmem + p.scale_col + word * p.set_cols;
                         copy_scales<PAIR>(to, scale_desc(at));
                         copy_scales<PAIR>(to + 4, scale_desc(at + 512));
                         if (N > 128) copy_scales<PAIR>(to + 8, scale_desc(at + 1024));
                     }
-                    const unsigned set = tmem + word * 256 + SCALE_COL;
+                    const unsigned set = tmem + p.scale_col + word * p.set_cols;
                     if (!wait_one(full + 8 * stage, phase, aborted)) {
                         give_up(aborted, p.status, ERR_MMA_WAIT);
                         ok = false;
@@ -339,18 +374,18 @@ __global__ void __launch_bounds__(NTHREADS, 1) gemm_fp8_kernel(const __grid_cons
                     const unsigned at = smem0 + stage * stage_bytes;
 #pragma unroll
                     for (int i = 0; i < BOXES; ++i) {
-                        if (kb + i < p.k_blocks) {
+                        if (kb + i < kb1) {
                             const unsigned idesc = instruction(SIDES * BM, N, (kb + i) & 3);
                             const unsigned long long a = operand_desc(at + i * w_bytes), b = operand_desc(at + BOXES * w_bytes + i * x_bytes);
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) mma<PAIR>(d, a + 2 * k, b + 2 * k, idesc, set, set + 4, (kb > 0 || i > 0 || k > 0) ? 1u : 0u);
+                            for (int k = 0; k < 4; ++k) mma<PAIR>(d, a + 2 * k, b + 2 * k, idesc, set, set + 4, (kb > kb0 || i > 0 || k > 0) ? 1u : 0u);
                         }
                     }
                     commit<PAIR>(empty + 8 * stage);
                     if (++stage == p.stages) { stage = 0; phase ^= 1; }
-                    if (kb % TURN == TURN - BOXES || kb + BOXES >= p.k_blocks) {
+                    if ((kb - kb0) % TURN == TURN - BOXES || kb + BOXES >= kb1) {
                         commit<PAIR>(sc_empty + 8 * buf);
-                        if (++buf == SCALE_BUFS) { buf = 0; sc_phase ^= 1; }
+                        if (++buf == p.scale_bufs) { buf = 0; sc_phase ^= 1; }
                     }
                 }
                 if (ok) commit<PAIR>(acc_full + 8 * acc);
@@ -364,11 +399,11 @@ __global__ void __launch_bounds__(NTHREADS, 1) gemm_fp8_kernel(const __grid_cons
     } else if (warp == 2 || warp == 3) {
         int turn = 0, buf = 0;
         unsigned phase = 1;
-        bool ok = true;
+        bool ok = true, waited = false;
         for (int u = first_unit; u < units && ok; u += step) {
             const Unit t = unit_of(p, u, n_tiles);
             const long long first = (long long)t.expert * p.N;
-            for (int kb = 0; kb < p.k_blocks; kb += TURN, ++turn) {
+            for (int kb = kb0; kb < kb1; kb += TURN, ++turn) {
                 if ((turn & 1) == warp - 2) {
                     if (!mbar_wait(sc_empty + 8 * buf, phase, aborted)) {
                         if (lane == 0) give_up(aborted, p.status, ERR_SCALE_WAIT);
@@ -376,14 +411,20 @@ __global__ void __launch_bounds__(NTHREADS, 1) gemm_fp8_kernel(const __grid_cons
                         break;
                     }
                     const unsigned at = scales_at + buf * turn_bytes + 16 * lane;
-                    const int words = min(4, (p.k_blocks - kb + 3) / 4);
+                    const int words = min(4, (kb1 - kb + 3) / 4);
+                    const bool whole = kb % TURN == 0;
                     unsigned v[12][4];
 #pragma unroll
-                    for (int j = 0; j < 12; ++j) {
-                        const int r = j < 4 ? (t.slab * SIDES + rank) * BM + 32 * j + lane : 32 * (j - 4) + lane;
-                        const bool there = j < 4 ? r < p.N : r < t.rows;
-                        const unsigned char* row = j < 4 ? p.w_scales + (first + r) * p.pitch : p.x_scales + (long long)(t.row0 + r) * p.pitch;
-                        load_words(there ? row + kb : nullptr, words, j < 4 ? p.w_whole : p.x_whole, v[j]);
+                    for (int j = 0; j < 4; ++j) {
+                        const int r = (t.slab * SIDES + rank) * BM + 32 * j + lane;
+                        load_words(r < p.N ? p.w_scales + (first + r) * p.pitch + kb : nullptr, words, whole && p.w_whole, v[j]);
+                    }
+                    if (ahead && !waited) grid_dependency_wait();
+                    waited = true;
+#pragma unroll
+                    for (int j = 4; j < 12; ++j) {
+                        const int r = 32 * (j - 4) + lane;
+                        load_words(r < t.rows ? p.x_scales + (long long)(t.row0 + r) * p.pitch + kb : nullptr, words, whole && p.x_whole, v[j]);
                     }
 #pragma unroll
                     for (int j = 0; j < 12; ++j) {
@@ -397,7 +438,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) gemm_fp8_kernel(const __grid_cons
                     __syncwarp();
                     arrive_elect<PAIR>(leader(sc_full + 8 * buf));
                 }
-                if (++buf == SCALE_BUFS) { buf = 0; phase ^= 1; }
+                if (++buf == p.scale_bufs) { buf = 0; phase ^= 1; }
             }
         }
     } else if (warp >= 4) {
@@ -417,9 +458,14 @@ __global__ void __launch_bounds__(NTHREADS, 1) gemm_fp8_kernel(const __grid_cons
             for (int c0 = 0; c0 < t.rows; c0 += 32) {
                 unsigned r[32];
                 // (a load of 32 columns may reach into the scales' columns behind the accumulator: read, not used)
-                tmem_load32(tmem + acc * 256 + ((unsigned)(quarter * 32) << 16) + c0, r);
+                tmem_load32(tmem + acc * ACC_COLS + ((unsigned)(quarter * 32) << 16) + c0, r);
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                if (wide) {
+                if (FORM == SPLIT) {
+                    // (every product of the CTA has been taken: the stages are free)
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        if (c0 + j < t.rows) reinterpret_cast<float*>(smem_at)[(c0 + j) * BM + quarter * 32 + lane] = __uint_as_float(r[j]);
+                } else if (wide) {
                     __syncwarp();
 #pragma unroll
                     for (int j = 0; j < 32; ++j)
@@ -450,6 +496,41 @@ __global__ void __launch_bounds__(NTHREADS, 1) gemm_fp8_kernel(const __grid_cons
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    if (FORM == SPLIT) {
+        // every CTA adds up, in the order of K, the rows cut, cut + splits, .. of x's tile: 32 threads a row, four rows of W a thread
+        cluster_sync();
+        const Unit t = unit_of(p, first_unit, n_tiles);
+        const unsigned sums = smem0 + (threadIdx.x & 31) * 16;
+        const int row = t.slab * BM + (threadIdx.x & 31) * 4;
+        for (int c = cut + (threadIdx.x >> 5) * p.splits; c < t.rows && !*aborted; c += (NTHREADS >> 5) * p.splits) {
+            float4 v[8];
+#pragma unroll
+            for (int s = 0; s < 8; ++s)
+                if (s < p.splits) v[s] = load_from(sums + c * (BM * 4), s);
+            float4 a = v[0];
+#pragma unroll
+            for (int s = 1; s < 8; ++s)
+                if (s < p.splits) { a.x += v[s].x; a.y += v[s].y; a.z += v[s].z; a.w += v[s].w; }
+            const size_t at = (size_t)(t.row0 + c) * p.N + row;
+            const float q[4] = {a.x, a.y, a.z, a.w};
+            if (p.N % 4 == 0 && row < p.N) {
+                if (p.out_is_f32) {
+                    *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + at) = a;
+                } else {
+                    const __nv_bfloat162 lo = __floats2bfloat162_rn(a.x, a.y), hi = __floats2bfloat162_rn(a.z, a.w);
+                    *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(p.out) + at) = make_uint2(reinterpret_cast<const unsigned&>(lo), reinterpret_cast<const unsigned&>(hi));
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (row + i >= p.N) break;
+                    if (p.out_is_f32) reinterpret_cast<float*>(p.out)[at + i] = q[i];
+                    else reinterpret_cast<__nv_bfloat16*>(p.out)[at + i] = __float2bfloat16_rn(q[i]);
+                }
+            }
+        }
+        cluster_sync();                // nobody reads this CTA's sums any more
+    }
     if (PAIR && rank == 1 && warp == 1) {
         // the second CTA issues nothing, but commits arrive at its barriers too, the last of them perhaps later than at the
         // first CTA's: it must not end before they have
@@ -461,8 +542,8 @@ __global__ void __launch_bounds__(NTHREADS, 1) gemm_fp8_kernel(const __grid_cons
     if (warp == 1) {
         __syncwarp();
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
-        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+        if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.tmem_cols) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.tmem_cols) : "memory");
     }
     if (PAIR) {                        // the pair gives its tensor memory back together, and ends together
         __syncthreads();
@@ -498,41 +579,76 @@ int make_map(CUtensorMap* map, const void* base, long long rows, long long K, in
               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? TL_OK : TL_BAD_SIZE;
 }
 
+constexpr int MAX_DEVICES = 64;
+int current_device() {
+    int dev = 0;
+    return cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < MAX_DEVICES ? dev : 0;
+}
+// (asked once a device; two threads that ask at once write the same number)
 int sm_count() {
-    int dev = 0, n = 148;
-    if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-    return n;
+    static int count[MAX_DEVICES];
+    const int dev = current_device();
+    if (count[dev] == 0) {
+        int n = 0;
+        count[dev] = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && n > 1 ? n : 148;
+    }
+    return count[dev];
 }
 
 // rows of x a tile: even shares of at most MAX_WIDTH
-int even_width(int M) {
-    const int tiles = (M + MAX_WIDTH - 1) / MAX_WIDTH;
+int even_width(int M, int most) {
+    const int tiles = (M + most - 1) / most;
     return ((M + tiles - 1) / tiles + 15) / 16 * 16;
 }
 
-template <bool PAIR>
+int whole_columns(int n) {
+    int c = 32;
+    while (c < n) c *= 2;
+    return c;
+}
+
+template <int FORM>
 int launch(Params& p, const void* x, const void* w, int experts, int K, cudaStream_t s) {
-    constexpr int SIDES = PAIR ? 2 : 1;
+    constexpr int SIDES = FORM == PAIRS ? 2 : 1;
     p.slabs = (p.N + SIDES * BM - 1) / (SIDES * BM);
-    if ((long long)p.slabs * p.n_tiles > 0x7fffffffll) return TL_BAD_SIZE;
-    const int stage_bytes = BOXES * (BM * BK + p.width / SIDES * BK);
-    const int most = 227 * 1024 - 1024 - 1024 - SCALE_BUFS * 4 * scale_bytes(p.width) - STAGING;       // (a kilobyte for barriers, one to align)
-    p.stages = most / stage_bytes;
+    if ((long long)p.slabs * p.n_tiles * 8 > 0x7fffffffll) return TL_BAD_SIZE;
+    const int units = p.slabs * p.n_tiles, sms = sm_count();
+    const int stage_bytes = boxes_of(FORM) * (BM * BK + p.width / SIDES * BK);
+    p.scale_bufs = FORM == SPLIT ? (p.split_blocks + TURN - 1) / TURN : MAX_SCALE_BUFS;
+    if (p.scale_bufs > MAX_SCALE_BUFS) p.scale_bufs = MAX_SCALE_BUFS;
+    const int fixed = 1024 + p.scale_bufs * 4 * scale_bytes(p.width) + (FORM == SPLIT ? 0 : STAGING);     // (1,024 to align)
+    int room = 226 * 1024;                          // (a kilobyte is left for barriers)
+    if (FORM == SPLIT) {
+        // one accumulator, one unit: narrow tiles leave room for a second CTA on an SM
+        const int sets = p.width <= 128 ? 8 : 12;
+        p.scale_col = p.width;
+        p.set_cols = sets;
+        p.tmem_cols = whole_columns(p.width + 2 * sets);
+        if (units * p.splits > sms && p.tmem_cols <= 256) room = 112 * 1024;
+    } else {
+        p.scale_col = MAX_WIDTH;
+        p.set_cols = ACC_COLS;
+        p.tmem_cols = 2 * ACC_COLS;
+    }
+    p.stages = (room - fixed) / stage_bytes;
     if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
+    if (p.stages < 1 || (FORM == SPLIT && p.stages * stage_bytes < p.width * BM * 4)) return TL_TOO_LARGE;
     CUtensorMap mw, mx;
     int rc = make_map(&mw, w, (long long)experts * p.N, K, BM);
     if (rc != TL_OK) return rc;
     rc = make_map(&mx, x, p.M, K, p.width / SIDES);
     if (rc != TL_OK) return rc;
-    const size_t smem = 1024 + (size_t)p.stages * stage_bytes + SCALE_BUFS * 4 * scale_bytes(p.width) + STAGING;
-    auto kern = gemm_fp8_kernel<PAIR>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024);
-    if (e != cudaSuccess) return (int)e;
-    const int units = p.slabs * p.n_tiles, most_units = sm_count() / SIDES;
-    const dim3 grid(SIDES * (units < most_units ? units : most_units));
-    if (!PAIR) return (int)tl_launch(kern, grid, dim3(NTHREADS), smem, s, mw, mx, p);
+    const size_t smem = fixed + (size_t)p.stages * stage_bytes;
+    auto kern = gemm_fp8_kernel<FORM>;
+    static bool raised[MAX_DEVICES];
+    const int dev = current_device();
+    if (!raised[dev]) {
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024);
+        if (e != cudaSuccess) return (int)e;
+        raised[dev] = true;
+    }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
+    cfg.gridDim = dim3(FORM == SPLIT ? units * p.splits : SIDES * (units < sms / SIDES ? units : sms / SIDES));
     cfg.blockDim = dim3(NTHREADS);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
@@ -540,12 +656,25 @@ int launch(Params& p, const void* x, const void* w, int experts, int K, cudaStre
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = SIDES;
+    attr[1].val.clusterDim.x = FORM == SPLIT ? p.splits : SIDES;
     attr[1].val.clusterDim.y = 1;
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 2;
+    cfg.numAttrs = FORM == SINGLE ? 1 : 2;
     return (int)cudaLaunchKernelEx(&cfg, kern, mw, mx, p);
+}
+
+// splits of K for `units` units: as many as find room at once (two CTAs an SM where tiles are narrow), no more than a cluster
+// holds, each with at least four blocks
+int splits_for(int units, int k_blocks, int width, int sms) {
+    const int slots = width <= 64 ? 2 * sms : sms;
+    int splits = units > 0 ? slots / units : 1;
+    if (splits > 8) splits = 8;
+    const int words = (k_blocks + 3) / 4;
+    if (splits > words) splits = words;
+    if (splits < 1) splits = 1;
+    const int per = (words + splits - 1) / splits;
+    return (words + per - 1) / per;                 // no empty split
 }
 
 int launch(const void* x, const void* x_scales, const void* w, const void* w_scales, void* out, int out_is_f32, int M, int N, int K, int experts,
@@ -562,11 +691,19 @@ int launch(const void* x, const void* x_scales, const void* w, const void* w_sca
     p.M = M; p.N = N; p.k_blocks = (K + BK - 1) / BK; p.pitch = fp8_scale_pitch(K);
     p.width = width;
     p.n_tiles = most_tiles;
-    if (form < 0 || form > 2) return TL_BAD_SIZE;
+    p.splits = 1;
+    p.split_blocks = p.k_blocks;
+    if (form < 0 || form > 3 || (form == SPLIT && (tiles != nullptr || width > MAX_SPLIT_WIDTH))) return TL_BAD_SIZE;
     // Pairs halve what a tile of x costs in copies, and that is what wide tiles wait for (2,048 rows of 28,672 x 4,096: 222 us
     // alone, 186 in pairs); narrow ones stream W, which nobody shares (8 rows: 22.3 and 22.4)
-    const bool pair = form == 0 ? width > 64 : form == 2;
-    return pair ? launch<true>(p, x, w, experts, K, s) : launch<false>(p, x, w, experts, K, s);
+    if (form == 0) form = width > 64 ? PAIRS : SINGLE;
+    if (form == SPLIT) {
+        p.splits = splits_for(((N + BM - 1) / BM) * most_tiles, p.k_blocks, width, sm_count());
+        const int words = (p.k_blocks + 3) / 4;
+        p.split_blocks = 4 * ((words + p.splits - 1) / p.splits);
+        return launch<SPLIT>(p, x, w, experts, K, s);
+    }
+    return form == PAIRS ? launch<PAIRS>(p, x, w, experts, K, s) : launch<SINGLE>(p, x, w, experts, K, s);
 }
 
 }  // namespace
@@ -576,7 +713,11 @@ int launch(const void* x, const void* x_scales, const void* w, const void* w_sca
 extern "C" int tl_gemm_fp8(const void* x, const void* x_scales, const void* w, const void* w_scales, void* out, int out_is_f32, int M, int N, int K,
                            int form, int* status, void* stream) {
     if (M <= 0) return TL_OK;
-    const int width = even_width(M);
+    int width = even_width(M, MAX_WIDTH);
+    // Few units leave SMs idle: their K is cut among the CTAs of a cluster.
+    const int narrow = even_width(M, MAX_SPLIT_WIDTH), units = ((N + BM - 1) / BM) * ((M + narrow - 1) / narrow);
+    if (form == 0 && 2 * units <= sm_count() && K > 4 * BK) form = SPLIT;
+    if (form == SPLIT) width = narrow;
     return launch(x, x_scales, w, w_scales, out, out_is_f32, M, N, K, 1, nullptr, (M + width - 1) / width, width, form, status, (cudaStream_t)stream);
 }
 

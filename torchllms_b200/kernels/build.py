@@ -45,12 +45,12 @@ NVCC_FLAGS += os.environ.get("TORCHLLMS_B200_NVCC_FLAGS", "").split()
 EXTRA_LINK: Dict[str, List[str]] = {}
 
 ALL_LIBRARIES = ("elementwise", "sublayer", "rope", "attention", "attention_mma", "attention_decode", "attention_prefill", "gemm_simt", "gemm_f32", "gemm_tcgen05", "sampling", "recurrent", "moe", "matrix_state", "stream_sum", "selective_scan", "conv_mixers", "matrix_recurrence",
-                 "rows_fp8", "gemm_fp8", "kv_fp4", "attention_fp4", "attention_fp4_decode", "attention_fp4_prefill", "fp4_calls")
+                 "rows_fp8", "gemm_fp8", "kv_fp4", "attention_fp4", "attention_fp4_decode", "attention_fp4_prefill", "fp4_calls", "fp8_calls")
 
 
 # Python modules (``csrc/<name>.cpp``, compiled with the host compiler against this Python's and this torch's headers): front ends of
 # operators whose calls cost more than their kernels
-EXTENSIONS = ("fp4_calls",)
+EXTENSIONS = ("fp4_calls", "fp8_calls")
 
 
 class KernelBuildError(RuntimeError):

@@ -134,6 +134,7 @@ class NativeOps:
         # (device, stream, inside a capture) -> ints that are zero between launches, and the capture they belong to
         self._counts: Dict[Tuple[int, int, bool], Tuple[int, torch.Tensor]] = {}
         self._fp4 = None           # the front end of the 4-bit cache's operators, once it is loaded
+        self._fp8 = None           # the same for the 8-bit rows'
         self.use_tcgen05 = True
         # SwiGLU in the epilogue of the gate/up product (TORCHLLMS_B200_NO_GATED=1 keeps the two kernels, for comparisons)
         self.use_gated = os.environ.get("TORCHLLMS_B200_NO_GATED", "") not in ("1", "true")
@@ -1485,6 +1486,17 @@ class NativeOps:
         return out
 
     # ------------------------------------------------------------- rows and weights in 8 bits
+    # The front end of what a step of few tokens calls is csrc/fp8_calls.cpp.  It returns None for arguments that do not fit, and for calls
+    # with no rows: the methods named _explained say what is wrong, or return what there is.
+    _FP8_FORMS = {"auto": 0, "single": 1, "pair": 2, "split": 3}
+
+    def _fp8_load(self):
+        calls = load_extension("fp8_calls")
+        names = (("rows_fp8", "tl_fp8_rows"), ("rows_fp8", "tl_fp8_norm"), ("gemm_fp8", "tl_gemm_fp8"))
+        calls.bind(*(ctypes.cast(getattr(self._lib(lib), name), ctypes.c_void_p).value for lib, name in names))
+        self._fp8 = calls
+        return calls
+
     @staticmethod
     def _fp8_empty(rows: int, width: int, device) -> Fp8Rows:
         return Fp8Rows(torch.empty((rows, width), dtype=FP8_CODES, device=device),
@@ -1514,90 +1526,108 @@ class NativeOps:
         _need(x.data_ptr() % 16 == 0, f"{name} must start on 16 bytes")
         return x.shape[1] // parts
 
-    @_timed
+    def _fp8_rows_explained(self, x: torch.Tensor, name: str, parts: int = 1) -> Fp8Rows:
+        K = self._fp8_width(x, name, parts)
+        self._fp8_here(x)
+        _need(x.shape[0] == 0, f"{name}: {x.shape[0]} rows of {K} numbers do not fit")
+        return self._fp8_empty(0, K, x.device)
+
+    @_timed_when_asked
     def quantize_fp8(self, x: torch.Tensor) -> Fp8Rows:
         """The rows of ``x`` (``[T, K]`` float32/bfloat16, ``K % 16 == 0``) in 8 bits: E4M3 numbers and a scale of a power of two for
         every 128 of them (:mod:`torchllms_b200.weights.fp8` has the format; what is not finite becomes NaN)."""
-        K = self._fp8_width(x, "quantize_fp8: x")
-        self._fp8_here(x)
-        out = self._fp8_empty(x.shape[0], K, x.device)
-        rc = self._lib("rows_fp8").tl_fp8_rows(_ptr(x), _DT[x.dtype], _ptr(out.codes), _ptr(out.scales), x.shape[0], K, 0, 0, ctypes.c_float(0.0),
-                                              ctypes.c_float(0.0), ctypes.c_float(0.0), _stream())
-        _check(rc, "quantize_fp8")
-        self.launches += x.shape[0] > 0
-        return out
+        rows = (self._fp8 or self._fp8_load()).rows(x, 0, 0, 0.0, 0.0, 0.0)
+        if type(rows) is tuple:
+            self.launches += 1
+            return Fp8Rows(*rows)
+        if rows is None:
+            return self._fp8_rows_explained(x, "quantize_fp8: x")
+        _check(rows, "quantize_fp8")
 
-    @_timed
+    @_timed_when_asked
     def activation_fp8(self, u: torch.Tensor, activation: str, *, gated: bool = False, act_params=None) -> Fp8Rows:
         """``act(u)``, or with ``gated`` ``act(g) * v`` of the halves ``[g | v]`` of ``u``'s rows, in 8 bits (as :meth:`quantize_fp8`); the
         activation is taken in float32 and rounded once.  Activations and ``act_params`` as in :meth:`moe_experts`."""
-        _need(activation in self._ACTS, f"unknown activation {activation!r}; known: {', '.join(self._ACTS)}")
-        clamped = activation == "clamped_swish"
-        _need(not clamped or (gated and act_params is not None and len(act_params) == 3 and act_params[0] > 0),
-              "the clamped activation is a gated one and goes with (limit, alpha, up_offset), the limit positive")
-        K = self._fp8_width(u, "activation_fp8: u", 2 if gated else 1)
-        self._fp8_here(u)
-        limit, alpha, offset = act_params if clamped else (0.0, 0.0, 0.0)
-        out = self._fp8_empty(u.shape[0], K, u.device)
-        rc = self._lib("rows_fp8").tl_fp8_rows(_ptr(u), _DT[u.dtype], _ptr(out.codes), _ptr(out.scales), u.shape[0], K, 2 if gated else 1,
-                                              self._ACTS[activation], ctypes.c_float(limit), ctypes.c_float(alpha), ctypes.c_float(offset), _stream())
-        _check(rc, "activation_fp8")
-        self.launches += u.shape[0] > 0
-        return out
+        code = self._ACTS.get(activation)
+        _need(code is not None, f"unknown activation {activation!r}; known: {', '.join(self._ACTS)}")
+        limit = alpha = offset = 0.0
+        if activation == "clamped_swish":
+            _need(gated and act_params is not None and len(act_params) == 3 and act_params[0] > 0,
+                  "the clamped activation is a gated one and goes with (limit, alpha, up_offset), the limit positive")
+            limit, alpha, offset = act_params
+        rows = (self._fp8 or self._fp8_load()).rows(u, 2 if gated else 1, code, limit, alpha, offset)
+        if type(rows) is tuple:
+            self.launches += 1
+            return Fp8Rows(*rows)
+        if rows is None:
+            return self._fp8_rows_explained(u, "activation_fp8: u", 2 if gated else 1)
+        _check(rows, "activation_fp8")
 
-    @_timed
+    @_timed_when_asked
     def rmsnorm_fp8(self, h: torch.Tensor, delta, weight: torch.Tensor, eps: float) -> Fp8Rows:
         """:meth:`rmsnorm` whose rows leave in 8 bits: ``h += delta`` in place (float32), then the rows of
         ``h / sqrt(mean(h^2) + eps) * weight``, taken in float32 and rounded once.  ``delta``: ``[T, dim]`` float32/bfloat16, float32 partial
         sums ``[splits, T, dim]``, a :class:`PendingProduct`, or ``None``."""
         if isinstance(delta, PendingProduct):
             delta = delta.take(self)
+        rows = (self._fp8 or self._fp8_load()).norm(h, delta, weight, eps)
+        if type(rows) is tuple:
+            self.launches += 1
+            return Fp8Rows(*rows)
+        if rows is None:
+            return self._rmsnorm_fp8_explained(h, delta, weight)
+        _check(rows, "rmsnorm_fp8")
+
+    def _rmsnorm_fp8_explained(self, h, delta, weight) -> Fp8Rows:
         _cuda_contig(h, "residual stream", torch.float32)
         K = self._fp8_width(h, "residual stream")
         _cuda_contig(weight, "norm weight", torch.float32)
-        _need(weight.numel() == K, "norm weight must match the stream's width")
+        _need(weight.numel() == K and weight.data_ptr() % 16 == 0, "norm weight must match the stream's width and start on 16 bytes")
         _need(K <= FP8_MAX_NORM_WIDTH, f"rmsnorm_fp8 keeps a row in registers: width {K} exceeds {FP8_MAX_NORM_WIDTH}")
-        splits, plane = 1, 0
         if delta is not None:
             _cuda_contig(delta, "delta")
-            _need(delta.dtype in _DT, "delta must be float32 or bfloat16")
+            _need(delta.dtype in _DT and delta.data_ptr() % 16 == 0, "delta must be float32 or bfloat16 and start on 16 bytes")
             if delta.dim() == 3:
                 _need(delta.shape[1:] == h.shape and delta.dtype == torch.float32 and delta.shape[0] >= 1,
                       "partial sums must be float32 [splits, tokens, width]")
-                splits, plane = delta.shape[0], delta.stride(0)
             else:
                 _need(delta.shape == h.shape, "delta must have the stream's shape")
         self._fp8_here(h, delta, weight)
-        out = self._fp8_empty(h.shape[0], K, h.device)
-        rc = self._lib("rows_fp8").tl_fp8_norm(_ptr(h), _ptr(delta), 0 if delta is None else _DT[delta.dtype], splits, ctypes.c_longlong(plane),
-                                              _ptr(weight), _ptr(out.codes), _ptr(out.scales), h.shape[0], K, ctypes.c_float(eps), _stream())
-        _check(rc, "rmsnorm_fp8")
-        self.launches += h.shape[0] > 0
-        return out
+        return self._fp8_rows_explained(h, "rmsnorm_fp8: stream, delta, weight and eps")
 
-    _FP8_FORMS = {"auto": 0, "single": 1, "pair": 2}
-
-    @_timed
+    @_timed_when_asked
     def linear_fp8(self, x, w: Fp8Rows, out_dtype: torch.dtype = torch.bfloat16, impl: str = "auto") -> torch.Tensor:
         """``x [M, K] @ w[N, K]^T`` of 8-bit rows, summed in float32.  ``x`` may be float32/bfloat16 rows, which are brought to 8 bits
         first (:meth:`quantize_fp8`).  The result is bfloat16 or float32 ``[M, N]``.  ``impl`` forces a form of the kernel (tests)."""
-        if not isinstance(x, Fp8Rows):
-            x = self.quantize_fp8(x)
-        self._fp8_need(x, "linear_fp8: x")
+        type_code, form = _DT.get(out_dtype), self._FP8_FORMS.get(impl)
+        if type_code is not None and form is not None and type(w) is Fp8Rows:
+            calls = self._fp8 or self._fp8_load()
+            if type(x) is Fp8Rows:
+                out = calls.product(x.codes, x.scales, w.codes, w.scales, type_code, form, self._status_at)
+                launches = 1
+            else:
+                out = calls.product(x, None, w.codes, w.scales, type_code, form, self._status_at)
+                launches = 2
+            if isinstance(out, torch.Tensor):
+                self.launches += launches
+                return out
+            if out is not None:
+                _check(out, "linear_fp8")
+        return self._linear_fp8_explained(x, w, out_dtype, impl)
+
+    def _linear_fp8_explained(self, x, w, out_dtype, impl) -> torch.Tensor:
         self._fp8_need(w, "linear_fp8: w")
-        (M, K), N = x.codes.shape, w.codes.shape[0]
-        _need(w.codes.shape[1] == K, f"linear_fp8: inner sizes differ ({K} and {w.codes.shape[1]})")
+        if isinstance(x, Fp8Rows):
+            self._fp8_need(x, "linear_fp8: x")
+            x = x.codes
+        else:
+            self._fp8_width(x, "linear_fp8: x")
+        _need(w.shape[1] == x.shape[1], f"linear_fp8: inner sizes differ ({x.shape[1]} and {w.shape[1]})")
         _need(out_dtype in _DT, f"linear_fp8: output dtype {out_dtype} unsupported")
         _need(impl in self._FP8_FORMS, f"linear_fp8: impl must be one of {', '.join(self._FP8_FORMS)}, got {impl!r}")
-        self._fp8_here(x.codes, w.codes)
-        out = torch.empty((M, N), dtype=out_dtype, device=x.codes.device)
-        if M == 0 or N == 0:
-            return out
-        rc = self._lib("gemm_fp8").tl_gemm_fp8(_ptr(x.codes), _ptr(x.scales), _ptr(w.codes), _ptr(w.scales), _ptr(out),
-                                              1 if out_dtype == torch.float32 else 0, M, N, K, self._FP8_FORMS[impl], ctypes.c_void_p(self._status_at), _stream())
-        _check(rc, "linear_fp8")
-        self.launches += 1
-        return out
+        self._fp8_here(x, w.codes)
+        _need(x.shape[0] == 0 or w.shape[0] == 0, "linear_fp8: rows must start on 16 bytes and their scales on 4")
+        return torch.empty((x.shape[0], w.shape[0]), dtype=out_dtype, device=x.device)
 
     @_timed
     def moe_experts_fp8(self, x: torch.Tensor, chosen: torch.Tensor, weights: torch.Tensor, w_up: Fp8Rows, w_down: Fp8Rows, *, activation: str,

@@ -41,7 +41,7 @@ def check_width(width: int, what: str = "8-bit rows") -> None:
         raise ValueError(f"{what} take a multiple of {ALIGN} numbers a row, got {width}")
 
 
-@dataclass(frozen=True)
+@dataclass(slots=True)
 class Fp8Rows:
     """``codes`` ``[..., rows, K]`` (float8_e4m3fn) and ``scales`` ``[..., rows, scale_pitch(K)]`` (float8_e8m0fnu)."""
 

@@ -81,11 +81,25 @@ def moved(y, d):
     return reach + (border * e * 2.0 ** -8).repeat_interleave(BLOCK, -1)[:, :y.shape[1]]
 
 
+def activated(x, w, kind, gated=False, params=None):
+    """``act(x @ w.T)`` and how far float32 arithmetic may be from it: the sums are off by 2^-24 of their magnitudes for every 32 terms (and 4
+    more), the activation by what that does to it, at the corners, and by 2^-20 of itself and 2^-21 of its argument's size."""
+    u = x @ w.T
+    du = (x.abs() @ w.abs().T) * (x.shape[1] / 32 + 4) * 2.0 ** -24
+    y = act(u, kind, gated, params)
+    if gated:
+        half = u.shape[1] // 2
+        sides = [torch.cat([a * du[:, :half], b * du[:, half:]], 1) for a in (-1, 1) for b in (-1, 1)]
+        size = u[:, :half].abs() * (u[:, half:].abs() + 1.0)
+    else:
+        sides, size = [-du, du], u.abs()
+    return y, torch.stack([(act(u + s, kind, gated, params) - y).abs() for s in sides]).amax(0) + y.abs() * 2.0 ** -20 + size * 2.0 ** -21
+
+
 def experts_bound(x, chosen, weights, up, down, kind, gated=False, params=None, result_eps=0.0):
-    """How far a result of float32 arithmetic may be from :func:`experts`, for every number of it: the first product's sums are off by 2^-24 of
-    their magnitudes for every 32 terms (and 4 more); the activation by what that does to it, at the corners, and by 2^-20 of itself and 2^-21
-    of its argument's size; a hidden number is then held as it is, or as its neighbour where the error reaches a border; the second
-    product's sums as the first one's; ``result_eps`` for the rounding of every expert's result, and of the sum."""
+    """How far a result of float32 arithmetic may be from :func:`experts`, for every number of it: the hidden numbers as in :func:`activated`;
+    each is then held as it is, or as its neighbour where the error reaches a border; the second product's sums as the first one's;
+    ``result_eps`` for the rounding of every expert's result, and of the sum."""
     rows = stands_for(x.double())
     out = torch.zeros_like(rows)
     total = torch.zeros_like(rows)
@@ -93,16 +107,7 @@ def experts_bound(x, chosen, weights, up, down, kind, gated=False, params=None, 
         token, choice = torch.nonzero(chosen == e, as_tuple=True)
         if not token.numel():
             continue
-        u = rows[token] @ up[e].T
-        du = (rows[token].abs() @ up[e].abs().T) * (rows.shape[1] / 32 + 4) * 2.0 ** -24
-        y = act(u, kind, gated, params)
-        if gated:
-            half = u.shape[1] // 2
-            sides = [torch.cat([a * du[:, :half], b * du[:, half:]], 1) for a in (-1, 1) for b in (-1, 1)]
-            size = u[:, :half].abs() * (u[:, half:].abs() + 1.0)
-        else:
-            sides, size = [-du, du], u.abs()
-        dy = torch.stack([(act(u + s, kind, gated, params) - y).abs() for s in sides]).amax(0) + y.abs() * 2.0 ** -20 + size * 2.0 ** -21
+        y, dy = activated(rows[token], up[e], kind, gated, params)
         held, off = stands_for(y), moved(y, dy)
         z = held @ down[e].T
         dz = off @ down[e].abs().T + ((held.abs() + off) @ down[e].abs().T) * (y.shape[1] / 32 + 4) * 2.0 ** -24

@@ -62,7 +62,7 @@ def bare_ops():
     """The front end without a GPU behind it: what it refuses, it refuses before anything is launched."""
     from torchllms_b200.kernels.native import NativeOps
     class Nothing:                       # (the C++ front end answers so where something does not fit)
-        rows = norm = product = experts = staticmethod(lambda *args: None)
+        rows = norm = product = act_product = experts = staticmethod(lambda *args: None)
     ops = object.__new__(NativeOps)
     ops._profile, ops.launches, ops._status_at, ops._fp8 = None, 0, 1, Nothing
     return ops
@@ -73,7 +73,7 @@ def test_calls_refuse_the_host():
     ops, x = bare_ops(), rows(4, 256)
     w = Fp8Rows(*encode(rows(32, 256)))
     for call in (lambda: ops.quantize_fp8(x), lambda: ops.activation_fp8(x, "silu"), lambda: ops.rmsnorm_fp8(x, None, x[0], 1e-5),
-                 lambda: ops.linear_fp8(x, w), lambda: ops.linear_fp8(w, w), lambda: ops.linear_fp8(w, x),
+                 lambda: ops.linear_fp8(x, w), lambda: ops.linear_fp8(w, w), lambda: ops.linear_fp8(w, x), lambda: ops.linear_activation_fp8(w, w, "silu"),
                  lambda: ops.moe_experts_fp8(x, torch.zeros((4, 1), dtype=torch.int32), torch.ones((4, 1)), w, w, activation="silu")):
         with pytest.raises(KernelError):
             call()

@@ -203,6 +203,37 @@ def test_rows_of_all_scales(ops):
     check_product(ops.linear_fp8(held(x), held(w), torch.float32), held(x), held(w), torch.float32)
 
 
+@pytest.mark.parametrize("impl", ["single", "pair"])
+@pytest.mark.parametrize("kind,gated", [("silu", True), ("silu", False), ("gelu_tanh", True), ("gelu_tanh", False), ("gelu", False), ("gelu", True),
+                                        ("relu2", False), ("relu2", True), ("clamped_swish", True)])
+@pytest.mark.parametrize("M,hidden,K", [(1, 16, 64), (9, 144, 528), (65, 1040, 256), (250, 384, 1040), (500, 4112, 640)])
+def test_product_behind_an_activation(ops, M, hidden, K, kind, gated, impl):
+    if gated:
+        impl = "auto"                   # (128 hidden numbers lie on a pair)
+    params = (3.0, 1.7, 1.0) if kind == "clamped_swish" else None
+    x, w = held(uneven(M, K, seed=M)), held(rand((hidden * (2 if gated else 1), K), seed=hidden, scale=K ** -0.5))
+    rows = ops.linear_activation_fp8(x, w, kind, gated=gated, act_params=params, impl=impl)
+    ops.check_status()
+    y, dy = plain.activated(plain.value(x), plain.value(w), kind, gated, params)
+    assert rows.shape == (M, hidden) and rows.scales.shape == (M, plain.pitch(hidden))
+    assert bool(((plain.value(rows) - plain.stands_for(y)).abs() <= plain.moved(y, dy)).all())
+    e = plain.hold(y)[1]
+    assert bool((rows.scales.view(torch.uint8)[:, e.shape[1]:] == 0).all())
+    # a scale is the format's, or its neighbour where the error reaches the border
+    off = (rows.scales.view(torch.uint8)[:, :e.shape[1]].double() - (e + 127)).abs()
+    assert bool((off <= 1).all()) and float((off > 0).double().mean()) < 0.01 + 2.0 / off.numel()
+
+
+def test_product_behind_an_activation_keeps_what_is_not_a_number(ops):
+    x, w = uneven(40, 640, seed=1), rand((512, 640), seed=2)
+    x[3, 200], w[130, 639] = math.nan, math.inf
+    for gated in (False, True):
+        bad = torch.isnan(plain.value(ops.linear_activation_fp8(held(x), held(w), "silu", gated=gated)))
+        want = torch.zeros_like(bad)
+        want[3], want[:, 130] = True, True
+        assert torch.equal(bad, want)
+
+
 # ------------------------------------------------------------------------------------------------- experts
 
 def routed(T, E, top, seed, skew=1.0):

@@ -66,8 +66,9 @@ __device__ __forceinline__ int fp8_encode8(const float (&v)[8], uint2& bytes) {
 enum : int { FP8_SILU = 0, FP8_GELU_TANH = 1, FP8_RELU2 = 2, FP8_CLAMPED_SWISH = 3, FP8_GELU = 4 };
 struct Fp8Gate { float limit, alpha, up_offset; };
 
+// (quotients of __fdividef and exponentials of __expf: two units off each, far below the step of E4M3 that follows)
 __device__ __forceinline__ float fp8_act(float x, int act) {
-    if (act == FP8_SILU) return x / (1.f + __expf(-x));
+    if (act == FP8_SILU) return __fdividef(x, 1.f + __expf(-x));
     if (act == FP8_GELU_TANH) return 0.5f * x * (1.f + tanhf(0.7978845608028654f * (x + 0.044715f * x * x * x)));
     if (act == FP8_GELU) return 0.5f * x * (1.f + erff(0.7071067811865476f * x));
     const float r = x < 0.f ? 0.f : x;           // (comparisons, not fmaxf: what is not a number stays so)
@@ -76,7 +77,7 @@ __device__ __forceinline__ float fp8_act(float x, int act) {
 __device__ __forceinline__ float fp8_gated(float gate, float up, int act, const Fp8Gate& p) {
     if (act == FP8_CLAMPED_SWISH) {
         const float g = gate > p.limit ? p.limit : gate, u = up > p.limit ? p.limit : (up < -p.limit ? -p.limit : up);
-        return g / (1.f + __expf(-p.alpha * g)) * (u + p.up_offset);
+        return __fdividef(g, 1.f + __expf(-p.alpha * g)) * (u + p.up_offset);
     }
     return fp8_act(gate, act) * up;
 }

@@ -27,12 +27,18 @@ constexpr int BM = 128;              // rows of W a CTA
 constexpr int BK = 128;              // bytes of K a box: a swizzle row, and a block of numbers that share a scale
 constexpr int MAX_WIDTH = 240;       // rows of x a tile: two accumulators and two sets of scales fill 512 columns
 constexpr int MAX_SPLIT_WIDTH = 224; // the same with one accumulator in 256 columns
+constexpr int COLUMNS = 256;
 constexpr int MAX_STAGES = 12;
 constexpr int MAX_SCALE_BUFS = 3;    // turns of scales under way
 constexpr int TURN = 16;             // blocks of 128 of a turn: four words a row
-constexpr int NTHREADS = 256;
-
-constexpr int STAGING = 4 * 2048;    // 32 x 32 results a warp
+enum : int { SINGLE = 1, PAIRS = 2, SPLIT = 3 };
+enum : int { PLAIN = 0, ACT = 1, GATED = 2 };       // what becomes of the sums: they leave; 8-bit rows of act(sum); of act(gate) * up
+// Warps that take the results: eight, two to a quarter of tensor memory's lanes, with every other 32 columns each (one warp a scheduler
+// waits for its own instructions: 524 us for 275 where 2,048 tokens go through gates and ups of 32 experts); split, four, where
+// two CTAs share an SM.
+__host__ __device__ constexpr int result_warps(int form) { return form == SPLIT ? 4 : 8; }
+__host__ __device__ constexpr int threads_of(int form) { return 32 * (4 + result_warps(form)); }
+constexpr int STAGING = 8 * 2048;    // 32 x 32 results a warp
 constexpr unsigned ACC_COLS = 256;   // a second accumulator lies so many columns behind the first
 constexpr unsigned long long WAIT_LIMIT_NS = 2000ull * 1000ull * 1000ull;   // two seconds, then give up
 
@@ -91,6 +97,13 @@ __device__ __forceinline__ void arrive_elect(unsigned bar) {
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// a word into another CTA's shared memory, counted by the barrier of the same place there
+__device__ __forceinline__ void store_async(unsigned addr, unsigned v, unsigned bar, int cta) {
+    unsigned at, there;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(addr), "r"(cta));
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(bar), "r"(cta));
+    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(at), "r"(v), "r"(there) : "memory");
+}
 // 16 bytes of another CTA's shared memory
 __device__ __forceinline__ float4 load_from(unsigned addr, int cta) {
     unsigned at;
@@ -108,15 +121,36 @@ __device__ __forceinline__ unsigned in_leader(unsigned addr) {
 __device__ __forceinline__ void expect_tx(unsigned bar, unsigned bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
+// A box of x, or of W with a mark on what becomes of it in L2.  PAIR: the barrier that counts the bytes is the first CTA's.
 template <bool PAIR>
-__device__ __forceinline__ void tma_load(unsigned dst, const CUtensorMap* map, unsigned bar, int x, int y) {
-    if (PAIR) {        // (the barrier that counts the bytes is the first CTA's)
-        asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-                     ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
-        return;
-    }
-    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-                 ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+__device__ __forceinline__ void tma_load(unsigned dst, const CUtensorMap* map, unsigned bar, int x, int y, unsigned long long policy) {
+#define TL_LOAD(G) \
+    asm volatile("cp.async.bulk.tensor.2d" G ".shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4}], [%2], %5;" \
+                 ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "l"(policy) : "memory")
+    if (PAIR) TL_LOAD(".cta_group::2");
+    else TL_LOAD("");
+#undef TL_LOAD
+}
+// a box of a gated weight: 16 rows of gates and the 16 matching rows of ups in turn, four times
+template <bool PAIR>
+__device__ __forceinline__ void tma_load_gated(unsigned dst, const CUtensorMap* map, unsigned bar, int x, int group, int expert, unsigned long long policy) {
+    const int zero = 0;
+#define TL_LOAD(G) \
+    asm volatile("cp.async.bulk.tensor.5d" G ".shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4, %4, %5, %6}], [%2], %7;" \
+                 ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(zero), "r"(group), "r"(expert), "l"(policy) : "memory")
+    if (PAIR) TL_LOAD(".cta_group::2");
+    else TL_LOAD("");
+#undef TL_LOAD
+}
+__device__ __forceinline__ unsigned long long policy_first() {
+    unsigned long long p;
+    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+    return p;
+}
+__device__ __forceinline__ unsigned long long policy_normal() {
+    unsigned long long p;
+    asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(p));
+    return p;
 }
 
 // shared-memory matrix descriptors.  Operands: K-major, rows of 128 bytes, 128-byte swizzle, groups of 8 rows 1,024 bytes
@@ -173,6 +207,41 @@ __device__ __forceinline__ void tmem_load32(unsigned taddr, unsigned (&r)[32]) {
                    "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
                  : "r"(taddr));
 }
+__device__ __forceinline__ void tmem_load16(unsigned taddr, unsigned (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+                   "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_store16(unsigned taddr, const float (&v)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                 ::"r"(taddr), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]),
+                   "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15]) : "memory");
+}
+// the result warps' barrier, which also tells whether all of them came through
+__device__ __forceinline__ bool meet(bool ok) {
+    unsigned all;
+    __syncwarp();
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\tbar.red.and.pred p, 1, 256, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(all) : "r"((unsigned)ok) : "memory");
+    return all != 0;
+}
+// The largest magnitude over LANES neighbouring lanes of each of their LANES values (bits of finite numbers): a lane is left with
+// that of value number lane % LANES.  Each step halves the values and doubles the lanes that they stand for.
+template <int LANES>
+__device__ __forceinline__ unsigned largest_of_lanes(unsigned (&m)[LANES]) {
+    const unsigned lane = threadIdx.x & 31;
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) {
+        const bool high = lane & o;
+#pragma unroll
+        for (int j = 0; j < o; ++j) {
+            const unsigned other = __shfl_xor_sync(0xffffffffu, high ? m[j] : m[j + o], o);
+            m[j] = max(high ? m[j + o] : m[j], other);
+        }
+    }
+    return m[0];
+}
 // up to four words of a row's scales, zeros where there is no row (null)
 __device__ __forceinline__ void load_words(const unsigned char* at, int words, bool whole, unsigned (&v)[4]) {
     if (at != nullptr && whole) {        // (every turn of every row starts on 16 bytes and has 16)
@@ -196,16 +265,20 @@ struct Params {
     int out_is_f32;
     bool w_whole, x_whole;           // scales: rows are a multiple of 16 bytes and start on 16
     int splits, split_blocks;        // SPLIT: CTAs of a cluster, and blocks of K of each (a multiple of 4)
+    // ACT, GATED: the 8-bit rows that leave, [M, N] (GATED: [M, N / 2]), and what is done to the sums
+    unsigned char *codes, *scales;
+    int hidden;
+    Fp8Gate gate;
     unsigned tmem_cols, scale_col, set_cols;     // columns of tensor memory; where the first set of scales lies, and how far the second is behind it
 };
 
 // shared memory of a word of scales: 512 bytes for the rows of W and for every 128 rows of x
 __host__ __device__ constexpr int scale_bytes(int width) { return 512 * (1 + (width + 127) / 128); }
 
-enum : int { SINGLE = 1, PAIRS = 2, SPLIT = 3 };
-// Boxes of W (and of x) a stage: what a stage costs its issuer (a wait, a fence, a commit) is as much as four products of 240 rows
-// take.  Split: one, the few blocks of a CTA would be a stage or two otherwise.
-__host__ __device__ constexpr int boxes_of(int form) { return form == SPLIT ? 1 : 2; }
+// Boxes of W (and of x) a stage.  Narrow tiles: two, what a stage costs its issuer (a wait, a fence, a commit) is more than its products
+// take.  Wide ones, whose boxes are large: one, for the more even stream (2,048 tokens through gates and ups of 32 experts: 303 us
+// and 249).  Split: one, the few blocks of a CTA would be a stage or two otherwise.
+__host__ __device__ constexpr int boxes_of(int form) { return form == SINGLE ? 2 : 1; }
 
 struct Unit { int expert, row0, rows, slab; };
 
@@ -225,8 +298,8 @@ __device__ __forceinline__ Unit unit_of(const Params& p, int u, int n_tiles) {
     return r;
 }
 
-template <int FORM>
-__global__ void __launch_bounds__(NTHREADS, FORM == SPLIT ? 2 : 1) gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
+template <int FORM, int EPI, int ACTIVATION>
+__global__ void __launch_bounds__(threads_of(FORM), FORM == SPLIT ? 2 : 1) gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                                                                const Params p) {
     extern __shared__ unsigned char smem_raw[];
     const unsigned smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u;            // tiles want 1,024-byte alignment for the swizzle
@@ -244,12 +317,17 @@ __global__ void __launch_bounds__(NTHREADS, FORM == SPLIT ? 2 : 1) gemm_fp8_kern
     const unsigned w_bytes = BM * BK, x_bytes = p.width / SIDES * BK, stage_bytes = BOXES * (w_bytes + x_bytes);
     const unsigned scales_at = smem0 + p.stages * stage_bytes, word_bytes = scale_bytes(p.width), turn_bytes = 4 * word_bytes;
     unsigned char* const staging = smem_at + p.stages * stage_bytes + p.scale_bufs * turn_bytes;
-    __shared__ __align__(8) unsigned long long bars[2 * MAX_STAGES + 2 * MAX_SCALE_BUFS + 5];
+    // ACT, GATED: a tile's largest magnitudes, by result warp; the other CTA's, of two units; what a row is multiplied by (a tile's
+    // columns are taken 32 at a time: room for whole ones)
+    unsigned* const tops = reinterpret_cast<unsigned*>(staging + STAGING);            // [4][COLUMNS]
+    unsigned* const theirs = tops + 4 * COLUMNS;                                      // [2][COLUMNS]
+    float* const inverse = reinterpret_cast<float*>(theirs + 2 * COLUMNS);            // [COLUMNS]
+    __shared__ __align__(8) unsigned long long bars[2 * MAX_STAGES + 2 * MAX_SCALE_BUFS + 7];
     __shared__ unsigned tmem_slot;
     __shared__ int abort_flag;
     const unsigned bar0 = smem_u32(bars);
     const unsigned full = bar0, empty = bar0 + 8 * MAX_STAGES, sc_full = bar0 + 16 * MAX_STAGES, sc_empty = sc_full + 8 * MAX_SCALE_BUFS;
-    const unsigned acc_full = sc_empty + 8 * MAX_SCALE_BUFS, acc_empty = acc_full + 16, drained = acc_empty + 16;
+    const unsigned acc_full = sc_empty + 8 * MAX_SCALE_BUFS, acc_empty = acc_full + 16, drained = acc_empty + 16, told = drained + 8;
     // (what the first CTA's issuing warp waits for counts arrivals of both)
     auto leader = [&](unsigned bar) { return PAIR ? in_leader(bar) : bar; };
 
@@ -258,8 +336,9 @@ __global__ void __launch_bounds__(NTHREADS, FORM == SPLIT ? 2 : 1) gemm_fp8_kern
         abort_flag = 0;
         for (int s = 0; s < MAX_STAGES; ++s) { mbar_init(full + 8 * s, 1); mbar_init(empty + 8 * s, 1); }
         for (int s = 0; s < MAX_SCALE_BUFS; ++s) { mbar_init(sc_full + 8 * s, SIDES); mbar_init(sc_empty + 8 * s, 1); }
-        for (int s = 0; s < 2; ++s) { mbar_init(acc_full + 8 * s, 1); mbar_init(acc_empty + 8 * s, 4 * SIDES); }
+        for (int s = 0; s < 2; ++s) { mbar_init(acc_full + 8 * s, 1); mbar_init(acc_empty + 8 * s, result_warps(FORM) * SIDES); }
         mbar_init(drained, 1);
+        if (EPI == GATED) { mbar_init(told, 1); mbar_init(told + 8, 1); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -282,6 +361,14 @@ __global__ void __launch_bounds__(NTHREADS, FORM == SPLIT ? 2 : 1) gemm_fp8_kern
     const bool ahead = p.tiles == nullptr;
     if (!(ahead && (warp == 0 || warp == 2 || warp == 3))) grid_dependency_wait();
 
+    // a slab's box: 128 rows of W, or 64 gates and their ups
+    // Experts: W is read by few tiles, side by side, x by every slab: W is the first to leave L2 (2,048 tokens through gates and ups of
+    // 32 experts: 1.28 GB from memory without the mark, 1.11 with it, 585,000 cycles and 524,000).
+    const unsigned long long x_policy = policy_normal(), w_policy = p.tiles != nullptr ? policy_first() : x_policy;
+    auto load_w = [&](unsigned at, unsigned bar, int k, int slab, int expert) {
+        if (EPI == GATED) tma_load_gated<PAIR>(at, &map_w, bar, k, slab * 4, expert, w_policy);
+        else tma_load<PAIR>(at, &map_w, bar, k, expert * p.N + slab * BM, w_policy);
+    };
     const int n_tiles = p.tiles != nullptr ? p.tiles[0] : p.n_tiles;
     const int units = n_tiles * p.slabs;
 
@@ -292,19 +379,19 @@ __global__ void __launch_bounds__(NTHREADS, FORM == SPLIT ? 2 : 1) gemm_fp8_kern
             bool ok = true;
             if (ahead) {
                 if (first_unit < units) {
-                    const int w_row = (first_unit / n_tiles * SIDES + rank) * BM;
+                    const int slab = first_unit / n_tiles * SIDES + rank;
                     for (int kb = kb0; kb < kb1 && early < p.stages; kb += BOXES, ++early) {
                         const unsigned at = smem0 + early * stage_bytes, bar = leader(full + 8 * early);
                         const int boxes = min(BOXES, kb1 - kb);
                         if (rank == 0) expect_tx(full + 8 * early, SIDES * boxes * (w_bytes + x_bytes));
-                        for (int i = 0; i < boxes; ++i) tma_load<PAIR>(at + i * w_bytes, &map_w, bar, (kb + i) * BK, w_row);
+                        for (int i = 0; i < boxes; ++i) load_w(at + i * w_bytes, bar, (kb + i) * BK, slab, 0);
                     }
                 }
                 grid_dependency_wait();
             }
             for (int u = first_unit; u < units && ok; u += step) {
                 const Unit t = unit_of(p, u, n_tiles);
-                const int w_row = t.expert * p.N + (t.slab * SIDES + rank) * BM, x_row = t.row0 + rank * (((t.rows + 15) & ~15) / 2);
+                const int slab = t.slab * SIDES + rank, x_row = t.row0 + rank * (((t.rows + 15) & ~15) / 2);
                 for (int kb = kb0; kb < kb1; kb += BOXES) {
                     if (!wait_one(empty + 8 * stage, phase, aborted)) {
                         give_up(aborted, p.status, ERR_TMA_WAIT);
@@ -319,8 +406,8 @@ __global__ void __launch_bounds__(NTHREADS, FORM == SPLIT ? 2 : 1) gemm_fp8_kern
 #pragma unroll
                     for (int i = 0; i < BOXES; ++i) {
                         if (i < boxes) {
-                            if (fresh) tma_load<PAIR>(at + i * w_bytes, &map_w, bar, (kb + i) * BK, w_row);
-                            tma_load<PAIR>(at + BOXES * w_bytes + i * x_bytes, &map_x, bar, (kb + i) * BK, x_row);
+                            if (fresh) load_w(at + i * w_bytes, bar, (kb + i) * BK, slab, t.expert);
+                            tma_load<PAIR>(at + BOXES * w_bytes + i * x_bytes, &map_x, bar, (kb + i) * BK, x_row, x_policy);
                         }
                     }
                     if (issued < p.stages) ++issued;
@@ -416,7 +503,11 @@ __global__ void __launch_bounds__(NTHREADS, FORM == SPLIT ? 2 : 1) gemm_fp8_kern
                     unsigned v[12][4];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const int r = (t.slab * SIDES + rank) * BM + 32 * j + lane;
+                        int r = (t.slab * SIDES + rank) * BM + 32 * j + lane;
+                        if (EPI == GATED) {        // (lanes 0 to 15 gates, 16 to 31 their ups)
+                            const int f = ((t.slab * SIDES + rank) * 4 + j) * 16 + (lane & 15);
+                            r = f < p.hidden ? f + (lane >= 16 ? p.hidden : 0) : p.N;
+                        }
                         load_words(r < p.N ? p.w_scales + (first + r) * p.pitch + kb : nullptr, words, whole && p.w_whole, v[j]);
                     }
                     if (ahead && !waited) grid_dependency_wait();
@@ -441,9 +532,11 @@ __global__ void __launch_bounds__(NTHREADS, FORM == SPLIT ? 2 : 1) gemm_fp8_kern
                 if (++buf == p.scale_bufs) { buf = 0; phase ^= 1; }
             }
         }
-    } else if (warp >= 4) {
+    } else if (warp >= 4 && EPI == PLAIN) {
         const int quarter = warp & 3;
-        unsigned char* const mine = staging + quarter * 2048;
+        constexpr int SHARES = result_warps(FORM) / 4;
+        const int share = (warp - 4) >> 2;
+        unsigned char* const mine = staging + (warp - 4) * 2048;
         const bool wide = !p.out_is_f32 && p.N % 8 == 0;
         int n = 0;
         for (int u = first_unit; u < units; u += step, ++n) {
@@ -455,7 +548,7 @@ __global__ void __launch_bounds__(NTHREADS, FORM == SPLIT ? 2 : 1) gemm_fp8_kern
             }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const int first = (t.slab * SIDES + rank) * BM + quarter * 32;          // this warp's first row of W
-            for (int c0 = 0; c0 < t.rows; c0 += 32) {
+            for (int c0 = 32 * share; c0 < t.rows; c0 += 32 * SHARES) {
                 unsigned r[32];
                 // (a load of 32 columns may reach into the scales' columns behind the accumulator: read, not used)
                 tmem_load32(tmem + acc * ACC_COLS + ((unsigned)(quarter * 32) << 16) + c0, r);
@@ -493,6 +586,123 @@ __global__ void __launch_bounds__(NTHREADS, FORM == SPLIT ? 2 : 1) gemm_fp8_kern
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             arrive_elect<PAIR>(leader(acc_empty + 8 * acc));
         }
+    } else if (warp >= 4) {
+        // The sums become 8-bit rows: the activation, the largest magnitude of every 128 for each row of x, the numbers under their
+        // scales.  A lane has a row of W (GATED: a half warp has the gates of 16, the other half their ups; they exchange half
+        // of their columns, and each lane then has 16 finished numbers of 32 columns), so the largest of a row of x is over lanes,
+        // warps and, GATED, where a CTA has 64 of the 128, both CTAs.  Meanwhile the numbers lie in tensor memory, over the sums.
+        constexpr int VALUES = EPI == GATED ? 16 : 32;          // finished numbers a lane and 32 columns
+        const int quarter = warp & 3, odd = (warp - 4) >> 2, thread = threadIdx.x - 128;
+        unsigned char* const mine = staging + (warp - 4) * 1024;
+        const unsigned lanes_at = (unsigned)(quarter * 32) << 16;
+        const int pitch = fp8_scale_pitch(p.hidden);
+        int n = 0;
+        for (int u = first_unit; u < units; u += step, ++n) {
+            const Unit t = unit_of(p, u, n_tiles);
+            const int acc = n & 1, slab = t.slab * SIDES + rank;
+            const unsigned d = tmem + acc * ACC_COLS + lanes_at;
+            bool ok = mbar_wait(acc_full + 8 * acc, (n / 2) & 1, aborted);
+            if (!ok && lane == 0) give_up(aborted, p.status, ERR_EPI_WAIT);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            // (GATED: the row of the hidden rows that a lane's numbers stand in, and whether there is one: the others are zeros, as W's rows are)
+            const bool there = EPI == GATED || slab * BM + quarter * 32 + lane < p.N;
+            for (int c0 = 32 * odd; ok && c0 < t.rows; c0 += 64) {
+                unsigned r[32];
+                tmem_load32(d + c0, r);
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                for (int half = 0; half < VALUES / 16; ++half) {
+                    float v[16];
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        if (EPI == GATED) {
+                            const unsigned other = __shfl_xor_sync(0xffffffffu, lane < 16 ? r[j + 16] : r[j], 16);
+                            v[j] = fp8_gated(__uint_as_float(lane < 16 ? r[j] : other), __uint_as_float(lane < 16 ? other : r[j + 16]), ACTIVATION, p.gate);
+                        } else {
+                            v[j] = there ? fp8_act(__uint_as_float(r[16 * half + j]), ACTIVATION) : 0.f;
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        const unsigned b = __float_as_uint(v[j]) & 0x7fffffffu;
+                        const bool fine = b < 0x7f800000u;
+                        r[16 * half + j] = fine ? b : 0u;
+                        if (!fine) v[j] = __int_as_float(0x7fffffff);
+                    }
+                    // (behind a tile's last columns lie scales of products under way)
+                    if (EPI == GATED || c0 + 16 * half < t.rows) tmem_store16(d + c0 + 16 * half, v);
+                }
+                if (EPI == GATED) {
+                    unsigned m[16];
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) m[j] = r[j];
+                    tops[quarter * COLUMNS + c0 + lane] = largest_of_lanes<16>(m);        // (columns c0 .. c0 + 15 by the first half warp)
+                } else {
+                    tops[quarter * COLUMNS + c0 + lane] = largest_of_lanes<32>(r);
+                }
+            }
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            if (!meet(ok)) break;
+            unsigned top = 0u;
+            if (thread < t.rows) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) top = max(top, tops[q * COLUMNS + thread]);
+                // (a store that counts itself when it has landed: a fence would wait for all that the warp has stored)
+                if (EPI == GATED) store_async(smem_u32(theirs + acc * COLUMNS + thread), top, told + 8 * acc, rank ^ 1);
+            }
+            if (EPI == GATED) {
+                // (the other CTA's next store to this place is behind two units of this one)
+                if (thread == 0) expect_tx(told + 8 * acc, 4 * t.rows);
+                __syncwarp();
+                ok = mbar_wait(told + 8 * acc, (n / 2) & 1, aborted);
+                if (!ok && lane == 0) give_up(aborted, p.status, ERR_EPI_WAIT);
+            }
+            if (thread < t.rows && ok) {
+                if (EPI == GATED) top = max(top, theirs[acc * COLUMNS + thread]);
+                const int e = fp8_exponent(top), block = EPI == GATED ? t.slab : slab;
+                inverse[thread] = fp8_inverse(e);
+                if ((EPI != GATED || rank == 0) && block * FP8_BLOCK < p.hidden) {
+                    unsigned char* s = p.scales + (size_t)(t.row0 + thread) * pitch;
+                    s[block] = (unsigned char)(e + 127);
+                    if ((block + 1) * FP8_BLOCK >= p.hidden)
+                        for (int k = block + 1; k < pitch; ++k) s[k] = 0;
+                }
+            }
+            if (!meet(ok)) break;
+            for (int c0 = 32 * odd; c0 < t.rows; c0 += 64) {
+#pragma unroll
+                for (int half = 0; half < VALUES / 16; ++half) {
+                    unsigned r[16];
+                    tmem_load16(d + c0 + 16 * half, r);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    const int first = EPI == GATED ? (lane >> 4) * 16 : 16 * half;       // the column of r[0], from c0 on
+                    __syncwarp();
+#pragma unroll
+                    for (int j = 0; j < 16; j += 4) {
+                        const float4 inv = *reinterpret_cast<const float4*>(inverse + c0 + first + j);
+                        const unsigned lo = fp8_pack2(__uint_as_float(r[j]) * inv.x, __uint_as_float(r[j + 1]) * inv.y);
+                        const unsigned hi = fp8_pack2(__uint_as_float(r[j + 2]) * inv.z, __uint_as_float(r[j + 3]) * inv.w);
+                        constexpr int ROW = EPI == GATED ? 16 : 32;
+                        unsigned char* to = mine + (first + j) * ROW + (lane & (ROW - 1));
+                        to[0] = (unsigned char)lo;
+                        to[ROW] = (unsigned char)(lo >> 8);
+                        to[2 * ROW] = (unsigned char)hi;
+                        to[3 * ROW] = (unsigned char)(hi >> 8);
+                    }
+                }
+                __syncwarp();
+                // 16 bytes a lane: GATED, a column's 16; else half of a column's 32
+#pragma unroll
+                for (int i = 0; i < VALUES / 16; ++i) {
+                    const int c = EPI == GATED ? lane : i * 16 + (lane >> 1);
+                    const int f = EPI == GATED ? (slab * 4 + quarter) * 16 : slab * BM + quarter * 32 + (lane & 1) * 16;
+                    const uint4 v = *reinterpret_cast<const uint4*>(mine + (EPI == GATED ? c * 16 : c * 32 + (lane & 1) * 16));
+                    if (c0 + c < t.rows && f < p.hidden) *reinterpret_cast<uint4*>(p.codes + (size_t)(t.row0 + c0 + c) * p.hidden + f) = v;
+                }
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            arrive_elect<PAIR>(leader(acc_empty + 8 * acc));
+        }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
@@ -502,7 +712,7 @@ __global__ void __launch_bounds__(NTHREADS, FORM == SPLIT ? 2 : 1) gemm_fp8_kern
         const Unit t = unit_of(p, first_unit, n_tiles);
         const unsigned sums = smem0 + (threadIdx.x & 31) * 16;
         const int row = t.slab * BM + (threadIdx.x & 31) * 4;
-        for (int c = cut + (threadIdx.x >> 5) * p.splits; c < t.rows && !*aborted; c += (NTHREADS >> 5) * p.splits) {
+        for (int c = cut + (threadIdx.x >> 5) * p.splits; c < t.rows && !*aborted; c += (threads_of(FORM) >> 5) * p.splits) {
             float4 v[8];
 #pragma unroll
             for (int s = 0; s < 8; ++s)
@@ -579,6 +789,18 @@ int make_map(CUtensorMap* map, const void* base, long long rows, long long K, in
               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? TL_OK : TL_BAD_SIZE;
 }
 
+// [experts, 2 hidden, K] bytes, an expert's rows [gates; ups]: boxes of 16 gates and their 16 ups in turn, four times
+int make_gated_map(CUtensorMap* map, const void* base, int experts, int hidden, long long K) {
+    EncodeTiledFn fn = encode_tiled();
+    if (fn == nullptr) return TL_BAD_SIZE;
+    cuuint64_t dims[5] = {(cuuint64_t)K, 16, 2, (cuuint64_t)hidden / 16, (cuuint64_t)experts};
+    cuuint64_t strides[4] = {(cuuint64_t)K, (cuuint64_t)hidden * K, 16 * (cuuint64_t)K, 2 * (cuuint64_t)hidden * K};
+    cuuint32_t box[5] = {(cuuint32_t)BK, 16, 2, 4, 1};
+    cuuint32_t elem[5] = {1, 1, 1, 1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 5, const_cast<void*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? TL_OK : TL_BAD_SIZE;
+}
+
 constexpr int MAX_DEVICES = 64;
 int current_device() {
     int dev = 0;
@@ -607,7 +829,7 @@ int whole_columns(int n) {
     return c;
 }
 
-template <int FORM>
+template <int FORM, int EPI = PLAIN, int ACTIVATION = 0>
 int launch(Params& p, const void* x, const void* w, int experts, int K, cudaStream_t s) {
     constexpr int SIDES = FORM == PAIRS ? 2 : 1;
     p.slabs = (p.N + SIDES * BM - 1) / (SIDES * BM);
@@ -616,7 +838,7 @@ int launch(Params& p, const void* x, const void* w, int experts, int K, cudaStre
     const int stage_bytes = boxes_of(FORM) * (BM * BK + p.width / SIDES * BK);
     p.scale_bufs = FORM == SPLIT ? (p.split_blocks + TURN - 1) / TURN : MAX_SCALE_BUFS;
     if (p.scale_bufs > MAX_SCALE_BUFS) p.scale_bufs = MAX_SCALE_BUFS;
-    const int fixed = 1024 + p.scale_bufs * 4 * scale_bytes(p.width) + (FORM == SPLIT ? 0 : STAGING);     // (1,024 to align)
+    const int fixed = 1024 + p.scale_bufs * 4 * scale_bytes(p.width) + (FORM == SPLIT ? 0 : STAGING) + (EPI == PLAIN ? 0 : 7 * COLUMNS * 4);     // (1,024 to align)
     int room = 226 * 1024;                          // (a kilobyte is left for barriers)
     if (FORM == SPLIT) {
         // one accumulator, one unit: narrow tiles leave room for a second CTA on an SM
@@ -634,12 +856,12 @@ int launch(Params& p, const void* x, const void* w, int experts, int K, cudaStre
     if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
     if (p.stages < 1 || (FORM == SPLIT && p.stages * stage_bytes < p.width * BM * 4)) return TL_TOO_LARGE;
     CUtensorMap mw, mx;
-    int rc = make_map(&mw, w, (long long)experts * p.N, K, BM);
+    int rc = EPI == GATED ? make_gated_map(&mw, w, experts, p.hidden, K) : make_map(&mw, w, (long long)experts * p.N, K, BM);
     if (rc != TL_OK) return rc;
     rc = make_map(&mx, x, p.M, K, p.width / SIDES);
     if (rc != TL_OK) return rc;
     const size_t smem = fixed + (size_t)p.stages * stage_bytes;
-    auto kern = gemm_fp8_kernel<FORM>;
+    auto kern = gemm_fp8_kernel<FORM, EPI, ACTIVATION>;
     static bool raised[MAX_DEVICES];
     const int dev = current_device();
     if (!raised[dev]) {
@@ -649,7 +871,7 @@ int launch(Params& p, const void* x, const void* w, int experts, int K, cudaStre
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(FORM == SPLIT ? units * p.splits : SIDES * (units < sms / SIDES ? units : sms / SIDES));
-    cfg.blockDim = dim3(NTHREADS);
+    cfg.blockDim = dim3(threads_of(FORM));
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cudaLaunchAttribute attr[2];
@@ -677,13 +899,13 @@ int splits_for(int units, int k_blocks, int width, int sms) {
     return (words + per - 1) / per;                 // no empty split
 }
 
-int launch(const void* x, const void* x_scales, const void* w, const void* w_scales, void* out, int out_is_f32, int M, int N, int K, int experts,
-           const int* tiles, int most_tiles, int width, int form, int* status, cudaStream_t s) {
-    if (N <= 0 || K <= 0 || K % 16 != 0 || experts <= 0 || (long long)experts * N > 0x7fffff00ll) return TL_BAD_SIZE;
-    if (!aligned16(x) || !aligned16(w) || !aligned16(out) || status == nullptr || ((uintptr_t)x_scales & 3u) != 0 || ((uintptr_t)w_scales & 3u) != 0)
-        return TL_BAD_ALIGN;
-    Params p = {};
-    p.out = out; p.status = status; p.out_is_f32 = out_is_f32;
+// what all forms need and check; tiles == null: one weight, tiles of `width` rows
+int fill(Params& p, const void* x, const void* x_scales, const void* w, const void* w_scales, int M, int N, int K, int experts, const int* tiles,
+         int most_tiles, int width, int* status) {
+    if (N <= 0 || K <= 0 || K % 16 != 0 || experts <= 0 || most_tiles <= 0 || (long long)experts * N > 0x7fffff00ll) return TL_BAD_SIZE;
+    if (!aligned16(x) || !aligned16(w) || status == nullptr || ((uintptr_t)x_scales & 3u) != 0 || ((uintptr_t)w_scales & 3u) != 0) return TL_BAD_ALIGN;
+    p = Params{};
+    p.status = status;
     p.w_scales = (const unsigned char*)w_scales; p.x_scales = (const unsigned char*)x_scales;
     p.w_whole = fp8_scale_pitch(K) % 16 == 0 && aligned16(w_scales);
     p.x_whole = fp8_scale_pitch(K) % 16 == 0 && aligned16(x_scales);
@@ -693,10 +915,23 @@ int launch(const void* x, const void* x_scales, const void* w, const void* w_sca
     p.n_tiles = most_tiles;
     p.splits = 1;
     p.split_blocks = p.k_blocks;
+    return TL_OK;
+}
+
+// Pairs halve what a tile of x costs in copies, and that is what wide tiles wait for (2,048 rows of 28,672 x 4,096: 222 us
+// alone, 186 in pairs); narrow ones stream W, which nobody shares (8 rows: 22.3 and 22.4)
+int form_for(int width) { return width > 64 ? PAIRS : SINGLE; }
+
+int sums(const void* x, const void* x_scales, const void* w, const void* w_scales, void* out, int out_is_f32, int M, int N, int K, int experts,
+         const int* tiles, int most_tiles, int width, int form, int* status, cudaStream_t s) {
+    Params p;
+    const int rc = fill(p, x, x_scales, w, w_scales, M, N, K, experts, tiles, most_tiles, width, status);
+    if (rc != TL_OK) return rc;
+    if (!aligned16(out)) return TL_BAD_ALIGN;
     if (form < 0 || form > 3 || (form == SPLIT && (tiles != nullptr || width > MAX_SPLIT_WIDTH))) return TL_BAD_SIZE;
-    // Pairs halve what a tile of x costs in copies, and that is what wide tiles wait for (2,048 rows of 28,672 x 4,096: 222 us
-    // alone, 186 in pairs); narrow ones stream W, which nobody shares (8 rows: 22.3 and 22.4)
-    if (form == 0) form = width > 64 ? PAIRS : SINGLE;
+    p.out = out;
+    p.out_is_f32 = out_is_f32;
+    if (form == 0) form = form_for(width);
     if (form == SPLIT) {
         p.splits = splits_for(((N + BM - 1) / BM) * most_tiles, p.k_blocks, width, sm_count());
         const int words = (p.k_blocks + 3) / 4;
@@ -706,10 +941,17 @@ int launch(const void* x, const void* x_scales, const void* w, const void* w_sca
     return form == PAIRS ? launch<PAIRS>(p, x, w, experts, K, s) : launch<SINGLE>(p, x, w, experts, K, s);
 }
 
+// rows of a tile of the experts' products: twice an even share, so that most experts need one tile
+int tile_rows(int pairs, int experts) {
+    const long long share = (2ll * pairs + experts - 1) / (experts > 0 ? experts : 1);
+    const int width = (int)(share > MAX_WIDTH ? MAX_WIDTH : (share + 15) / 16 * 16);
+    return width < 16 ? 16 : width;
+}
+
 }  // namespace
 
 // out[M, N] (float32 or bfloat16) = x . w^T for 8-bit rows x [M, K] and w [N, K] with their scales.  form: 0 the one that fits, 1 a CTA
-// to a unit, 2 a pair of CTAs.
+// to a unit, 2 a pair of CTAs, 3 a cluster that shares K.
 extern "C" int tl_gemm_fp8(const void* x, const void* x_scales, const void* w, const void* w_scales, void* out, int out_is_f32, int M, int N, int K,
                            int form, int* status, void* stream) {
     if (M <= 0) return TL_OK;
@@ -718,23 +960,56 @@ extern "C" int tl_gemm_fp8(const void* x, const void* x_scales, const void* w, c
     const int narrow = even_width(M, MAX_SPLIT_WIDTH), units = ((N + BM - 1) / BM) * ((M + narrow - 1) / narrow);
     if (form == 0 && 2 * units <= sm_count() && K > 4 * BK) form = SPLIT;
     if (form == SPLIT) width = narrow;
-    return launch(x, x_scales, w, w_scales, out, out_is_f32, M, N, K, 1, nullptr, (M + width - 1) / width, width, form, status, (cudaStream_t)stream);
+    return sums(x, x_scales, w, w_scales, out, out_is_f32, M, N, K, 1, nullptr, (M + width - 1) / width, width, form, status, (cudaStream_t)stream);
 }
 
-// Rows of a tile of the experts' products, and how many tiles there can be.
-extern "C" int tl_gemm_fp8_tile_rows(int pairs, int experts) {
-    // twice an even share, so that most experts need one tile
-    const long long share = (2ll * pairs + experts - 1) / (experts > 0 ? experts : 1);
-    const int width = (int)(share > MAX_WIDTH ? MAX_WIDTH : (share + 15) / 16 * 16);
-    return width < 16 ? 16 : width;
-}
+// Rows of a tile of the experts' products.
+extern "C" int tl_gemm_fp8_tile_rows(int pairs, int experts) { return tile_rows(pairs, experts); }
 
-// The experts' products: x [pairs, K] sorted by expert, w [experts, N, K], out [pairs, N]; tiles as moe_plan leaves them, with
+// The experts' products: x [pairs, K] sorted by expert, w [experts, N, K], out [pairs, N]; tiles as tl_fp8_plan leaves them, with
 // tl_gemm_fp8_tile_rows(pairs, experts) rows at most and most_tiles of them at most.
 extern "C" int tl_gemm_fp8_experts(const void* x, const void* x_scales, const void* w, const void* w_scales, void* out, int out_is_f32, int pairs,
-                                   int N, int K, int experts, const int* tiles, int most_tiles, int form, int* status, void* stream) {
+                                   int N, int K, int experts, const int* tiles, int most_tiles, int form, int* status,
+                                   void* stream) {
     if (pairs <= 0) return TL_OK;
-    if (tiles == nullptr || most_tiles <= 0) return TL_BAD_SIZE;
-    return launch(x, x_scales, w, w_scales, out, out_is_f32, pairs, N, K, experts, tiles, most_tiles, tl_gemm_fp8_tile_rows(pairs, experts), form, status,
-                  (cudaStream_t)stream);
+    if (tiles == nullptr) return TL_BAD_SIZE;
+    return sums(x, x_scales, w, w_scales, out, out_is_f32, pairs, N, K, experts, tiles, most_tiles, tile_rows(pairs, experts), form, status,
+                (cudaStream_t)stream);
+}
+
+// 8-bit rows codes [M, hidden], scales [M, fp8_scale_pitch(hidden)] of act(x . w^T), w [experts, hidden, K], or, gated, of
+// act(x . gate^T) * (x . up^T), w [experts, 2 hidden, K] with an expert's rows [gates; ups].  hidden % 16 == 0; act as in fp8.cuh.
+// tiles == null: one expert; else as tl_gemm_fp8_experts.  form: 0, 1 or 2 (gated: 0 or 2, 128 hidden numbers lie on a pair).
+extern "C" int tl_gemm_fp8_act(const void* x, const void* x_scales, const void* w, const void* w_scales, void* codes, void* scales, int M, int hidden,
+                               int K, int gated, int act, float limit, float alpha, float up_offset, int experts, const int* tiles,
+                               int most_tiles, int form, int* status, void* stream) {
+    if (M <= 0) return TL_OK;
+    if (hidden <= 0 || hidden % 16 != 0 || hidden > (1 << 26) || act < 0 || act > 4 || (act == FP8_CLAMPED_SWISH && !gated) ||
+        form < 0 || form > 2 || (gated && form == SINGLE))
+        return TL_BAD_SIZE;
+    const int width = tiles == nullptr ? even_width(M, MAX_WIDTH) : tile_rows(M, experts);
+    Params p;
+    const int rc = fill(p, x, x_scales, w, w_scales, M, gated ? 2 * hidden : hidden, K, experts, tiles,
+                        tiles == nullptr ? (M + width - 1) / width : most_tiles, width, status);
+    if (rc != TL_OK) return rc;
+    if (!aligned16(codes)) return TL_BAD_ALIGN;
+    p.codes = (unsigned char*)codes;
+    p.scales = (unsigned char*)scales;
+    p.hidden = hidden;
+    p.gate = Fp8Gate{limit, alpha, up_offset};
+    cudaStream_t s = (cudaStream_t)stream;
+    if (form == 0) form = form_for(width);
+    if (gated) {
+        if (act == FP8_SILU) return launch<PAIRS, GATED, FP8_SILU>(p, x, w, experts, K, s);
+        if (act == FP8_GELU_TANH) return launch<PAIRS, GATED, FP8_GELU_TANH>(p, x, w, experts, K, s);
+        if (act == FP8_RELU2) return launch<PAIRS, GATED, FP8_RELU2>(p, x, w, experts, K, s);
+        if (act == FP8_GELU) return launch<PAIRS, GATED, FP8_GELU>(p, x, w, experts, K, s);
+        return launch<PAIRS, GATED, FP8_CLAMPED_SWISH>(p, x, w, experts, K, s);
+    }
+#define TL_ACT(A) return form == PAIRS ? launch<PAIRS, ACT, A>(p, x, w, experts, K, s) : launch<SINGLE, ACT, A>(p, x, w, experts, K, s)
+    if (act == FP8_SILU) TL_ACT(FP8_SILU);
+    if (act == FP8_GELU_TANH) TL_ACT(FP8_GELU_TANH);
+    if (act == FP8_RELU2) TL_ACT(FP8_RELU2);
+    TL_ACT(FP8_GELU);
+#undef TL_ACT
 }

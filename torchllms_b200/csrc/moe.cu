@@ -311,7 +311,7 @@ __global__ void moe_combine_kernel(const T* __restrict__ y, const int* __restric
     grid_dependency_wait();
     const int t = blockIdx.x;
     if (threadIdx.x < top) {
-        pl[threadIdx.x] = place[(size_t)t * top + threadIdx.x];
+        pl[threadIdx.x] = max(place[(size_t)t * top + threadIdx.x], 0);        // (-1: an expert that there is not; stay in bounds)
         wt[threadIdx.x] = weights[(size_t)t * top + threadIdx.x];
     }
     __syncthreads();
@@ -531,15 +531,6 @@ extern "C" int tl_moe_plan(const int* chosen, int n_pairs, int n_experts, int* o
     const size_t smem = (size_t)(2 * n_experts + 1) * sizeof(int);
     return (int)tl_launch(moe_plan_kernel, dim3(1), dim3(1024), smem, (cudaStream_t)stream, chosen, n_pairs, n_experts,
                           tl_moe_tile_rows(n_pairs), order, place, tiles, tl_moe_max_tiles(n_pairs, n_experts), ends);
-}
-
-// The same for tiles of so many rows as the caller says: tiles has room for 1 + 3 * min(n_pairs, ceil(n_pairs / tile_rows) + n_experts).
-extern "C" int tl_moe_plan_tiles(const int* chosen, int n_pairs, int n_experts, int tile_rows, int* order, int* place, int* tiles, void* stream) {
-    if (n_pairs <= 0) return TL_OK;
-    if (n_experts <= 0 || n_experts > 4096 || tile_rows <= 0) return TL_BAD_SIZE;
-    const long long most = ((long long)n_pairs + tile_rows - 1) / tile_rows + n_experts;
-    return (int)tl_launch(moe_plan_kernel, dim3(1), dim3(1024), (size_t)(2 * n_experts + 1) * sizeof(int), (cudaStream_t)stream, chosen, n_pairs,
-                          n_experts, tile_rows, order, place, tiles, (int)(most < n_pairs ? most : n_pairs), (int*)nullptr);
 }
 
 // The experts' products over the sorted rows.  A: [rows][K]; with gather_div > 0 row r of the sorted order

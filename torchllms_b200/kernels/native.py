@@ -1492,7 +1492,9 @@ class NativeOps:
 
     def _fp8_load(self):
         calls = load_extension("fp8_calls")
-        names = (("rows_fp8", "tl_fp8_rows"), ("rows_fp8", "tl_fp8_norm"), ("gemm_fp8", "tl_gemm_fp8"))
+        names = (("rows_fp8", "tl_fp8_rows"), ("rows_fp8", "tl_fp8_norm"), ("gemm_fp8", "tl_gemm_fp8"), ("gemm_fp8", "tl_gemm_fp8_act"),
+                 ("gemm_fp8", "tl_gemm_fp8_tile_rows"), ("rows_fp8", "tl_fp8_plan"), ("rows_fp8", "tl_fp8_rows_placed"),
+                 ("gemm_fp8", "tl_gemm_fp8_experts"), ("moe", "tl_moe_combine"))
         calls.bind(*(ctypes.cast(getattr(self._lib(lib), name), ctypes.c_void_p).value for lib, name in names))
         self._fp8 = calls
         return calls
@@ -1548,13 +1550,7 @@ class NativeOps:
     def activation_fp8(self, u: torch.Tensor, activation: str, *, gated: bool = False, act_params=None) -> Fp8Rows:
         """``act(u)``, or with ``gated`` ``act(g) * v`` of the halves ``[g | v]`` of ``u``'s rows, in 8 bits (as :meth:`quantize_fp8`); the
         activation is taken in float32 and rounded once.  Activations and ``act_params`` as in :meth:`moe_experts`."""
-        code = self._ACTS.get(activation)
-        _need(code is not None, f"unknown activation {activation!r}; known: {', '.join(self._ACTS)}")
-        limit = alpha = offset = 0.0
-        if activation == "clamped_swish":
-            _need(gated and act_params is not None and len(act_params) == 3 and act_params[0] > 0,
-                  "the clamped activation is a gated one and goes with (limit, alpha, up_offset), the limit positive")
-            limit, alpha, offset = act_params
+        code, limit, alpha, offset = self._fp8_activation(activation, gated, act_params)
         rows = (self._fp8 or self._fp8_load()).rows(u, 2 if gated else 1, code, limit, alpha, offset)
         if type(rows) is tuple:
             self.launches += 1
@@ -1629,21 +1625,65 @@ class NativeOps:
         _need(x.shape[0] == 0 or w.shape[0] == 0, "linear_fp8: rows must start on 16 bytes and their scales on 4")
         return torch.empty((x.shape[0], w.shape[0]), dtype=out_dtype, device=x.device)
 
-    @_timed
+    def _fp8_activation(self, activation: str, gated: bool, act_params):
+        """The activation's code and its parameters."""
+        code = self._ACTS.get(activation)
+        _need(code is not None, f"unknown activation {activation!r}; known: {', '.join(self._ACTS)}")
+        if activation != "clamped_swish":
+            return code, 0.0, 0.0, 0.0
+        _need(gated and act_params is not None and len(act_params) == 3 and act_params[0] > 0,
+              "the clamped activation is a gated one and goes with (limit, alpha, up_offset), the limit positive")
+        return (code, *act_params)
+
+    @_timed_when_asked
+    def linear_activation_fp8(self, x, w: Fp8Rows, activation: str, *, gated: bool = False, act_params=None, impl: str = "auto") -> Fp8Rows:
+        """:meth:`linear_fp8` and :meth:`activation_fp8` of its float32 sums in one kernel: 8-bit rows of ``act(x @ w^T)``, or with ``gated``
+        of ``act(x @ w[:H]^T) * (x @ w[H:]^T)``.  ``w`` has a multiple of 16 rows (``gated``: twice that)."""
+        code, limit, alpha, offset = self._fp8_activation(activation, gated, act_params)
+        form = self._FP8_FORMS.get(impl)
+        if form is not None and type(w) is Fp8Rows:
+            held = type(x) is Fp8Rows
+            rows = (self._fp8 or self._fp8_load()).act_product(x.codes if held else x, x.scales if held else None, w.codes, w.scales, code,
+                                                               1 if gated else 0, limit, alpha, offset, form, self._status_at)
+            if type(rows) is tuple:
+                self.launches += 1 if held else 2
+                return Fp8Rows(*rows)
+            if rows is not None:
+                _check(rows, "linear_activation_fp8")
+        self._fp8_need(w, "linear_activation_fp8: w")
+        hidden = w.shape[0] // 2 if gated else w.shape[0]
+        _need(hidden % FP8_ALIGN == 0 and (not gated or w.shape[0] % 2 == 0),
+              f"linear_activation_fp8: 8-bit rows take a multiple of {FP8_ALIGN} numbers, got {hidden}")
+        empty = self._linear_fp8_explained(x, w, torch.float32, impl)
+        return self._fp8_empty(empty.shape[0], hidden, empty.device)
+
+    @_timed_when_asked
     def moe_experts_fp8(self, x: torch.Tensor, chosen: torch.Tensor, weights: torch.Tensor, w_up: Fp8Rows, w_down: Fp8Rows, *, activation: str,
                         shared: Optional[torch.Tensor] = None, shared_gate: Optional[torch.Tensor] = None, gated: bool = False,
                         act_params=None, impl: str = "auto") -> torch.Tensor:
         """:meth:`moe_experts` with weights in 8 bits: ``w_up`` ``[E, hidden, dim]`` (``gated``: ``[E, 2 * hidden, dim]``, rows ``[gate; up]``) and
         ``w_down`` ``[E, dim, hidden]``.  A token's row is brought to 8 bits once, the hidden rows behind the activation again (taken in
-        float32, rounded once); both products run over the rows sorted by expert.  Experts that nobody chose are not read."""
+        float32, rounded once); both products run over the rows sorted by expert.  Experts that nobody chose are not read.  ``chosen`` must lie
+        in ``0 .. E - 1``; what a token with another number gets is not defined."""
+        code, limit, alpha, offset = self._fp8_activation(activation, gated, act_params)
+        form = self._FP8_FORMS.get(impl)
+        if form is not None and type(w_up) is Fp8Rows and type(w_down) is Fp8Rows:
+            out = (self._fp8 or self._fp8_load()).experts(x, chosen, weights, w_up.codes, w_up.scales, w_down.codes, w_down.scales, code, 1 if gated else 0,
+                                                          limit, alpha, offset, shared, shared_gate, form, self._status_at)
+            if isinstance(out, torch.Tensor):
+                self.launches += 5
+                return out
+            if out is not None:
+                _check(out, "moe_experts_fp8")
+        return self._moe_experts_fp8_explained(x, chosen, weights, w_up, w_down, shared, shared_gate, gated, impl)
+
+    def _moe_experts_fp8_explained(self, x, chosen, weights, w_up, w_down, shared, shared_gate, gated, impl) -> torch.Tensor:
         _cuda_contig(x, "experts' input")
         _cuda_contig(chosen, "chosen", torch.int32)
         _cuda_contig(weights, "weights", torch.float32)
         self._fp8_need(w_up, "experts' up weights", 3)
         self._fp8_need(w_down, "experts' down weights", 3)
-        _need(activation in self._ACTS, f"unknown activation {activation!r}; known: {', '.join(self._ACTS)}")
         _need(impl in self._FP8_FORMS, f"experts: impl must be one of {', '.join(self._FP8_FORMS)}, got {impl!r}")
-        form = self._FP8_FORMS[impl]
         dim = self._fp8_width(x, "experts' input")
         _need(chosen.dim() == 2 and chosen.shape == weights.shape and chosen.shape[0] == x.shape[0], "experts: x [T, dim], chosen and weights [T, top]")
         T, top = chosen.shape
@@ -1653,42 +1693,16 @@ class NativeOps:
         _need((not gated or up_rows % 2 == 0) and w_up.codes.shape[2] == dim and w_down.codes.shape == (E, dim, hidden),
               "experts: w_up [E, hidden, dim] (gated: 2 * hidden), w_down [E, dim, hidden]")
         _need(1 <= E <= 4096, f"between 1 and 4096 experts, got {E}")
-        splits, plane = 1, 0
         if shared is not None:
             _cuda_contig(shared, "shared expert's output")
             _need(shared.shape[-2:] == (T, dim) and (shared.dtype == x.dtype or shared.dtype == torch.float32), "shared must be [T, dim] or float32 partial sums of it")
-            if shared.dim() == 3:
-                _need(shared.dtype == torch.float32, "partial sums must be float32")
-                splits, plane = shared.shape[0], shared.stride(0)
+            _need(shared.dim() == 2 or (shared.dim() == 3 and shared.dtype == torch.float32 and shared.shape[0] >= 1), "partial sums must be float32")
         if shared_gate is not None:
             _cuda_contig(shared_gate, "shared gate", torch.float32)
             _need(shared is not None and shared_gate.numel() == T, "one gate value per token, with a shared expert")
         self._fp8_here(x, chosen, weights, w_up.codes, w_down.codes, shared, shared_gate)
-        out = torch.empty((T, dim), dtype=x.dtype, device=x.device)
-        if T == 0:
-            return out
-        pairs = T * top
-        moe, rows_lib, gemm = self._lib("moe"), self._lib("rows_fp8"), self._lib("gemm_fp8")
-        tile_rows = gemm.tl_gemm_fp8_tile_rows(pairs, E)
-        most = min(pairs, -(-pairs // tile_rows) + E)
-        index = torch.empty(2 * pairs + 1 + 3 * most, dtype=torch.int32, device=x.device)
-        order, place, tiles = index[:pairs], index[pairs:2 * pairs], index[2 * pairs:]
-        _check(moe.tl_moe_plan_tiles(_ptr(chosen), pairs, E, tile_rows, _ptr(order), _ptr(place), _ptr(tiles), _stream()), "moe_plan")
-        rows = self._fp8_empty(pairs, dim, x.device)
-        _check(rows_lib.tl_fp8_rows_placed(_ptr(x), _DT[x.dtype], _ptr(rows.codes), _ptr(rows.scales), T, dim, _ptr(place), top, _stream()), "experts' rows")
-        u = torch.empty((pairs, up_rows), dtype=torch.float32, device=x.device)
-        status = ctypes.c_void_p(self._status_at)
-        _check(gemm.tl_gemm_fp8_experts(_ptr(rows.codes), _ptr(rows.scales), _ptr(w_up.codes), _ptr(w_up.scales), _ptr(u), 1, pairs, up_rows, dim, E,
-                                        _ptr(tiles), most, form, status, _stream()), "experts' products (up)")
-        hid = self.activation_fp8(u, activation, gated=gated, act_params=act_params)
-        y = torch.empty((pairs, dim), dtype=x.dtype, device=x.device)
-        _check(gemm.tl_gemm_fp8_experts(_ptr(hid.codes), _ptr(hid.scales), _ptr(w_down.codes), _ptr(w_down.scales), _ptr(y),
-                                        1 if x.dtype == torch.float32 else 0, pairs, dim, hidden, E, _ptr(tiles), most, form, status, _stream()),
-               "experts' products (down)")
-        _check(moe.tl_moe_combine(_ptr(y), _DT[x.dtype], _ptr(place), _ptr(weights), _ptr(shared), _DT[shared.dtype] if shared is not None else 0,
-                                  splits, ctypes.c_longlong(plane), _ptr(shared_gate), _ptr(out), T, dim, top, _stream()), "moe_combine")
-        self.launches += 5
-        return out
+        _need(T == 0, "experts: rows must start on 16 bytes and their scales on 4")
+        return torch.empty((0, dim), dtype=x.dtype, device=x.device)
 
     def can_fuse_residual(self, pending, h: torch.Tensor) -> bool:
         """Whether :meth:`linear_residual_norm` takes this pending product for this stream."""

@@ -40,7 +40,7 @@ def model_dir_of(path) -> Path:
 
 
 def load_model(path, *, dtype="bfloat16", device="cuda", overrides: Optional[Mapping[str, Any]] = None,
-               max_positions: Optional[int] = None, ops=None, kv_format: str = "full") -> Tuple[Architecture, Any, Model]:
+               max_positions: Optional[int] = None, ops=None, kv_format: str = "full", weight_format: str = "full") -> Tuple[Architecture, Any, Model]:
     """``path`` is a model folder, a safetensors file, a ``torch.save``d checkpoint of plain tensors
     (the reference's ``consolidated.00.pth`` beside its ``params.json``), or a list of them: tensors of later
     entries replace those of earlier ones (the reference loads several checkpoint paths in order,
@@ -50,7 +50,7 @@ def load_model(path, *, dtype="bfloat16", device="cuda", overrides: Optional[Map
     arch, config = load_config(folder, overrides)
     spec = arch.build_spec(config)
     model = Model(spec, dtype=parse_dtype(dtype), device=device, ops=ops or get_ops(),
-                  max_positions=max_positions, kv_format=kv_format)
+                  max_positions=max_positions, kv_format=kv_format, weight_format=weight_format)
     found: Dict[str, LazyTensor] = {}
     for p in paths:
         p = Path(p)
@@ -73,11 +73,11 @@ def load_model(path, *, dtype="bfloat16", device="cuda", overrides: Optional[Map
 
 
 def random_model(config, seed: int, *, dtype="bfloat16", device="cuda", arch: Optional[Architecture] = None,
-                 max_positions: Optional[int] = None, ops=None, kv_format: str = "full") -> Tuple[Architecture, Any, Model]:
+                 max_positions: Optional[int] = None, ops=None, kv_format: str = "full", weight_format: str = "full") -> Tuple[Architecture, Any, Model]:
     """Random weights drawn on ``device`` without a file (for models too large to write)."""
     arch = arch or get_architecture(config.architecture)
     model = Model(arch.build_spec(config), dtype=parse_dtype(dtype), device=device, ops=ops or get_ops(),
-                  max_positions=max_positions, kv_format=kv_format)
+                  max_positions=max_positions, kv_format=kv_format, weight_format=weight_format)
     # the architecture draws its tensors under the names a checkpoint of it uses; they take the same
     # way to the parts' names as a checkpoint's do
     tensors: Dict[str, torch.Tensor] = dict(arch.random_tensors(config, seed, device=device, dtype=model.dtype))

@@ -17,14 +17,19 @@ import torch
 from ..parts import attention, block, ffn, latent_attention, moe, norm, pair, recurrent, rope  # noqa: F401  (register the built-in parts)
 from ..parts.base import BLOCKS, NORMS, BuildEnv, CacheNeed, Residual, StateNeed, as_compute
 from ..parts.spec import ModelSpec
+from ..weights.fp8 import WEIGHT_FORMATS
 from ..weights.loader import ExpectedTensor
 
 
 class Model:
     def __init__(self, spec: ModelSpec, *, dtype: torch.dtype, device, ops, max_positions: Optional[int] = None,
-                 kv_format: str = "full"):
+                 kv_format: str = "full", weight_format: str = "full"):
         if dtype not in (torch.float32, torch.bfloat16):
             raise ValueError(f"the engine computes in float32 or bfloat16, not {dtype}")
+        if weight_format not in WEIGHT_FORMATS:
+            raise ValueError(f"weights must be one of {', '.join(WEIGHT_FORMATS)}, got {weight_format!r}")
+        if weight_format == "fp8" and dtype != torch.bfloat16:
+            raise ValueError("weights in 8 bits go with bfloat16 (float32 is the engine's true 32-bit path)")
         self.spec = spec
         self.dtype = dtype
         self.device = torch.device(device)
@@ -34,9 +39,11 @@ class Model:
             # a learned position table ends where it ends: no request can grow past its last row
             self.max_positions = min(self.max_positions, spec.max_positions)
         self.env = BuildEnv(dim=spec.dim, dtype=dtype, device=self.device,
-                            max_positions=self.max_positions, ops=ops, kv_format=kv_format)
+                            max_positions=self.max_positions, ops=ops, kv_format=kv_format, weight_format=weight_format)
         self.blocks = [BLOCKS.build(layer.block, self.env) for layer in spec.layers]
-        self.kv_format = kv_format
+        self.kv_format, self.weight_format = kv_format, weight_format
+        if weight_format != "full" and not any(weight_format in part.weight_formats for b in self.blocks for part in b.parts_within()):
+            raise ValueError(f"no part of this architecture holds its matrices as {weight_format!r}")
         for layer, blk in zip(spec.layers, self.blocks):
             need = blk.cache_need()
             if need is not None and need.format != kv_format:

@@ -13,6 +13,7 @@ import json
 from pathlib import Path
 
 from ..cache.fp4 import CACHE_FORMATS
+from ..weights.fp8 import WEIGHT_FORMATS
 from . import LLM
 
 
@@ -31,6 +32,8 @@ def parse_args(argv=None):
     p.add_argument("--seed", type=int, default=0, help="Seed of the sampling noise.")
     p.add_argument("--kv_cache", type=str, default="full", choices=CACHE_FORMATS,
                    help="How keys and values are held: in the precision's own type, or in 4 bits (fp4).")
+    p.add_argument("--weights", type=str, default="full", choices=WEIGHT_FORMATS,
+                   help="How the layers' matrices are held: in the precision's own type, or in 8 bits (fp8).")
     return p.parse_args(argv)
 
 
@@ -38,7 +41,7 @@ def main(argv=None):
     args = parse_args(argv)
     print("Loading model and tokenizer...")
     llm = LLM(ckpt_paths=args.ckpt_paths, template_config=args.template_config, device=args.device,
-              precision=args.precision, model_kwargs=args.model_kwargs, max_len=args.max_len, max_bsz=1, kv_cache=args.kv_cache)
+              precision=args.precision, model_kwargs=args.model_kwargs, max_len=args.max_len, max_bsz=1, kv_cache=args.kv_cache, weights=args.weights)
     text_mode = llm._load_tokenizer(required=False) is not None and llm.template is not None
     kw = dict(max_new_tokens=args.max_new_tokens, temperature=args.temperature, top_k=args.top_k, seed=args.seed)
 

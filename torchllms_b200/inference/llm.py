@@ -24,6 +24,7 @@ from ..engine.scheduler import Request, Scheduler
 from ..engine.step import Engine
 from ..kernels import get_ops
 from ..sampling.sampler import Sampler, SamplingParams
+from ..weights.fp8 import WEIGHT_FORMATS
 from .template import ChatTemplate, get_template
 
 
@@ -66,6 +67,7 @@ class LLM:
         random_seed: Optional[int] = None,
         ops=None,
         kv_cache: str = "full",
+        weights: str = "full",
     ):
         """``ckpt_paths``: a model folder (``config.json`` + ``model.safetensors``), a file in
         one, or a list of them loaded in order, later tensors overriding earlier ones (the
@@ -78,7 +80,11 @@ class LLM:
         (50 to 350 MB at 2,048 to 14,336 numbers a row).  ``kv_cache`` is how keys and values are held: ``"full"`` (the
         precision's own type) or ``"fp4"`` (4.5 bits a number: 3.6 times the tokens of bfloat16 in the same memory, and as
         much less to read in a decode step; for architectures whose layers are rotary grouped-query attention, with pages
-        of a multiple of 16 tokens; others are refused)."""
+        of a multiple of 16 tokens; others are refused).  ``weights`` is how the layers' matrices are held: ``"full"``, or ``"fp8"`` (8 bits
+        and a scale of a power of two for 128 of them; bfloat16 only): attention, SwiGLU and routed experts hold theirs so, and the
+        rows that meet them are brought to 8 bits too; embedding, head, routers and other parts' matrices stay as they are."""
+        if weights not in WEIGHT_FORMATS:
+            raise ValueError(f"weights must be one of {', '.join(WEIGHT_FORMATS)}, got {weights!r}")
         if kv_cache not in CACHE_FORMATS:
             raise ValueError(f"kv_cache must be one of {', '.join(CACHE_FORMATS)}, got {kv_cache!r}")
         if kv_cache == "fp4":
@@ -89,21 +95,22 @@ class LLM:
         ops = ops or get_ops()
         precision = precision or "bfloat16"
         self.dtype = parse_dtype(precision)
-        if kv_cache == "full":
-            ops.prepare(self.dtype)
-        else:
-            ops.prepare(self.dtype, kv_format=kv_cache)
+        if weights == "fp8" and self.dtype != torch.bfloat16:
+            raise ValueError("weights in 8 bits go with bfloat16 (float32 is the engine's true 32-bit path)")
+        # (what is as usual is not mentioned: an ops object of the caller's own may know nothing else)
+        ops.prepare(self.dtype, **{k: v for k, v in (("kv_format", kv_cache), ("weight_format", weights)) if v != "full"})
         if ckpt_paths is not None:
             paths = [ckpt_paths] if isinstance(ckpt_paths, (str, Path)) else list(ckpt_paths)
             self.model_dir: Optional[Path] = model_dir_of(paths[0])
             self.arch, self.config, self.model = load_model(
                 paths, dtype=self.dtype, device=device, overrides=model_kwargs, max_positions=max_len, ops=ops,
-                kv_format=kv_cache)
+                kv_format=kv_cache, weight_format=weights)
         elif config is not None:
             self.model_dir = None
             config = config.with_overrides(model_kwargs)
             self.arch, self.config, self.model = random_model(
-                config, random_seed or 0, dtype=self.dtype, device=device, max_positions=max_len, ops=ops, kv_format=kv_cache)
+                config, random_seed or 0, dtype=self.dtype, device=device, max_positions=max_len, ops=ops, kv_format=kv_cache,
+                weight_format=weights)
         else:
             raise ValueError("give ckpt_paths (a model folder) or config and random_seed")
         self.max_len = min(int(max_len), self.model.max_positions)     # (a learned position table ends where it ends)

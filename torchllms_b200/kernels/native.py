@@ -170,13 +170,15 @@ class NativeOps:
             _check(self._lib(lib_name).tl_debug_set_limit(which, ctypes.c_longlong(int(value)), _stream()), "debug limit")
 
     # ------------------------------------------------------------ libraries
-    def prepare(self, dtype: torch.dtype, sampling: bool = True, kv_format: str = "full") -> None:
-        """Compile, side by side, what a model of this dtype (and cache format) will call."""
+    def prepare(self, dtype: torch.dtype, sampling: bool = True, kv_format: str = "full", weight_format: str = "full") -> None:
+        """Compile, side by side, what a model of this dtype (and these formats of cache and weights) will call."""
         names = ["elementwise", "sublayer", "rope", "attention", "gemm_simt", "gemm_f32", "recurrent", "moe", "matrix_state", "stream_sum", "conv_mixers", "matrix_recurrence"]
         if dtype == torch.bfloat16:
             names += ["attention_mma", "attention_decode", "gemm_tcgen05"]
         if kv_format == "fp4":
             names += ["kv_fp4", "attention_fp4", "attention_fp4_decode", "attention_fp4_prefill", "fp4_calls"]
+        if weight_format == "fp8":
+            names += ["rows_fp8", "gemm_fp8", "fp8_calls"]
         if sampling:
             names.append("sampling")
         build_libraries(names)
@@ -1709,7 +1711,7 @@ class NativeOps:
         if not (self.use_fused_residual and self.use_tcgen05 and isinstance(pending, PendingProduct)):
             return False
         x, w = pending.x, pending.w
-        if not (x.is_cuda and x.dtype == torch.bfloat16 and w.dtype == torch.bfloat16 and x.dim() == 2 and w.dim() == 2):
+        if isinstance(w, Fp8Rows) or not (x.is_cuda and x.dtype == torch.bfloat16 and w.dtype == torch.bfloat16 and x.dim() == 2 and w.dim() == 2):
             return False
         M, K = x.shape
         N = w.shape[0]
@@ -1772,12 +1774,15 @@ class NativeOps:
                partials_ok: bool = False) -> torch.Tensor:
         """``x [M, K] @ w[N, K]^T``.  float32 is multiplied in true 32-bit (see :meth:`gemm_simt`).  bfloat16 with
         at most 64 rows (decode steps) runs on the tcgen05 kernel that streams the weight once;
-        more rows use the library product, as the reference's ``nn.Linear`` does.
+        more rows use the library product, as the reference's ``nn.Linear`` does.  A weight in 8 bits goes to
+        :meth:`linear_fp8` (whole sums, whatever the number of rows).
 
         With ``partials_ok`` the result may be float32 partial sums ``[splits, M, N]`` of a
         split-K product, for callers that hand it to a kernel which adds them up (residual +
         norm, rope, swiglu).  A :class:`RowScaled` input gives a :class:`RowScaled` result: the
         product is taken of the rows as they are and the scale follows it."""
+        if type(w) is Fp8Rows:
+            return self.linear_fp8(x, w, out_dtype or torch.bfloat16)
         if isinstance(x, RowScaled):
             return x.follow(self.linear(x.x, w, out_dtype, partials_ok))
         _cuda_contig(x, "linear input")

@@ -19,13 +19,16 @@ import torch
 
 from ..kernels.lazy import PendingProduct
 from ..weights.loader import ExpectedTensor
-from .base import (POSITION_ENCODINGS, BuildEnv, CacheNeed, Mixer, StateNeed, as_compute, register_mixer)
+from .base import (POSITION_ENCODINGS, BuildEnv, CacheNeed, Mixer, StateNeed, as_compute, as_held, check_held_width, register_mixer,
+                   stack_held)
 from .rope import precise_rotary_table
 from .spec import PartSpec
 
 
 @register_mixer("attention")
 class PagedAttention(Mixer):
+    weight_formats = ("full", "fp8")
+
     def __init__(self, env: BuildEnv, *, dim: int, n_heads: int, n_kv_heads: int, head_dim: int,
                  scale: float, position: PartSpec, window: Optional[int] = None):
         if n_heads % n_kv_heads != 0:
@@ -38,6 +41,11 @@ class PagedAttention(Mixer):
         self.graph_safe = self.position.graph_safe
         # x only goes into the q/k/v product, whose result the position encoding's kernel may scale
         self.takes_row_scaled = self.position.takes_row_scaled
+        self.held = env.weight_format == "fp8"
+        if self.held:
+            check_held_width(self.dim, "the attention's input")
+            check_held_width(self.n_heads * self.head_dim, "the attention's result")
+            self.takes_row_scaled, self.takes_fp8_rows = False, True
         env.ops.check_attention_sizes(self.n_heads, self.n_kv_heads, self.head_dim, env.dtype)
         self.format = env.kv_format
         if self.format not in self.position.cache_formats:
@@ -65,8 +73,12 @@ class PagedAttention(Mixer):
 
     def load(self, tensors: Mapping[str, torch.Tensor]) -> None:
         # One projection for q, k and v: rows [wq; wk; wv].
-        self.wqkv = torch.cat([as_compute(tensors[n], self.env) for n in ("wq.weight", "wk.weight", "wv.weight")])
-        self.wo = as_compute(tensors["wo.weight"], self.env)
+        names = ("wq.weight", "wk.weight", "wv.weight")
+        if self.held:
+            self.wqkv, self.wo = stack_held([as_held(tensors[n], self.env) for n in names]), as_held(tensors["wo.weight"], self.env)
+        else:
+            self.wqkv = torch.cat([as_compute(tensors[n], self.env) for n in names])
+            self.wo = as_compute(tensors["wo.weight"], self.env)
         self.position.load({name: tensors[f"position.{name}"] for name in self.position.expected_tensors()})
 
     def forward(self, x: torch.Tensor, ctx, cache) -> torch.Tensor:

@@ -29,6 +29,7 @@ from typing import Any, Callable, Dict, Mapping, Optional, Tuple
 import torch
 
 from ..cache.fp4 import CACHE_FORMATS, RECORD, check_head_dim, record_bytes
+from ..weights.fp8 import Fp8Rows, WEIGHT_FORMATS, check_width, encode
 from ..weights.loader import ExpectedTensor
 from .spec import PartSpec
 
@@ -43,6 +44,7 @@ class BuildEnv:
     max_positions: int       # the longest sequence the engine will hold
     ops: Any                 # the kernel library (see torchllms_b200.kernels)
     kv_format: str = "full"  # how keys and values are to be kept (``CacheNeed.format``)
+    weight_format: str = "full"  # how parts that can are to hold their matrices (``Part.weight_formats``)
 
 
 @dataclass(frozen=True)
@@ -185,6 +187,9 @@ class Part:
     # step's token and request counts alone (no read-back, no host-side branching on device
     # data): such a part may be captured into a CUDA graph and replayed.
     graph_safe = False
+    # how this part can hold the matrices of its products: ``"full"`` (the activation dtype) and perhaps ``"fp8"``
+    # (:class:`~torchllms_b200.weights.fp8.Fp8Rows`); one that cannot hold them as ``env.weight_format`` says holds them in full
+    weight_formats: Tuple[str, ...] = ("full",)
 
     def expected_tensors(self) -> Dict[str, ExpectedTensor]:
         return {}
@@ -192,12 +197,21 @@ class Part:
     def load(self, tensors: Mapping[str, torch.Tensor]) -> None:
         pass
 
+    def parts_within(self):
+        """This part and the parts inside it."""
+        yield self
+        for v in vars(self).values():
+            if isinstance(v, Part):
+                yield from v.parts_within()
+
     def weight_bytes(self) -> int:
         """Bytes of the weights this part (and the parts inside it) reads in a step."""
         total = 0
         for v in vars(self).values():
             if isinstance(v, torch.Tensor) and v.is_floating_point():
                 total += v.numel() * v.element_size()
+            elif isinstance(v, Fp8Rows):
+                total += v.nbytes()
             elif isinstance(v, Part):
                 total += v.weight_bytes()
         return total
@@ -214,9 +228,12 @@ class Norm(Part):
     norm with ``can_defer`` also accepts ``deferred_ok=True`` and may then return a
     :class:`~torchllms_b200.kernels.lazy.RowScaled` (rows weighted but not yet normalised, the
     scale to be applied by whoever consumes them); a block passes that flag only to such a norm
-    and only when the part that reads the rows has ``takes_row_scaled``."""
+    and only when the part that reads the rows has ``takes_row_scaled``.  A norm with ``can_hold`` accepts ``fp8_ok=True``
+    and then returns its rows in 8 bits (:class:`~torchllms_b200.weights.fp8.Fp8Rows`); a block passes that flag only when the
+    part that reads the rows has ``takes_fp8_rows``."""
 
     can_defer = False
+    can_hold = False
 
     def forward(self, residual: "Residual", rows: Optional[torch.Tensor] = None) -> torch.Tensor:
         raise NotImplementedError
@@ -257,6 +274,7 @@ class Mixer(Part):
     """
 
     takes_row_scaled = False
+    takes_fp8_rows = False       # ``x`` may be an :class:`~torchllms_b200.weights.fp8.Fp8Rows`
     # A mixer that starts with one product of its input and ends with one product may be run in halves, so that a
     # part that holds several of them can stack their products: ``w_in`` and ``wo`` are the two weights, and
     # ``mix(proj, ctx, cache, out)`` is all that lies between: ``proj`` is ``x @ w_in.T``, a column range of wider rows or
@@ -278,9 +296,10 @@ class Mixer(Part):
 
 class FeedForward(Part):
     """``forward(x [T, dim], ctx) -> [T, dim]`` (activation dtype); tokens do not interact.
-    ``takes_row_scaled`` and a pending last projection as for a mixer."""
+    ``takes_row_scaled``, ``takes_fp8_rows`` and a pending last projection as for a mixer."""
 
     takes_row_scaled = False
+    takes_fp8_rows = False
 
     def forward(self, x: torch.Tensor, ctx) -> torch.Tensor:
         raise NotImplementedError
@@ -392,3 +411,19 @@ register_block = BLOCKS.register
 def as_compute(t: torch.Tensor, env: BuildEnv) -> torch.Tensor:
     """A matrix weight on the device in the activation dtype, contiguous."""
     return t.to(device=env.device, dtype=env.dtype).contiguous()
+
+
+def check_held_width(width: int, what: str) -> None:
+    """8-bit rows take a multiple of 16 numbers: said when a part is built, not when its weights arrive."""
+    check_width(width, f"8-bit weights: {what}")
+
+
+def as_held(t: torch.Tensor, env: BuildEnv, rows_at_once: int = 4096) -> Fp8Rows:
+    """A matrix weight ``[rows, width]`` on the device in 8 bits (some rows at a time: bringing them there takes several times their memory)."""
+    parts = [encode(t[a:a + rows_at_once].to(env.device)) for a in range(0, t.shape[0], rows_at_once)]
+    return Fp8Rows(torch.cat([c for c, _s in parts]), torch.cat([s.view(torch.uint8) for _c, s in parts]).view(parts[0][1].dtype))
+
+
+def stack_held(parts) -> Fp8Rows:
+    """Matrices of equal width as one, rows behind rows."""
+    return Fp8Rows(torch.cat([p.codes for p in parts]), torch.cat([p.scales.view(torch.uint8) for p in parts]).view(parts[0].scales.dtype))

@@ -80,7 +80,9 @@ class PreNormBlock(Block):
 
     @staticmethod
     def _normed(norm, reader, residual: Residual):
-        """The rows for ``reader``: with their normalisation deferred where both sides can."""
+        """The rows for ``reader``: in 8 bits, or with their normalisation deferred, where both sides can."""
+        if norm.can_hold and reader.takes_fp8_rows:
+            return norm.forward(residual, fp8_ok=True)
         if norm.can_defer and reader.takes_row_scaled:
             return norm.forward(residual, deferred_ok=True)
         return norm.forward(residual)

@@ -13,17 +13,23 @@ import torch
 
 from ..kernels.lazy import PendingProduct
 from ..weights.loader import ExpectedTensor
-from .base import BuildEnv, FeedForward, as_compute, register_feed_forward
+from .base import BuildEnv, FeedForward, as_compute, as_held, check_held_width, register_feed_forward, stack_held
 
 
 @register_feed_forward("swiglu")
 class SwiGLU(FeedForward):
     graph_safe = True
     takes_row_scaled = True      # x only goes into the gate/up product, whose activation applies the scale
+    weight_formats = ("full", "fp8")
 
     def __init__(self, env: BuildEnv, *, dim: int, hidden: int):
         self.env = env
         self.dim, self.hidden = int(dim), int(hidden)
+        self.held = env.weight_format == "fp8"
+        if self.held:
+            check_held_width(self.dim, "the feed-forward's input")
+            check_held_width(self.hidden, "the feed-forward's hidden rows")
+            self.takes_row_scaled, self.takes_fp8_rows = False, True
         self.w13: Optional[torch.Tensor] = None
         self.w2: Optional[torch.Tensor] = None
 
@@ -35,6 +41,10 @@ class SwiGLU(FeedForward):
         }
 
     def load(self, tensors: Mapping[str, torch.Tensor]) -> None:
+        if self.held:
+            self.w13 = stack_held([as_held(tensors["w1.weight"], self.env), as_held(tensors["w3.weight"], self.env)])
+            self.w2 = as_held(tensors["w2.weight"], self.env)
+            return
         self.w13 = torch.cat([as_compute(tensors["w1.weight"], self.env), as_compute(tensors["w3.weight"], self.env)])
         self.w2 = as_compute(tensors["w2.weight"], self.env)
 
@@ -43,6 +53,8 @@ class SwiGLU(FeedForward):
         # gate and up in one product over the stacked weight, the activation in its epilogue where the
         # kernel can (decode steps), else product [T, 2 * hidden] + SwiGLU kernel
         # the down projection is left to the norm that follows (see PendingProduct)
+        if self.held:             # gate, up, the activation and the 8-bit rows of it in one kernel, whatever the number of rows
+            return PendingProduct(ops.linear_activation_fp8(x, self.w13, "silu", gated=True), self.w2)
         return PendingProduct(ops.linear_swiglu(x, self.w13), self.w2)
 
 

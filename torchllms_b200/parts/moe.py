@@ -17,7 +17,8 @@ import torch
 
 from ..kernels.lazy import PendingProduct
 from ..weights.loader import ExpectedTensor
-from .base import BuildEnv, FeedForward, as_compute, register_feed_forward
+from ..weights.fp8 import Fp8Rows
+from .base import BuildEnv, FeedForward, as_compute, as_held, check_held_width, register_feed_forward, stack_held
 
 EXPERT_ACTIVATIONS = ("relu2", "silu", "gelu_tanh", "gelu", "clamped_swish")      # ("gelu" is the exact form, with erf)
 
@@ -49,6 +50,7 @@ class RoutedExperts(FeedForward):
     ``shared.gate.weight [1, dim]``."""
 
     graph_safe = True
+    weight_formats = ("full", "fp8")     # (the experts' and the shared expert's matrices; the router's stays in 32-bit)
 
     def __init__(self, env: BuildEnv, *, dim: int, n_experts: int, top: int, hidden: int, activation: str = "relu2",
                  router_scale: float = 1.0, choice_correction: bool = False, renormalize: bool = False,
@@ -64,6 +66,12 @@ class RoutedExperts(FeedForward):
             raise ValueError("a gate of the shared expert needs a shared expert")
         self.env = env
         self.dim, self.n_experts, self.top, self.hidden = int(dim), int(n_experts), int(top), int(hidden)
+        self.held = env.weight_format == "fp8"
+        if self.held:
+            check_held_width(self.dim, "the experts' input")
+            check_held_width(self.hidden, "the experts' hidden rows")
+            if shared_hidden:
+                check_held_width(int(shared_hidden), "the shared expert's hidden rows")
         self.activation = activation
         self.router_scale = float(router_scale)
         self.choice_correction, self.renormalize = bool(choice_correction), bool(renormalize)
@@ -100,6 +108,7 @@ class RoutedExperts(FeedForward):
         self.w_up_all: Optional[torch.Tensor] = None
         self.w_down_all: Optional[torch.Tensor] = None
         self.w_up: Optional[torch.Tensor] = None           # [E, hidden, dim], a view of w_up_all
+        self.w_down: Optional[Fp8Rows] = None              # 8-bit experts only: [E, dim, hidden]
         self.w_shared_up: Optional[torch.Tensor] = None    # a view of w_up_all
         self.w_shared_down: Optional[torch.Tensor] = None  # a copy of its own (the products want whole rows)
 
@@ -133,6 +142,9 @@ class RoutedExperts(FeedForward):
             self.correction = tensors["correction"].to(**f32).contiguous()
         if self.router_bias:
             self.logit_bias = tensors["router.bias"].to(**f32).contiguous()
+        if self.held:
+            self._load_held(tensors)
+            return
         ups = [as_compute(tensors[f"experts.{e}.up.weight"], self.env) for e in range(self.n_experts)]
         if self.gated:        # an expert's rows are [gate; up], so that one product yields both
             ups = [torch.cat([as_compute(tensors[f"experts.{e}.gate.weight"], self.env), up]) for e, up in enumerate(ups)]
@@ -150,9 +162,25 @@ class RoutedExperts(FeedForward):
         if self.shared_hidden:
             self.w_shared_up = self.w_up_all[n:]
 
+    def _load_held(self, tensors: Mapping[str, torch.Tensor]) -> None:
+        """8-bit experts: ``w_up`` ``[E, hidden (gated: 2 * hidden), dim]``, ``w_down`` ``[E, dim, hidden]``, the shared expert by itself."""
+        held = lambda name: as_held(tensors[name], self.env)  # noqa: E731
+        ups = [stack_held([held(f"experts.{e}.gate.weight"), held(f"experts.{e}.up.weight")]) if self.gated else held(f"experts.{e}.up.weight")
+               for e in range(self.n_experts)]
+        downs = [held(f"experts.{e}.down.weight") for e in range(self.n_experts)]
+        each = lambda rows, n: Fp8Rows(rows.codes.unflatten(0, (n, -1)), rows.scales.unflatten(0, (n, -1)))  # noqa: E731
+        self.w_up, self.w_down = each(stack_held(ups), self.n_experts), each(stack_held(downs), self.n_experts)
+        if self.shared_hidden:
+            up = held("shared.up.weight")
+            self.w_shared_up = stack_held([held("shared.w_gate.weight"), up]) if self.gated else up
+            self.w_shared_down = held("shared.down.weight")
+
     def weight_bytes(self) -> int:
         """What a step reads at most: the router and every expert (a step of few tokens leaves most
         experts alone; this counts all of them)."""
+        if self.held:
+            held = [t for t in (self.w_up, self.w_down, self.w_shared_up, self.w_shared_down) if t is not None]
+            return self.w_router.numel() * self.w_router.element_size() + sum(t.nbytes() for t in held)
         return sum(t.numel() * t.element_size() for t in (self.w_router, self.w_up_all, self.w_down_all))
 
     def forward(self, x: torch.Tensor, ctx):
@@ -162,6 +190,13 @@ class RoutedExperts(FeedForward):
                                               shared_gate=self.shared_gate, logit_bias=self.logit_bias, score=self.score,
                                               n_groups=self.n_groups, keep_groups=self.keep_groups,
                                               group_score_top=self.group_score_top, renorm_eps=self.renorm_eps)
+        if self.held:
+            shared = None
+            if self.shared_hidden:
+                u = ops.linear_activation_fp8(x, self.w_shared_up, self.activation, gated=self.gated, act_params=self.shared_act_params)
+                shared = ops.linear(u, self.w_shared_down)
+            return ops.moe_experts_fp8(x, chosen, weights, self.w_up, self.w_down, activation=self.activation, shared=shared, shared_gate=gate,
+                                       gated=self.gated, act_params=self.act_params)
         if ops.moe_prefers_dense(x.shape[0], self.top, self.n_experts, x.dtype):
             # few tokens that touch most experts between them: every expert (and the shared one) as one
             # matrix each way, the rows of experts a token did not choose multiplied by zero

@@ -24,6 +24,7 @@ from typing import Dict, Mapping, Optional
 import torch
 
 from ..kernels.lazy import PendingProduct
+from ..weights.fp8 import ALIGN as FP8_ALIGN, MAX_NORM_WIDTH
 from ..weights.loader import ExpectedTensor
 from .base import BuildEnv, Norm, Residual, register_norm
 
@@ -45,6 +46,7 @@ class RMSNorm(Norm):
             raise ValueError(f"a norm over {dim} coordinates cannot have {groups} equal groups")
         self.groups = int(groups)
         self.can_defer = self.groups == 1
+        self.can_hold = self.groups == 1 and dim % FP8_ALIGN == 0 and dim <= MAX_NORM_WIDTH
         self.env = env
         self.scalar = bool(scalar)
         self.dim = int(dim)
@@ -62,11 +64,15 @@ class RMSNorm(Norm):
             w = w * self.weight_scale
         self.weight = (w.reshape(1).expand(self.dim) if self.scalar else w).contiguous()
 
-    def forward(self, residual: Residual, rows: Optional[torch.Tensor] = None, deferred_ok: bool = False):
+    def forward(self, residual: Residual, rows: Optional[torch.Tensor] = None, deferred_ok: bool = False, fp8_ok: bool = False):
         ops = self.env.ops
         # 32-bit mode keeps the reference's order of operations to the letter
         deferred = bool(deferred_ok and rows is None and self.env.dtype == torch.bfloat16)
         delta, scale = residual.delta, residual.delta_scale
+        if fp8_ok and rows is None and scale is None:
+            out = ops.rmsnorm_fp8(residual.h, delta, self.weight, self.eps)
+            residual.delta = residual.rows = None
+            return out
         if self.groups > 1 or scale is not None:
             out = ops.rmsnorm(residual.h, delta, self.weight, self.eps, out_dtype=self.env.dtype, rows=rows, groups=self.groups,
                               delta_scale=scale)

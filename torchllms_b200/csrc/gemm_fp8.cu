@@ -26,6 +26,10 @@ namespace {
 constexpr int BM = 128;              // rows of W a CTA
 constexpr int BK = 128;              // bytes of K a box: a swizzle row, and a block of numbers that share a scale
 constexpr int MAX_WIDTH = 240;       // rows of x a tile: two accumulators and two sets of scales fill 512 columns
+// Split: tiles so narrow send their sums to where they are added up, wider ones, whose sums would take room from the stages, leave them to
+// be fetched (8 rows of 4,096 x 14,336: 13.5 us sent, 14.6 fetched; 64 rows 16.0 and 15.4); and tiles so narrow share an SM.
+constexpr int PUSH_WIDTH = 32;
+constexpr int SHARED_WIDTH = 64;
 constexpr int MAX_SPLIT_WIDTH = 224; // the same with one accumulator in 256 columns
 constexpr int COLUMNS = 256;
 constexpr int MAX_STAGES = 12;
@@ -36,7 +40,7 @@ enum : int { PLAIN = 0, ACT = 1, GATED = 2 };       // what becomes of the sums:
 // Warps that take the results: eight, two to a quarter of tensor memory's lanes, with every other 32 columns each (one warp a scheduler
 // waits for its own instructions: 524 us for 275 where 2,048 tokens go through gates and ups of 32 experts); split, four, where
 // two CTAs share an SM.
-__host__ __device__ constexpr int result_warps(int form) { return form == SPLIT ? 4 : 8; }
+__host__ __device__ constexpr int result_warps(int form) { return form == SPLIT ? 4 : 8; }       // (two CTAs of SPLIT may share an SM)
 __host__ __device__ constexpr int threads_of(int form) { return 32 * (4 + result_warps(form)); }
 constexpr int STAGING = 8 * 2048;    // 32 x 32 results a warp
 constexpr unsigned ACC_COLS = 256;   // a second accumulator lies so many columns behind the first
@@ -94,6 +98,8 @@ __device__ __forceinline__ void arrive_elect(unsigned bar) {
     }
     asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t@e mbarrier.arrive.shared::cluster.b64 _, [%0];\n\t}" ::"r"(bar) : "memory");
 }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -104,6 +110,10 @@ __device__ __forceinline__ void store_async(unsigned addr, unsigned v, unsigned 
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(bar), "r"(cta));
     asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(at), "r"(v), "r"(there) : "memory");
 }
+__device__ __forceinline__ void store_async4(unsigned at, const unsigned* v, unsigned bar) {
+    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];"
+                 ::"r"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(bar) : "memory");
+}
 // 16 bytes of another CTA's shared memory
 __device__ __forceinline__ float4 load_from(unsigned addr, int cta) {
     unsigned at;
@@ -112,10 +122,10 @@ __device__ __forceinline__ float4 load_from(unsigned addr, int cta) {
     asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
     return v;
 }
-// the address of the pair's first CTA's variable of the same place
-__device__ __forceinline__ unsigned in_leader(unsigned addr) {
+// the address of another CTA's variable of the same place
+__device__ __forceinline__ unsigned in_cta(unsigned addr, int cta) {
     unsigned r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(cta));
     return r;
 }
 __device__ __forceinline__ void expect_tx(unsigned bar, unsigned bytes) {
@@ -191,10 +201,9 @@ __device__ __forceinline__ void copy_scales(unsigned taddr, unsigned long long d
 #undef TL_COPY
 }
 template <bool PAIR>
-__device__ __forceinline__ void commit(unsigned bar) {
+__device__ __forceinline__ void commit(unsigned bar, unsigned short both) {
     if (PAIR)
-        asm volatile("{\n\t.reg .b16 m;\n\tmov.b16 m, 3;\n\t"
-                     "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], m;\n\t}" ::"r"(bar) : "memory");
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"(both) : "memory");
     else
         asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
@@ -264,6 +273,7 @@ struct Params {
     int slabs, n_tiles, stages, scale_bufs;
     int out_is_f32;
     bool w_whole, x_whole;           // scales: rows are a multiple of 16 bytes and start on 16
+    int push_bytes;                  // SPLIT, narrow tiles: where the CTAs of a cluster send what this one adds up
     int splits, split_blocks;        // SPLIT: CTAs of a cluster, and blocks of K of each (a multiple of 4)
     // ACT, GATED: the 8-bit rows that leave, [M, N] (GATED: [M, N / 2]), and what is done to the sums
     unsigned char *codes, *scales;
@@ -298,6 +308,12 @@ __device__ __forceinline__ Unit unit_of(const Params& p, int u, int n_tiles) {
     return r;
 }
 
+// SPLIT: groups of four rows of x are dealt out to the CTAs of a cluster: how many of a tile's one adds up
+__device__ __forceinline__ int groups_of(int rows, int cta, int ctas) {
+    const int groups = (rows + 3) / 4;
+    return groups > cta ? (groups - cta - 1) / ctas + 1 : 0;
+}
+
 template <int FORM, int EPI, int ACTIVATION>
 __global__ void __launch_bounds__(threads_of(FORM), FORM == SPLIT ? 2 : 1) gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                                                                const Params p) {
@@ -305,15 +321,15 @@ __global__ void __launch_bounds__(threads_of(FORM), FORM == SPLIT ? 2 : 1) gemm_
     const unsigned smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u;            // tiles want 1,024-byte alignment for the swizzle
     unsigned char* const smem_at = smem_raw + (smem0 - smem_u32(smem_raw));
     // a pair shares a unit of 256 rows of W: each CTA has 128 of them and half of the tile's rows of x
-    constexpr bool PAIR = FORM == PAIRS;
+    constexpr bool PAIR = FORM == PAIRS, CUT = FORM == SPLIT;
     constexpr int BOXES = boxes_of(FORM);
     constexpr int SIDES = PAIR ? 2 : 1;
     const int rank = PAIR ? (int)(blockIdx.x & 1) : 0;
     // split: a cluster to a unit, every CTA with a run of its blocks of K
-    const int cut = FORM == SPLIT ? (int)(blockIdx.x % (unsigned)p.splits) : 0;
-    const int first_unit = FORM == SPLIT ? (int)(blockIdx.x / (unsigned)p.splits) : (int)blockIdx.x / SIDES;
-    const int step = FORM == SPLIT ? p.n_tiles * p.slabs : (int)gridDim.x / SIDES;
-    const int kb0 = cut * p.split_blocks, kb1 = FORM == SPLIT ? min(kb0 + p.split_blocks, p.k_blocks) : p.k_blocks;
+    const int group = (int)blockIdx.x / SIDES, cut = CUT ? group % p.splits : 0;
+    const int first_unit = CUT ? group / p.splits : group;
+    const int step = CUT ? p.n_tiles * p.slabs : (int)gridDim.x / SIDES;
+    const int kb0 = cut * p.split_blocks, kb1 = CUT ? min(kb0 + p.split_blocks, p.k_blocks) : p.k_blocks;
     const unsigned w_bytes = BM * BK, x_bytes = p.width / SIDES * BK, stage_bytes = BOXES * (w_bytes + x_bytes);
     const unsigned scales_at = smem0 + p.stages * stage_bytes, word_bytes = scale_bytes(p.width), turn_bytes = 4 * word_bytes;
     unsigned char* const staging = smem_at + p.stages * stage_bytes + p.scale_bufs * turn_bytes;
@@ -325,20 +341,25 @@ __global__ void __launch_bounds__(threads_of(FORM), FORM == SPLIT ? 2 : 1) gemm_
     __shared__ __align__(8) unsigned long long bars[2 * MAX_STAGES + 2 * MAX_SCALE_BUFS + 7];
     __shared__ unsigned tmem_slot;
     __shared__ int abort_flag;
+    unsigned char* const pushed = staging;               // SPLIT (which stages nothing): [group of four rows of x of this CTA's][split][row of W][4]
     const unsigned bar0 = smem_u32(bars);
     const unsigned full = bar0, empty = bar0 + 8 * MAX_STAGES, sc_full = bar0 + 16 * MAX_STAGES, sc_empty = sc_full + 8 * MAX_SCALE_BUFS;
     const unsigned acc_full = sc_empty + 8 * MAX_SCALE_BUFS, acc_empty = acc_full + 16, drained = acc_empty + 16, told = drained + 8;
     // (what the first CTA's issuing warp waits for counts arrivals of both)
-    auto leader = [&](unsigned bar) { return PAIR ? in_leader(bar) : bar; };
+    auto leader = [&](unsigned bar) { return PAIR ? in_cta(bar, 0) : bar; };
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 32) {           // (descriptors come from memory: on their way while the barriers are set up)
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_x) : "memory");
+    }
     if (threadIdx.x == 0) {
         abort_flag = 0;
         for (int s = 0; s < MAX_STAGES; ++s) { mbar_init(full + 8 * s, 1); mbar_init(empty + 8 * s, 1); }
         for (int s = 0; s < MAX_SCALE_BUFS; ++s) { mbar_init(sc_full + 8 * s, SIDES); mbar_init(sc_empty + 8 * s, 1); }
         for (int s = 0; s < 2; ++s) { mbar_init(acc_full + 8 * s, 1); mbar_init(acc_empty + 8 * s, result_warps(FORM) * SIDES); }
         mbar_init(drained, 1);
-        if (EPI == GATED) { mbar_init(told, 1); mbar_init(told + 8, 1); }
+        if (EPI == GATED || CUT) { mbar_init(told, 1); mbar_init(told + 8, 1); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -353,9 +374,16 @@ __global__ void __launch_bounds__(threads_of(FORM), FORM == SPLIT ? 2 : 1) gemm_
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     if (PAIR) cluster_sync();          // both CTAs' barriers are set up and both have their tensor memory
+    if (CUT && p.push_bytes > 0) {
+        // (said here, waited for by those that send, when they do)
+        if (threadIdx.x == 0) expect_tx(told, groups_of(unit_of(p, first_unit, p.n_tiles).rows, cut, p.splits) * p.splits * (BM * 16));
+        __syncwarp();
+        cluster_arrive();
+    }
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const unsigned tmem = tmem_slot;
     volatile int* aborted = &abort_flag;
+    bool met = false;                  // SPLIT: whether the cluster has been waited for
     grid_launch_dependents();
     // W and its scales depend on no earlier kernel: the first boxes of a product without a list of tiles are asked for ahead
     const bool ahead = p.tiles == nullptr;
@@ -425,6 +453,7 @@ __global__ void __launch_bounds__(threads_of(FORM), FORM == SPLIT ? 2 : 1) gemm_
         __syncwarp();
     } else if (warp == 1 && rank == 0) {
         if (elect_one()) {
+            const unsigned short both = 3;         // (CTAs of the pair)
             int stage = 0, buf = 0, n = 0;
             unsigned phase = 0, sc_phase = 0, word = 0;
             bool ok = true;
@@ -468,18 +497,18 @@ __global__ void __launch_bounds__(threads_of(FORM), FORM == SPLIT ? 2 : 1) gemm_
                             for (int k = 0; k < 4; ++k) mma<PAIR>(d, a + 2 * k, b + 2 * k, idesc, set, set + 4, (kb > kb0 || i > 0 || k > 0) ? 1u : 0u);
                         }
                     }
-                    commit<PAIR>(empty + 8 * stage);
+                    commit<PAIR>(empty + 8 * stage, both);
                     if (++stage == p.stages) { stage = 0; phase ^= 1; }
                     if ((kb - kb0) % TURN == TURN - BOXES || kb + BOXES >= kb1) {
-                        commit<PAIR>(sc_empty + 8 * buf);
+                        commit<PAIR>(sc_empty + 8 * buf, both);
                         if (++buf == p.scale_bufs) { buf = 0; sc_phase ^= 1; }
                     }
                 }
-                if (ok) commit<PAIR>(acc_full + 8 * acc);
+                if (ok) commit<PAIR>(acc_full + 8 * acc, both);
             }
             // (the products read shared memory and their commits write barriers: all of it ends before the CTA does)
             int none = 0;
-            commit<PAIR>(drained);
+            commit<PAIR>(drained, both);
             wait_one(drained, 0, &none);
         }
         __syncwarp();
@@ -553,7 +582,17 @@ __global__ void __launch_bounds__(threads_of(FORM), FORM == SPLIT ? 2 : 1) gemm_
                 // (a load of 32 columns may reach into the scales' columns behind the accumulator: read, not used)
                 tmem_load32(tmem + acc * ACC_COLS + ((unsigned)(quarter * 32) << 16) + c0, r);
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                if (FORM == SPLIT) {
+                if (CUT && p.push_bytes > 0) {
+                    if (!met) cluster_wait();          // (all barriers of the cluster are set up)
+                    met = true;
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4) {
+                        const int g = (c0 + j) / 4;
+                        if (c0 + j < t.rows)
+                            store_async4(in_cta(smem_u32(pushed) + ((g / p.splits * p.splits + cut) * BM + quarter * 32 + lane) * 16, g % p.splits), r + j,
+                                         in_cta(told, g % p.splits));
+                    }
+                } else if (CUT) {
                     // (every product of the CTA has been taken: the stages are free)
 #pragma unroll
                     for (int j = 0; j < 32; ++j)
@@ -585,6 +624,31 @@ __global__ void __launch_bounds__(threads_of(FORM), FORM == SPLIT ? 2 : 1) gemm_
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             arrive_elect<PAIR>(leader(acc_empty + 8 * acc));
+            if (CUT && p.push_bytes > 0) {
+                // this CTA's groups, added up in the order of K: a row of W a lane, four rows of x
+                const int own = groups_of(t.rows, cut, p.splits), row = t.slab * BM + quarter * 32 + lane;
+                if (own > 0 && !mbar_wait(told, 0, aborted)) {
+                    if (lane == 0) give_up(aborted, p.status, ERR_EPI_WAIT);
+                    break;
+                }
+                for (int i = 0; i < own; ++i) {
+                    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+                    for (int s = 0; s < p.splits; ++s) {
+                        const float4 v = *reinterpret_cast<const float4*>(pushed + ((i * p.splits + s) * BM + quarter * 32 + lane) * 16);
+                        if (s == 0) a = v;
+                        else { a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w; }
+                    }
+                    const float q[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int c = (i * p.splits + cut) * 4 + j;
+                        if (c >= t.rows || row >= p.N) break;
+                        const size_t at = (size_t)(t.row0 + c) * p.N + row;
+                        if (p.out_is_f32) reinterpret_cast<float*>(p.out)[at] = q[j];
+                        else reinterpret_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(q[j]);
+                    }
+                }
+            }
         }
     } else if (warp >= 4) {
         // The sums become 8-bit rows: the activation, the largest magnitude of every 128 for each row of x, the numbers under their
@@ -705,13 +769,17 @@ __global__ void __launch_bounds__(threads_of(FORM), FORM == SPLIT ? 2 : 1) gemm_
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    if (CUT && p.push_bytes > 0 && !met) cluster_wait();       // (every thread waits once; the result warps did when they sent)
     __syncthreads();
-    if (FORM == SPLIT) {
-        // every CTA adds up, in the order of K, the rows cut, cut + splits, .. of x's tile: 32 threads a row, four rows of W a thread
+    // a CTA that gave up does not end before the others have (whatever they send it has somewhere to land)
+    if (CUT && p.push_bytes > 0 && *aborted) cluster_sync();
+    if (CUT && p.push_bytes == 0) {
+        // every CTA adds up, in the order of K, the rows cut, cut + splits, .. of x's tile for its rows of W: 32 threads a row, four
+        // rows of W a thread
         cluster_sync();
         const Unit t = unit_of(p, first_unit, n_tiles);
         const unsigned sums = smem0 + (threadIdx.x & 31) * 16;
-        const int row = t.slab * BM + (threadIdx.x & 31) * 4;
+        const int row = (t.slab * SIDES + rank) * BM + (threadIdx.x & 31) * 4;
         for (int c = cut + (threadIdx.x >> 5) * p.splits; c < t.rows && !*aborted; c += (threads_of(FORM) >> 5) * p.splits) {
             float4 v[8];
 #pragma unroll
@@ -838,7 +906,11 @@ int launch(Params& p, const void* x, const void* w, int experts, int K, cudaStre
     const int stage_bytes = boxes_of(FORM) * (BM * BK + p.width / SIDES * BK);
     p.scale_bufs = FORM == SPLIT ? (p.split_blocks + TURN - 1) / TURN : MAX_SCALE_BUFS;
     if (p.scale_bufs > MAX_SCALE_BUFS) p.scale_bufs = MAX_SCALE_BUFS;
-    const int fixed = 1024 + p.scale_bufs * 4 * scale_bytes(p.width) + (FORM == SPLIT ? 0 : STAGING) + (EPI == PLAIN ? 0 : 7 * COLUMNS * 4);     // (1,024 to align)
+    if (FORM == SPLIT && p.width <= PUSH_WIDTH) {
+        const int groups = p.width / 4;
+        p.push_bytes = (groups + p.splits - 1) / p.splits * p.splits * BM * 16;
+    }
+    const int fixed = 1024 + p.push_bytes + p.scale_bufs * 4 * scale_bytes(p.width) + (FORM == SPLIT ? 0 : STAGING) + (EPI == PLAIN ? 0 : 7 * COLUMNS * 4);     // (1,024 to align)
     int room = 226 * 1024;                          // (a kilobyte is left for barriers)
     if (FORM == SPLIT) {
         // one accumulator, one unit: narrow tiles leave room for a second CTA on an SM
@@ -846,7 +918,7 @@ int launch(Params& p, const void* x, const void* w, int experts, int K, cudaStre
         p.scale_col = p.width;
         p.set_cols = sets;
         p.tmem_cols = whole_columns(p.width + 2 * sets);
-        if (units * p.splits > sms && p.tmem_cols <= 256) room = 112 * 1024;
+        if (p.width <= SHARED_WIDTH && units * p.splits > sms) room = 112 * 1024;
     } else {
         p.scale_col = MAX_WIDTH;
         p.set_cols = ACC_COLS;
@@ -854,7 +926,7 @@ int launch(Params& p, const void* x, const void* w, int experts, int K, cudaStre
     }
     p.stages = (room - fixed) / stage_bytes;
     if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
-    if (p.stages < 1 || (FORM == SPLIT && p.stages * stage_bytes < p.width * BM * 4)) return TL_TOO_LARGE;
+    if (p.stages < 1 || (FORM == SPLIT && p.push_bytes == 0 && p.stages * stage_bytes < p.width * BM * 4)) return TL_TOO_LARGE;
     CUtensorMap mw, mx;
     int rc = EPI == GATED ? make_gated_map(&mw, w, experts, p.hidden, K) : make_map(&mw, w, (long long)experts * p.N, K, BM);
     if (rc != TL_OK) return rc;
@@ -870,7 +942,7 @@ int launch(Params& p, const void* x, const void* w, int experts, int K, cudaStre
         raised[dev] = true;
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(FORM == SPLIT ? units * p.splits : SIDES * (units < sms / SIDES ? units : sms / SIDES));
+    cfg.gridDim = dim3(FORM == SPLIT ? SIDES * units * p.splits : SIDES * (units < sms / SIDES ? units : sms / SIDES));
     cfg.blockDim = dim3(threads_of(FORM));
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
@@ -878,7 +950,7 @@ int launch(Params& p, const void* x, const void* w, int experts, int K, cudaStre
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = FORM == SPLIT ? p.splits : SIDES;
+    attr[1].val.clusterDim.x = SIDES * (FORM == SPLIT ? p.splits : 1);
     attr[1].val.clusterDim.y = 1;
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
@@ -886,15 +958,40 @@ int launch(Params& p, const void* x, const void* w, int experts, int K, cudaStre
     return (int)cudaLaunchKernelEx(&cfg, kern, mw, mx, p);
 }
 
-// splits of K for `units` units: as many as find room at once (two CTAs an SM where tiles are narrow), no more than a cluster
-// holds, each with at least four blocks
-int splits_for(int units, int k_blocks, int width, int sms) {
-    const int slots = width <= 64 ? 2 * sms : sms;
-    int splits = units > 0 ? slots / units : 1;
-    if (splits > 8) splits = 8;
-    const int words = (k_blocks + 3) / 4;
-    if (splits > words) splits = words;
-    if (splits < 1) splits = 1;
+// Clusters of so many CTAs that find room at the same time, with this much shared memory a CTA: asked once.
+int clusters_at_once(int ctas, int room) {
+    static int known[MAX_DEVICES][2][9];
+    int& n = known[current_device()][room < 200 * 1024 ? 1 : 0][ctas];
+    if (n == 0) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(ctas * 64);
+        cfg.blockDim = dim3(threads_of(SPLIT));
+        cfg.dynamicSmemBytes = room;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = ctas;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        auto kern = gemm_fp8_kernel<SPLIT, PLAIN, 0>;
+        int found = 0;
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024) != cudaSuccess ||
+            cudaOccupancyMaxActiveClusters(&found, kern, &cfg) != cudaSuccess) {
+            cudaGetLastError();
+            found = 128 / ctas;
+        }
+        n = found < 1 ? 1 : found;
+    }
+    return n;
+}
+
+// splits of K for `units` units: as many as let all clusters run at once (two CTAs an SM where tiles are narrow), at most eight, each
+// with at least four blocks
+int splits_for(int units, int k_blocks, int width) {
+    const int words = (k_blocks + 3) / 4, room = (width <= SHARED_WIDTH ? 112 : 226) * 1024;
+    int splits = words < 8 ? words : 8;
+    while (splits > 1 && units > clusters_at_once(splits, room)) --splits;
     const int per = (words + splits - 1) / splits;
     return (words + per - 1) / per;                 // no empty split
 }
@@ -928,12 +1025,12 @@ int sums(const void* x, const void* x_scales, const void* w, const void* w_scale
     const int rc = fill(p, x, x_scales, w, w_scales, M, N, K, experts, tiles, most_tiles, width, status);
     if (rc != TL_OK) return rc;
     if (!aligned16(out)) return TL_BAD_ALIGN;
-    if (form < 0 || form > 3 || (form == SPLIT && (tiles != nullptr || width > MAX_SPLIT_WIDTH))) return TL_BAD_SIZE;
+    if (form < 0 || form > 3 || (form == SPLIT && tiles != nullptr) || (form == SPLIT && width > MAX_SPLIT_WIDTH)) return TL_BAD_SIZE;
     p.out = out;
     p.out_is_f32 = out_is_f32;
     if (form == 0) form = form_for(width);
     if (form == SPLIT) {
-        p.splits = splits_for(((N + BM - 1) / BM) * most_tiles, p.k_blocks, width, sm_count());
+        p.splits = splits_for(((N + BM - 1) / BM) * most_tiles, p.k_blocks, width);
         const int words = (p.k_blocks + 3) / 4;
         p.split_blocks = 4 * ((words + p.splits - 1) / p.splits);
         return launch<SPLIT>(p, x, w, experts, K, s);
@@ -955,12 +1052,12 @@ int tile_rows(int pairs, int experts) {
 extern "C" int tl_gemm_fp8(const void* x, const void* x_scales, const void* w, const void* w_scales, void* out, int out_is_f32, int M, int N, int K,
                            int form, int* status, void* stream) {
     if (M <= 0) return TL_OK;
-    int width = even_width(M, MAX_WIDTH);
-    // Few units leave SMs idle: their K is cut among the CTAs of a cluster.
+    // Few units leave SMs idle: their K is cut among the CTAs of a cluster.  (64 rows of 4,096 x 14,336: 25 us whole, 15.4 cut; 701 of
+    // 2,048 x 8,192: 23.4 in pairs, 18.2 cut; 512 of 6,144 x 4,096, 144 units: 14.7 in pairs, 20.4 cut.)
     const int narrow = even_width(M, MAX_SPLIT_WIDTH), units = ((N + BM - 1) / BM) * ((M + narrow - 1) / narrow);
     if (form == 0 && 2 * units <= sm_count() && K > 4 * BK) form = SPLIT;
-    if (form == SPLIT) width = narrow;
-    return sums(x, x_scales, w, w_scales, out, out_is_f32, M, N, K, 1, nullptr, (M + width - 1) / width, width, form, status, (cudaStream_t)stream);
+    const int width = form == SPLIT ? narrow : even_width(M, MAX_WIDTH), tiles = (M + width - 1) / width;
+    return sums(x, x_scales, w, w_scales, out, out_is_f32, M, N, K, 1, nullptr, tiles, width, form, status, (cudaStream_t)stream);
 }
 
 // Rows of a tile of the experts' products.

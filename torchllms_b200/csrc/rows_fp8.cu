@@ -28,6 +28,28 @@ __device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&v)[8]) {
     }
 }
 
+// eight numbers as they lie in memory
+template <typename T> struct Eight;
+template <> struct Eight<float> {
+    float4 a, b;
+    __device__ __forceinline__ void load(const float* p) { a = __ldcs(reinterpret_cast<const float4*>(p)); b = __ldcs(reinterpret_cast<const float4*>(p + 4)); }
+    __device__ __forceinline__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
+    __device__ __forceinline__ void get(float (&v)[8]) const { v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w; }
+};
+template <> struct Eight<__nv_bfloat16> {
+    uint4 r;
+    __device__ __forceinline__ void load(const __nv_bfloat16* p) { r = __ldcs(reinterpret_cast<const uint4*>(p)); }
+    __device__ __forceinline__ void zero() { r = make_uint4(0u, 0u, 0u, 0u); }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+        const unsigned w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = __uint_as_float(w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    }
+};
+
 // codes of the eight numbers at column d of a row and, from the first lane of a block, its scale byte; the last block of a
 // row also clears the places behind it
 __device__ __forceinline__ void keep8(const uint2& bytes, int e, unsigned char* codes, unsigned char* scales, int d, int K) {
@@ -47,42 +69,53 @@ __device__ __forceinline__ void leave8(const float (&v)[8], unsigned char* codes
 }
 
 // FORM 0: the rows; 1: act(x); 2: gated act of the row's halves (x has 2 K columns); 3: the rows, each left at `top` places
-// (the rows that a token's choices of experts have in the sorted order).  grid (rows, chunks of 2,048 columns).
-template <typename T, int FORM>
+// (the rows that a token's choices of experts have in the sorted order).  grid (groups of ROWS rows, chunks of 2,048 columns): a
+// thread has the same eight columns of ROWS rows, all asked for before the first is used (1,531 rows of gates and ups of 14,336 each: 23.7 us
+// with one row, 20.2 with two; rows alone gain nothing).
+template <typename T, int FORM, int ACT, int ROWS>
 __global__ void __launch_bounds__(ROWS_THREADS) rows_kernel(const T* __restrict__ x, unsigned char* __restrict__ codes,
-                                                            unsigned char* __restrict__ scales, int K, int act, Fp8Gate gp,
+                                                            unsigned char* __restrict__ scales, int rows, int K, Fp8Gate gp,
                                                             const int* __restrict__ place, int top) {
     grid_launch_dependents();
     grid_dependency_wait();
-    const size_t row = blockIdx.x;
-    const int d = (blockIdx.y * ROWS_THREADS + threadIdx.x) * 8;
-    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (d < K) {
+    const size_t row0 = (size_t)blockIdx.x * ROWS;
+    const int d = (blockIdx.y * ROWS_THREADS + threadIdx.x) * 8, pitch = fp8_scale_pitch(K);
+    constexpr int HALVES = FORM == 2 ? 2 : 1;
+    Eight<T> raw[ROWS][HALVES];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h)
+            if (d < K && (ROWS == 1 || row0 + r < rows)) raw[r][h].load(x + ((row0 + r) * HALVES + h) * K + d);
+            else raw[r][h].zero();
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+        const size_t row = row0 + r;
+        if (ROWS > 1 && row >= rows) break;
+        float v[8];
+        raw[r][0].get(v);
+        if (FORM == 1)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = fp8_act(v[i], ACT);
         if (FORM == 2) {
             float u[8];
-            load8(x + row * 2 * K + d, v);
-            load8(x + row * 2 * K + K + d, u);
+            raw[r][HALVES - 1].get(u);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = fp8_gated(v[i], u[i], act, gp);
+            for (int i = 0; i < 8; ++i) v[i] = fp8_gated(v[i], u[i], ACT, gp);
+        }
+        if (FORM == 3) {
+            uint2 bytes;
+            const int e = fp8_encode8(v, bytes);
+            for (int k = 0; k < top; ++k) {
+                const int to_row = place[row * top + k];
+                if (to_row < 0) continue;
+                const size_t to = to_row;
+                keep8(bytes, e, codes + to * K, scales + to * pitch, d, K);
+            }
         } else {
-            load8(x + row * K + d, v);
-            if (FORM == 1)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = fp8_act(v[i], act);
+            leave8(v, codes + row * K, scales + row * pitch, d, K);
         }
     }
-    if (FORM == 3) {
-        uint2 bytes;
-        const int e = fp8_encode8(v, bytes);
-        for (int k = 0; k < top; ++k) {
-            const int to_row = place[row * top + k];
-            if (to_row < 0) continue;
-            const size_t to = to_row;
-            keep8(bytes, e, codes + to * K, scales + to * fp8_scale_pitch(K), d, K);
-        }
-        return;
-    }
-    leave8(v, codes + row * K, scales + row * fp8_scale_pitch(K), d, K);
 }
 
 // A CTA to a row, which stays in registers: SLOTS times eight numbers a thread.  delta: splits planes `plane` elements apart
@@ -91,13 +124,13 @@ template <typename TD, int SLOTS>
 __global__ void __launch_bounds__(1024) norm_kernel(float* __restrict__ h, const TD* __restrict__ delta, int splits, long long plane,
                                                     const float* __restrict__ weight, unsigned char* __restrict__ codes,
                                                     unsigned char* __restrict__ scales, int K, float eps) {
-    __shared__ double part[32];
+    __shared__ float part[32];
     grid_launch_dependents();
     grid_dependency_wait();
     const size_t row = blockIdx.x;
     float* hr = h + row * K;
     float x[SLOTS][8];
-    float ss = 0.f;              // (of at most 32 squares; beyond a warp, 64 bits)
+    float ss = 0.f;              // (of at most 32 squares, summed in pairs)
 #pragma unroll
     for (int s = 0; s < SLOTS; ++s) {
         const int d = (s * blockDim.x + threadIdx.x) * 8;
@@ -139,10 +172,9 @@ __global__ void __launch_bounds__(1024) norm_kernel(float* __restrict__ h, const
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n_warps = blockDim.x >> 5;
     if (lane == 0) part[warp] = ss;
     __syncthreads();
-    double total = 0.0;
-    for (int i = 0; i < n_warps; ++i) total += part[i];
-    // (an error of the factor moves a whole row against E4M3's borders: 64 bits here, once a row)
-    const float factor = (float)(1.0 / sqrt(total / (double)K + (double)eps));
+    const float total = warp_sum(lane < n_warps ? part[lane] : 0.f);
+    // (a true root and quotient: an error of the factor moves a whole row against E4M3's borders)
+    const float factor = 1.f / sqrtf(total / (float)K + eps);
 #pragma unroll
     for (int s = 0; s < SLOTS; ++s) {
         const int d = (s * blockDim.x + threadIdx.x) * 8;
@@ -248,15 +280,31 @@ __global__ void __launch_bounds__(1024) plan_kernel(const int* __restrict__ chos
     }
 }
 
+template <typename T, int FORM, int ACT, int ROWS>
+int launch_rows_of(const void* x, void* codes, void* scales, int rows, int K, const Fp8Gate& gp, const int* place, int top, cudaStream_t s) {
+    const dim3 grid((rows + ROWS - 1) / ROWS, (K + 8 * ROWS_THREADS - 1) / (8 * ROWS_THREADS));
+    return (int)tl_launch(rows_kernel<T, FORM, ACT, ROWS>, grid, dim3(ROWS_THREADS), 0, s, (const T*)x, (unsigned char*)codes, (unsigned char*)scales, rows, K,
+                          gp, place, top);
+}
+template <typename T, int FORM, int ACT>
+int launch_rows_act(const void* x, void* codes, void* scales, int rows, int K, const Fp8Gate& gp, const int* place, int top, cudaStream_t s) {
+    // gates and ups: two rows a thread as long as eight CTAs an SM are left
+    const long long ctas = (long long)rows * ((K + 8 * ROWS_THREADS - 1) / (8 * ROWS_THREADS));
+    if (FORM == 2 && ctas >= 2 * 8 * 148) return launch_rows_of<T, FORM, ACT, FORM == 2 ? 2 : 1>(x, codes, scales, rows, K, gp, place, top, s);
+    return launch_rows_of<T, FORM, ACT, 1>(x, codes, scales, rows, K, gp, place, top, s);
+}
 template <typename T>
 int launch_rows(const void* x, void* codes, void* scales, int rows, int K, int form, int act, const Fp8Gate& gp, const int* place, int top,
                 cudaStream_t s) {
-    const dim3 grid(rows, (K + 8 * ROWS_THREADS - 1) / (8 * ROWS_THREADS));
-    unsigned char *c = (unsigned char*)codes, *b = (unsigned char*)scales;
-    if (form == 0) return (int)tl_launch(rows_kernel<T, 0>, grid, dim3(ROWS_THREADS), 0, s, (const T*)x, c, b, K, act, gp, place, top);
-    if (form == 1) return (int)tl_launch(rows_kernel<T, 1>, grid, dim3(ROWS_THREADS), 0, s, (const T*)x, c, b, K, act, gp, place, top);
-    if (form == 3) return (int)tl_launch(rows_kernel<T, 3>, grid, dim3(ROWS_THREADS), 0, s, (const T*)x, c, b, K, act, gp, place, top);
-    return (int)tl_launch(rows_kernel<T, 2>, grid, dim3(ROWS_THREADS), 0, s, (const T*)x, c, b, K, act, gp, place, top);
+    if (form == 0) return launch_rows_act<T, 0, 0>(x, codes, scales, rows, K, gp, place, top, s);
+    if (form == 3) return launch_rows_act<T, 3, 0>(x, codes, scales, rows, K, gp, place, top, s);
+#define TL_ACT(A) return form == 1 ? launch_rows_act<T, 1, A>(x, codes, scales, rows, K, gp, place, top, s) : launch_rows_act<T, 2, A>(x, codes, scales, rows, K, gp, place, top, s)
+    if (act == FP8_SILU) TL_ACT(FP8_SILU);
+    if (act == FP8_GELU_TANH) TL_ACT(FP8_GELU_TANH);
+    if (act == FP8_RELU2) TL_ACT(FP8_RELU2);
+    if (act == FP8_GELU) TL_ACT(FP8_GELU);
+#undef TL_ACT
+    return launch_rows_act<T, 2, FP8_CLAMPED_SWISH>(x, codes, scales, rows, K, gp, place, top, s);
 }
 
 template <typename TD>

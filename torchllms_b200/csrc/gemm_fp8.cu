@@ -9,14 +9,28 @@
 // The operands are swapped as in gemm_tcgen05.cu: rows of W are the M of the instruction (128 a CTA), rows of x its N (`width`,
 // up to 240, chosen per call, so that few rows waste little).  D[w_row, token] lies with a row of W to a TMEM lane.
 //
-// A persistent CTA per SM walks units (a slab of 128 rows of W, a tile of rows of x), tiles fastest, so that a slab of W comes from
-// memory once and the rows of x, which are fewer, from L2.  Inside a CTA (256 threads):
-//   warp 0    TMA: two [128 x 128] boxes of W and two [width x 128] boxes of x a stage, 128-byte swizzle
-//   warp 1    tcgen05.cp of scales (a word a row: four blocks of 128) and tcgen05.mma, four of K 32 a stage
-//   warps 2, 3  scales from memory to shared memory, four words a row and turn (2,048 of K), in turns; in the order that
-//             tcgen05.cp wants: row r of a chunk of 128 at 16 (r % 32) + 4 (r / 32).  (The fence behind them waits for all loads
-//             under way: a word a turn, copied ahead, kept the products waiting - 620 cycles of every 880 a stage.)
-//   warps 4-7 results: tcgen05.ld, through shared memory to rows of C; two accumulators, so that the next unit's products run meanwhile
+// Three forms, by a rule on sizes at the end of this file:
+//   single  a persistent CTA per SM walks units (a slab of 128 rows of W, a tile of rows of x), tiles fastest, so that a slab of W comes
+//           from memory once and the rows of x, which are fewer, from L2;
+//   pairs   the same by two CTAs that share a unit of 256 rows of W (cta_group::2): each brings its half of the tile's rows of x;
+//   split   few units: the blocks of K of each are dealt out to the CTAs of a cluster, whose sums meet through distributed shared memory
+//           and are added up in the order of K.
+// And three ends: the sums leave (float32 or bfloat16), or 8-bit rows of act(sum) do, or of act(gate) * up.
+//
+// Inside a CTA:
+//   warp 0     TMA: boxes of W [128 x 128] and of x [width x 128], 128-byte swizzle, one or two of each a stage; the first ones of W before the
+//              kernel ahead of this one has ended
+//   warp 1     tcgen05.cp of scales (a word a row: four blocks of 128) and tcgen05.mma, four of K 32 a box; by one lane, as warp 0's loads
+//              (64 rows of 4,096 x 14,336 by pairs: 34.2 us with the lane elected at each instruction, 24.6 so, 21.9 with warp 0 so too)
+//   warps 2, 3 scales from memory to shared memory, four words a row and turn (2,048 of K), in turns; in the order that tcgen05.cp
+//              wants: row r of a chunk of 128 at 16 (r % 32) + 4 (r / 32).  (The fence behind them waits for all loads under way: a
+//              word a turn, copied ahead, kept the products waiting, 49 us for 39 in the same case and 225 for 203 with 2,048 rows of 28,672 x 4,096.)
+//   the rest   results: tcgen05.ld, through shared memory to rows of C; two accumulators, so that the next unit's products run meanwhile
+//
+// Measured (microseconds of repeated calls; floors at 6.57 TB/s and twice 1.65 PFLOP/s): 8 rows of 28,672 x 4,096 22.9 (floor 18.1: 224
+// slabs on 148 SMs, one or two each), 64 of 4,096 x 14,336 16.0 (9.2), 2,048 of 28,672 x 4,096 218 under the power cap that
+// long runs of it meet, 183 in short ones (146).  What bounds the last, from copies of an earlier step (203 us in short runs)
+// with a part left out: no copies of scales 168, no loads 158, one product in four 126, no products 105.
 // Every wait is bounded: on a time-out the CTA records a code, lets its copies land, frees its tensor memory and returns.
 #include "fp8.cuh"
 #include <cuda.h>
@@ -54,8 +68,8 @@ __device__ __forceinline__ void mbar_init(unsigned bar, unsigned count) {
 }
 __device__ __forceinline__ bool mbar_try_wait(unsigned bar, unsigned parity) {
     unsigned ok;
-    // (what a wait guards is read by the tensor cores and the copy engine, not by the waiting thread: an acquire at the scope of the
-    // cluster, which empties L1, cost a quarter of a decode step's product)
+    // (what a wait guards is read by the tensor cores and the copy engine, not by the waiting thread; an acquire at the scope of the
+    // cluster took 8 rows of 28,672 x 4,096 from 34.7 us to 35.9)
     asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
                  : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     return ok != 0;
@@ -88,8 +102,8 @@ __device__ __forceinline__ void give_up(volatile int* aborted, int* status, int 
     atomicExch(status, code);
 }
 // One elected lane of a warp in step arrives.  PAIR: at a barrier that may be the other CTA's.  (Neither form orders more than this CTA
-// sees: what it guards has gone through a proxy fence or has been read from tensor memory.  With release at the cluster's scope,
-// which waits for everything the warp has stored, a decode step's product took a quarter longer.)
+// sees: what it guards has gone through a proxy fence or has been read from tensor memory.  Release at the cluster's scope, which waits for
+// everything the warp has stored, took 8 rows of 28,672 x 4,096 from 31.2 us to 34.7.)
 template <bool PAIR>
 __device__ __forceinline__ void arrive_elect(unsigned bar) {
     if (!PAIR) {
@@ -1052,7 +1066,7 @@ int tile_rows(int pairs, int experts) {
 extern "C" int tl_gemm_fp8(const void* x, const void* x_scales, const void* w, const void* w_scales, void* out, int out_is_f32, int M, int N, int K,
                            int form, int* status, void* stream) {
     if (M <= 0) return TL_OK;
-    // Few units leave SMs idle: their K is cut among the CTAs of a cluster.  (64 rows of 4,096 x 14,336: 25 us whole, 15.4 cut; 701 of
+    // Few units leave SMs idle: their K is cut among the CTAs of a cluster.  (64 rows of 4,096 x 14,336: 25 us whole, 15.9 cut; 701 of
     // 2,048 x 8,192: 23.4 in pairs, 18.2 cut; 512 of 6,144 x 4,096, 144 units: 14.7 in pairs, 20.4 cut.)
     const int narrow = even_width(M, MAX_SPLIT_WIDTH), units = ((N + BM - 1) / BM) * ((M + narrow - 1) / narrow);
     if (form == 0 && 2 * units <= sm_count() && K > 4 * BK) form = SPLIT;

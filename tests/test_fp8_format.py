@@ -82,3 +82,21 @@ def test_calls_refuse_the_host():
     with pytest.raises(KernelError, match="clamped"):
         ops.activation_fp8(x, "clamped_swish")
     assert ops.launches == 0
+
+
+def test_sizes_at_the_end_of_an_int_are_refused():
+    """The products' entries say so before they reckon with them, or ask a device anything."""
+    import ctypes
+    from torchllms_b200.kernels.build import compile_library
+    lib = ctypes.CDLL(str(compile_library("gemm_fp8")))
+    some, status = ctypes.c_void_p(1 << 20), (ctypes.c_int * 1)()
+    end = 2 ** 31 - 1
+    i, f, at = ctypes.c_int, ctypes.c_float, ctypes.byref(status)
+    for M, N in ((end, 16), (1, end), (2 ** 31 - 255, 16)):
+        for form in range(4):
+            assert lib.tl_gemm_fp8(some, some, some, some, some, i(0), i(M), i(N), i(16), i(form), at, None) != 0
+    for form in range(3):
+        assert lib.tl_gemm_fp8_act(some, some, some, some, some, some, i(end), i(16), i(16), i(0), i(0), f(0), f(0), f(0), i(1), None, i(0), i(form), at,
+                                   None) != 0
+        assert lib.tl_gemm_fp8_experts(some, some, some, some, some, i(0), i(end), i(16), i(16), i(2), some, i(1), i(form), at, None) != 0
+    assert status[0] == 0

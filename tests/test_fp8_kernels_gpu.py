@@ -106,6 +106,17 @@ def test_norm(ops, dtype, T, K, splits):
     near_rows(rows, y, 64 * 2.0 ** -24)
 
 
+@pytest.mark.parametrize("T,K", [(591, 4096), (592, 4096), (592, 16), (700, 2032), (593, 2064), (600, 4112), (595, 8192), (600, 8208)])
+def test_norm_of_many_rows(ops, T, K):
+    """Both sides of the number of rows and of the widths from which CTAs are smaller; bounds as above (32 terms a thread, 8 sums in a tree)."""
+    h, w, delta = uneven(T, K, seed=1), 1.0 + 0.3 * rand((K,), seed=2), rand((T, K), torch.bfloat16, seed=4)
+    want_h = h.double() + delta.double()
+    rows = ops.rmsnorm_fp8(h, delta, w, 1e-5)
+    assert bool(((h.double() - want_h).abs() <= 2.0 ** -24 * (want_h.abs() + 1e-30) * (1 + 2.0 ** -20)).all())
+    x = h.double()
+    near_rows(rows, x / torch.sqrt((x * x).mean(-1, keepdim=True) + 1e-5) * w.double(), 64 * 2.0 ** -24)
+
+
 def test_norm_without_a_delta_leaves_the_stream(ops):
     h, w = uneven(5, 512, seed=1), 1.0 + 0.3 * rand((512,), seed=2)
     before = h.clone()

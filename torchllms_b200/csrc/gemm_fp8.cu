@@ -931,6 +931,8 @@ int launch(Params& p, const void* x, const void* w, int experts, int K, cudaStre
         const int sets = p.width <= 128 ? 8 : 12;
         p.scale_col = p.width;
         p.set_cols = sets;
+        // (128 columns at most where there is room for another kernel's CTA: none that takes more than 384 fits beside 112 KB, so clusters
+        // never wait in a circle for each other's columns)
         p.tmem_cols = whole_columns(p.width + 2 * sets);
         if (p.width <= SHARED_WIDTH && units * p.splits > sms) room = 112 * 1024;
     } else {
@@ -1052,6 +1054,9 @@ int sums(const void* x, const void* x_scales, const void* w, const void* w_scale
     return form == PAIRS ? launch<PAIRS>(p, x, w, experts, K, s) : launch<SINGLE>(p, x, w, experts, K, s);
 }
 
+// (so that a tile's last row, worked out as its first plus its width, and a count of tiles stay within an int)
+constexpr int MOST_ROWS = 0x7fffff00;
+
 // rows of a tile of the experts' products: twice an even share, so that most experts need one tile
 int tile_rows(int pairs, int experts) {
     const long long share = (2ll * pairs + experts - 1) / (experts > 0 ? experts : 1);
@@ -1066,6 +1071,7 @@ int tile_rows(int pairs, int experts) {
 extern "C" int tl_gemm_fp8(const void* x, const void* x_scales, const void* w, const void* w_scales, void* out, int out_is_f32, int M, int N, int K,
                            int form, int* status, void* stream) {
     if (M <= 0) return TL_OK;
+    if (M > MOST_ROWS || N > MOST_ROWS) return TL_BAD_SIZE;
     // Few units leave SMs idle: their K is cut among the CTAs of a cluster.  (64 rows of 4,096 x 14,336: 25 us whole, 15.9 cut; 701 of
     // 2,048 x 8,192: 23.4 in pairs, 18.2 cut; 512 of 6,144 x 4,096, 144 units: 14.7 in pairs, 20.4 cut.)
     const int narrow = even_width(M, MAX_SPLIT_WIDTH), units = ((N + BM - 1) / BM) * ((M + narrow - 1) / narrow);
@@ -1083,7 +1089,7 @@ extern "C" int tl_gemm_fp8_experts(const void* x, const void* x_scales, const vo
                                    int N, int K, int experts, const int* tiles, int most_tiles, int form, int* status,
                                    void* stream) {
     if (pairs <= 0) return TL_OK;
-    if (tiles == nullptr) return TL_BAD_SIZE;
+    if (tiles == nullptr || pairs > MOST_ROWS) return TL_BAD_SIZE;
     return sums(x, x_scales, w, w_scales, out, out_is_f32, pairs, N, K, experts, tiles, most_tiles, tile_rows(pairs, experts), form, status,
                 (cudaStream_t)stream);
 }
@@ -1095,7 +1101,7 @@ extern "C" int tl_gemm_fp8_act(const void* x, const void* x_scales, const void* 
                                int K, int gated, int act, float limit, float alpha, float up_offset, int experts, const int* tiles,
                                int most_tiles, int form, int* status, void* stream) {
     if (M <= 0) return TL_OK;
-    if (hidden <= 0 || hidden % 16 != 0 || hidden > (1 << 26) || act < 0 || act > 4 || (act == FP8_CLAMPED_SWISH && !gated) ||
+    if (M > MOST_ROWS || hidden <= 0 || hidden % 16 != 0 || hidden > (1 << 26) || act < 0 || act > 4 || (act == FP8_CLAMPED_SWISH && !gated) ||
         form < 0 || form > 2 || (gated && form == SINGLE))
         return TL_BAD_SIZE;
     const int width = tiles == nullptr ? even_width(M, MAX_WIDTH) : tile_rows(M, experts);

@@ -4,7 +4,11 @@ import pytest
 import torch
 
 import fp8_plain as plain
+import bomotar_cases
+import lagusun_cases
+import nunosun_cases
 import rakuvik_cases
+import zusitar_cases
 from helpers import TINY, TINY_C, make_tensors, tiny_folder, write_model_folder
 from torch_ops import TorchOps
 from torchllms_b200.engine.loading import load_model
@@ -13,6 +17,8 @@ from torchllms_b200.engine.step import StepEntry
 from torchllms_b200.inference import LLM
 from torchllms_b200.inference.chat import parse_args
 from torchllms_b200.kernels.lazy import PendingProduct
+from torchllms_b200.parts.attention import PagedAttention
+from torchllms_b200.parts.pair import SideBySide
 from torchllms_b200.weights.fp8 import Fp8Rows, encode
 
 
@@ -134,6 +140,33 @@ def test_what_is_refused(tmp_path):
         LLM(dense, device="cpu", ops=Fp8TorchOps(), weights="fp8")
 
 
+def test_a_part_inside_a_pair_is_found():
+    """A model whose only matrices in 8 bits are those of one of two mixers side by side is not refused."""
+    pair, members = object.__new__(SideBySide), [object.__new__(PagedAttention) for _ in range(2)]
+    pair.members = (("left", members[0]), ("right", members[1]))
+    assert list(pair.parts_within()) == [pair, *members]
+
+
+def expert_family(tmp, name, width=48):
+    """A folder of each family that has routed experts, their widths a multiple of 16."""
+    if name == "rakuvik":
+        c, layers = rakuvik_cases, [rakuvik_cases.attention_layer(mlp=rakuvik_cases.moe(ff=32, shared=48))]
+    elif name == "nunosun":
+        c, layers = nunosun_cases, [nunosun_cases.parallel_layer(mlp=nunosun_cases.moe(ff=32)), nunosun_cases.delta_layer(mlp=nunosun_cases.moe(ff=16))]
+    elif name == "zusitar":
+        c, layers = zusitar_cases, [zusitar_cases.attention_layer(mlp=zusitar_cases.moe(ff=32, shared=(16, 1.2))),
+                                    zusitar_cases.scan_layer(mlp=zusitar_cases.moe(ff=16, shared=(32, 1.2)))]
+    elif name == "lagusun":
+        c, layers = lagusun_cases, [lagusun_cases.windowed(mlp=lagusun_cases.moe(ff=32, shared=16)), lagusun_cases.chunked(mlp=lagusun_cases.moe(ff=16, shared=32))]
+    else:
+        c, layers = bomotar_cases, [bomotar_cases.layer(mlp=bomotar_cases.moe(ff=32)), bomotar_cases.layer(mlp=bomotar_cases.moe(ff=16))]
+    cfg = c.config(layers, width=width)
+    return c.write_folder(tmp, name, cfg, c.tensors_for(cfg, 1), torch.bfloat16)
+
+
+FAMILIES = ("rakuvik", "nunosun", "zusitar", "lagusun", "bomotar")
+
+
 # ------------------------------------------------------------------------------------------------- on a GPU
 
 @pytest.mark.gpu
@@ -186,3 +219,21 @@ def test_generation(tmp_path):
     out = llm.generate(prompt_token_ids=PROMPTS, max_new_tokens=8)
     assert all(r.error is None and len(r.token_ids) == 8 for r in out)
     llm.engine.model.ops.check_status()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", FAMILIES)
+def test_every_family_with_experts(tmp_path, name):
+    """Its experts are held and run; recorded steps give the bits of eager ones, and every number is one."""
+    folder, runs = expert_family(tmp_path, name), []
+    for graphs in (False, True):
+        engine = Replayer(folder, "bfloat16", 512, weight_format="fp8").engine
+        engine.use_graphs = engine.use_graphs and graphs
+        held = [p for b in engine.model.blocks for p in b.parts_within() if type(p).__name__ == "RoutedExperts"]
+        assert held and all(type(p.w_up) is Fp8Rows for p in held)
+        a, b = engine.claim(), engine.claim()
+        run = [engine.step([StepEntry(a, [(5 * i) % 83 for i in range(70)], [69]), StepEntry(b, [1, 2], [1])]).clone()]
+        run += [engine.step([StepEntry(a, [s], [0]), StepEntry(b, [s + 20], [0])]).clone() for s in range(6)]
+        engine.model.ops.check_status()
+        runs.append(torch.stack(run))
+    assert bool(torch.isfinite(runs[0]).all()) and torch.equal(*runs)

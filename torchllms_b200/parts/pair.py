@@ -30,6 +30,11 @@ class _Pair(Mixer):
         self.graph_safe = all(m.graph_safe for _p, m in self.members)
         self._need = join_states([(p, m.state_need()) for p, m in self.members])
 
+    def parts_within(self):
+        yield self
+        for _p, m in self.members:
+            yield from m.parts_within()
+
     def cache_need(self):
         for _p, m in self.members:
             if m.cache_need() is not None:

@@ -41,7 +41,7 @@ constexpr int BM = 128;              // rows of W a CTA
 constexpr int BK = 128;              // bytes of K a box: a swizzle row, and a block of numbers that share a scale
 constexpr int MAX_WIDTH = 240;       // rows of x a tile: two accumulators and two sets of scales fill 512 columns
 // Split: tiles so narrow send their sums to where they are added up, wider ones, whose sums would take room from the stages, leave them to
-// be fetched (8 rows of 4,096 x 14,336: 13.5 us sent, 14.6 fetched; 64 rows 16.0 and 15.4); and tiles so narrow share an SM.
+// be fetched (8 rows of 4,096 x 14,336: 13.5 us sent, 14.6 fetched; 64 rows 15.9 and 15.7); and tiles so narrow share an SM.
 constexpr int PUSH_WIDTH = 32;
 constexpr int SHARED_WIDTH = 64;
 constexpr int MAX_SPLIT_WIDTH = 224; // the same with one accumulator in 256 columns

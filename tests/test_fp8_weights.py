@@ -212,7 +212,7 @@ def test_recorded_steps_are_eager_ones(tmp_path):
 
 @pytest.mark.gpu
 def test_generation(tmp_path):
-    """Requests in a batch and alone, cut into portions or not, follow the same logits up to the kernels' order of sums: judged by the twins."""
+    """Requests in a batch, cut into portions, beside keys and values in 4 bits: all are answered and no wait ran out."""
     folder = write_model_folder(tmp_path / "m", TINY_C, make_tensors(TINY_C, 2, std=0.05, qk_std=0.25), torch.bfloat16)
     llm = LLM(folder, precision="bfloat16", max_len=256, max_bsz=4, max_num_batched_tokens=64, prefill_chunk=48, weights="fp8", kv_cache="fp4")
     llm.warmup(batch_sizes=[3])

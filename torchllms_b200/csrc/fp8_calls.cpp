@@ -59,6 +59,20 @@ long long pitch(long long width) { return 4 * ((width + 511) / 512); }
 at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& like) {
     return at::Tensor(at::detail::empty_cuda(sizes, type, like.device(), c10::nullopt));
 }
+// What lives in one call only comes in one piece (an allocation takes the host some 0.6 us): parts of it, each on 256 bytes
+struct Pieces {
+    long long bytes = 0;
+    at::Tensor memory;
+    long long add(long long n) {
+        const long long at = bytes;
+        bytes += (n + 255) / 256 * 256;
+        return at;
+    }
+    char* take(const at::Tensor& like) {
+        memory = fresh({bytes}, at::kByte, like);
+        return (char*)memory.data_ptr();
+    }
+};
 void* stream_of(int device) { return (void*)c10::cuda::getCurrentCUDAStream(device).stream(); }
 // float32/bfloat16 rows whose width is `parts` times a multiple of 16
 bool plain_rows(const at::Tensor* x, int device, int parts) {
@@ -168,16 +182,19 @@ PyObject* product(PyObject*, PyObject* const* args, Py_ssize_t n) {
     }
     const long long M = x->size(0), N = w->size(0), K = x->size(1);
     void* stream = stream_of(device);
-    at::Tensor codes, scales;
+    Pieces held;
+    void *codes, *scales;
     if (xs == nullptr) {
-        codes = fresh({M, K}, at::kFloat8_e4m3fn, *x);
-        scales = fresh({M, pitch(K)}, at::kFloat8_e8m0fnu, *x);
-        const int rc = entry.rows(x->data_ptr(), code_of(*x), codes.data_ptr(), scales.data_ptr(), (int)M, (int)K, 0, 0, 0.f, 0.f, 0.f, stream);
+        const long long codes_at = held.add(M * K), scales_at = held.add(M * pitch(K));
+        char* memory = held.take(*x);
+        codes = memory + codes_at, scales = memory + scales_at;
+        const int rc = entry.rows(x->data_ptr(), code_of(*x), codes, scales, (int)M, (int)K, 0, 0, 0.f, 0.f, 0.f, stream);
         if (rc != 0) return PyLong_FromLong(rc);
+    } else {
+        codes = x->data_ptr(), scales = xs->data_ptr();
     }
     at::Tensor out = fresh({M, N}, type == 0 ? at::kFloat : at::kBFloat16, *x);
-    const int rc = entry.product(xs == nullptr ? codes.data_ptr() : x->data_ptr(), xs == nullptr ? scales.data_ptr() : xs->data_ptr(), w->data_ptr(),
-                                 ws->data_ptr(), out.data_ptr(), type == 0 ? 1 : 0, (int)M, (int)N, (int)K, form, status, stream);
+    const int rc = entry.product(codes, scales, w->data_ptr(), ws->data_ptr(), out.data_ptr(), type == 0 ? 1 : 0, (int)M, (int)N, (int)K, form, status, stream);
     if (rc != 0) return PyLong_FromLong(rc);
     return THPVariable_Wrap(std::move(out));
     END_HANDLE_TH_ERRORS
@@ -203,16 +220,19 @@ PyObject* act_product(PyObject*, PyObject* const* args, Py_ssize_t n) {
         Py_RETURN_NONE;
     }
     void* stream = stream_of(device);
-    at::Tensor codes, scales;
+    Pieces held;
+    void *codes, *scales;
     if (xs == nullptr) {
-        codes = fresh({M, K}, at::kFloat8_e4m3fn, *x);
-        scales = fresh({M, pitch(K)}, at::kFloat8_e8m0fnu, *x);
-        const int rc = entry.rows(x->data_ptr(), code_of(*x), codes.data_ptr(), scales.data_ptr(), (int)M, (int)K, 0, 0, 0.f, 0.f, 0.f, stream);
+        const long long codes_at = held.add(M * K), scales_at = held.add(M * pitch(K));
+        char* memory = held.take(*x);
+        codes = memory + codes_at, scales = memory + scales_at;
+        const int rc = entry.rows(x->data_ptr(), code_of(*x), codes, scales, (int)M, (int)K, 0, 0, 0.f, 0.f, 0.f, stream);
         if (rc != 0) return PyLong_FromLong(rc);
+    } else {
+        codes = x->data_ptr(), scales = xs->data_ptr();
     }
     at::Tensor out = fresh({M, hidden}, at::kFloat8_e4m3fn, *x), out_scales = fresh({M, pitch(hidden)}, at::kFloat8_e8m0fnu, *x);
-    const int rc = entry.act_product(xs == nullptr ? codes.data_ptr() : x->data_ptr(), xs == nullptr ? scales.data_ptr() : xs->data_ptr(), w->data_ptr(),
-                                     ws->data_ptr(), out.data_ptr(), out_scales.data_ptr(), (int)M, (int)hidden, (int)K, gated, act, (float)limit,
+    const int rc = entry.act_product(codes, scales, w->data_ptr(), ws->data_ptr(), out.data_ptr(), out_scales.data_ptr(), (int)M, (int)hidden, (int)K, gated, act, (float)limit,
                                      (float)alpha, (float)offset, 1, nullptr, 0, form, status, stream);
     if (rc != 0) return PyLong_FromLong(rc);
     return both(std::move(out), std::move(out_scales));
@@ -257,21 +277,23 @@ PyObject* experts(PyObject*, PyObject* const* args, Py_ssize_t n) {
     void* stream = stream_of(device);
     const int P = (int)pairs, width = entry.tile_rows(P, (int)E);
     const long long tiles_most = (pairs + width - 1) / width + E, most = tiles_most < pairs ? tiles_most : pairs;
-    at::Tensor index = fresh({2 * pairs + 1 + 3 * most}, at::kInt, *x);
-    int *order = index.data_ptr<int>(), *place = order + pairs, *tiles = place + pairs;
-    at::Tensor rows = fresh({pairs, dim}, at::kFloat8_e4m3fn, *x), rows_s = fresh({pairs, pitch(dim)}, at::kFloat8_e8m0fnu, *x);
-    at::Tensor hid = fresh({pairs, hidden}, at::kFloat8_e4m3fn, *x), hid_s = fresh({pairs, pitch(hidden)}, at::kFloat8_e8m0fnu, *x);
-    at::Tensor y = fresh({pairs, dim}, x->scalar_type(), *x), out = fresh({T, dim}, x->scalar_type(), *x);
+    Pieces held;
+    const long long index_at = held.add(4 * (2 * pairs + 1 + 3 * most)), rows_at = held.add(pairs * dim), rows_s_at = held.add(pairs * pitch(dim)),
+                    hid_at = held.add(pairs * hidden), hid_s_at = held.add(pairs * pitch(hidden)), y_at = held.add(pairs * dim * x->element_size());
+    at::Tensor out = fresh({T, dim}, x->scalar_type(), *x);
+    char* memory = held.take(*x);
+    int *order = (int*)(memory + index_at), *place = order + pairs, *tiles = place + pairs;
+    void *rows = memory + rows_at, *rows_s = memory + rows_s_at, *hid = memory + hid_at, *hid_s = memory + hid_s_at, *y = memory + y_at;
     int rc = entry.plan(chosen->data_ptr<int>(), P, (int)E, width, order, place, tiles, (int)most, stream);
-    if (rc == 0) rc = entry.placed(x->data_ptr(), code, rows.data_ptr(), rows_s.data_ptr(), (int)T, (int)dim, place, (int)top, stream);
+    if (rc == 0) rc = entry.placed(x->data_ptr(), code, rows, rows_s, (int)T, (int)dim, place, (int)top, stream);
     if (rc == 0)
-        rc = entry.act_product(rows.data_ptr(), rows_s.data_ptr(), up->data_ptr(), up_s->data_ptr(), hid.data_ptr(), hid_s.data_ptr(), P, (int)hidden, (int)dim,
+        rc = entry.act_product(rows, rows_s, up->data_ptr(), up_s->data_ptr(), hid, hid_s, P, (int)hidden, (int)dim,
                                gated, act, (float)limit, (float)alpha, (float)offset, (int)E, tiles, (int)most, gated ? 0 : form, status, stream);
     if (rc == 0)
-        rc = entry.experts(hid.data_ptr(), hid_s.data_ptr(), down->data_ptr(), down_s->data_ptr(), y.data_ptr(), code == 0 ? 1 : 0, P, (int)dim, (int)hidden,
+        rc = entry.experts(hid, hid_s, down->data_ptr(), down_s->data_ptr(), y, code == 0 ? 1 : 0, P, (int)dim, (int)hidden,
                            (int)E, tiles, (int)most, form, status, stream);
     if (rc == 0)
-        rc = entry.combine(y.data_ptr(), code, place, weights->data_ptr<float>(), shared == nullptr ? nullptr : shared->data_ptr(),
+        rc = entry.combine(y, code, place, weights->data_ptr<float>(), shared == nullptr ? nullptr : shared->data_ptr(),
                            shared == nullptr ? 0 : code_of(*shared), (int)splits, plane, gate == nullptr ? nullptr : gate->data_ptr<float>(), out.data_ptr(),
                            (int)T, (int)dim, (int)top, stream);
     if (rc != 0) return PyLong_FromLong(rc);

@@ -200,6 +200,25 @@ def test_what_is_not_finite_stays_in_its_row(ops):
     assert torch.equal(got[~bad], clean[~bad])
 
 
+@pytest.mark.parametrize("impl", ["single", "pair", "split"])
+def test_few_rows_are_the_first_of_more(ops, impl):
+    """Products of 1 to 15 rows, behind products of rows that are not numbers (which stay in shared memory): the bits of the first of 16."""
+    w, x = held(rand((640, 2064), seed=1, scale=1 / 32)), held(uneven(16, 2064, seed=2))
+    poison = held(torch.full((240, 2064), math.nan, device="cuda"))
+    want = ops.linear_fp8(x, w, torch.float32, impl=impl)
+    acted = None if impl == "split" else ops.linear_activation_fp8(x, w, "silu", gated=impl == "pair", impl=impl)
+    for M in range(1, 16):
+        ops.linear_fp8(poison, w, impl="pair")
+        ops.linear_fp8(poison[:16], w, impl=impl)
+        assert torch.equal(ops.linear_fp8(x[:M], w, torch.float32, impl=impl), want[:M])
+        if acted is not None:
+            ops.linear_fp8(poison, w, impl="pair")
+            got = ops.linear_activation_fp8(x[:M], w, "silu", gated=impl == "pair", impl=impl)
+            assert torch.equal(got.codes.view(torch.uint8), acted.codes[:M].view(torch.uint8))
+            assert torch.equal(got.scales.view(torch.uint8), acted.scales[:M].view(torch.uint8))
+    ops.check_status()
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_product_of_rows_that_come_unheld(ops, dtype):
     x, w = uneven(21, 1040, dtype, seed=5), held(rand((512, 1040), seed=6))

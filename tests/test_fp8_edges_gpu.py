@@ -1,0 +1,65 @@
+"""The 8-bit rows' operators where a rounding too many, a value far out or the order of launches would show: each case by itself."""
+
+import pytest
+import torch
+
+import fp8_plain as plain
+from torchllms_b200.weights.fp8 import Fp8Rows, encode
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from torchllms_b200.kernels import get_ops
+    return get_ops()
+
+
+def rand(shape, dtype=torch.float32, seed=0, scale=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(shape, generator=g, device="cuda") * scale).to(dtype)
+
+
+def whole(lo, hi, shape, seed):
+    return torch.randint(lo, hi + 1, shape, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda").float()
+
+
+def held(x):
+    return Fp8Rows(*encode(x))
+
+
+# ------------------------------------------------------------------------------------------------- one rounding
+
+def check_one_rounding(got, x, chosen, share, up, down, extra=None):
+    """Small whole numbers, which 8 bits hold as they are, all the way to the experts' results: those are exact in float32, and what is left
+    are the weighted sum's errors in float32 (an error of half a step for each of its terms) and one rounding to the result's type."""
+    terms = torch.zeros(x.shape, dtype=torch.float64, device="cuda")
+    want = torch.zeros_like(terms)
+    for k in range(chosen.shape[1]):
+        u = torch.einsum("td,thd->th", x.double(), up[chosen[:, k].long()].double())
+        z = torch.einsum("th,tdh->td", u.clamp(min=0) ** 2, down[chosen[:, k].long()].double()) * share[:, k, None].double()
+        want, terms = want + z, terms + z.abs()
+    if extra is not None:
+        want, terms = want + extra, terms + extra.abs()
+    slack = terms * (chosen.shape[1] + 2) * 2.0 ** -24
+    bound = slack + (want.abs() + slack) * (torch.finfo(got.dtype).eps / 2)
+    assert bool(((got.double() - want).abs() <= bound).all()), float(((got.double() - want).abs() / (bound + 1e-30)).max())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T,E,top,dim,hidden", [(1, 4, 3, 16, 64), (40, 8, 4, 144, 128), (300, 4, 4, 512, 256), (33, 16, 7, 272, 144)])
+def test_experts_results_are_rounded_once(ops, dtype, T, E, top, dim, hidden):
+    # (a token's row has one number, and the hidden ones are squares of 0 to 3: all of them numbers of E4M3 under one scale)
+    x = torch.zeros((T, dim), device="cuda")
+    x[torch.arange(T), whole(0, dim - 1, (T,), 1).long()] = 1.0
+    up, down = whole(-1, 3, (E, hidden, dim), 2), whole(-15, 15, (E, dim, hidden), 3)
+    chosen = whole(0, E - 1, (T, top), 4).int()
+    share = rand((T, top), seed=5)                    # (of either sign: results that cancel keep their experts' errors)
+    out = ops.moe_experts_fp8(x.to(dtype), chosen, share, held(up), held(down), activation="relu2")
+    check_one_rounding(out, x, chosen, share, up, down)
+    gate = torch.rand(T, generator=torch.Generator(device="cuda").manual_seed(7), device="cuda")
+    for shared in (rand((T, dim), dtype, seed=6, scale=100.0), rand((2, T, dim), seed=6, scale=100.0)):
+        out = ops.moe_experts_fp8(x.to(dtype), chosen, share, held(up), held(down), activation="relu2", shared=shared, shared_gate=gate)
+        extra = (shared.double().sum(0) if shared.dim() == 3 else shared.double()) * gate.double()[:, None]
+        check_one_rounding(out, x, chosen, share, up, down, extra)
+    ops.check_status()

@@ -298,11 +298,24 @@ __global__ void __launch_bounds__(NT) moe_gemm_kernel(const T* __restrict__ A, c
     }
 }
 
-// One CTA per token.  y: [pairs][dim] in sorted order; shared: [splits][T][dim] or null.  The token's places and
-// weights are fetched once; VEC: sixteen bytes of a row per thread and turn, four choices' loads in flight.
+// N numbers from a 16-byte boundary on
+template <int N, typename T>
+__device__ __forceinline__ void load_run(const T* p, float (&v)[N]) {
+    constexpr int M = Vec16<T>::N;
+#pragma unroll
+    for (int i = 0; i < N; i += M) {
+        Vec16<T> r;
+        r.load(p + i);
+#pragma unroll
+        for (int e = 0; e < M; ++e) v[i + e] = r.get(e);
+    }
+}
+
+// One CTA per token.  y: [pairs][dim] in sorted order, of the result's type or in float32; shared: [splits][T][dim] or null.  The token's
+// places and weights are fetched once; VEC: sixteen bytes of the result per thread and turn, four choices' loads in flight.
 constexpr int COMBINE_TOP = 64;
-template <typename T, typename TS, bool VEC>
-__global__ void moe_combine_kernel(const T* __restrict__ y, const int* __restrict__ place, const float* __restrict__ weights,
+template <typename TY, typename T, typename TS, bool VEC>
+__global__ void moe_combine_kernel(const TY* __restrict__ y, const int* __restrict__ place, const float* __restrict__ weights,
                                    const TS* __restrict__ shared, int shared_splits, long long shared_plane,
                                    const float* __restrict__ gate, T* __restrict__ out, int dim, int top) {
     __shared__ int pl[COMBINE_TOP];
@@ -324,19 +337,19 @@ __global__ void moe_combine_kernel(const T* __restrict__ y, const int* __restric
             for (int e = 0; e < N; ++e) acc[e] = 0.f;
             int k = 0;
             for (; k + 4 <= top; k += 4) {
-                Vec16<T> v[4];
+                float v[4][N];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[i].load(y + (size_t)pl[k + i] * dim + d);
+                for (int i = 0; i < 4; ++i) load_run(y + (size_t)pl[k + i] * dim + d, v[i]);
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int e = 0; e < N; ++e) acc[e] = fmaf(wt[k + i], v[i].get(e), acc[e]);
+                    for (int e = 0; e < N; ++e) acc[e] = fmaf(wt[k + i], v[i][e], acc[e]);
             }
             for (; k < top; ++k) {
-                Vec16<T> v;
-                v.load(y + (size_t)pl[k] * dim + d);
+                float v[N];
+                load_run(y + (size_t)pl[k] * dim + d, v);
 #pragma unroll
-                for (int e = 0; e < N; ++e) acc[e] = fmaf(wt[k], v.get(e), acc[e]);
+                for (int e = 0; e < N; ++e) acc[e] = fmaf(wt[k], v[e], acc[e]);
             }
             if (shared != nullptr) {
 #pragma unroll
@@ -555,9 +568,9 @@ extern "C" int tl_moe_gemm(const void* A, const void* W, void* C, int dtype, con
     return TL_BAD_DTYPE;
 }
 
-// y: [n_tokens * top][dim] of dtype in sorted order; shared: [shared_splits][n_tokens][dim] of shared_dtype or
+// y: [n_tokens * top][dim] in sorted order, of dtype or (y_dtype) float32; shared: [shared_splits][n_tokens][dim] of shared_dtype or
 // null; gate: float32 [n_tokens] or null; out: [n_tokens][dim] of dtype.
-extern "C" int tl_moe_combine(const void* y, int dtype, const int* place, const float* weights, const void* shared,
+extern "C" int tl_moe_combine(const void* y, int y_dtype, int dtype, const int* place, const float* weights, const void* shared,
                               int shared_dtype, int shared_splits, long long shared_plane, const float* gate, void* out,
                               int n_tokens, int dim, int top, void* stream) {
     if (n_tokens <= 0) return TL_OK;
@@ -568,14 +581,19 @@ extern "C" int tl_moe_combine(const void* y, int dtype, const int* place, const 
     threads = threads < 64 ? 64 : (threads > 256 ? 256 : threads);
     const dim3 grid(n_tokens), block(threads);
     cudaStream_t s = (cudaStream_t)stream;
-#define TL_MOE_COMBINE(T, TS)                                                                                          \
-    (vec ? tl_launch(moe_combine_kernel<T, TS, true>, grid, block, 0, s, (const T*)y, place, weights, (const TS*)shared,   \
-                     shared_splits, shared_plane, gate, (T*)out, dim, top)                                             \
-         : tl_launch(moe_combine_kernel<T, TS, false>, grid, block, 0, s, (const T*)y, place, weights, (const TS*)shared,  \
-                     shared_splits, shared_plane, gate, (T*)out, dim, top))
-    if (dtype == TL_F32 && (shared == nullptr || shared_dtype == TL_F32)) return (int)TL_MOE_COMBINE(float, float);
-    if (dtype == TL_BF16 && (shared == nullptr || shared_dtype == TL_BF16)) return (int)TL_MOE_COMBINE(__nv_bfloat16, __nv_bfloat16);
-    if (dtype == TL_BF16 && shared_dtype == TL_F32) return (int)TL_MOE_COMBINE(__nv_bfloat16, float);
+#define TL_MOE_COMBINE(TY, T, TS)                                                                                          \
+    return (int)(vec ? tl_launch(moe_combine_kernel<TY, T, TS, true>, grid, block, 0, s, (const TY*)y, place, weights, (const TS*)shared,   \
+                                 shared_splits, shared_plane, gate, (T*)out, dim, top)                                             \
+                     : tl_launch(moe_combine_kernel<TY, T, TS, false>, grid, block, 0, s, (const TY*)y, place, weights, (const TS*)shared,  \
+                                 shared_splits, shared_plane, gate, (T*)out, dim, top))
+    const bool shared_f32 = shared != nullptr && shared_dtype == TL_F32;
+    if (shared != nullptr && shared_dtype != dtype && !shared_f32) return TL_BAD_DTYPE;
+    if (dtype == TL_F32 && y_dtype == TL_F32) TL_MOE_COMBINE(float, float, float);
+    if (dtype != TL_BF16) return TL_BAD_DTYPE;
+    if (y_dtype == TL_BF16 && shared_f32) TL_MOE_COMBINE(__nv_bfloat16, __nv_bfloat16, float);
+    if (y_dtype == TL_BF16) TL_MOE_COMBINE(__nv_bfloat16, __nv_bfloat16, __nv_bfloat16);
+    if (y_dtype == TL_F32 && shared_f32) TL_MOE_COMBINE(float, __nv_bfloat16, float);
+    if (y_dtype == TL_F32) TL_MOE_COMBINE(float, __nv_bfloat16, __nv_bfloat16);
 #undef TL_MOE_COMBINE
     return TL_BAD_DTYPE;
 }

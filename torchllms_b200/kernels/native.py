@@ -1434,7 +1434,7 @@ class NativeOps:
             _cuda_contig(shared_gate, "shared gate", torch.float32)
             _need(shared is not None and shared_gate.numel() == T, "one gate value per token, with a shared expert")
         out = torch.empty((T, dim), dtype=x.dtype, device=x.device)
-        rc = lib.tl_moe_combine(_ptr(y), _DT[x.dtype], _ptr(place), _ptr(weights), _ptr(shared),
+        rc = lib.tl_moe_combine(_ptr(y), _DT[y.dtype], _DT[x.dtype], _ptr(place), _ptr(weights), _ptr(shared),
                                 _DT[shared.dtype] if shared is not None else 0, splits, ctypes.c_longlong(plane), _ptr(shared_gate),
                                 _ptr(out), T, dim, top, _stream())
         _check(rc, "moe_combine")

@@ -63,3 +63,65 @@ def test_experts_results_are_rounded_once(ops, dtype, T, E, top, dim, hidden):
         extra = (shared.double().sum(0) if shared.dim() == 3 else shared.double()) * gate.double()[:, None]
         check_one_rounding(out, x, chosen, share, up, down, extra)
     ops.check_status()
+
+
+# ------------------------------------------------------------------------------------------------- weights that were made just before
+
+MADE = [("linear", "single"), ("linear", "pair"), ("linear", "split"), ("linear", "auto"), ("act", "single"), ("act", "pair"), ("gated", "auto")]
+
+
+def made_and_used(ops, kind, impl, weight, x):
+    """A weight brought to 8 bits by the kernel in front of the product (held rows), or in front of the rows' kernel (others)."""
+    w = ops.quantize_fp8(weight)
+    if kind == "linear":
+        return ops.linear_fp8(x, w, torch.float32, impl=impl)
+    rows = ops.linear_activation_fp8(x, w, "silu", gated=kind == "gated", impl=impl)
+    return torch.cat([rows.codes.view(torch.uint8), rows.scales.view(torch.uint8)], 1)
+
+
+def used_alone(ops, kind, impl, weight, x):
+    w = held(weight)
+    torch.cuda.synchronize()
+    if kind == "linear":
+        return ops.linear_fp8(x, w, torch.float32, impl=impl)
+    rows = ops.linear_activation_fp8(x, w, "silu", gated=kind == "gated", impl=impl)
+    return torch.cat([rows.codes.view(torch.uint8), rows.scales.view(torch.uint8)], 1)
+
+
+@pytest.mark.parametrize("unheld", [False, True])
+@pytest.mark.parametrize("kind,impl", MADE)
+@pytest.mark.parametrize("N,K", [(512, 640), (8192, 2048)])
+def test_a_weight_made_by_the_kernel_before(ops, N, K, kind, impl, unheld):
+    """Other weights from run to run, in the same place of a recorded graph, where nothing stands between the two launches."""
+    x = rand((24, K), torch.bfloat16, seed=1)
+    x = x if unheld else held(x)
+    weights = [rand((N, K), seed=10 + i, scale=K ** -0.5 * 4.0 ** i) for i in range(3)]
+    want = [used_alone(ops, kind, impl, w, x) for w in weights]
+    place = weights[0].clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        made_and_used(ops, kind, impl, place, x)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = [made_and_used(ops, kind, impl, place, x) for _ in range(8)]
+    for i in (0, 1, 2, 0, 2, 1):
+        place.copy_(weights[i])
+        graph.replay()
+        assert all(torch.equal(o, want[i]) for o in out)
+    for i in range(3):                                   # (the same without a graph, launches queued one behind the other)
+        assert all(torch.equal(o, want[i]) for o in [made_and_used(ops, kind, impl, weights[i], x) for _ in range(8)])
+    ops.check_status()
+
+
+def test_rows_times_themselves(ops):
+    """The same rows on both sides, straight from the norm that made them."""
+    h, w = rand((300, 1040), seed=1), torch.ones(1040, device="cuda")
+    rows = ops.rmsnorm_fp8(h, None, w, 1e-5)
+    torch.cuda.synchronize()
+    want = ops.linear_fp8(rows, rows, torch.float32)
+    for _ in range(20):
+        rows = ops.rmsnorm_fp8(h, None, w, 1e-5)
+        assert torch.equal(ops.linear_fp8(rows, rows, torch.float32), want)
+    ops.check_status()

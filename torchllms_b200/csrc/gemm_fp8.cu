@@ -18,8 +18,8 @@
 // And three ends: the sums leave (float32 or bfloat16), or 8-bit rows of act(sum) do, or of act(gate) * up.
 //
 // Inside a CTA:
-//   warp 0     TMA: boxes of W [128 x 128] and of x [width x 128], 128-byte swizzle, one or two of each a stage; the first ones of W before the
-//              kernel ahead of this one has ended
+//   warp 0     TMA: boxes of W [128 x 128] and of x [width x 128], 128-byte swizzle, one or two of each a stage; the first ones of W are asked
+//              for into L2 before the kernel ahead of this one has ended
 //   warp 1     tcgen05.cp of scales (a word a row: four blocks of 128) and tcgen05.mma, four of K 32 a box; by one lane, as warp 0's loads
 //              (64 rows of 4,096 x 14,336 by pairs: 34.2 us with the lane elected at each instruction, 24.6 so, 21.9 with warp 0 so too)
 //   warps 2, 3 scales from memory to shared memory, four words a row and turn (2,048 of K), in turns; in the order that tcgen05.cp
@@ -166,6 +166,15 @@ __device__ __forceinline__ void tma_load_gated(unsigned dst, const CUtensorMap* 
     else TL_LOAD("");
 #undef TL_LOAD
 }
+// The same boxes into L2 only.  L2 is where all writes to memory meet, so what a kernel that still runs writes later is read all the same.
+__device__ __forceinline__ void prefetch_box(const CUtensorMap* map, int x, int y) {
+    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void prefetch_box_gated(const CUtensorMap* map, int x, int group) {
+    const int zero = 0;
+    asm volatile("cp.async.bulk.prefetch.tensor.5d.L2.global.tile [%0, {%1, %2, %2, %3, %2}];" ::"l"(map), "r"(x), "r"(zero), "r"(group) : "memory");
+}
+__device__ __forceinline__ void prefetch_line(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 __device__ __forceinline__ unsigned long long policy_first() {
     unsigned long long p;
     asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
@@ -400,9 +409,35 @@ __global__ void __launch_bounds__(threads_of(FORM), FORM == SPLIT ? 2 : 1) gemm_
     volatile int* aborted = &abort_flag;
     bool met = false;                  // SPLIT: whether the cluster has been waited for
     grid_launch_dependents();
-    // W and its scales depend on no earlier kernel: the first boxes of a product without a list of tiles are asked for ahead
-    const bool ahead = p.tiles == nullptr;
-    if (!(ahead && (warp == 0 || warp == 2 || warp == 3))) grid_dependency_wait();
+    // the row of W's scales that a lane copies as number j of four, of a slab; N and beyond: none
+    auto scale_row = [&](int slab, int j) {
+        if (EPI != GATED) return slab * BM + 32 * j + lane;
+        const int f = (slab * 4 + j) * 16 + (lane & 15);        // (lanes 0 to 15 gates, 16 to 31 their ups)
+        return f < p.hidden ? f + (lane >= 16 ? p.hidden : 0) : p.N;
+    };
+    // Nothing is read before the kernel ahead of this one has ended: rows in 8 bits are made by kernels of this library, which let their
+    // successors start early, and W is such rows.  But what a product without a list of tiles reads first is known: it comes into L2 meanwhile
+    // (decode steps of 8, by 32 layers: 2.668 ms so, 2.644 when W was loaded outright, which read rows that were not there yet).
+    if (p.tiles == nullptr && first_unit < p.n_tiles * p.slabs) {
+        const int slab = first_unit / p.n_tiles * SIDES + rank;
+        if (warp == 0 && elect_one()) {
+            const int until = min(kb1, kb0 + p.stages * BOXES);
+            for (int kb = kb0; kb < until; ++kb) {
+                if (EPI == GATED) prefetch_box_gated(&map_w, kb * BK, slab * 4);
+                else prefetch_box(&map_w, kb * BK, slab * BM);
+            }
+        }
+        const int kb = kb0 + (warp - 2) * TURN;
+        if ((warp == 2 || warp == 3) && kb < kb1) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int r = scale_row(slab, j);
+                if (r < p.N) prefetch_line(p.w_scales + (long long)r * p.pitch + kb);
+            }
+        }
+        __syncwarp();
+    }
+    grid_dependency_wait();
 
     // a slab's box: 128 rows of W, or 64 gates and their ups
     // Experts: W is read by few tiles, side by side, x by every slab: W is the first to leave L2 (2,048 tokens through gates and ups of
@@ -417,21 +452,9 @@ __global__ void __launch_bounds__(threads_of(FORM), FORM == SPLIT ? 2 : 1) gemm_
 
     if (warp == 0) {
         if (elect_one()) {
-            int stage = 0, issued = 0, early = 0;
+            int stage = 0, issued = 0;
             unsigned phase = 1;                // (a barrier that has completed nothing counts as having completed phase 1)
             bool ok = true;
-            if (ahead) {
-                if (first_unit < units) {
-                    const int slab = first_unit / n_tiles * SIDES + rank;
-                    for (int kb = kb0; kb < kb1 && early < p.stages; kb += BOXES, ++early) {
-                        const unsigned at = smem0 + early * stage_bytes, bar = leader(full + 8 * early);
-                        const int boxes = min(BOXES, kb1 - kb);
-                        if (rank == 0) expect_tx(full + 8 * early, SIDES * boxes * (w_bytes + p.x_box * BK));
-                        for (int i = 0; i < boxes; ++i) load_w(at + i * w_bytes, bar, (kb + i) * BK, slab, 0);
-                    }
-                }
-                grid_dependency_wait();
-            }
             for (int u = first_unit; u < units && ok; u += step) {
                 const Unit t = unit_of(p, u, n_tiles);
                 const int slab = t.slab * SIDES + rank, x_row = t.row0 + rank * (((t.rows + 15) & ~15) / 2);
@@ -443,13 +466,11 @@ __global__ void __launch_bounds__(threads_of(FORM), FORM == SPLIT ? 2 : 1) gemm_
                     }
                     const unsigned at = smem0 + stage * stage_bytes, bar = leader(full + 8 * stage);
                     const int boxes = min(BOXES, kb1 - kb);
-                    const bool fresh = early == 0;             // (else W's boxes are under way already)
-                    if (!fresh) --early;
-                    if (fresh && rank == 0) expect_tx(full + 8 * stage, SIDES * boxes * (w_bytes + p.x_box * BK));
+                    if (rank == 0) expect_tx(full + 8 * stage, SIDES * boxes * (w_bytes + p.x_box * BK));
 #pragma unroll
                     for (int i = 0; i < BOXES; ++i) {
                         if (i < boxes) {
-                            if (fresh) load_w(at + i * w_bytes, bar, (kb + i) * BK, slab, t.expert);
+                            load_w(at + i * w_bytes, bar, (kb + i) * BK, slab, t.expert);
                             tma_load<PAIR>(at + BOXES * w_bytes + i * x_bytes, &map_x, bar, (kb + i) * BK, x_row, x_policy);
                         }
                     }
@@ -530,7 +551,7 @@ __global__ void __launch_bounds__(threads_of(FORM), FORM == SPLIT ? 2 : 1) gemm_
     } else if (warp == 2 || warp == 3) {
         int turn = 0, buf = 0;
         unsigned phase = 1;
-        bool ok = true, waited = false;
+        bool ok = true;
         for (int u = first_unit; u < units && ok; u += step) {
             const Unit t = unit_of(p, u, n_tiles);
             const long long first = (long long)t.expert * p.N;
@@ -547,15 +568,9 @@ __global__ void __launch_bounds__(threads_of(FORM), FORM == SPLIT ? 2 : 1) gemm_
                     unsigned v[12][4];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        int r = (t.slab * SIDES + rank) * BM + 32 * j + lane;
-                        if (EPI == GATED) {        // (lanes 0 to 15 gates, 16 to 31 their ups)
-                            const int f = ((t.slab * SIDES + rank) * 4 + j) * 16 + (lane & 15);
-                            r = f < p.hidden ? f + (lane >= 16 ? p.hidden : 0) : p.N;
-                        }
+                        const int r = scale_row(t.slab * SIDES + rank, j);
                         load_words(r < p.N ? p.w_scales + (first + r) * p.pitch + kb : nullptr, words, whole && p.w_whole, v[j]);
                     }
-                    if (ahead && !waited) grid_dependency_wait();
-                    waited = true;
 #pragma unroll
                     for (int j = 4; j < 12; ++j) {
                         const int r = 32 * (j - 4) + lane;

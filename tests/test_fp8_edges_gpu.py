@@ -125,3 +125,37 @@ def test_rows_times_themselves(ops):
         rows = ops.rmsnorm_fp8(h, None, w, 1e-5)
         assert torch.equal(ops.linear_fp8(rows, rows, torch.float32), want)
     ops.check_status()
+
+
+# ------------------------------------------------------------------------------------------------- what CTAs of a cluster send each other
+
+@pytest.mark.parametrize("M", [1, 7, 32])
+def test_sums_sent_between_ctas(ops, M):
+    """K cut among the CTAs of a cluster, whole numbers: every sum is exact, in every one of many launches one behind the other."""
+    x, w = whole(-3, 3, (M, 8192), 1), whole(-3, 3, (640, 8192), 2)
+    want = (x.double() @ w.double().T).float()
+    xs, ws = held(x), held(w)
+    assert all(torch.equal(ops.linear_fp8(xs, ws, torch.float32, impl="split"), want) for _ in range(100))
+    ops.check_status()
+
+
+@pytest.mark.parametrize("M", [3, 200, 481])
+def test_magnitudes_sent_between_ctas(ops, M):
+    """The largest of 128 gated numbers is now one CTA's, now the other's: scales by the definition, in every launch."""
+    hidden, K = 1024, 128
+    x = torch.zeros((M, K), device="cuda")
+    x[torch.arange(M), torch.arange(M) % K] = 1.0
+    # u of column d is 2^(-20 .. 20) in one place of the 128, one beside it: squares of them leave
+    up = torch.full((hidden, K), 2.0 ** -24, device="cuda")
+    place = whole(0, 127, (hidden // 128, K), 3).long()
+    power = torch.exp2(whole(-20, 20, (hidden // 128, K), 4))
+    up.view(hidden // 128, 128, K).scatter_(1, place[:, None], power[:, None])
+    ws = held(torch.cat([up, up]))
+    value = plain.value(ws)[:hidden]
+    want = value[:, torch.arange(M, device="cuda") % K].T.clamp(min=0) ** 3            # relu2(g) * u, exact
+    codes, e = plain.hold(want)
+    for _ in range(50):
+        rows = ops.linear_activation_fp8(held(x), ws, "relu2", gated=True)
+        assert torch.equal(rows.scales.view(torch.uint8)[:, :e.shape[1]].double(), e + 127)
+        assert torch.equal(rows.codes.double(), codes)
+    ops.check_status()

@@ -66,12 +66,17 @@ __device__ __forceinline__ unsigned smem_u32(const void* p) { return (unsigned)_
 __device__ __forceinline__ void mbar_init(unsigned bar, unsigned count) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count));
 }
+// OTHERS: the waiting thread itself reads what another CTA of the cluster has stored here, so the wait acquires at the cluster's scope.  What the
+// other waits guard is read by the tensor cores and the copy engine, or from tensor memory (an acquire at the cluster's scope in all of
+// them took 8 rows of 28,672 x 4,096 from 34.7 us to 35.9).
+template <bool OTHERS>
 __device__ __forceinline__ bool mbar_try_wait(unsigned bar, unsigned parity) {
     unsigned ok;
-    // (what a wait guards is read by the tensor cores and the copy engine, not by the waiting thread; an acquire at the scope of the
-    // cluster took 8 rows of 28,672 x 4,096 from 34.7 us to 35.9)
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    if (OTHERS)
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    else asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                      : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     return ok != 0;
 }
 __device__ __forceinline__ unsigned long long global_ns() {
@@ -80,12 +85,13 @@ __device__ __forceinline__ unsigned long long global_ns() {
     return t;
 }
 // false once the limit has passed, or as soon as another role has given up
+template <bool OTHERS = false>
 __device__ __forceinline__ bool wait_one(unsigned bar, unsigned parity, volatile int* aborted) {
-    bool ok = mbar_try_wait(bar, parity);
+    bool ok = mbar_try_wait<OTHERS>(bar, parity);
     unsigned long long t0 = 0;
     // (the timer is read rarely: a read takes as long as a stage's products)
     for (unsigned i = 1; !ok; ++i) {
-        ok = mbar_try_wait(bar, parity);
+        ok = mbar_try_wait<OTHERS>(bar, parity);
         if (!ok && (i & 255u) == 0u) {
             if (t0 == 0) t0 = global_ns();
             if (*aborted || global_ns() - t0 > WAIT_LIMIT_NS) break;
@@ -94,8 +100,9 @@ __device__ __forceinline__ bool wait_one(unsigned bar, unsigned parity, volatile
     return ok;
 }
 // the same for a whole warp that waits together
+template <bool OTHERS = false>
 __device__ __forceinline__ bool mbar_wait(unsigned bar, unsigned parity, volatile int* aborted) {
-    return __all_sync(0xffffffffu, wait_one(bar, parity, aborted));
+    return __all_sync(0xffffffffu, wait_one<OTHERS>(bar, parity, aborted));
 }
 __device__ __forceinline__ void give_up(volatile int* aborted, int* status, int code) {
     *aborted = 1;
@@ -657,7 +664,7 @@ __global__ void __launch_bounds__(threads_of(FORM), FORM == SPLIT ? 2 : 1) gemm_
             if (CUT && p.push_bytes > 0) {
                 // this CTA's groups, added up in the order of K: a row of W a lane, four rows of x
                 const int own = groups_of(t.rows, cut, p.splits), row = t.slab * BM + quarter * 32 + lane;
-                if (own > 0 && !mbar_wait(told, 0, aborted)) {
+                if (own > 0 && !mbar_wait<true>(told, 0, aborted)) {
                     if (lane == 0) give_up(aborted, p.status, ERR_EPI_WAIT);
                     break;
                 }
@@ -748,7 +755,7 @@ __global__ void __launch_bounds__(threads_of(FORM), FORM == SPLIT ? 2 : 1) gemm_
                 // (the other CTA's next store to this place is behind two units of this one)
                 if (thread == 0) expect_tx(told + 8 * acc, 4 * t.rows);
                 __syncwarp();
-                ok = mbar_wait(told + 8 * acc, (n / 2) & 1, aborted);
+                ok = mbar_wait<true>(told + 8 * acc, (n / 2) & 1, aborted);
                 if (!ok && lane == 0) give_up(aborted, p.status, ERR_EPI_WAIT);
             }
             if (thread < t.rows && ok) {

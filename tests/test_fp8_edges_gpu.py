@@ -159,3 +159,59 @@ def test_magnitudes_sent_between_ctas(ops, M):
         assert torch.equal(rows.scales.view(torch.uint8)[:, :e.shape[1]].double(), e + 127)
         assert torch.equal(rows.codes.double(), codes)
     ops.check_status()
+
+
+# ------------------------------------------------------------------------------------------------- choices that are no experts
+
+def padded(T, E, top, seed):
+    """Choices of which some are no experts, with weights that would spoil a sum; one token has no expert at all."""
+    chosen, share = whole(0, E - 1, (T, top), seed).int(), rand((T, top), seed=seed + 1).abs()
+    real = torch.rand((T, top), generator=torch.Generator(device="cuda").manual_seed(seed + 2), device="cuda") < 0.7
+    real[T // 2] = False
+    odd = torch.tensor([-1, E, -2 ** 31, 2 ** 31 - 1], dtype=torch.int32, device="cuda")[whole(0, 3, (T, top), seed + 3).long()]
+    spoilt = torch.where(whole(0, 1, (T, top), seed + 4) == 1, torch.full_like(share, float("nan")), torch.full_like(share, float("inf")))
+    zero = torch.zeros_like(share)
+    return torch.where(real, chosen, odd), torch.where(real, share, spoilt), torch.where(real, chosen, torch.zeros_like(chosen)), torch.where(real, share, zero)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T,E,top", [(1, 4, 2), (20, 8, 2), (300, 8, 4), (33, 16, 7)])
+def test_choices_that_are_no_experts_add_nothing(ops, dtype, T, E, top):
+    chosen, share, instead, nothing = padded(T, E, top, 11)
+    x = rand((T, 128), dtype, seed=1)
+    up, down = rand((E, 96, 128), dtype, seed=2, scale=0.1), rand((E, 128, 96), dtype, seed=3, scale=0.1)
+    shared = rand((T, 128), dtype, seed=4)
+    for extra in (None, shared):
+        got = ops.moe_experts_fp8(x, chosen, share, held(up), held(down), activation="silu", shared=extra)
+        assert torch.equal(got, ops.moe_experts_fp8(x, instead, nothing, held(up), held(down), activation="silu", shared=extra))
+        assert torch.equal(got[T // 2], torch.zeros_like(got[0]) if extra is None else shared[T // 2])
+        side = down.permute(1, 0, 2).reshape(128, E * 96).contiguous()
+        got = ops.moe_experts(x, chosen, share, up, side, activation="silu", shared=extra)
+        assert bool(torch.isfinite(got).all())
+        assert torch.equal(got[T // 2], torch.zeros_like(got[0]) if extra is None else shared[T // 2])
+        if T * top < ops.GROUPED_MIN_PAIRS or dtype == torch.float32:
+            assert torch.equal(got, ops.moe_experts(x, instead, nothing, up, side, activation="silu", shared=extra))
+    ops.check_status()
+
+
+def test_no_choice_is_an_expert(ops):
+    chosen = torch.full((5, 3), -1, dtype=torch.int32, device="cuda")
+    share = torch.full((5, 3), float("nan"), device="cuda")
+    up, down = held(rand((4, 32, 128), seed=1)), held(rand((4, 128, 32), seed=2))
+    for _ in range(3):
+        assert bool((ops.moe_experts_fp8(rand((5, 128), seed=3), chosen, share, up, down, activation="gelu") == 0).all())
+    ops.check_status()
+
+
+def test_layers_of_experts_as_one_matrix_take_padding(ops):
+    """The form for few tokens: all experts' hidden rows, a column times its expert's weight."""
+    chosen, share, instead, nothing = padded(6, 4, 2, 21)
+    keep = nothing != 0
+    x, up = rand((6, 128), torch.bfloat16, seed=1), rand((4 * 96, 128), torch.bfloat16, seed=2, scale=0.1)
+    got = ops.moe_dense_hidden(x, chosen, share, None, up, n_experts=4, hidden=96, activation="silu")
+    weight = torch.zeros((6, 4), device="cuda")
+    for t in range(6):
+        for k in range(2):
+            if keep[t, k]:
+                weight[t, int(chosen[t, k])] = share[t, k]
+    assert bool(torch.isfinite(got).all()) and bool(((got.view(6, 4, 96) != 0).any(-1) == (weight != 0)).all())

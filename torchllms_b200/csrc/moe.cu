@@ -15,6 +15,7 @@
 //           expert; float32 multiply-adds on the CUDA cores, operands float32 or bfloat16.
 // combine:  out[t] = sum_k weight[t, k] * Y[place(t, k)]  (+ gate[t] * shared[t]), summed in the
 //           order of the choices, so a token's result does not depend on what else is in the batch.
+// A choice that is no expert (below 0, or beyond the last: padding) has no row and adds nothing, whatever its weight.
 #include "common.cuh"
 #include <math.h>
 
@@ -198,6 +199,7 @@ __global__ void __launch_bounds__(1024) moe_plan_kernel(const int* __restrict__ 
     for (int a = threadIdx.x; a < n_pairs; a += blockDim.x) {
         const int e = chosen[a];
         if (e >= 0 && e < n_experts) atomicAdd(&counts[e], 1);
+        else place[a] = -1;               // (an expert that there is not: the pair has no row)
     }
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -213,10 +215,13 @@ __global__ void __launch_bounds__(1024) moe_plan_kernel(const int* __restrict__ 
             off += counts[e];
             if (ends != nullptr) ends[e] = off;
         }
+        // (places of pairs without a row are the last expert's, for those who walk all of them; nobody adds them up)
+        if (ends != nullptr) ends[n_experts - 1] = n_pairs;
         offsets[n_experts] = off;
         tiles[0] = n_tiles;
     }
     __syncthreads();
+    for (int a = offsets[n_experts] + threadIdx.x; a < n_pairs; a += blockDim.x) order[a] = 0;
     // stable placement: a warp per expert walks the pairs in order
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n_warps = blockDim.x >> 5;
     for (int e = warp; e < n_experts; e += n_warps) {
@@ -298,14 +303,17 @@ __global__ void __launch_bounds__(NT) moe_gemm_kernel(const T* __restrict__ A, c
     }
 }
 
-// N numbers from a 16-byte boundary on
+// N numbers of a row, from a 16-byte boundary on; zeros where there is no row
 template <int N, typename T>
-__device__ __forceinline__ void load_run(const T* p, float (&v)[N]) {
+__device__ __forceinline__ void load_place(const T* y, int row, int dim, int d, float (&v)[N]) {
     constexpr int M = Vec16<T>::N;
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] = 0.f;
+    if (row < 0) return;
 #pragma unroll
     for (int i = 0; i < N; i += M) {
         Vec16<T> r;
-        r.load(p + i);
+        r.load(y + (size_t)row * dim + d + i);
 #pragma unroll
         for (int e = 0; e < M; ++e) v[i + e] = r.get(e);
     }
@@ -324,8 +332,9 @@ __global__ void moe_combine_kernel(const TY* __restrict__ y, const int* __restri
     grid_dependency_wait();
     const int t = blockIdx.x;
     if (threadIdx.x < top) {
-        pl[threadIdx.x] = max(place[(size_t)t * top + threadIdx.x], 0);        // (-1: an expert that there is not; stay in bounds)
-        wt[threadIdx.x] = weights[(size_t)t * top + threadIdx.x];
+        const int at = place[(size_t)t * top + threadIdx.x];
+        pl[threadIdx.x] = at;
+        wt[threadIdx.x] = at >= 0 ? weights[(size_t)t * top + threadIdx.x] : 0.f;
     }
     __syncthreads();
     const float g = gate != nullptr ? gate[t] : 1.f;
@@ -339,7 +348,7 @@ __global__ void moe_combine_kernel(const TY* __restrict__ y, const int* __restri
             for (; k + 4 <= top; k += 4) {
                 float v[4][N];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) load_run(y + (size_t)pl[k + i] * dim + d, v[i]);
+                for (int i = 0; i < 4; ++i) load_place(y, pl[k + i], dim, d, v[i]);
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -347,7 +356,7 @@ __global__ void moe_combine_kernel(const TY* __restrict__ y, const int* __restri
             }
             for (; k < top; ++k) {
                 float v[N];
-                load_run(y + (size_t)pl[k] * dim + d, v);
+                load_place(y, pl[k], dim, d, v);
 #pragma unroll
                 for (int e = 0; e < N; ++e) acc[e] = fmaf(wt[k], v[e], acc[e]);
             }
@@ -367,7 +376,7 @@ __global__ void moe_combine_kernel(const TY* __restrict__ y, const int* __restri
     } else {
         for (int d = threadIdx.x; d < dim; d += blockDim.x) {
             float acc = 0.f;
-            for (int k = 0; k < top; ++k) acc = fmaf(wt[k], to_float(y[(size_t)pl[k] * dim + d]), acc);
+            for (int k = 0; k < top; ++k) acc = fmaf(wt[k], pl[k] >= 0 ? to_float(y[(size_t)pl[k] * dim + d]) : 0.f, acc);
             if (shared != nullptr) {
                 float sh = 0.f;
                 for (int s = 0; s < shared_splits; ++s) sh += to_float(shared[(size_t)s * shared_plane + (size_t)t * dim + d]);
@@ -412,7 +421,10 @@ __global__ void moe_scale_act_kernel(const TI* __restrict__ u, int splits, long 
     const int t = blockIdx.x, width = n_experts * hidden + extra;
     for (int e = threadIdx.x; e < n_experts; e += blockDim.x) wexp[e] = 0.f;
     __syncthreads();
-    if (threadIdx.x < top) wexp[chosen[(size_t)t * top + threadIdx.x]] = weights[(size_t)t * top + threadIdx.x];
+    if (threadIdx.x < top) {
+        const int e = chosen[(size_t)t * top + threadIdx.x];
+        if (e >= 0 && e < n_experts) wexp[e] = weights[(size_t)t * top + threadIdx.x];
+    }
     __syncthreads();
     const float g = gate != nullptr ? gate[t] : 1.f;
     if (gated) {
@@ -536,7 +548,7 @@ extern "C" int tl_moe_max_tiles(int n_pairs, int n_experts) {
 
 // chosen: int32 [n_pairs]; order, place: int32 [n_pairs]; tiles: int32 [1 + 3 * max_tiles] (count, then
 // expert, first row, rows of every tile)
-// ends: int32 [n_experts] or null: where every expert's rows end in the sorted order
+// ends: int32 [n_experts] or null: where every expert's rows end in the sorted order (the last one's: n_pairs)
 extern "C" int tl_moe_plan(const int* chosen, int n_pairs, int n_experts, int* order, int* place, int* tiles, int* ends,
                            void* stream) {
     if (n_pairs <= 0) return TL_OK;

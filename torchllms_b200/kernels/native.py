@@ -1365,7 +1365,8 @@ class NativeOps:
                     w_down: torch.Tensor, *, activation: str, shared: Optional[torch.Tensor] = None,
                     shared_gate: Optional[torch.Tensor] = None, gated: bool = False, act_params=None) -> torch.Tensor:
         """``out[t] = sum_k weights[t, k] * down_e(act(up_e x[t]))`` with ``e = chosen[t, k]``, plus
-        ``shared[t]`` (``[T, dim]`` or float32 partial sums) times ``shared_gate[t]`` where given.
+        ``shared[t]`` (``[T, dim]`` or float32 partial sums) times ``shared_gate[t]`` where given.  A choice outside ``0 .. E - 1``
+        (padding) adds nothing, whatever its weight.
         With ``gated`` an expert is ``down_e(act(gate_e x) * up_e x)`` and ``w_up`` is ``[E, 2 * hidden, dim]``, an expert's
         rows being ``[gate; up]``; ``activation="clamped_swish"`` (gated only) with ``act_params = (limit, alpha, up_offset)``
         is ``g * sigmoid(alpha g) * (u + up_offset)``, ``g = min(gate, limit)``, ``u = clamp(up, +-limit)``.
@@ -1665,8 +1666,7 @@ class NativeOps:
                         act_params=None, impl: str = "auto") -> torch.Tensor:
         """:meth:`moe_experts` with weights in 8 bits: ``w_up`` ``[E, hidden, dim]`` (``gated``: ``[E, 2 * hidden, dim]``, rows ``[gate; up]``) and
         ``w_down`` ``[E, dim, hidden]``.  A token's row is brought to 8 bits once, the hidden rows behind the activation again (taken in
-        float32, rounded once); both products run over the rows sorted by expert.  Experts that nobody chose are not read.  ``chosen`` must lie
-        in ``0 .. E - 1``; what a token with another number gets is not defined."""
+        float32, rounded once); both products run over the rows sorted by expert.  Experts that nobody chose are not read."""
         code, limit, alpha, offset = self._fp8_activation(activation, gated, act_params)
         form = self._FP8_FORMS.get(impl)
         if form is not None and type(w_up) is Fp8Rows and type(w_down) is Fp8Rows:

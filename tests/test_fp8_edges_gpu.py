@@ -215,3 +215,59 @@ def test_layers_of_experts_as_one_matrix_take_padding(ops):
             if keep[t, k]:
                 weight[t, int(chosen[t, k])] = share[t, k]
     assert bool(torch.isfinite(got).all()) and bool(((got.view(6, 4, 96) != 0).any(-1) == (weight != 0)).all())
+
+
+# ------------------------------------------------------------------------------------------------- activations that vanish
+
+def check_far_rows(rows, y, slack):
+    """Half a step of E4M3 (2^-4 of the number, 2^-10 of the scale), ``slack`` and a relative 2^-14: exponentials are off by 2 + 1.173 times their
+    argument units of 2^-23 (2^-16 at 100), a quotient by two, an argument of 2^-24 of itself three times over shifts them by as much again."""
+    got, scale = plain.value(rows), rows.scales.double().repeat_interleave(128, -1)[:, :y.shape[1]]
+    bound = torch.maximum(y.abs() * 2.0 ** -4, scale * 2.0 ** -10) * 1.0001 + y.abs() * 2.0 ** -14 + slack
+    assert bool(((got - y).abs() <= bound).all()), float(((got - y).abs() / bound).max())
+    # scales follow the numbers of their block
+    top = torch.nn.functional.pad(y.abs() + 0 * scale, (0, -y.shape[1] % 128)).unflatten(-1, (-1, 128)).amax(-1)
+    used = rows.scales.double()[:, :top.shape[1]]
+    far = torch.nn.functional.pad(slack, (0, -y.shape[1] % 128)).unflatten(-1, (-1, 128)).amax(-1)
+    assert bool((top * (1 + 2.0 ** -14) + far >= 224.0 * used)[used > 2.0 ** -126].all()) and bool((top * (1 - 2.0 ** -14) - far <= 448.0 * used).all())
+
+
+@pytest.mark.parametrize("kind,lo,hi", [("silu", -100.0, -20.0), ("gelu", -5.5, -3.0), ("gelu_tanh", -5.5, -3.0), ("clamped_swish", -55.0, -10.0)])
+def test_activations_of_gates_far_below_zero(ops, kind, lo, hi):
+    """Blocks of 128 whose numbers are all of one small size: from gates of nearly the same value, steps apart from row to row."""
+    T, K = 400, 256
+    params = (1e32, 1.7, 0.0) if kind == "clamped_swish" else None
+    gate = torch.linspace(lo, hi, T, device="cuda")[:, None] * (1.0 + 0.001 * torch.rand((T, K), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda"))
+    up = rand((T, K), seed=2) * 1e30
+    y = plain.act(torch.cat([gate, up], 1).double(), kind, True, params)
+    # (an exponential, and its product with the gate, may be below float32's smallest normal number: steps of 2^-149, before the large factor)
+    tiny = (gate.double().abs() + 1.0) * up.double().abs() * 2.0 ** -148
+    check_far_rows(ops.activation_fp8(torch.cat([gate, up], 1), kind, gated=True, act_params=params), y, tiny)
+    if kind != "clamped_swish":
+        y = plain.act(gate.double(), kind)
+        check_far_rows(ops.activation_fp8(gate, kind), y, (gate.double().abs() + 1.0) * 2.0 ** -148)
+
+
+@pytest.mark.parametrize("kind,values", [("silu", (-104.0, -96.0, -88.0, -80.0, -36.0, -20.0)), ("gelu", (-5.5, -5.0, -4.5, -4.0, -3.5)),
+                                         ("gelu_tanh", (-5.5, -5.0, -4.5, -4.0, -3.5)), ("clamped_swish", (-60.0, -48.0, -22.0, -9.0))])
+def test_products_behind_activations_of_gates_far_below_zero(ops, kind, values):
+    """The same behind a product: a row of x picks a column of W, whose rows all hold one gate and numbers of E4M3 beside it."""
+    params = (2.0 ** 100, 1.75, 0.0) if kind == "clamped_swish" else None
+    hidden, K, M = 256, 128, len(values)
+    x = torch.zeros((M, K), device="cuda")
+    x[torch.arange(M), torch.arange(M)] = 1.0
+    up = torch.zeros((hidden, K), device="cuda")
+    up[:, :M] = whole(8, 15, (hidden, M), 3) * 2.0 ** 96                 # (four significant bits)
+    for m, v in enumerate(values):
+        gate = torch.zeros((hidden, K), device="cuda")
+        gate[:, m] = v
+        w = torch.cat([gate, up])
+        u = torch.zeros((M, 2 * hidden), device="cuda", dtype=torch.float64)
+        u[m, :hidden] = v
+        u[:, hidden:] = plain.value(held(up))[:, :M].T
+        y = plain.act(u, kind, True, params)
+        slack = (u[:, :hidden].abs() + 1.0) * u[:, hidden:].abs() * 2.0 ** -148
+        check_far_rows(ops.linear_activation_fp8(held(x), held(w), kind, gated=True, act_params=params), y, slack)
+        if params is None:
+            check_far_rows(ops.linear_activation_fp8(held(x), held(gate), kind), plain.act(u[:, :hidden], kind), (u[:, :hidden].abs() + 1.0) * 2.0 ** -148)
+    ops.check_status()

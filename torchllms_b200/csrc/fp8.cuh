@@ -62,22 +62,30 @@ __device__ __forceinline__ int fp8_encode8(const float (&v)[8], uint2& bytes) {
     return e;
 }
 
-// ---- activations of feed-forwards: the codes and the arithmetic of csrc/moe.cu
+// ---- activations of feed-forwards: the codes and the functions of csrc/moe.cu, in forms that keep their relative error where they vanish
+// (a block may hold nothing else, and its scale follows its numbers)
 enum : int { FP8_SILU = 0, FP8_GELU_TANH = 1, FP8_RELU2 = 2, FP8_CLAMPED_SWISH = 3, FP8_GELU = 4 };
 struct Fp8Gate { float limit, alpha, up_offset; };
 
-// (quotients of __fdividef and exponentials of __expf: two units off each, far below the step of E4M3 that follows)
+// x / (1 + e^-y) by e^-|y|, which is at most 1, so the divisor lies between 1 and 2, where its approximate reciprocal is off by one unit; __expf is
+// off by 2 + 1.17 |y| of them (2^-16 at 95): far below the step of E4M3 that follows.
+__device__ __forceinline__ float fp8_times_sigmoid(float x, float y) {
+    const float e = __expf(-fabsf(y));
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+    return (y < 0.f ? x * e : x) * r;
+}
 __device__ __forceinline__ float fp8_act(float x, int act) {
-    if (act == FP8_SILU) return __fdividef(x, 1.f + __expf(-x));
-    if (act == FP8_GELU_TANH) return 0.5f * x * (1.f + tanhf(0.7978845608028654f * (x + 0.044715f * x * x * x)));
-    if (act == FP8_GELU) return 0.5f * x * (1.f + erff(0.7071067811865476f * x));
+    if (act == FP8_SILU) return fp8_times_sigmoid(x, x);
+    if (act == FP8_GELU_TANH) return fp8_times_sigmoid(x, 1.5957691216057308f * (x + 0.044715f * x * x * x));      // (1 + tanh y) / 2 = sigmoid(2 y)
+    if (act == FP8_GELU) return x * normcdff(x);             // (1 + erf(x / sqrt 2)) / 2, without the difference that cancels below 0
     const float r = x < 0.f ? 0.f : x;           // (comparisons, not fmaxf: what is not a number stays so)
     return r * r;
 }
 __device__ __forceinline__ float fp8_gated(float gate, float up, int act, const Fp8Gate& p) {
     if (act == FP8_CLAMPED_SWISH) {
         const float g = gate > p.limit ? p.limit : gate, u = up > p.limit ? p.limit : (up < -p.limit ? -p.limit : up);
-        return __fdividef(g, 1.f + __expf(-p.alpha * g)) * (u + p.up_offset);
+        return fp8_times_sigmoid(g, p.alpha * g) * (u + p.up_offset);
     }
     return fp8_act(gate, act) * up;
 }

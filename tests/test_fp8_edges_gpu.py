@@ -271,3 +271,57 @@ def test_products_behind_activations_of_gates_far_below_zero(ops, kind, values):
         if params is None:
             check_far_rows(ops.linear_activation_fp8(held(x), held(gate), kind), plain.act(u[:, :hidden], kind), (u[:, :hidden].abs() + 1.0) * 2.0 ** -148)
     ops.check_status()
+
+
+# ------------------------------------------------------------------------------------------------- a run of them, recorded
+
+@pytest.mark.parametrize("T", [1, 9, 200])
+def test_every_output_of_a_recorded_run(ops, T):
+    """Codes, scales, sums and the stream of a replayed run against an eager one's, byte by byte, with other inputs from replay to replay."""
+    dim, hidden, E = 512, 640, 8
+    w13, w2 = held(rand((2 * hidden, dim), seed=4, scale=dim ** -0.5)), held(rand((dim, hidden), seed=5, scale=hidden ** -0.5))
+    up, down = held(rand((E, hidden, dim), seed=6, scale=dim ** -0.5)), held(rand((E, dim, hidden), seed=7, scale=hidden ** -0.5))
+    norm = 1.0 + 0.1 * rand((dim,), seed=3)
+
+    def inputs(seed):
+        best, chosen = torch.topk(rand((T, E), seed=seed), 2, dim=-1)
+        chosen = chosen.int().contiguous()
+        chosen[T // 2, 1] = -1                          # (padding)
+        return [rand((T, dim), seed=seed + 1), rand((T, dim), torch.bfloat16, seed=seed + 2), chosen, torch.softmax(best, -1).contiguous()]
+
+    def chain(h, delta, chosen, share):
+        rows = ops.rmsnorm_fp8(h, delta, norm, 1e-5)
+        act = ops.linear_activation_fp8(rows, w13, "silu", gated=True)
+        y = ops.linear_fp8(act, w2)
+        z = ops.moe_experts_fp8(y, chosen, share, up, down, activation="gelu")
+        again = ops.quantize_fp8(z)
+        last = ops.activation_fp8(z, "relu2")
+        return [t.view(torch.uint8) for r in (rows, act, again, last) for t in (r.codes, r.scales)] + [y, z, h]
+
+    place = [t.clone() for t in inputs(0)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        chain(*[t.clone() for t in place])
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = chain(*place)
+    for seed in (0, 30, 60, 30):
+        for t, v in zip(place, inputs(seed)):
+            t.copy_(v)
+        graph.replay()
+        want = chain(*inputs(seed))
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    ops.check_status()
+
+
+@pytest.mark.parametrize("T,E,top", [(700, 4096, 64), (1, 4096, 64), (2000, 3, 64)])
+def test_the_most_experts_and_choices(ops, T, E, top):
+    """As many experts and choices of a token as there may be: exact results, so that every pair is seen to be placed once."""
+    x = torch.zeros((T, 16), device="cuda")
+    x[torch.arange(T), whole(0, 15, (T,), 1).long()] = 1.0
+    up, down = whole(-1, 3, (E, 16, 16), 2), whole(-15, 15, (E, 16, 16), 3)
+    chosen, share = whole(0, E - 1, (T, top), 4).int(), rand((T, top), seed=5)
+    check_one_rounding(ops.moe_experts_fp8(x, chosen, share, held(up), held(down), activation="relu2"), x, chosen, share, up, down)
+    ops.check_status()

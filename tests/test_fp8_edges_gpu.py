@@ -325,3 +325,40 @@ def test_the_most_experts_and_choices(ops, T, E, top):
     chosen, share = whole(0, E - 1, (T, top), 4).int(), rand((T, top), seed=5)
     check_one_rounding(ops.moe_experts_fp8(x, chosen, share, held(up), held(down), activation="relu2"), x, chosen, share, up, down)
     ops.check_status()
+
+
+# ------------------------------------------------------------------------------------------------- norms, next to borders
+
+@pytest.mark.parametrize("T,K", [(2048, 4096), (500, 4096), (60, 16384), (40000, 16), (900, 1040)])
+def test_norms_are_rounded_once(ops, T, K):
+    """Every code and scale is that of the 64-bit row of the stream as it was left: what lies ahead of E4M3's rounding is off by some 2^-42 (eps
+    as a float32; all else 2^-47), so one number in 2^37 may stand that close to a border."""
+    h, w = rand((T, K), seed=1) * torch.exp(rand((K,), seed=2)), 1.0 + 0.2 * rand((K,), seed=3)
+    rows = ops.rmsnorm_fp8(h, rand((T, K), torch.bfloat16, seed=4), w, 1e-5)
+    x = h.double()
+    codes, e = plain.hold(x / torch.sqrt((x * x).mean(-1, keepdim=True) + 1e-5) * w.double())
+    assert torch.equal(rows.scales.view(torch.uint8)[:, :e.shape[1]].double(), e + 127)
+    assert torch.equal(rows.codes.double(), codes)
+
+
+def test_norms_of_rows_far_out(ops):
+    """Rows whose squares leave float32's range, weights of any size, rows that end a block's scale exactly, rows of one number."""
+    T, K = 64, 256
+    h = rand((T, K), seed=1) * torch.exp2(torch.linspace(-100, 100, T, device="cuda").round())[:, None]
+    w = torch.exp2(whole(-60, 20, (K,), 2)) * (1.0 + whole(0, 7, (K,), 3) / 8)
+    h[5], h[6] = 0.0, torch.where(torch.arange(K, device="cuda") == 9, 3.0, 0.0)
+    rows = ops.rmsnorm_fp8(h, None, w, 1e-30)
+    x = h.double()
+    codes, e = plain.hold(x / torch.sqrt((x * x).mean(-1, keepdim=True) + torch.tensor(1e-30, dtype=torch.float32).double()) * w.double())
+    assert torch.equal(rows.scales.view(torch.uint8)[:, :e.shape[1]].double(), e + 127)
+    assert torch.equal(rows.codes.double(), codes)
+
+
+def test_norms_keep_what_is_not_finite(ops):
+    h, w = rand((6, 256), seed=1), torch.ones(256, device="cuda")
+    h[1, 3], h[2, 200], w[7] = float("nan"), float("inf"), float("inf")
+    bad = torch.isnan(plain.value(ops.rmsnorm_fp8(h, None, w, 1e-5)))
+    want = torch.zeros_like(bad)
+    want[1], want[:, 7] = True, True
+    want[2, 200] = True                       # (an infinite row: the others are divided by infinity)
+    assert torch.equal(bad, want)

@@ -1,7 +1,7 @@
 // Rows into 8 bits (format: fp8.cuh): as they are, behind a residual sum and an RMS norm, behind an activation.
 //
 // rows:  codes, scales of x.
-// norm:  x = h + delta, h <- x;  y = x * rsqrt(mean(x^2) + eps) * w, all in float32;  codes, scales of y.
+// norm:  x = h + delta, h <- x, in float32;  y = x * rsqrt(mean(x^2) + eps) * w;  codes, scales of y.
 //        (RMSNorm, torchllms/models/networks.py:195-200: the rows go straight to 8 bits, rounded once.)
 // act:   y = act(u), or act(g) * u of the halves of a row, in float32;  codes, scales of y.
 //
@@ -118,19 +118,39 @@ __global__ void __launch_bounds__(ROWS_THREADS) rows_kernel(const T* __restrict_
     }
 }
 
+// y = x * (f_hi + f_lo) * w, rounded to float32 once: t + rest_t is the row's number under the norm, u what rest_t makes of y.
+struct Product { float t, u, y; };
+__device__ __forceinline__ Product product_of(float x, float f_hi, float f_lo, float w) {
+    const float t = x * f_hi, u = fmaf(x, f_lo, fmaf(x, f_hi, -t)) * w;
+    return {t, u, fmaf(t, w, u)};
+}
+// Rounded twice, a number next to a border of E4M3 may land on the border and fall to the wrong side.  Borders, those of the scales among them,
+// end in 19 bits of 0.  (So does one number in 2^19.)
+__device__ __forceinline__ bool may_be_a_border(float y) { return (__float_as_uint(y) & 0x7ffffu) == 0u; }
+// such a y, moved to its neighbour on the number's own side
+__device__ __forceinline__ float beside_border(const Product& p, float w) {
+    const float rest = fmaf(p.t, w, -p.y) + p.u;
+    const unsigned b = __float_as_uint(p.y);
+    // (a rest of less than 2^-44 is what the sums and the two halves of the factor are off by: the number itself may well stand on the border)
+    if (fabsf(rest) > fabsf(p.y) * 0x1p-44f && fabsf(rest) < INFINITY && p.y != 0.f) return __uint_as_float((rest > 0.f) == (p.y > 0.f) ? b + 1u : b - 1u);
+    return p.y;
+}
+
 // A CTA to a row, which stays in registers: SLOTS times eight numbers a thread.  delta: splits planes `plane` elements apart
-// (partial sums, added in order), or null.
+// (partial sums, added in order), or null.  The squares are summed in 64 bits and the factor is held in two float32, so that the one
+// rounding is E4M3's (in 32 bits one number in a million fell to the wrong side of a border, up to ten in 2,048 rows of 4,096; 19.3 us then,
+// 20.5 so).  Registers are held to what lets as many CTAs onto an SM as before: without that 21.5.
 template <typename TD, int SLOTS, int THREADS>
-__global__ void __launch_bounds__(THREADS) norm_kernel(float* __restrict__ h, const TD* __restrict__ delta, int splits, long long plane,
+__global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 1 : SLOTS == 1 ? 6 : SLOTS == 2 ? 5 : sizeof(TD) == 2 ? 4 : 3) norm_kernel(float* __restrict__ h, const TD* __restrict__ delta, int splits, long long plane,
                                                     const float* __restrict__ weight, unsigned char* __restrict__ codes,
                                                     unsigned char* __restrict__ scales, int K, float eps) {
-    __shared__ float part[32];
+    __shared__ double part[32];
     grid_launch_dependents();
     grid_dependency_wait();
     const size_t row = blockIdx.x;
     float* hr = h + row * K;
     float x[SLOTS][8];
-    float ss = 0.f;              // (of at most 32 squares, summed in pairs)
+    double ss = 0.0;
 #pragma unroll
     for (int s = 0; s < SLOTS; ++s) {
         const int d = (s * blockDim.x + threadIdx.x) * 8;
@@ -163,18 +183,25 @@ __global__ void __launch_bounds__(THREADS) norm_kernel(float* __restrict__ h, co
     }
 #pragma unroll
     for (int s = 0; s < SLOTS; ++s) {
-        float q[8];
+        double q[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) q[i] = x[s][i] * x[s][i];
-        ss += ((q[0] + q[1]) + (q[2] + q[3])) + ((q[4] + q[5]) + (q[6] + q[7]));
+        for (int i = 0; i < 4; ++i) {
+            const double lo = x[s][i], hi = x[s][i + 4];
+            q[i] = fma(hi, hi, lo * lo);
+        }
+        ss += (q[0] + q[1]) + (q[2] + q[3]);
     }
-    ss = warp_sum(ss);
+    auto sum64 = [](double v) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        return v;
+    };
+    ss = sum64(ss);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n_warps = blockDim.x >> 5;
     if (lane == 0) part[warp] = ss;
     __syncthreads();
-    const float total = warp_sum(lane < n_warps ? part[lane] : 0.f);
-    // (a true root and quotient: an error of the factor moves a whole row against E4M3's borders)
-    const float factor = 1.f / sqrtf(total / (float)K + eps);
+    const double factor = rsqrt(sum64(lane < n_warps ? part[lane] : 0.0) / K + (double)eps);
+    const float f_hi = (float)factor, f_lo = (float)(factor - (double)f_hi);
 #pragma unroll
     for (int s = 0; s < SLOTS; ++s) {
         const int d = (s * blockDim.x + threadIdx.x) * 8;
@@ -182,8 +209,19 @@ __global__ void __launch_bounds__(THREADS) norm_kernel(float* __restrict__ h, co
         if (d < K) {
             float w[8];
             load8(weight + d, w);
+            bool border = false;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[s][i] = x[s][i] * factor * w[i];
+            for (int i = 0; i < 8; ++i) border |= may_be_a_border(product_of(x[s][i], f_hi, f_lo, w[i]).y);
+            if (border) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const Product p = product_of(x[s][i], f_hi, f_lo, w[i]);
+                    x[s][i] = may_be_a_border(p.y) ? beside_border(p, w[i]) : p.y;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[s][i] = product_of(x[s][i], f_hi, f_lo, w[i]).y;
+            }
         }
         leave8(x[s], codes + row * K, scales + row * fp8_scale_pitch(K), d, K);
     }

@@ -75,10 +75,24 @@ __device__ __forceinline__ float fp8_times_sigmoid(float x, float y) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
     return (y < 0.f ? x * e : x) * r;
 }
+// The normal distribution below -t, for t >= 0: e^(-t^2 / 2) q P(q), q = 1 / (1 + 0.345 t).  P was fitted to Mills' ratio over sqrt(2 pi)
+// from 0 to 15 by least squares of the relative error, weighted until its largest was least (2.6e-8; 3e-7 with float32's roundings).  (CUDA's
+// normcdff, which does not cancel either: 1,531 rows of gates and ups of 14,336 by gelu 56 us; erff, which does, 34; this 30.)
+__device__ __forceinline__ float fp8_normal_tail(float t) {
+    float q, p = -0.0279335193f;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(fmaf(0.345f, t, 1.f)));
+    const float c[8] = {0.137620866f, 0.137990683f, 0.117477998f, 0.110766202f, -0.0349472314f, 0.183022812f, -0.267236143f, 0.143238321f};
+#pragma unroll
+    for (int i = 7; i >= 0; --i) p = fmaf(p, q, c[i]);
+    return __expf(-0.5f * t * t) * (p * q);
+}
 __device__ __forceinline__ float fp8_act(float x, int act) {
     if (act == FP8_SILU) return fp8_times_sigmoid(x, x);
     if (act == FP8_GELU_TANH) return fp8_times_sigmoid(x, 1.5957691216057308f * (x + 0.044715f * x * x * x));      // (1 + tanh y) / 2 = sigmoid(2 y)
-    if (act == FP8_GELU) return x * normcdff(x);             // (1 + erf(x / sqrt 2)) / 2, without the difference that cancels below 0
+    if (act == FP8_GELU) {                       // (1 + erf(x / sqrt 2)) / 2, without the difference that cancels below 0
+        const float p = fp8_normal_tail(fabsf(x));
+        return x < 0.f ? x * p : fmaf(-x, p, x);
+    }
     const float r = x < 0.f ? 0.f : x;           // (comparisons, not fmaxf: what is not a number stays so)
     return r * r;
 }

@@ -69,52 +69,44 @@ __device__ __forceinline__ void leave8(const float (&v)[8], unsigned char* codes
 }
 
 // FORM 0: the rows; 1: act(x); 2: gated act of the row's halves (x has 2 K columns); 3: the rows, each left at `top` places
-// (the rows that a token's choices of experts have in the sorted order).  grid (groups of ROWS rows, chunks of 2,048 columns): a
-// thread has the same eight columns of ROWS rows, all asked for before the first is used (1,531 rows of gates and ups of 14,336 each: 23.7 us
-// with one row, 20.2 with two; rows alone gain nothing).
-template <typename T, int FORM, int ACT, int ROWS>
+// (the rows that a token's choices of experts have in the sorted order).  grid (rows, chunks of 2,048 columns): eight columns a thread.  (Two rows a
+// thread, all asked for before the first is used: 1,531 rows of gates and ups of 14,336 22.4 us by silu, 25.6 by gelu's tanh form; one 22.3 and 24.8.)
+template <typename T, int FORM, int ACT>
 __global__ void __launch_bounds__(ROWS_THREADS) rows_kernel(const T* __restrict__ x, unsigned char* __restrict__ codes,
-                                                            unsigned char* __restrict__ scales, int rows, int K, Fp8Gate gp,
+                                                            unsigned char* __restrict__ scales, int K, Fp8Gate gp,
                                                             const int* __restrict__ place, int top) {
     grid_launch_dependents();
     grid_dependency_wait();
-    const size_t row0 = (size_t)blockIdx.x * ROWS;
+    const size_t row = blockIdx.x;
     const int d = (blockIdx.y * ROWS_THREADS + threadIdx.x) * 8, pitch = fp8_scale_pitch(K);
     constexpr int HALVES = FORM == 2 ? 2 : 1;
-    Eight<T> raw[ROWS][HALVES];
+    Eight<T> raw[HALVES];
 #pragma unroll
-    for (int r = 0; r < ROWS; ++r)
+    for (int h = 0; h < HALVES; ++h)
+        if (d < K) raw[h].load(x + (row * HALVES + h) * K + d);
+        else raw[h].zero();
+    float v[8];
+    raw[0].get(v);
+    if (FORM == 1)
 #pragma unroll
-        for (int h = 0; h < HALVES; ++h)
-            if (d < K && (ROWS == 1 || row0 + r < rows)) raw[r][h].load(x + ((row0 + r) * HALVES + h) * K + d);
-            else raw[r][h].zero();
+        for (int i = 0; i < 8; ++i) v[i] = fp8_act(v[i], ACT);
+    if (FORM == 2) {
+        float u[8];
+        raw[HALVES - 1].get(u);
 #pragma unroll
-    for (int r = 0; r < ROWS; ++r) {
-        const size_t row = row0 + r;
-        if (ROWS > 1 && row >= rows) break;
-        float v[8];
-        raw[r][0].get(v);
-        if (FORM == 1)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = fp8_act(v[i], ACT);
-        if (FORM == 2) {
-            float u[8];
-            raw[r][HALVES - 1].get(u);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = fp8_gated(v[i], u[i], ACT, gp);
+        for (int i = 0; i < 8; ++i) v[i] = fp8_gated(v[i], u[i], ACT, gp);
+    }
+    uint2 bytes;
+    const int e = fp8_encode8(v, bytes);
+    if (FORM == 3) {
+        for (int k = 0; k < top; ++k) {
+            const int to_row = place[row * top + k];
+            if (to_row < 0) continue;
+            const size_t to = to_row;
+            keep8(bytes, e, codes + to * K, scales + to * pitch, d, K);
         }
-        if (FORM == 3) {
-            uint2 bytes;
-            const int e = fp8_encode8(v, bytes);
-            for (int k = 0; k < top; ++k) {
-                const int to_row = place[row * top + k];
-                if (to_row < 0) continue;
-                const size_t to = to_row;
-                keep8(bytes, e, codes + to * K, scales + to * pitch, d, K);
-            }
-        } else {
-            leave8(v, codes + row * K, scales + row * pitch, d, K);
-        }
+    } else {
+        keep8(bytes, e, codes + row * K, scales + row * pitch, d, K);
     }
 }
 
@@ -318,18 +310,10 @@ __global__ void __launch_bounds__(1024) plan_kernel(const int* __restrict__ chos
     }
 }
 
-template <typename T, int FORM, int ACT, int ROWS>
-int launch_rows_of(const void* x, void* codes, void* scales, int rows, int K, const Fp8Gate& gp, const int* place, int top, cudaStream_t s) {
-    const dim3 grid((rows + ROWS - 1) / ROWS, (K + 8 * ROWS_THREADS - 1) / (8 * ROWS_THREADS));
-    return (int)tl_launch(rows_kernel<T, FORM, ACT, ROWS>, grid, dim3(ROWS_THREADS), 0, s, (const T*)x, (unsigned char*)codes, (unsigned char*)scales, rows, K,
-                          gp, place, top);
-}
 template <typename T, int FORM, int ACT>
 int launch_rows_act(const void* x, void* codes, void* scales, int rows, int K, const Fp8Gate& gp, const int* place, int top, cudaStream_t s) {
-    // gates and ups: two rows a thread as long as eight CTAs an SM are left
-    const long long ctas = (long long)rows * ((K + 8 * ROWS_THREADS - 1) / (8 * ROWS_THREADS));
-    if (FORM == 2 && ctas >= 2 * 8 * 148) return launch_rows_of<T, FORM, ACT, FORM == 2 ? 2 : 1>(x, codes, scales, rows, K, gp, place, top, s);
-    return launch_rows_of<T, FORM, ACT, 1>(x, codes, scales, rows, K, gp, place, top, s);
+    const dim3 grid(rows, (K + 8 * ROWS_THREADS - 1) / (8 * ROWS_THREADS));
+    return (int)tl_launch(rows_kernel<T, FORM, ACT>, grid, dim3(ROWS_THREADS), 0, s, (const T*)x, (unsigned char*)codes, (unsigned char*)scales, K, gp, place, top);
 }
 template <typename T>
 int launch_rows(const void* x, void* codes, void* scales, int rows, int K, int form, int act, const Fp8Gate& gp, const int* place, int top,

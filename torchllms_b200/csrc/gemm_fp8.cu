@@ -27,10 +27,10 @@
 //              word a turn, copied ahead, kept the products waiting, 49 us for 39 in the same case and 225 for 203 with 2,048 rows of 28,672 x 4,096.)
 //   the rest   results: tcgen05.ld, through shared memory to rows of C; two accumulators, so that the next unit's products run meanwhile
 //
-// Measured (microseconds of repeated calls; floors at 6.57 TB/s and twice 1.65 PFLOP/s): 8 rows of 28,672 x 4,096 22.9 (floor 18.1: 224
-// slabs on 148 SMs, one or two each), 64 of 4,096 x 14,336 16.0 (9.2), 2,048 of 28,672 x 4,096 218 under the power cap that
-// long runs of it meet, 183 in short ones (146).  What bounds the last, from copies of an earlier step (203 us in short runs)
-// with a part left out: no copies of scales 168, no loads 158, one product in four 126, no products 105.
+// Measured (microseconds of repeated calls; floors at 6.57 TB/s and twice the 16-bit rate of 1.65 PFLOP/s): 8 rows of 28,672 x 4,096 22.9 (floor
+// 18.1: 224 slabs on 148 SMs, one or two each), 64 of 4,096 x 14,336 15.8 (9.2), 2,048 of 28,672 x 4,096 208 to 217 under the power cap that
+// long runs of it meet, 172 to 181 in short ones (146; 122 is what the tensor pipe is busy for).  What bounds the last, from copies of an
+// earlier step (203 us in short runs) with a part left out: no copies of scales 168, no loads 158, one product in four 126, no products 105.
 // Every wait is bounded: on a time-out the CTA records a code, lets its copies land, frees its tensor memory and returns.
 #include "fp8.cuh"
 #include <cuda.h>

@@ -337,7 +337,8 @@ int launch_norm(float* h, const void* delta, int splits, long long plane, const 
     unsigned char *c = (unsigned char*)codes, *b = (unsigned char*)scales;
 #define TL_NORM(S, T) return (int)tl_launch(norm_kernel<TD, S, T>, dim3(rows), dim3(threads(S)), 0, s, h, (const TD*)delta, splits, plane, weight, c, b, K, eps)
     // Few rows: as many threads as there are eights of numbers.  Many: small CTAs, of which more fit an SM, each somewhere else on its
-    // way from loads to stores (2,048 rows of 4,096 18.9 us, with 512 threads 20.4; floor 14.1).
+    // way from loads to stores (2,048 rows of 4,096 20.5 us, with 512 threads 22.7, floor 14.1; of 2,048 10.6 and 12.2, of 8,192 41.7 and 47.3; 512
+    // rows, as many threads as eights, 7.9).
     if (rows >= 4 * 148) {
         if (lanes <= 256) TL_NORM(1, 256);
         if (lanes <= 512) TL_NORM(2, 256);

@@ -81,8 +81,9 @@ class LLM:
         precision's own type) or ``"fp4"`` (4.5 bits a number: 3.6 times the tokens of bfloat16 in the same memory, and as
         much less to read in a decode step; for architectures whose layers are rotary grouped-query attention, with pages
         of a multiple of 16 tokens; others are refused).  ``weights`` is how the layers' matrices are held: ``"full"``, or ``"fp8"`` (8 bits
-        and a scale of a power of two for 128 of them; bfloat16 only): attention, SwiGLU and routed experts hold theirs so, and the
-        rows that meet them are brought to 8 bits too; embedding, head, routers and other parts' matrices stay as they are."""
+        and a scale of a power of two for 128 of them; bfloat16 only): Llama's attention and SwiGLU, and routed experts of any architecture,
+        hold theirs so, and the rows that meet them are brought to 8 bits too; embedding, head, routers and other parts' matrices (of
+        architectures other than Llama: all but the experts') stay as they are."""
         if weights not in WEIGHT_FORMATS:
             raise ValueError(f"weights must be one of {', '.join(WEIGHT_FORMATS)}, got {weights!r}")
         if kv_cache not in CACHE_FORMATS:

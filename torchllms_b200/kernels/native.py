@@ -1565,8 +1565,8 @@ class NativeOps:
     @_timed_when_asked
     def rmsnorm_fp8(self, h: torch.Tensor, delta, weight: torch.Tensor, eps: float) -> Fp8Rows:
         """:meth:`rmsnorm` whose rows leave in 8 bits: ``h += delta`` in place (float32), then the rows of
-        ``h / sqrt(mean(h^2) + eps) * weight``, taken in float32 and rounded once.  ``delta``: ``[T, dim]`` float32/bfloat16, float32 partial
-        sums ``[splits, T, dim]``, a :class:`PendingProduct`, or ``None``."""
+        ``h / sqrt(mean(h^2) + eps) * weight``, bit for bit those of 64-bit arithmetic on the new ``h``.  ``delta``: ``[T, dim]``
+        float32/bfloat16, float32 partial sums ``[splits, T, dim]``, a :class:`PendingProduct`, or ``None``."""
         if isinstance(delta, PendingProduct):
             delta = delta.take(self)
         rows = (self._fp8 or self._fp8_load()).norm(h, delta, weight, eps)
@@ -1597,7 +1597,8 @@ class NativeOps:
     @_timed_when_asked
     def linear_fp8(self, x, w: Fp8Rows, out_dtype: torch.dtype = torch.bfloat16, impl: str = "auto") -> torch.Tensor:
         """``x [M, K] @ w[N, K]^T`` of 8-bit rows, summed in float32.  ``x`` may be float32/bfloat16 rows, which are brought to 8 bits
-        first (:meth:`quantize_fp8`).  The result is bfloat16 or float32 ``[M, N]``.  ``impl`` forces a form of the kernel (tests)."""
+        first (:meth:`quantize_fp8`).  The result is bfloat16 or float32 ``[M, N]``.  ``w`` may be what any call before this one left.
+        ``impl`` forces a form of the kernel (tests)."""
         type_code, form = _DT.get(out_dtype), self._FP8_FORMS.get(impl)
         if type_code is not None and form is not None and type(w) is Fp8Rows:
             calls = self._fp8 or self._fp8_load()
@@ -1666,7 +1667,8 @@ class NativeOps:
                         act_params=None, impl: str = "auto") -> torch.Tensor:
         """:meth:`moe_experts` with weights in 8 bits: ``w_up`` ``[E, hidden, dim]`` (``gated``: ``[E, 2 * hidden, dim]``, rows ``[gate; up]``) and
         ``w_down`` ``[E, dim, hidden]``.  A token's row is brought to 8 bits once, the hidden rows behind the activation again (taken in
-        float32, rounded once); both products run over the rows sorted by expert.  Experts that nobody chose are not read."""
+        float32, rounded once); both products run over the rows sorted by expert, and the experts' results stay in float32 until they are added up.
+        Experts that nobody chose are not read."""
         code, limit, alpha, offset = self._fp8_activation(activation, gated, act_params)
         form = self._FP8_FORMS.get(impl)
         if form is not None and type(w_up) is Fp8Rows and type(w_down) is Fp8Rows:
@@ -1774,8 +1776,9 @@ class NativeOps:
                partials_ok: bool = False) -> torch.Tensor:
         """``x [M, K] @ w[N, K]^T``.  float32 is multiplied in true 32-bit (see :meth:`gemm_simt`).  bfloat16 with
         at most 64 rows (decode steps) runs on the tcgen05 kernel that streams the weight once;
-        more rows use the library product, as the reference's ``nn.Linear`` does.  A weight in 8 bits goes to
-        :meth:`linear_fp8` (whole sums, whatever the number of rows).
+        more rows use the library product, as the reference's ``nn.Linear`` does.  (The kernel for few rows asks for ``w`` before the
+        launch ahead of it has ended: a ``w`` that a call of this library has just left wants a kernel of PyTorch's in between.)  A
+        weight in 8 bits goes to :meth:`linear_fp8` (whole sums, whatever the number of rows), where that does not matter.
 
         With ``partials_ok`` the result may be float32 partial sums ``[splits, M, N]`` of a
         split-K product, for callers that hand it to a kernel which adds them up (residual +

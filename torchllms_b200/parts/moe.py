@@ -194,7 +194,7 @@ class RoutedExperts(FeedForward):
             shared = None
             if self.shared_hidden:
                 u = ops.linear_activation_fp8(x, self.w_shared_up, self.activation, gated=self.gated, act_params=self.shared_act_params)
-                shared = ops.linear(u, self.w_shared_down)
+                shared = ops.linear(u, self.w_shared_down, out_dtype=torch.float32)      # (rounded where it has been added to the experts)
             return ops.moe_experts_fp8(x, chosen, weights, self.w_up, self.w_down, activation=self.activation, shared=shared, shared_gate=gate,
                                        gated=self.gated, act_params=self.act_params)
         if ops.moe_prefers_dense(x.shape[0], self.top, self.n_experts, x.dtype):
